@@ -568,6 +568,148 @@ int nb_attention_batch(const float* q, const float* k_cache, const float* v_cach
                        void* stream);
 
 /* ------------------------------------------------------------------------
+ * Serving: requests of different lengths over one 8-bit key / value cache.
+ * No counterpart in the reference (one fp32 cache of fixed shape for each
+ * sequence, inference/generate_torch.py:269-277).
+ *
+ * The cache is an array of blocks of NB_KV_BLOCK consecutive tokens of one
+ * request; block i of a layer holds, for each key / value head h < n_kv_head,
+ *     k        int8 [n_blocks][n_kv_head][NB_KV_BLOCK][head_dim]
+ *     v        int8 [n_blocks][n_kv_head][head_dim][NB_KV_BLOCK]
+ *     k_scale, v_scale   fp32 [n_blocks][n_kv_head]
+ * the key being k * k_scale, the value v * v_scale.  table[r][j] (row stride
+ * table_stride) is the block with positions 64 j .. 64 j + 63 of request r,
+ * -1 where there is none; slot 64 b + i is token i of block b.  All layers
+ * share the tables.
+ *
+ * A step brings new tokens of some requests, their rows one after the other
+ * in the order of the requests; nb_kv_plan says where they go, and the other
+ * calls follow its output.  A row that the plan gave no slot (a row behind
+ * the last request's, one that no block was free for) is skipped: its output
+ * rows are left as they were.  head_dim: a multiple of 16, <= 256; n_head: a
+ * multiple of n_kv_head.
+ * ------------------------------------------------------------------------ */
+#define NB_KV_BLOCK 64
+
+/* Entries (of 4 int32) of the chunk list of a step of n_tokens rows of
+ * n_requests requests: a chunk is a run of rows of one request within one
+ * block.  min(n_tokens, (n_tokens + 126 min(n_tokens, n_requests)) / 64). */
+int64_t nb_kv_plan_chunks(int n_tokens, int n_requests);
+/*
+ * The plan of a step, from lengths in device memory: request r < n_requests
+ * (<= 4096) has lens[r] tokens cached and brings new_tokens[r] (less than 0
+ * counts as 0).  Rows are given to the requests in order while n_tokens
+ * last; blocks from the end of the free list (free_blocks[state[0] - 1],
+ * ..[state[0] - 2], ...), in the order of requests and positions, while they
+ * last and max_blocks holds them.  Outputs:
+ *   table      the new blocks' entries (no other entry is written)
+ *   slots      [n_tokens] the slot of each row, -1 where it has none
+ *   positions  [n_tokens] its position (0 where it has no slot)
+ *   chunks     [nb_kv_plan_chunks(n_tokens, n_requests)][4]: first row, rows,
+ *              request, first position; 0 rows past the last
+ *   lens_out   [n_requests] lengths after the step
+ *   state_out  [2] free blocks after it; tokens of new_tokens without a slot
+ * lens_out and state_out are memory of their own: a call writes no input but
+ * table, and the same call again gives the same.
+ */
+int nb_kv_plan(int32_t* table, int64_t table_stride, const int32_t* lens,
+               const int32_t* new_tokens, const int32_t* free_blocks, const int32_t* state,
+               int n_requests, int max_blocks, int n_blocks, int n_tokens, int32_t* slots,
+               int32_t* positions, int32_t* chunks, int32_t* lens_out, int32_t* state_out,
+               void* stream);
+/*
+ * The blocks of every request r with finished[r] != 0 go to the end of the
+ * free list (in place, with state[0], its count), its table entries become -1
+ * and its length 0.  A block that several tables hold must be in one finished
+ * request's only.
+ */
+int nb_kv_release(int32_t* table, int64_t table_stride, int32_t* lens, const int32_t* finished,
+                  int32_t* free_blocks, int32_t* state, int n_requests, int max_blocks,
+                  int n_blocks, void* stream);
+/*
+ * RoPE and append: qkv has n_tokens rows (stride ld_qkv, NB_F32 or NB_BF16) of
+ * (n_head + 2 n_kv_head) head_dim values q | k | v.  Queries and keys are
+ * turned in pairs (2i, 2i + 1) by the angles cos_t / sin_t [n_pos][head_dim /
+ * 2] of the row's position (NaN where it is not under n_pos); q_out row =
+ * turned q * head_dim^-0.5 (stride ld_q, NB_F32 or NB_BF16).  Keys and values
+ * go to the cache: with s the block's scale (0 before its first token), a
+ * chunk's rows x set it to s' = max(s, max|x| / 127), their codes to
+ * clamp(rint(x / s'), -127, 127) and, where s' > s, the block's earlier codes
+ * to rint(code * s / s'), in fp32.  A NaN or infinity sets s' = inf: the block
+ * reads as NaN.  slots, positions and chunks as nb_kv_plan writes them.  Two
+ * chunks of a call must not lie in one block.
+ */
+int nb_kv8_append(const void* qkv, int qkv_dtype, int64_t ld_qkv, const int32_t* slots,
+                  const int32_t* positions, const int32_t* chunks, int n_chunks,
+                  const float* cos_t, const float* sin_t, int n_pos, int8_t* k, int8_t* v,
+                  float* k_scale, float* v_scale, int n_blocks, void* q_out, int q_dtype,
+                  int64_t ld_q, int n_tokens, int n_head, int n_kv_head, int head_dim,
+                  void* stream);
+/*
+ * keys / values [n][n_kv_head][head_dim] (NB_F32 or NB_BF16) of n slots of the
+ * cache, in any order; zeros for a slot outside it (-1).
+ */
+int nb_kv8_read(const int32_t* slots, int64_t n, const int8_t* k, const int8_t* v,
+                const float* k_scale, const float* v_scale, int n_blocks, int n_kv_head,
+                int head_dim, void* keys, void* values, int dtype, void* stream);
+/*
+ * Attention of the step's rows over the cache (appended first): row t of
+ * request r at position i, head h with key / value head h / (n_head /
+ * n_kv_head):
+ *     s(j)  = q[t][h] . k(j)                       (q scaled, as q_out above)
+ *     s(j)  = softcap * tanh(s(j) / softcap)       if softcap > 0
+ *     s(j) += slopes[h] * (j - i)                  if slopes
+ *     out[t][h] = sum_j softmax_j(s) v(j)
+ * over the cached positions j that it sees: j <= i, with window > 0 only
+ * i - window < j, and with prefix all j < prefix[r] besides (of those that
+ * the request has after the step, lens).  A block whose table entry lies
+ * outside the cache is not seen; a row that sees nothing is 0.  q, out:
+ * n_tokens rows of n_head * head_dim (strides ld_q, ld_out; NB_F32 or
+ * NB_BF16).  Sums and statistics in fp32; with NB_F32 outputs products of 24
+ * bits of q and of the softmax weights (each relative to the largest of its row) with the
+ * exact codes, with NB_BF16 outputs of 16.  The workspace needs
+ * nb_kv8_attention_ws_bytes(...) bytes, 16-byte aligned (0: may be NULL).
+ */
+int64_t nb_kv8_attention_ws_bytes(int n_tokens, int n_chunks, int max_blocks, int n_head,
+                                  int n_kv_head, int head_dim);
+int nb_kv8_attention(const void* q, int q_dtype, int64_t ld_q, const int32_t* chunks, int n_chunks,
+                     const int32_t* lens, const int32_t* table, int64_t table_stride,
+                     int n_requests, int max_blocks, const int8_t* k, const int8_t* v,
+                     const float* k_scale, const float* v_scale, int n_blocks, void* out,
+                     int out_dtype, int64_t ld_out, int n_tokens, int n_head, int n_kv_head,
+                     int head_dim, float softcap, int window, const float* slopes,
+                     const int32_t* prefix, void* workspace, int64_t ws_bytes, void* stream);
+/*
+ * Rules on `rows` rows of V logits (NB_F32 or NB_BF16, stride ld) and the
+ * greedy choice; out fp32 (stride ld_out; may be logits).  For row b, token v,
+ * in this order, each operation rounded by itself:
+ *     x = logits[b][v]
+ *     x = x > 0 ? x / repetition[b] : x * repetition[b]
+ *                                   if v is in history[b][0 .. lens[b])
+ *     x = (x - frequency[b] * n) - presence[b]
+ *                                   if v is n > 0 times in
+ *                                   history[b][prompt_lens[b] .. lens[b])
+ *     x = x + bias[b][i]            for the last i with bias_ids[b][i] == v
+ *     x = -inf                      if bit v % 32 of mask[b][v / 32] is 0
+ * tokens[b] (if tokens) = the lowest v with the largest x; a NaN is never
+ * chosen, and where all are -inf or NaN it is -1.  NULL leaves a rule out:
+ * history (with lens, row stride ld_history, max_history entries a row;
+ * prompt_lens NULL counts all of it), repetition, frequency, presence (rows
+ * fp32 each, with a history), bias_ids and bias (n_bias a row, stride
+ * ld_bias), mask (stride ld_mask).  Ids outside 0 .. V - 1 are passed over.
+ * The workspace needs nb_logits_rules_ws_bytes(rows, V) bytes if tokens are
+ * chosen, 8-byte aligned (0: may be NULL).
+ */
+int64_t nb_logits_rules_ws_bytes(int rows, int V);
+int nb_logits_rules(const void* logits, int dtype, int64_t ld, int rows, int V,
+                    const int32_t* history, int64_t ld_history, int max_history,
+                    const int32_t* lens, const int32_t* prompt_lens, const float* repetition,
+                    const float* frequency, const float* presence, const int32_t* bias_ids,
+                    const float* bias, int64_t ld_bias, int n_bias, const int32_t* mask,
+                    int64_t ld_mask, float* out, int64_t ld_out, int32_t* tokens, void* workspace,
+                    int64_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Persistent decode: many greedy tokens of the whole packed decoder in one
  * cooperative launch (one workgroup per CU), the phases of a token separated
  * by grid barriers instead of kernel boundaries, and the packed weights of

@@ -95,6 +95,18 @@ SIGNATURES = {
     "nb_lm_head_argmax": (_I, [_P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _P]),
     "nb_rmsnorm_lm_head_argmax": (_I, [_P, _P, ctypes.c_float, _P, _P, _P, _P, _I, _P, _I, _I,
                                        _I, _P]),
+    "nb_kv_plan_chunks": (_L, [_I, _I]),
+    "nb_kv_plan": (_I, [_P, _L, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P]),
+    "nb_kv_release": (_I, [_P, _L, _P, _P, _P, _P, _I, _I, _I, _P]),
+    "nb_kv8_append": (_I, [_P, _I, _L, _P, _P, _P, _I, _P, _P, _I, _P, _P, _P, _P, _I, _P, _I, _L,
+                           _I, _I, _I, _I, _P]),
+    "nb_kv8_read": (_I, [_P, _L, _P, _P, _P, _P, _I, _I, _I, _P, _P, _I, _P]),
+    "nb_kv8_attention_ws_bytes": (_L, [_I, _I, _I, _I, _I, _I]),
+    "nb_kv8_attention": (_I, [_P, _I, _L, _P, _I, _P, _P, _L, _I, _I, _P, _P, _P, _P, _I, _P, _I,
+                              _L, _I, _I, _I, _I, ctypes.c_float, _I, _P, _P, _P, _L, _P]),
+    "nb_logits_rules_ws_bytes": (_L, [_I, _I]),
+    "nb_logits_rules": (_I, [_P, _I, _L, _I, _I, _P, _L, _I, _P, _P, _P, _P, _P, _P, _P, _L, _I,
+                             _P, _L, _P, _L, _P, _P, _L, _P]),
     "nb_decode_workspace_bytes": (_L, [_P]),
     "nb_decode_persistent": (_I, [_P, _P, _L, _P, _P, _P, _I, _P, _I, _I, _I, _P]),
 }

@@ -10,6 +10,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
 #include <cmath>
 #include <mutex>
 #include <vector>
@@ -1107,3 +1108,295 @@ extern "C" int nb_decode_persistent(const nb_decode_model* model, void* workspac
                 "%s: switched off (an illegal memory access on a 26-layer model is not yet "
                 "explained); use the per-launch decode step", fn);
 }
+
+// ---------------------------------------------------------------------------
+// serving step over an 8-bit block cache
+// ---------------------------------------------------------------------------
+namespace {
+int64_t plan_chunks(int n_tokens, int n_requests) {
+    const int64_t n = std::max(n_tokens, 0), r = std::max(n_requests, 0);
+    return std::min<int64_t>(n, (n + 2 * (NB_KV_BLOCK - 1) * std::min(n, r)) / NB_KV_BLOCK);
+}
+
+// Shapes of the tables (their kernels count positions and slots in 31 bits).
+int check_tables(const char* fn, const void* table, int64_t table_stride, int n_requests,
+                 int max_blocks, int n_blocks) {
+    constexpr int kMost = 0x7fffffff / NB_KV_BLOCK;
+    if (n_requests < 1 || max_blocks < 1 || n_blocks < 1) {
+        return fail(NB_EINVAL, "%s: n_requests=%d max_blocks=%d n_blocks=%d", fn, n_requests,
+                    max_blocks, n_blocks);
+    }
+    if (max_blocks > kMost || n_blocks > kMost) {
+        return fail(NB_EUNSUPPORTED, "%s: max_blocks=%d, n_blocks=%d (<= %d)", fn, max_blocks,
+                    n_blocks, kMost);
+    }
+    if (!table) return fail(NB_EINVAL, "%s: table is NULL", fn);
+    if (table_stride < max_blocks) {
+        return fail(NB_EINVAL, "%s: table_stride=%lld < %d", fn, (long long)table_stride, max_blocks);
+    }
+    if (!aligned(table, 4)) return fail(NB_EALIGN, "%s: table not 4-byte aligned", fn);
+    return NB_OK;
+}
+
+int check_cache(const char* fn, const void* k, const void* v, const void* k_scale,
+                const void* v_scale, int n_blocks, int n_kv_head, int head_dim) {
+    if (n_blocks < 1 || n_kv_head < 1) {
+        return fail(NB_EINVAL, "%s: n_blocks=%d n_kv_head=%d", fn, n_blocks, n_kv_head);
+    }
+    if (n_blocks > 0x7fffffff / NB_KV_BLOCK) return fail(NB_EUNSUPPORTED, "%s: n_blocks=%d", fn, n_blocks);
+    if (head_dim < 16 || head_dim % 16 || head_dim > kv8_max_head_dim()) {
+        return fail(NB_EUNSUPPORTED, "%s: head_dim=%d (a multiple of 16, <= %d)", fn, head_dim,
+                    kv8_max_head_dim());
+    }
+    if (!k || !v || !k_scale || !v_scale) return fail(NB_EINVAL, "%s: NULL cache", fn);
+    if (!aligned(k, 16) || !aligned(v, 16) || !aligned(k_scale, 4) || !aligned(v_scale, 4)) {
+        return fail(NB_EALIGN, "%s: codes 16-byte, scales 4-byte alignment", fn);
+    }
+    return NB_OK;
+}
+
+int check_heads(const char* fn, int n_tokens, int n_head, int n_kv_head) {
+    if (n_tokens < 0 || n_head < 1 || n_kv_head < 1 || n_head % n_kv_head) {
+        return fail(NB_EINVAL, "%s: n_tokens=%d n_head=%d n_kv_head=%d", fn, n_tokens, n_head, n_kv_head);
+    }
+    if (n_head > 21845) return fail(NB_EUNSUPPORTED, "%s: n_head=%d", fn, n_head);
+    return NB_OK;
+}
+
+int check_rows(const char* fn, const char* name, const void* p, int dtype, int64_t ld, int64_t width) {
+    if (dtype != NB_F32 && dtype != NB_BF16) return fail(NB_EINVAL, "%s: %s dtype=%d", fn, name, dtype);
+    if (!p) return fail(NB_EINVAL, "%s: %s is NULL", fn, name);
+    if (ld < width) return fail(NB_EINVAL, "%s: %s row stride %lld < %lld", fn, name, (long long)ld,
+                                (long long)width);
+    if (!aligned(p, dtype_size(dtype))) return fail(NB_EALIGN, "%s: %s misaligned", fn, name);
+    return NB_OK;
+}
+
+// Chunks times the workgroups of each in one dimension of a grid of 256
+// threads each (under 2^32 work-items).
+int check_chunks(const char* fn, const void* chunks, int n_chunks, int64_t per_chunk) {
+    if (n_chunks < 0) return fail(NB_EINVAL, "%s: n_chunks=%d", fn, n_chunks);
+    if (!chunks) return fail(NB_EINVAL, "%s: chunks is NULL", fn);
+    if (!aligned(chunks, 4)) return fail(NB_EALIGN, "%s: chunks misaligned", fn);
+    if (n_chunks * per_chunk >= (1LL << 24)) return fail(NB_EUNSUPPORTED, "%s: n_chunks=%d", fn, n_chunks);
+    return NB_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int64_t nb_kv_plan_chunks(int n_tokens, int n_requests) { return plan_chunks(n_tokens, n_requests); }
+
+int nb_kv_plan(int32_t* table, int64_t table_stride, const int32_t* lens,
+               const int32_t* new_tokens, const int32_t* free_blocks, const int32_t* state,
+               int n_requests, int max_blocks, int n_blocks, int n_tokens, int32_t* slots,
+               int32_t* positions, int32_t* chunks, int32_t* lens_out, int32_t* state_out,
+               void* stream) {
+    const char* fn = "nb_kv_plan";
+    int st = check_tables(fn, table, table_stride, n_requests, max_blocks, n_blocks);
+    if (st) return st;
+    if (n_tokens < 0) return fail(NB_EINVAL, "%s: n_tokens=%d", fn, n_tokens);
+    if (n_requests > kv_plan_max_requests()) {
+        return fail(NB_EUNSUPPORTED, "%s: n_requests=%d (<= %d)", fn, n_requests, kv_plan_max_requests());
+    }
+    if ((int64_t)n_tokens * n_requests >= (1LL << 31)) {
+        return fail(NB_EUNSUPPORTED, "%s: n_tokens=%d of %d requests", fn, n_tokens, n_requests);
+    }
+    if (!lens || !new_tokens || !free_blocks || !state || !lens_out || !state_out ||
+        (n_tokens && (!slots || !positions || !chunks))) {
+        return fail(NB_EINVAL, "%s: NULL pointer", fn);
+    }
+    const void* in[] = {lens, new_tokens, free_blocks, state, table};
+    const void* out[] = {lens_out, state_out, slots, positions, chunks};
+    for (const void* o : out) {
+        if (!aligned(o, 4)) return fail(NB_EALIGN, "%s: misaligned pointer", fn);
+        for (const void* i : in) {
+            if (!aligned(i, 4)) return fail(NB_EALIGN, "%s: misaligned pointer", fn);
+            if (o && o == i) return fail(NB_EINVAL, "%s: an output is an input", fn);
+        }
+    }
+    st = ensure_device();
+    if (st) return st;
+    return launch_kv_plan(table, table_stride, lens, new_tokens, free_blocks, state, n_requests,
+                          max_blocks, n_blocks, n_tokens, (int)plan_chunks(n_tokens, n_requests),
+                          slots, positions, chunks, lens_out, state_out,
+                          static_cast<hipStream_t>(stream));
+}
+
+int nb_kv_release(int32_t* table, int64_t table_stride, int32_t* lens, const int32_t* finished,
+                  int32_t* free_blocks, int32_t* state, int n_requests, int max_blocks,
+                  int n_blocks, void* stream) {
+    const char* fn = "nb_kv_release";
+    int st = check_tables(fn, table, table_stride, n_requests, max_blocks, n_blocks);
+    if (st) return st;
+    if (n_requests > kv_plan_max_requests()) {
+        return fail(NB_EUNSUPPORTED, "%s: n_requests=%d (<= %d)", fn, n_requests, kv_plan_max_requests());
+    }
+    if ((int64_t)n_requests * max_blocks >= (1LL << 31)) {
+        return fail(NB_EUNSUPPORTED, "%s: %d requests of %d blocks", fn, n_requests, max_blocks);
+    }
+    if (!lens || !finished || !free_blocks || !state) return fail(NB_EINVAL, "%s: NULL pointer", fn);
+    if (!aligned(lens, 4) || !aligned(finished, 4) || !aligned(free_blocks, 4) || !aligned(state, 4)) {
+        return fail(NB_EALIGN, "%s: misaligned pointer", fn);
+    }
+    st = ensure_device();
+    if (st) return st;
+    return launch_kv_release(table, table_stride, lens, finished, free_blocks, state, n_requests,
+                             max_blocks, n_blocks, static_cast<hipStream_t>(stream));
+}
+
+int nb_kv8_append(const void* qkv, int qkv_dtype, int64_t ld_qkv, const int32_t* slots,
+                  const int32_t* positions, const int32_t* chunks, int n_chunks,
+                  const float* cos_t, const float* sin_t, int n_pos, int8_t* k, int8_t* v,
+                  float* k_scale, float* v_scale, int n_blocks, void* q_out, int q_dtype,
+                  int64_t ld_q, int n_tokens, int n_head, int n_kv_head, int head_dim,
+                  void* stream) {
+    const char* fn = "nb_kv8_append";
+    int st = check_heads(fn, n_tokens, n_head, n_kv_head);
+    if (st) return st;
+    st = check_cache(fn, k, v, k_scale, v_scale, n_blocks, n_kv_head, head_dim);
+    if (st || n_tokens == 0) return st;
+    st = check_rows(fn, "qkv", qkv, qkv_dtype, ld_qkv, (int64_t)(n_head + 2 * n_kv_head) * head_dim);
+    if (st) return st;
+    st = check_rows(fn, "q_out", q_out, q_dtype, ld_q, (int64_t)n_head * head_dim);
+    if (st) return st;
+    st = check_chunks(fn, chunks, n_chunks, 1);
+    if (st) return st;
+    if (n_pos < 0) return fail(NB_EINVAL, "%s: n_pos=%d", fn, n_pos);
+    if (!slots || !positions || !cos_t || !sin_t) return fail(NB_EINVAL, "%s: NULL pointer", fn);
+    if (!aligned(slots, 4) || !aligned(positions, 4) || !aligned(cos_t, 4) || !aligned(sin_t, 4)) {
+        return fail(NB_EALIGN, "%s: misaligned pointer", fn);
+    }
+    if (n_chunks == 0) return NB_OK;
+    st = ensure_device();
+    if (st) return st;
+    return launch_kv8_append(qkv, qkv_dtype, ld_qkv, slots, positions, chunks, n_chunks, cos_t,
+                             sin_t, n_pos, k, v, k_scale, v_scale, n_blocks, q_out, q_dtype, ld_q,
+                             n_tokens, n_head, n_kv_head, head_dim,
+                             static_cast<hipStream_t>(stream));
+}
+
+int nb_kv8_read(const int32_t* slots, int64_t n, const int8_t* k, const int8_t* v,
+                const float* k_scale, const float* v_scale, int n_blocks, int n_kv_head,
+                int head_dim, void* keys, void* values, int dtype, void* stream) {
+    const char* fn = "nb_kv8_read";
+    if (n < 0) return fail(NB_EINVAL, "%s: n=%lld", fn, (long long)n);
+    int st = check_heads(fn, 0, n_kv_head, n_kv_head);
+    if (st) return st;
+    st = check_cache(fn, k, v, k_scale, v_scale, n_blocks, n_kv_head, head_dim);
+    if (st || n == 0) return st;
+    if (n >= 1LL << 29) return fail(NB_EUNSUPPORTED, "%s: n=%lld", fn, (long long)n);
+    st = check_rows(fn, "keys", keys, dtype, 0, 0);
+    if (st) return st;
+    st = check_rows(fn, "values", values, dtype, 0, 0);
+    if (st) return st;
+    if (!slots) return fail(NB_EINVAL, "%s: slots is NULL", fn);
+    if (!aligned(slots, 4)) return fail(NB_EALIGN, "%s: slots misaligned", fn);
+    st = ensure_device();
+    if (st) return st;
+    return launch_kv8_read(slots, n, k, v, k_scale, v_scale, n_blocks, n_kv_head, head_dim, keys,
+                           values, dtype, static_cast<hipStream_t>(stream));
+}
+
+int64_t nb_kv8_attention_ws_bytes(int n_tokens, int n_chunks, int max_blocks, int n_head,
+                                  int n_kv_head, int head_dim) {
+    if (n_tokens < 1 || n_chunks < 1 || n_kv_head < 1 || n_head < n_kv_head) return 0;
+    if (ensure_device() != NB_OK) g_last_error[0] = '\0';   // (256 CUs without a device)
+    return kv8_attention_bytes(n_chunks, n_tokens, max_blocks, n_head, n_kv_head, head_dim);
+}
+
+int nb_kv8_attention(const void* q, int q_dtype, int64_t ld_q, const int32_t* chunks, int n_chunks,
+                     const int32_t* lens, const int32_t* table, int64_t table_stride,
+                     int n_requests, int max_blocks, const int8_t* k, const int8_t* v,
+                     const float* k_scale, const float* v_scale, int n_blocks, void* out,
+                     int out_dtype, int64_t ld_out, int n_tokens, int n_head, int n_kv_head,
+                     int head_dim, float softcap, int window, const float* slopes,
+                     const int32_t* prefix, void* workspace, int64_t ws_bytes, void* stream) {
+    const char* fn = "nb_kv8_attention";
+    int st = check_heads(fn, n_tokens, n_head, n_kv_head);
+    if (st) return st;
+    st = check_cache(fn, k, v, k_scale, v_scale, n_blocks, n_kv_head, head_dim);
+    if (st) return st;
+    st = check_tables(fn, table, table_stride, n_requests, max_blocks, n_blocks);
+    if (st || n_tokens == 0) return st;
+    const int64_t width = (int64_t)n_head * head_dim;
+    st = check_rows(fn, "q", q, q_dtype, ld_q, width);
+    if (st) return st;
+    st = check_rows(fn, "out", out, out_dtype, ld_out, width);
+    if (st) return st;
+    st = check_chunks(fn, chunks, n_chunks, n_kv_head);
+    if (st) return st;
+    if (!(softcap >= 0.f) || !std::isfinite(softcap)) return fail(NB_EINVAL, "%s: softcap=%g", fn, (double)softcap);
+    if (window < 0) return fail(NB_EINVAL, "%s: window=%d", fn, window);
+    if (!lens) return fail(NB_EINVAL, "%s: lens is NULL", fn);
+    if (n_chunks == 0) return NB_OK;
+    if (!aligned(lens, 4) || !aligned(slopes, 4) || !aligned(prefix, 4)) {
+        return fail(NB_EALIGN, "%s: misaligned pointer", fn);
+    }
+    const int dev_st = ensure_device();
+    const int64_t need = kv8_attention_bytes(n_chunks, n_tokens, max_blocks, n_head, n_kv_head, head_dim);
+    if (ws_bytes < need || (need && !workspace)) {
+        return fail(NB_EINVAL, "%s: workspace of %lld bytes < %lld", fn, (long long)ws_bytes, (long long)need);
+    }
+    if (!aligned(workspace, 16)) return fail(NB_EALIGN, "%s: workspace not 16-byte aligned", fn);
+    if (dev_st) return dev_st;
+    return launch_kv8_attention(q, q_dtype, ld_q, chunks, n_chunks, lens, table, table_stride,
+                                n_requests, max_blocks, k, v, k_scale, v_scale, n_blocks, out,
+                                out_dtype, ld_out, n_tokens, n_head, n_kv_head, head_dim, softcap,
+                                window, slopes, prefix, workspace, static_cast<hipStream_t>(stream));
+}
+
+int64_t nb_logits_rules_ws_bytes(int rows, int V) {
+    return rows < 1 || V < 1 ? 0 : logits_rules_bytes(rows, V);
+}
+
+int nb_logits_rules(const void* logits, int dtype, int64_t ld, int rows, int V,
+                    const int32_t* history, int64_t ld_history, int max_history,
+                    const int32_t* lens, const int32_t* prompt_lens, const float* repetition,
+                    const float* frequency, const float* presence, const int32_t* bias_ids,
+                    const float* bias, int64_t ld_bias, int n_bias, const int32_t* mask,
+                    int64_t ld_mask, float* out, int64_t ld_out, int32_t* tokens, void* workspace,
+                    int64_t ws_bytes, void* stream) {
+    const char* fn = "nb_logits_rules";
+    if (rows < 0 || V < 1 || V > 0x7fffffff - 8) return fail(NB_EINVAL, "%s: rows=%d V=%d", fn, rows, V);
+    if (rows > 65535) return fail(NB_EUNSUPPORTED, "%s: rows=%d (<= 65535)", fn, rows);
+    if (rows == 0) return NB_OK;
+    int st = check_rows(fn, "logits", logits, dtype, ld, V);
+    if (st) return st;
+    st = check_rows(fn, "out", out, NB_F32, ld_out, V);
+    if (st) return st;
+    if (out == logits && (dtype != NB_F32 || ld != ld_out)) {
+        return fail(NB_EINVAL, "%s: in place only over fp32 logits of the same stride", fn);
+    }
+    if ((history == nullptr) != (lens == nullptr)) return fail(NB_EINVAL, "%s: history and lens go together", fn);
+    if (!history && (prompt_lens || repetition || frequency || presence)) {
+        return fail(NB_EINVAL, "%s: penalties need a history", fn);
+    }
+    if (history && (max_history < 0 || ld_history < 0 || (ld_history && ld_history < max_history))) {
+        return fail(NB_EINVAL, "%s: max_history=%d ld_history=%lld", fn, max_history, (long long)ld_history);
+    }
+    if (n_bias < 0 || ld_bias < 0 || (n_bias && (!bias_ids || !bias || (ld_bias && ld_bias < n_bias)))) {
+        return fail(NB_EINVAL, "%s: n_bias=%d ld_bias=%lld", fn, n_bias, (long long)ld_bias);
+    }
+    if (mask && ld_mask && ld_mask < ((int64_t)V + 31) / 32) {
+        return fail(NB_EINVAL, "%s: ld_mask=%lld < %lld", fn, (long long)ld_mask, ((long long)V + 31) / 32);
+    }
+    const void* four[] = {history, lens, prompt_lens, repetition, frequency, presence, bias_ids,
+                          bias, mask, tokens};
+    for (const void* p : four) {
+        if (!aligned(p, 4)) return fail(NB_EALIGN, "%s: misaligned pointer", fn);
+    }
+    const int64_t need = tokens ? logits_rules_bytes(rows, V) : 0;
+    if (ws_bytes < need || (need && !workspace)) {
+        return fail(NB_EINVAL, "%s: workspace of %lld bytes < %lld", fn, (long long)ws_bytes, (long long)need);
+    }
+    if (!aligned(workspace, 8)) return fail(NB_EALIGN, "%s: workspace not 8-byte aligned", fn);
+    st = ensure_device();
+    if (st) return st;
+    return launch_logits_rules(logits, dtype, ld, rows, V, history, ld_history, max_history, lens,
+                               prompt_lens, repetition, frequency, presence, bias_ids, bias, ld_bias,
+                               n_bias, mask, ld_mask, out, ld_out, tokens, workspace,
+                               static_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"

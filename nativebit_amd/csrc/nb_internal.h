@@ -215,6 +215,49 @@ int launch_attention_mfma(const float* q, const float* k, const float* v, int po
                           hipStream_t stream);
 int attention_rows_max_head_dim();
 
+// Serving step over an 8-bit block cache; arguments validated.
+constexpr int kKvBlock = NB_KV_BLOCK;   // tokens of a cache block
+// nb_kv_plan.hip
+int kv_plan_max_requests();
+int launch_kv_plan(int32_t* table, int64_t table_stride, const int32_t* lens,
+                   const int32_t* new_tokens, const int32_t* free_blocks, const int32_t* state,
+                   int R, int max_blocks, int n_blocks, int n_tokens, int n_chunks, int32_t* slots,
+                   int32_t* positions, int32_t* chunks, int32_t* lens_out, int32_t* state_out,
+                   hipStream_t stream);
+int launch_kv_release(int32_t* table, int64_t table_stride, int32_t* lens, const int32_t* finished,
+                      int32_t* free_blocks, int32_t* state, int R, int max_blocks, int n_blocks,
+                      hipStream_t stream);
+// nb_kv8.hip
+int kv8_max_head_dim();
+int launch_kv8_append(const void* qkv, int qkv_dtype, int64_t ld_qkv, const int32_t* slots,
+                      const int32_t* positions, const int32_t* chunks, int n_chunks,
+                      const float* cos_t, const float* sin_t, int n_pos, int8_t* k, int8_t* v,
+                      float* k_scale, float* v_scale, int n_blocks, void* q_out, int q_dtype,
+                      int64_t ld_q, int n_tokens, int n_head, int n_kv, int D,
+                      hipStream_t stream);
+int launch_kv8_read(const int32_t* slots, int64_t n, const int8_t* k, const int8_t* v,
+                    const float* k_scale, const float* v_scale, int n_blocks, int n_kv, int D,
+                    void* keys, void* values, int dtype, hipStream_t stream);
+// nb_kv8_attention.hip: workspace of kv8_attention_bytes(...) bytes (0: none)
+int64_t kv8_attention_bytes(int n_chunks, int n_tokens, int max_blocks, int n_head, int n_kv, int D);
+int launch_kv8_attention(const void* q, int q_dtype, int64_t ld_q, const int32_t* chunks,
+                         int n_chunks, const int32_t* lens, const int32_t* table,
+                         int64_t table_stride, int R, int max_blocks, const int8_t* k,
+                         const int8_t* v, const float* k_scale, const float* v_scale, int n_blocks,
+                         void* out, int out_dtype, int64_t ld_out, int n_tokens, int n_head,
+                         int n_kv, int D, float softcap, int window, const float* slopes,
+                         const int32_t* prefix, void* workspace, hipStream_t stream);
+// nb_logits.hip: workspace of logits_rules_bytes(rows, V) bytes (0: none) where
+// tokens are chosen
+int64_t logits_rules_bytes(int rows, int V);
+int launch_logits_rules(const void* logits, int dtype, int64_t ld, int rows, int V,
+                        const int32_t* history, int64_t ld_history, int max_history,
+                        const int32_t* lens, const int32_t* prompt_lens, const float* repetition,
+                        const float* frequency, const float* presence, const int32_t* bias_ids,
+                        const float* bias, int64_t ld_bias, int n_bias, const int32_t* mask,
+                        int64_t ld_mask, float* out, int64_t ld_out, int32_t* tokens,
+                        void* workspace, hipStream_t stream);
+
 // Persistent decode (nb_decode_persistent.hip); arguments validated.
 int64_t decode_persistent_workspace_bytes(int C, int H, int F);
 int decode_persistent_limits(int* max_c, int* max_f, int* max_d, int* max_ctx, int* max_heads,

@@ -1,0 +1,83 @@
+// nb_kv8_attention: the launch (its shape and split) and the join of split
+// results.  The kernel and its mathematics: nb_kv8_attention.h.
+#include <algorithm>
+
+#include "nb_kv8_attention.h"
+
+namespace nb {
+namespace {
+
+// Workgroups over a row's blocks.  Enough for three workgroups of four waves a
+// CU, but no less than 32 blocks each: the joining launch costs as much as
+// they take.
+int splits_of(int n_chunks, int n_tokens, int max_blocks, int n_head, int n_kv) {
+    const int64_t groups = (int64_t)n_chunks * n_kv;
+    const int64_t want = 3 * device_cu_count();
+    if (groups >= want || (int64_t)n_tokens * (n_head / n_kv) > 16LL * n_chunks) return 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({want / groups, max_blocks / 32, 64}));
+}
+
+// One wave a row and head: the splits' maxima and sums in its lanes, then
+// the dims.
+__global__ __launch_bounds__(64) void kv8_join_kernel(Kv8AttentionArgs a, int splits) {
+    const Kv8Chunk ch = kv8_chunk(a, blockIdx.x);
+    const int head = blockIdx.y, lane = threadIdx.x;
+    for (int t = 0; t < ch.n; ++t) {
+        const int64_t row = ch.row0 + t, at = (row * a.n_head + head) * splits;
+        const float* ml = a.part + (int64_t)a.n_tokens * a.n_head * splits * a.D + 2 * at;
+        const float m = lane < splits ? ml[2 * lane] : -INFINITY;
+        const float l = lane < splits ? ml[2 * lane + 1] : 0.f;
+        const float top = fmaxf(wave64_max(m), kLowest);
+        const float w = __builtin_amdgcn_exp2f(m - top);
+        const float sum = wave64_sum(l * w);
+        const float scaled = l == 0.f ? 0.f : w * (sum == 0.f ? 0.f : 1.f / sum);
+        const uint64_t used = __ballot(lane < splits && l != 0.f);
+        for (int d = lane; d < a.D; d += 64) {
+            float v = 0.f;
+            for (uint64_t u = used; u; u &= u - 1) {
+                const int s = __ffsll((unsigned long long)u) - 1;
+                v = fmaf(a.part[(at + s) * a.D + d], lane_value(scaled, s), v);
+            }
+            const int64_t to = row * a.ld_out + head * a.D + d;
+            if (a.out_dtype == NB_F32) static_cast<float*>(a.out)[to] = v;
+            else static_cast<bf16_bits*>(a.out)[to] = f32_to_bf16_rne(v);
+        }
+    }
+}
+
+}  // namespace
+
+int64_t kv8_attention_bytes(int n_chunks, int n_tokens, int max_blocks, int n_head, int n_kv, int D) {
+    const int splits = splits_of(n_chunks, n_tokens, max_blocks, n_head, n_kv);
+    return splits == 1 ? 0 : (int64_t)n_tokens * n_head * splits * (D + 2) * 4;
+}
+
+int launch_kv8_attention(const void* q, int q_dtype, int64_t ld_q, const int32_t* chunks,
+                         int n_chunks, const int32_t* lens, const int32_t* table,
+                         int64_t table_stride, int R, int max_blocks, const int8_t* k,
+                         const int8_t* v, const float* k_scale, const float* v_scale, int n_blocks,
+                         void* out, int out_dtype, int64_t ld_out, int n_tokens, int n_head,
+                         int n_kv, int D, float softcap, int window, const float* slopes,
+                         const int32_t* prefix, void* workspace, hipStream_t stream) {
+    auto four = [](const void* p, int dtype, int64_t ld) {
+        return reinterpret_cast<uintptr_t>(p) % (dtype == NB_F32 ? 16 : 8) == 0 && ld % 4 == 0;
+    };
+    const int splits = splits_of(n_chunks, n_tokens, max_blocks, n_head, n_kv);
+    Kv8AttentionArgs a{q, ld_q, chunks, lens, table, table_stride, k, v, k_scale, v_scale, out,
+                       ld_out, slopes, prefix, static_cast<float*>(workspace), q_dtype, out_dtype,
+                       four(q, q_dtype, ld_q), four(out, out_dtype, ld_out), n_chunks, n_tokens, R,
+                       max_blocks, n_blocks, n_head, n_kv, D, window, softcap};
+    // a chunk of 64 tokens makes G groups of 64 rows
+    const int64_t rows = ((int64_t)n_tokens + n_chunks - 1) / n_chunks * (n_head / n_kv);
+    const int groups = (int)std::min<int64_t>(std::max<int64_t>(1, (rows + 63) / 64), 64);
+    const dim3 grid((unsigned)(n_chunks * n_kv), groups, splits);
+    const bool rules = softcap > 0.f || window > 0 || slopes || prefix;
+    if (out_dtype == NB_BF16) launch_kv8_attention_2(a, grid, rules, stream);
+    else launch_kv8_attention_3(a, grid, rules, stream);
+    if (splits > 1) {
+        hipLaunchKernelGGL(kv8_join_kernel, dim3(n_chunks, n_head), dim3(64), 0, stream, a, splits);
+    }
+    return check_launch("nb_kv8_attention");
+}
+
+}  // namespace nb

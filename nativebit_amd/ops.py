@@ -7,6 +7,7 @@ torch's current stream and raises NativeBitError on a non-zero status.
 from __future__ import annotations
 
 import math
+from typing import NamedTuple
 
 import torch
 
@@ -505,3 +506,339 @@ def dequant(packed: torch.Tensor, codebook: torch.Tensor, total: int, bits: int,
         packed.data_ptr(), codebook.data_ptr(), w.data_ptr(), _DT[out_dtype], total,
         codebook.shape[0], bits, codebook.shape[1], block_size, _stream(packed)))
     return w
+
+
+# ---------------------------------------------------------------------------
+# serving: requests of different lengths over an 8-bit block cache
+# ---------------------------------------------------------------------------
+KV_BLOCK = 64   # tokens of a cache block (NB_KV_BLOCK)
+
+
+class KVPlan(NamedTuple):
+    """A serving step's plan (``kv_plan``): for each row its slot (-1: none)
+    and position, the chunks (first row, rows, request, first position; 0 rows
+    past the last), the requests' lengths after the step, and (free blocks,
+    tokens without a slot) after it.  int32 on the GPU."""
+    slots: torch.Tensor
+    positions: torch.Tensor
+    chunks: torch.Tensor
+    lens: torch.Tensor
+    state: torch.Tensor
+
+
+def _launch(t: torch.Tensor, fn, *args):
+    """fn(*args, stream) on t's device and torch's current stream there."""
+    stream = _stream(t)
+    device = t.get_device()
+    if device == torch._C._cuda_getDevice():
+        status = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, stream)
+    if status:
+        _lib.check(status)
+
+
+def _int32(name: str, t: torch.Tensor, shape, like: torch.Tensor | None = None):
+    """t is a contiguous int32 GPU tensor of this shape (None: any size)."""
+    _require_cuda(name, t)
+    if t.dtype != torch.int32 or not t.is_contiguous():
+        raise TypeError(f"{name} must be a contiguous int32 tensor")
+    if t.dim() != len(shape) or any(want is not None and have != want
+                                    for have, want in zip(t.shape, shape)):
+        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    if like is not None:
+        _same_device(like, t)
+
+
+def _table(table: torch.Tensor):
+    _require_cuda("table", table)
+    if table.dtype != torch.int32 or table.dim() != 2 or table.numel() == 0 or \
+            (table.shape[1] > 1 and table.stride(1) != 1):
+        raise TypeError("table must be an int32 (requests, blocks) tensor, rows contiguous")
+    # (a table of one row may have any row stride)
+    return table.stride(0) if table.shape[0] > 1 else table.shape[1]
+
+
+def kv_plan_chunks(n_tokens: int, n_requests: int) -> int:
+    """Chunks that a plan of n_tokens rows of n_requests requests has room
+    for (nb_kv_plan_chunks)."""
+    n = max(int(n_tokens), 0)
+    return min(n, (n + 2 * (KV_BLOCK - 1) * min(n, max(int(n_requests), 0))) // KV_BLOCK)
+
+
+def kv_plan(table: torch.Tensor, lens: torch.Tensor, new: torch.Tensor, free: torch.Tensor,
+            state: torch.Tensor, n_tokens: int, out: KVPlan | None = None) -> KVPlan:
+    """The plan of a serving step from the requests' lengths, on the GPU
+    (nb_kv_plan): request r has ``lens[r]`` tokens cached and brings ``new[r]``;
+    its new blocks come from the end of ``free[:state[0]]`` and are entered in
+    ``table`` (requests, blocks), which is updated in place.  ``n_tokens`` is
+    the rows of the step (the sum of ``new``, or more: the rows behind have no
+    slot).  ``lens`` and ``state`` are left as they are; the plan's are those
+    after the step.  ``out``: a plan of the same sizes to write."""
+    stride = _table(table)
+    R, width = table.shape
+    n_tokens = int(n_tokens)
+    _int32("lens", lens, (R,), table)
+    _int32("new", new, (R,), table)
+    _int32("free", free, (None,), table)
+    _int32("state", state, (2,), table)
+    chunks = kv_plan_chunks(n_tokens, R)
+    if out is None:
+        if n_tokens < 0:
+            raise ValueError(f"n_tokens={n_tokens}")
+        buf = torch.empty(4 * chunks + 2 * n_tokens + R + 2, dtype=torch.int32, device=table.device)
+        c, s, p, l, st = buf.split_with_sizes([4 * chunks, n_tokens, n_tokens, R, 2])
+        out = KVPlan(s, p, c.view(chunks, 4), l, st)
+    else:
+        for name, t, shape in (("slots", out.slots, (n_tokens,)),
+                               ("positions", out.positions, (n_tokens,)),
+                               ("chunks", out.chunks, (chunks, 4)), ("lens", out.lens, (R,)),
+                               ("state", out.state, (2,))):
+            _int32(f"out.{name}", t, shape, table)
+    _launch(table, _lib.load().nb_kv_plan, table.data_ptr(), stride, lens.data_ptr(),
+            new.data_ptr(), free.data_ptr(), state.data_ptr(), R, width, free.numel(), n_tokens,
+            out.slots.data_ptr(), out.positions.data_ptr(), out.chunks.data_ptr(),
+            out.lens.data_ptr(), out.state.data_ptr())
+    return out
+
+
+def kv_release(table: torch.Tensor, lens: torch.Tensor, finished: torch.Tensor,
+               free: torch.Tensor, state: torch.Tensor) -> None:
+    """The blocks of the requests with ``finished[r] != 0`` back on the free
+    list, their lengths 0 and table entries -1, all in place
+    (nb_kv_release)."""
+    stride = _table(table)
+    R, width = table.shape
+    _int32("lens", lens, (R,), table)
+    _int32("finished", finished, (R,), table)
+    _int32("free", free, (None,), table)
+    _int32("state", state, (2,), table)
+    _launch(table, _lib.load().nb_kv_release, table.data_ptr(), stride, lens.data_ptr(),
+            finished.data_ptr(), free.data_ptr(), state.data_ptr(), R, width, free.numel())
+
+
+def _kv8_cache(k, v, k_scale, v_scale):
+    """(blocks, heads, head dim) of an 8-bit cache, its tensors checked."""
+    for name, t in (("k", k), ("v", v), ("k_scale", k_scale), ("v_scale", v_scale)):
+        _require_cuda(name, t)
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+    _same_device(k, v, k_scale, v_scale)
+    if k.dtype != torch.int8 or v.dtype != torch.int8 or k.dim() != 4 or k.shape[2] != KV_BLOCK:
+        raise ValueError(f"k must be int8 (blocks, heads, {KV_BLOCK}, head_dim), v int8 "
+                         f"(blocks, heads, head_dim, {KV_BLOCK})")
+    n, h, _, d = k.shape
+    if v.shape != (n, h, d, KV_BLOCK):
+        raise ValueError(f"v must be {(n, h, d, KV_BLOCK)}, got {tuple(v.shape)}")
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t.dtype != torch.float32 or t.shape != (n, h):
+            raise ValueError(f"{name} must be float32 {(n, h)}")
+    return n, h, d
+
+
+def _rows(name, t, rows, width, like):
+    """Row stride of a (rows, width) float32 / bfloat16 tensor."""
+    _require_cuda(name, t)
+    _same_device(like, t)
+    if t.dtype not in _DT:
+        raise TypeError(f"{name} dtype {t.dtype} not supported (float32 or bfloat16)")
+    if t.dim() != 2 or t.shape[0] != rows or (width is not None and t.shape[1] != width) or \
+            (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be ({rows}, {width}), rows contiguous; got "
+                         f"{tuple(t.shape)}, strides {t.stride()}")
+    if rows > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError(f"{name}: rows overlap")
+    return t.stride(0) if rows > 1 else t.shape[1]
+
+
+def _plan(plan: KVPlan, rows: int, like):
+    _int32("plan.slots", plan.slots, (rows,), like)
+    _int32("plan.positions", plan.positions, (rows,), like)
+    _int32("plan.chunks", plan.chunks, (None, 4), like)
+
+
+def kv8_append(qkv: torch.Tensor, plan: KVPlan, cos: torch.Tensor, sin: torch.Tensor,
+               k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+               n_head: int, q: torch.Tensor | None = None) -> torch.Tensor:
+    """RoPE of a step's rows and the append of their keys and values to the
+    8-bit cache (nb_kv8_append).  ``qkv`` (rows, (n_head + 2 heads) head_dim)
+    float32 or bfloat16, ``cos`` / ``sin`` (positions, head_dim / 2) float32.
+    Returns the turned queries times head_dim^-0.5, (rows, n_head head_dim) in
+    qkv's dtype (or into ``q``); rows without a slot are not written."""
+    n_blocks, n_kv, D = _kv8_cache(k, v, k_scale, v_scale)
+    n_head = int(n_head)
+    if qkv.dim() != 2:
+        raise ValueError(f"qkv must be (rows, {(n_head + 2 * n_kv) * D})")
+    n = qkv.shape[0]
+    ld = _rows("qkv", qkv, n, (n_head + 2 * n_kv) * D, k)
+    _plan(plan, n, k)
+    for name, t in (("cos", cos), ("sin", sin)):
+        _require_cuda(name, t)
+        if t.dtype != torch.float32 or not t.is_contiguous() or t.dim() != 2 or \
+                t.shape[1] * 2 != D or t.shape != cos.shape:
+            raise ValueError(f"{name} must be a contiguous float32 (positions, {D // 2}) tensor")
+        _same_device(k, t)
+    if q is None:
+        q = torch.empty((n, n_head * D), dtype=qkv.dtype, device=qkv.device)
+    ld_q = _rows("q", q, n, n_head * D, k)
+    if n:
+        _launch(k, _lib.load().nb_kv8_append, qkv.data_ptr(), _DT[qkv.dtype], ld,
+                plan.slots.data_ptr(), plan.positions.data_ptr(), plan.chunks.data_ptr(),
+                plan.chunks.shape[0], cos.data_ptr(), sin.data_ptr(), cos.shape[0], k.data_ptr(),
+                v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_blocks, q.data_ptr(),
+                _DT[q.dtype], ld_q, n, n_head, n_kv, D)
+    return q
+
+
+def kv8_read(slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor,
+             v_scale: torch.Tensor, dtype: torch.dtype = torch.float32):
+    """(keys, values), each (n, heads, head_dim), that the cache holds at
+    ``slots`` (n,); zeros for slots outside it, -1 among them
+    (nb_kv8_read)."""
+    n_blocks, n_kv, D = _kv8_cache(k, v, k_scale, v_scale)
+    _int32("slots", slots, (None,), k)
+    if dtype not in _DT:
+        raise TypeError(f"dtype {dtype} not supported")
+    n = slots.numel()
+    keys = torch.empty((n, n_kv, D), dtype=dtype, device=k.device)
+    values = torch.empty_like(keys)
+    if n:
+        _launch(k, _lib.load().nb_kv8_read, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(),
+                k_scale.data_ptr(), v_scale.data_ptr(), n_blocks, n_kv, D, keys.data_ptr(),
+                values.data_ptr(), _DT[dtype])
+    return keys, values
+
+
+def kv8_attention(q: torch.Tensor, plan: KVPlan, table: torch.Tensor, k: torch.Tensor,
+                  v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, *,
+                  softcap: float = 0.0, window: int = 0, slopes: torch.Tensor | None = None,
+                  prefix: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                  out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """Attention of a step's queries ``q`` (rows, heads * head_dim), as
+    ``kv8_append`` returns them, over the cached tokens of their requests, the
+    step's own among them (nb_kv8_attention).  Scores s become softcap *
+    tanh(s / softcap) (softcap > 0), then get slopes[head] * (key position -
+    query position); a query sees the positions up to its own, with ``window``
+    > 0 only the last ``window`` of them, and with ``prefix`` (requests,)
+    besides all before prefix[request].  Returns (rows, heads * head_dim) in
+    q's dtype or ``out_dtype`` (or into ``out``); rows without a slot are not
+    written."""
+    n_blocks, n_kv, D = _kv8_cache(k, v, k_scale, v_scale)
+    stride = _table(table)
+    _same_device(k, table)
+    R, width = table.shape
+    if q.dim() != 2 or q.shape[1] == 0 or q.shape[1] % (n_kv * D):
+        raise ValueError(f"q must be (rows, heads * {D}), heads a multiple of {n_kv}")
+    n, n_head = q.shape[0], q.shape[1] // D
+    ld_q = _rows("q", q, n, None, k)
+    _plan(plan, n, k)
+    _int32("plan.lens", plan.lens, (R,), k)
+    if slopes is not None:
+        _require_cuda("slopes", slopes)
+        _same_device(k, slopes)
+        if slopes.dtype != torch.float32 or slopes.shape != (n_head,) or not slopes.is_contiguous():
+            raise ValueError(f"slopes must be a contiguous float32 ({n_head},) tensor")
+    if prefix is not None:
+        _int32("prefix", prefix, (R,), k)
+    if out is None:
+        out = torch.empty((n, n_head * D), dtype=out_dtype or q.dtype, device=q.device)
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
+    ld_out = _rows("out", out, n, n_head * D, k)
+    if n:
+        lib = _lib.load()
+        n_chunks = plan.chunks.shape[0]
+        nbytes = lib.nb_kv8_attention_ws_bytes(n, n_chunks, width, n_head, n_kv, D)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        _launch(k, lib.nb_kv8_attention, q.data_ptr(), _DT[q.dtype], ld_q, plan.chunks.data_ptr(),
+                n_chunks, plan.lens.data_ptr(), table.data_ptr(), stride, R, width, k.data_ptr(),
+                v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_blocks, out.data_ptr(),
+                _DT[out.dtype], ld_out, n, n_head, n_kv, D, float(softcap), int(window),
+                slopes.data_ptr() if slopes is not None else None,
+                prefix.data_ptr() if prefix is not None else None,
+                ws.data_ptr() if nbytes else None, nbytes)
+    return out
+
+
+def logits_rules(logits: torch.Tensor, *, history: torch.Tensor | None = None,
+                 lens: torch.Tensor | None = None, prompt_lens: torch.Tensor | None = None,
+                 repetition: torch.Tensor | None = None, frequency: torch.Tensor | None = None,
+                 presence: torch.Tensor | None = None, bias_ids: torch.Tensor | None = None,
+                 bias: torch.Tensor | None = None, mask: torch.Tensor | None = None,
+                 out: torch.Tensor | None = None, choose: bool = False):
+    """Rules on a batch of logits (B, V), float32 or bfloat16, and the greedy
+    choice (nb_logits_rules).  In this order: the penalties of the tokens in
+    ``history[b, :lens[b]]`` (B, n) -- logits divided (positive) or multiplied
+    by ``repetition[b]``, less ``frequency[b]`` times their count from
+    ``prompt_lens[b]`` on and ``presence[b]`` where that is not 0; ``bias`` at
+    ``bias_ids`` (B, n), an id listed twice having its last value; -inf where
+    bit v % 32 of ``mask[b, v // 32]`` (int32) is 0.  Returns float32 (B, V)
+    (or ``out``, which may be ``logits``), and with ``choose`` also the int32
+    (B,) tokens with the largest logit, the lowest on ties, -1 where nothing is
+    left."""
+    _require_cuda("logits", logits)
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError(f"logits must be (B, V), got {tuple(logits.shape)}")
+    B, V = logits.shape
+    ld = _rows("logits", logits, B, V, logits)
+    if (history is None) != (lens is None):
+        raise ValueError("history and lens go together")
+    if history is None and not (prompt_lens is None and repetition is None and
+                                frequency is None and presence is None):
+        raise ValueError("penalties need a history")
+    if (bias_ids is None) != (bias is None):
+        raise ValueError("bias_ids and bias go together")
+    p = {}
+
+    def matrix(name, t, dtype, columns):
+        if t is None:
+            return 0, 0
+        _require_cuda(name, t)
+        _same_device(logits, t)
+        if t.dtype != dtype or t.dim() != 2 or t.shape[0] != B or t.shape[1] < columns or \
+                (t.shape[1] > 1 and t.stride(1) != 1):
+            raise ValueError(f"{name} must be a {dtype} ({B}, >= {columns}) tensor, rows contiguous")
+        if t.numel():
+            p[name] = t.data_ptr()
+        # (a row stride of 0 gives every row the same entries)
+        return t.stride(0) if B > 1 else t.shape[1], t.shape[1]
+
+    def vector(name, t, dtype):
+        if t is None:
+            return
+        _require_cuda(name, t)
+        _same_device(logits, t)
+        if t.dtype != dtype or t.shape != (B,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {dtype} ({B},) tensor")
+        p[name] = t.data_ptr()
+
+    ld_history, n_history = matrix("history", history, torch.int32, 0)
+    ld_ids, n_bias = matrix("bias_ids", bias_ids, torch.int32, 0)
+    ld_bias, n_values = matrix("bias", bias, torch.float32, 0)
+    ld_mask, _ = matrix("mask", mask, torch.int32, (V + 31) // 32)
+    if n_bias != n_values or ld_ids != ld_bias:
+        raise ValueError("bias_ids and bias must have the same shape and strides")
+    if n_history:   # (an empty history has no penalties)
+        vector("lens", lens, torch.int32)
+        vector("prompt_lens", prompt_lens, torch.int32)
+        vector("repetition", repetition, torch.float32)
+        vector("frequency", frequency, torch.float32)
+        vector("presence", presence, torch.float32)
+    if out is None:
+        out = torch.empty((B, V), dtype=torch.float32, device=logits.device)
+    ld_out = _rows("out", out, B, V, logits)
+    if out.dtype != torch.float32:
+        raise TypeError("out must be float32")
+    tokens = torch.empty(B, dtype=torch.int32, device=logits.device) if choose else None
+    if B:
+        lib = _lib.load()
+        nbytes = lib.nb_logits_rules_ws_bytes(B, V) if choose else 0
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
+        g = p.get
+        _launch(logits, lib.nb_logits_rules, logits.data_ptr(), _DT[logits.dtype], ld, B, V,
+                g("history"), ld_history, n_history, g("lens"), g("prompt_lens"),
+                g("repetition"), g("frequency"), g("presence"), g("bias_ids"), g("bias"), ld_bias,
+                n_bias, g("mask"), ld_mask, out.data_ptr(), ld_out,
+                tokens.data_ptr() if choose else None, ws.data_ptr() if nbytes else None, nbytes)
+    return (out, tokens) if choose else out
