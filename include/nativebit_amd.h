@@ -633,7 +633,7 @@ int nb_kv_release(int32_t* table, int64_t table_stride, int32_t* lens, const int
  * 2] of the row's position (NaN where it is not under n_pos); q_out row =
  * turned q * head_dim^-0.5 (stride ld_q, NB_F32 or NB_BF16).  Keys and values
  * go to the cache: with s the block's scale (0 before its first token), a
- * chunk's rows x set it to s' = max(s, max|x| / 127), their codes to
+ * chunk's rows x set it to s' = max(s, max|x| * (1 / 127)), their codes to
  * clamp(rint(x / s'), -127, 127) and, where s' > s, the block's earlier codes
  * to rint(code * s / s'), in fp32.  A NaN or infinity sets s' = inf: the block
  * reads as NaN.  slots, positions and chunks as nb_kv_plan writes them.  Two

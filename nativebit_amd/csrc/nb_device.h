@@ -41,6 +41,14 @@ __device__ __forceinline__ __attribute__((address_space(1))) T* as_global_mut(T*
     return (__attribute__((address_space(1))) T*)p;
 }
 
+// Memory that no kernel in flight writes, read at wave-uniform addresses: the
+// loads go through the scalar cache into scalar registers and wait on their own
+// counter, not on the vector loads issued before them.
+template <typename T>
+__device__ __forceinline__ const __attribute__((address_space(4))) T* as_constant(const T* p) {
+    return (const __attribute__((address_space(4))) T*)p;
+}
+
 template <typename T>
 __device__ __forceinline__ T stream_load(const T* p) {
 #if NB_STREAM_NT

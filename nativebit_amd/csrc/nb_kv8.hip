@@ -7,7 +7,7 @@
 // with one fp32 scale each.  With x the new rows of a chunk (the rows of one
 // request inside one block), `before` the tokens that the block already
 // holds and s its scale (0 where it holds none)
-//     s'   = max(s, max |x| / 127)
+//     s'   = max(s, max |x| * (1 / 127))
 //     code = clamp(rint(x / s'), -127, 127)             of the new rows
 //     code = clamp(rint((code * s) / s'), -127, 127)    of the earlier ones
 // each operation rounded to nearest in fp32, so that the codes follow from
@@ -196,7 +196,7 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(AppendArgs a) {
     most = fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3]));
     float* scale = (part == 0 ? a.k_scale : a.v_scale) + bh;
     const float s = before > 0 ? *scale : 0.f;
-    const float s2 = fmaxf(s, most / 127.f);
+    const float s2 = fmaxf(s, most * (1.f / 127.f));
     const bool again = before > 0 && s2 > s;   // the earlier codes change
     __syncthreads();   // every thread has the old scale
     if (threadIdx.x == 0 && (again || before == 0)) *scale = s2;

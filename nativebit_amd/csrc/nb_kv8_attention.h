@@ -1,19 +1,21 @@
 // Attention of a step's queries over the 8-bit block cache on int8 MFMAs
-// (gfx950): the kernel of nb_kv8_attention.  nb_kv8_attention_2.hip and _3.hip
-// build it for two and three digits, nb_kv8_attention.hip launches it.
+// (gfx950): the kernel of nb_kv8_attention.  nb_kv8_attention_tokens_2.hip,
+// _tokens_3.hip, _prompts_2.hip and _prompts_3.hip build it, nb_kv8_attention.hip
+// launches it.
 //
 // Mathematics.  The cache's codes are int8, and a scale belongs to a block of
 // 64 tokens and head, so that both products are int8 ones if the other factor
 // is cut into signed base-256 digits: a row of q is written as
 //     q[d] = inv (a[d] 2^16 + b[d] 2^8 + c[d]),   inv = max |q| / (127 * 2^16)
-// (rounded to nearest; digits -128 .. 127) and q . k = inv * k_scale * (A 2^16
-// + B 2^8 + C) with A, B, C exact 32-bit sums of int8 products: 24 bits of q
-// relative to its row's largest value, what fp32 has of that value.  Likewise the softmax
+// (rounded to nearest; digits -128 .. 127) and q . k = inv * k_scale * 2^8 (A 2^8
+// + B + C / 2^8) with A, B, C exact 32-bit sums of int8 products, C / 2^8 rounded
+// to a whole number: 24 bits of q relative to its row's largest value, what fp32
+// has of that value, and half a unit of 2^-15 of it in the sum.  Likewise the softmax
 // weights of a block of 64 tokens, w = exp(s - m) in [0, 1] with m the block's
 // largest score of the row, are three digits, and V's dims get
-//     O = O exp(M - M') + (A 2^16 + B 2^8 + C) / (127 * 2^16) v_scale exp(m - M')
-// with M, M' the running maximum before and after.  Scores, statistics and O
-// are fp32.  Two digits (16 bits of q and of w, each relative to the largest of its row)
+//     O = O + (A 2^8 + B + C / 2^8) / (127 * 2^8) v_scale exp(m - M)
+// with M the row's running reference, its largest score or up to 16 binary
+// orders less (O is scaled when it moves).  Scores, statistics and O are fp32.  Two digits (16 bits of q and of w, each relative to the largest of its row)
 // serve bf16 outputs, whose own rounding is 2^-9: 2^-17 is lost of q and w.
 // The codes go from memory into the MFMAs as they are.
 //
@@ -38,6 +40,8 @@
 #pragma once
 
 #include <math.h>
+
+#include <type_traits>
 
 #include "nb_device.h"
 #include "nb_internal.h"
@@ -64,7 +68,7 @@ struct Kv8AttentionArgs {
 // A chunk that holds rows of the call (else n = 0).
 struct Kv8Chunk { int row0, n, request, pos0; };
 __device__ __forceinline__ Kv8Chunk kv8_chunk(const Kv8AttentionArgs& a, int i) {
-    const int32_t* c = a.chunks + 4 * (int64_t)i;
+    const auto* c = as_constant(a.chunks) + 4 * (int64_t)i;
     Kv8Chunk h{c[0], c[1], c[2], c[3]};
     if (h.n < 0 || h.n > kKvBlock || h.row0 < 0 || h.row0 > a.n_tokens - h.n || h.request < 0 ||
         h.request >= a.R || h.pos0 < 0 || h.pos0 > a.max_blocks * kKvBlock - h.n) {
@@ -117,13 +121,31 @@ struct Digits {
     static constexpr int kBias = ND == 3 ? 0x8080 : 0x80;
 };
 
-// tanh to 3e-7 of its value: the odd series up to 0.3 (next term 1.3e-10 of
-// it), above it 1 - 2 / (e^2t + 1), whose 6e-8 are 2e-7 of 0.29.  For bf16
-// outputs the latter alone: 6e-8 of the cap in the exponent.
+// o *= beta where flag (the same in all lanes) is not 0.  One instruction to
+// the compiler: a branch in the program makes it keep O twice, with a copy of
+// all of it on the way round.
+__device__ __forceinline__ void scale_if(int flag, float beta, float (&o)[4]) {
+    asm("s_cmp_eq_u32 %5, 0\n\t"
+        "s_cbranch_scc1 .Lkv8_kept_%=\n\t"
+        "v_mul_f32 %0, %0, %4\n\t"
+        "v_mul_f32 %1, %1, %4\n\t"
+        "v_mul_f32 %2, %2, %4\n\t"
+        "v_mul_f32 %3, %3, %4\n"
+        ".Lkv8_kept_%=:"
+        : "+v"(o[0]), "+v"(o[1]), "+v"(o[2]), "+v"(o[3])
+        : "v"(beta), "s"(flag)
+        : "scc");
+}
+
+// cap * tanh(x f) + add.  The tanh to 3e-7 of its value: the odd series up to
+// 0.3 (next term 1.3e-10 of it), above it 1 - 2 / (e^2t + 1), whose 6e-8 are
+// 2e-7 of 0.29.  For bf16 outputs the latter alone: 6e-8 of the cap in the
+// exponent.
 template <int ND>
-__device__ __forceinline__ float tanh_of(float t) {
+__device__ __forceinline__ float capped(float x, float f, float cap, float add) {
+    const float t = x * f;
     const float e = __builtin_amdgcn_exp2f(t * (2.f * kLog2e));
-    const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
+    const float far = fmaf(__builtin_amdgcn_rcpf(e + 1.f), -2.f * cap, cap + add);
     if constexpr (ND == 2) return far;
     const float z = t * t;
     float p = 0.0035921280f;
@@ -132,83 +154,183 @@ __device__ __forceinline__ float tanh_of(float t) {
     p = fmaf(p, z, -0.0539682540f);
     p = fmaf(p, z, 0.1333333333f);
     p = fmaf(p, z, -0.3333333333f);
-    const float near = fmaf(t * z, p, t);
-    return z < 0.09f ? near : far;
+    return z < 0.09f ? fmaf(fmaf(t * z, p, t), cap, add) : far;
 }
 
-template <int DT, int ND, bool kRules, int NW>
-__global__ __launch_bounds__(NW * 64, (DT <= 8 ? 2 : 1)) void kv8_attention_kernel(
-    Kv8AttentionArgs a) {
+// 16 bytes a lane from `src` to LDS at m0 + 16 * lane, m0 = `lds`; counted by
+// vmcnt, unseen by the compiler.
+__device__ __forceinline__ void to_lds16(uint32_t lds, const void* src) {
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :
+                 : "s"(lds), "v"(src)
+                 : "memory", "m0");
+}
+
+constexpr int kWavesKv8 = 4;   // of a workgroup
+
+// LDS of a workgroup: the waves' results to join, or two blocks' codes.
+template <int DT, bool kShared>
+constexpr int kv8_lds_bytes() {
+    const int join = kWavesKv8 / 2 * (DT * 4 + 2) * 64 * 4, codes = 4 * 64 * 16 * DT;
+    return kShared && codes > join ? codes : join;
+}
+
+template <int DT, int ND, bool kRules, bool kWhole, bool kShared>
+__device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chunk& ch, int h, char* lds) {
+    constexpr int NW = kWavesKv8;
     constexpr int DS = (DT + 3) / 4;   // steps of 64 dims of the first product
     constexpr float kTop = Digits<ND>::kTop;
-    constexpr int kSlot = (DT * 4 + 2) * 64;   // floats of a wave's result
-    __shared__ float joined[NW / 2 * kSlot];
-    // Heads vary fastest (neighbouring workgroups, dealt to the XCDs in turn,
-    // then share no keys, and with heads a multiple of 8 an XCD's L2 holds its
-    // own heads only); the last chunks, which see the longest caches, go first.
-    const int h = blockIdx.x % a.n_kv;
-    const Kv8Chunk ch = kv8_chunk(a, a.n_chunks - 1 - blockIdx.x / a.n_kv);
-    if (ch.n == 0) return;
+    constexpr int kSlot = (DT * 4 + 2) * 64;      // floats of a wave's result
+    constexpr int kCodes = 64 * 16 * DT;          // bytes of a block's keys or values
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int G = a.n_head / a.n_kv, D = a.D;
+    const int D = kWhole ? 16 * DT : a.D;
+    const int per = kWhole ? DT : D / 16;   // 16-byte pieces of a key
+    const int G = a.n_head / a.n_kv;
     const int rows = ch.n * G, tiles = (rows + 15) / 16;
     // waves of a row group (rw) and of a row's blocks (kw)
-    int rw = 1;
-    while (rw < NW && rw < tiles) rw *= 2;
-    const int kw = NW / rw, wr = wave & (rw - 1), wk = wave / rw;
+    const int rw = kShared || tiles > 2 ? NW : tiles, kw = NW / rw;
+    const int wr = wave & (rw - 1), wk = wave / rw;
     const int split = blockIdx.z, splits = gridDim.z;
-    const int32_t* blocks = a.table + ch.request * a.table_stride;
-    const int cached = min(max(a.lens[ch.request], 0), a.max_blocks * kKvBlock);
+    const auto* blocks = as_constant(a.table) + ch.request * a.table_stride;
+    const int cached = min(max(as_constant(a.lens)[ch.request], 0), a.max_blocks * kKvBlock);
+    const int pre = kRules && a.prefix ? min(max(as_constant(a.prefix)[ch.request], 0), cached) : 0;
+    const bool windowed = kRules && a.window > 0;
 
     for (int group = blockIdx.y; group * rw < tiles; group += gridDim.y) {
         const int tile = group * rw + wr;
-        const bool idle = tile >= tiles;
         const int row = min(tile * 16 + c, rows - 1);   // (rows past the last repeat it)
         const int tok = row / G, head = h * G + row - tok * G;
         const int pos = ch.pos0 + tok;
-        const int64_t q_row = ch.row0 + tok;
+        const int q_row = ch.row0 + tok;
+
+        // ---- what the rows see --------------------------------------------------
+        // a row: positions [lo, hi) and [0, pre); the tile's rows pos_lo .. pos_hi;
+        // the waves that walk together: blocks [0, pt) and [wt, t_end)
+        auto position = [&](int r) { return ch.pos0 + min(r, rows - 1) / G; };
+        const int pos_lo = position(tile * 16), pos_hi = position(tile * 16 + 15);
+        const int hi = pos + 1, lo = windowed ? max(0, hi - a.window) : 0;
+        const int lo_max = windowed ? max(0, pos_hi + 1 - a.window) : 0;
+        const int first = kShared ? position(group * NW * 16) : pos_lo;
+        const int last = kShared ? position(group * NW * 16 + NW * 16 - 1) : pos_hi;
+        const int t_end = (max(last + 1, pre) + kKvBlock - 1) / kKvBlock;
+        int wt = windowed ? max(0, first + 1 - a.window) / kKvBlock : 0;
+        int pt = (pre + kKvBlock - 1) / kKvBlock;
+        if (wt <= pt) wt = pt = 0;
+        const int count = !kShared && tile >= tiles ? 0 : pt + t_end - wt;
+        const int i_end = (int)((int64_t)count * (split + 1) / splits);
+        int i = (int)((int64_t)count * split / splits) + wk;
+
+        // ---- the row of q, and the first block on its way -----------------------
+        float x[DS][16];
+#pragma unroll
+        for (int s = 0; s < DS; ++s) {
+            const int d0 = 64 * s + 16 * g;
+            const int64_t at = q_row * a.ld_q + head * D + d0;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[s][e] = 0.f;
+            if (d0 < D) {   // (D is a multiple of 16)
+                if (a.q_dtype == NB_F32) {
+                    const float* p = static_cast<const float*>(a.q) + at;
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        if (a.vec_q) {
+                            const f4 v = *reinterpret_cast<const f4*>(p + e);
+                            x[s][e] = v[0], x[s][e + 1] = v[1], x[s][e + 2] = v[2], x[s][e + 3] = v[3];
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) x[s][e + r] = p[e + r];
+                        }
+                    }
+                } else {
+                    const bf16_bits* p = static_cast<const bf16_bits*>(a.q) + at;
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        if (a.vec_q) {
+                            const h4 v = *reinterpret_cast<const h4*>(p + e);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) x[s][e + r] = bf16_to_f32(v[r]);
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) x[s][e + r] = bf16_to_f32(p[e + r]);
+                        }
+                    }
+                }
+            }
+        }
+        // Lane's places in a block, in memory: dims past D are read at the row's
+        // start (their digits of q are zero), value dims past D at the last one
+        // (not stored).
+        const int key_row = 16 * (c >> 2) + (c & 3);   // (+ 4 mt)
+        auto place = [&](int n) { return n < pt ? n : n - pt + wt; };
+        auto block_at = [&](int n) { return blocks[place(min(n, i_end - 1))]; };
+        auto valid = [&](int b) { return b >= 0 && b < a.n_blocks; };
+        auto codes_at = [&](const int8_t* p, int b) {
+            return p + ((int64_t)(valid(b) ? b : 0) * a.n_kv + h) * kKvBlock * D;
+        };
+        i4 kf[4][DS], vf[DT];
+        auto load_keys = [&](int b) {
+            const auto* p = as_global(codes_at(a.k, b));
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt) {
+#pragma unroll
+                for (int s = 0; s < DS; ++s) {
+                    const int d0 = 64 * s + 16 * g;
+                    kf[mt][s] = *reinterpret_cast<const __attribute__((address_space(1))) i4*>(
+                        p + key_row * D + (d0 < D ? d0 : 0) + 4 * mt * D);
+                }
+            }
+        };
+        auto load_values = [&](int b) {
+            const auto* p = as_global(codes_at(a.v, b));
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                vf[dt] = *reinterpret_cast<const __attribute__((address_space(1))) i4*>(
+                    p + (kWhole ? 16 * dt + c : min(16 * dt + c, D - 1)) * kKvBlock + 16 * g);
+            }
+        };
+        // In LDS the 16-byte pieces of a key (and of a dim's values) are exchanged
+        // by its row, so that the 8 lanes that are served together (rows c ..
+        // c + 7, one piece) reach all 32 banks: keys of 8 or 16 pieces by c & 7
+        // (token bits 0, 1, 4), of 4 by token bits 1, 4; values by dim bits 1, 2.
+        auto key_swap = [&](int token) {
+            return per % 8 == 0 ? (token & 3) | (token >> 4 & 1) << 2
+                   : per == 4   ? (token >> 1 & 1) | (token >> 4 & 1) << 1
+                                : 0;
+        };
+        const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+        constexpr int kIns = (DT + NW - 1) / NW;   // loads of a wave for a block's keys
+        auto stage = [&](int b, int buffer) {
+            const int8_t *kp = codes_at(a.k, b), *vp = codes_at(a.v, b);
+#pragma unroll
+            for (int n = 0; n < kIns; ++n) {
+                const int ins = wave + NW * n;   // 64 pieces each
+                if (DT % NW != 0 || !kWhole) {
+                    if (ins >= per) break;
+                }
+                const int l = 64 * ins + lane;
+                const int token = l / per, piece = l - token * per;
+                const uint32_t to = lds0 + buffer * 2 * kCodes + 1024 * ins;
+                to_lds16(to, kp + token * D + 16 * (piece ^ key_swap(token)));
+                const int dim = l >> 2;
+                to_lds16(to + kCodes, vp + dim * kKvBlock + 16 * ((l & 3) ^ (dim >> 1 & 3)));
+            }
+        };
+        int b = 0, b_next = 0;
+        if (i < i_end) {
+            b = block_at(i);
+            b_next = block_at(i + kw);
+            if constexpr (kShared) stage(b, 0);
+            else load_keys(b);
+        }
 
         // ---- the row's digits -------------------------------------------------
         i4 qd[ND][DS];
         float inv;
         {
-            float x[DS][16];
             float most = 0.f, odd = 0.f;
 #pragma unroll
             for (int s = 0; s < DS; ++s) {
-                const int d0 = 64 * s + 16 * g;
-                const int64_t at = q_row * a.ld_q + head * D + d0;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[s][e] = 0.f;
-                if (d0 < D) {   // (D is a multiple of 16)
-                    if (a.q_dtype == NB_F32) {
-                        const float* p = static_cast<const float*>(a.q) + at;
-#pragma unroll
-                        for (int e = 0; e < 16; e += 4) {
-                            if (a.vec_q) {
-                                const f4 v = *reinterpret_cast<const f4*>(p + e);
-                                x[s][e] = v[0], x[s][e + 1] = v[1], x[s][e + 2] = v[2], x[s][e + 3] = v[3];
-                            } else {
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) x[s][e + i] = p[e + i];
-                            }
-                        }
-                    } else {
-                        const bf16_bits* p = static_cast<const bf16_bits*>(a.q) + at;
-#pragma unroll
-                        for (int e = 0; e < 16; e += 4) {
-                            if (a.vec_q) {
-                                const h4 v = *reinterpret_cast<const h4*>(p + e);
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) x[s][e + i] = bf16_to_f32(v[i]);
-                            } else {
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) x[s][e + i] = bf16_to_f32(p[e + i]);
-                            }
-                        }
-                    }
-                }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     most = fmaxf(most, fabsf(x[s][e]));
@@ -220,15 +342,16 @@ __global__ __launch_bounds__(NW * 64, (DT <= 8 ? 2 : 1)) void kv8_attention_kern
             odd = rows_sum(odd);
             const float f = kTop / most;
             inv = most / kTop + odd;
+            if constexpr (ND == 3) inv *= 256.f;   // (the first product is in units of 2^8)
 #pragma unroll
             for (int s = 0; s < DS; ++s) {
 #pragma unroll
                 for (int e = 0; e < 16; e += 4) {
                     uint32_t w[4], d[3];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float y = fminf(fmaxf(rintf(x[s][e + i] * f), -kTop), kTop);
-                        w[i] = (uint32_t)((int)y + Digits<ND>::kBias);
+                    for (int r = 0; r < 4; ++r) {
+                        const float y = fminf(fmaxf(rintf(x[s][e + r] * f), -kTop), kTop);
+                        w[r] = (uint32_t)((int)y + Digits<ND>::kBias);
                     }
                     digits4<ND>(w, d);
 #pragma unroll
@@ -237,136 +360,89 @@ __global__ __launch_bounds__(NW * 64, (DT <= 8 ? 2 : 1)) void kv8_attention_kern
             }
         }
         const float to_log2 = inv * kLog2e;
-        const float slope = kRules && a.slopes ? a.slopes[head] : 0.f;
+        // (for exponents of 2)
+        const float slope = kRules && a.slopes ? a.slopes[head] * kLog2e : 0.f;
+        const float cap = a.softcap * kLog2e, per_cap = a.softcap > 0.f ? 1.f / a.softcap : 0.f;
 
-        // ---- what the tile's rows see -----------------------------------------
-        // row: positions [lo, hi) and [0, pre); the tile: blocks [0, pt) and
-        // [wt, t_end)
-        const int tok_lo = min(tile * 16, rows - 1) / G, tok_hi = min(tile * 16 + 15, rows - 1) / G;
-        const int pos_lo = ch.pos0 + tok_lo, pos_hi = ch.pos0 + tok_hi;
-        const int pre = kRules && a.prefix ? min(max(a.prefix[ch.request], 0), cached) : 0;
-        const bool windowed = kRules && a.window > 0;
-        const int hi = pos + 1, lo = windowed ? max(0, hi - a.window) : 0;
-        const int lo_max = windowed ? max(0, pos_hi + 1 - a.window) : 0;
-        const int t_end = (max(pos_hi + 1, pre) + kKvBlock - 1) / kKvBlock;
-        int wt = windowed ? max(0, pos_lo + 1 - a.window) / kKvBlock : 0;
-        int pt = (pre + kKvBlock - 1) / kKvBlock;
-        if (wt <= pt) wt = pt = 0;
-        const int count = idle ? 0 : pt + t_end - wt;
-        const int i_end = (int)((int64_t)count * (split + 1) / splits);
-        int i = (int)((int64_t)count * split / splits) + wk;
-
-        f4 o[DT];
+        float o[DT][4];   // (no vectors: their elements would move in and out of them)
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[dt] = f4{0.f, 0.f, 0.f, 0.f};
+        for (int dt = 0; dt < DT; ++dt) o[dt][0] = o[dt][1] = o[dt][2] = o[dt][3] = 0.f;
         float m = -INFINITY, l = 0.f;   // l: of the lane's own tokens
 
-        i4 kf[4][DS], vf[DT];
-        // lane's places in a block: dims past D are read at the row's start
-        // (their digits of q are zero), value dims past D at the last one (not
-        // stored)
-        int k_at[DS];
-#pragma unroll
-        for (int s = 0; s < DS; ++s) {
-            const int d0 = 64 * s + 16 * g;
-            k_at[s] = (16 * (c >> 2) + (c & 3)) * D + (d0 < D ? d0 : 0);
-        }
-        auto place = [&](int n) { return n < pt ? n : n - pt + wt; };
-        auto block_at = [&](int n) {
-            return __builtin_amdgcn_readfirstlane(blocks[place(min(n, i_end - 1))]);
-        };
-        auto valid = [&](int b) { return b >= 0 && b < a.n_blocks; };
-        auto load_keys = [&](int b) {
-            const auto* p = as_global(a.k + ((int64_t)(valid(b) ? b : 0) * a.n_kv + h) * kKvBlock * D);
-#pragma unroll
-            for (int mt = 0; mt < 4; ++mt) {
-#pragma unroll
-                for (int s = 0; s < DS; ++s) {
-                    kf[mt][s] = *reinterpret_cast<const __attribute__((address_space(1))) i4*>(
-                        p + k_at[s] + 4 * mt * D);
-                }
-            }
-        };
-        auto load_values = [&](int b) {
-            const auto* p = as_global(a.v + ((int64_t)(valid(b) ? b : 0) * a.n_kv + h) * kKvBlock * D);
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                vf[dt] = *reinterpret_cast<const __attribute__((address_space(1))) i4*>(
-                    p + min(16 * dt + c, D - 1) * kKvBlock + 16 * g);
-            }
-        };
-        int b = 0, b_next = 0;
-        if (i < i_end) {
-            b = block_at(i);
-            b_next = block_at(i + kw);
-            load_keys(b);
-            load_values(b);
-        }
-        for (; i < i_end; i += kw) {
-            const int64_t bh = (int64_t)(valid(b) ? b : 0) * a.n_kv + h;
-            const float ks = a.k_scale[bh], vs = a.v_scale[bh];
-            const int j0 = place(i) * kKvBlock;
-            const bool more = i + kw < i_end;
+        // one block: key(mt, s) and value(dt) give the codes; between() runs
+        // after the first product
+        auto walk = [&](int block, int n, auto&& key, auto&& between, auto&& value)
+                        __attribute__((always_inline)) {
+            const int64_t bh = (int64_t)(valid(block) ? block : 0) * a.n_kv + h;
+            const float ks = as_constant(a.k_scale)[bh], vs = as_constant(a.v_scale)[bh];
+            const int j0 = place(n) * kKvBlock;
             // ---- scores -------------------------------------------------------
             float x[16];
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt) {
-                i4 acc = {0, 0, 0, 0}, low = {0, 0, 0, 0};
+                i4 acc = {0, 0, 0, 0}, low = {128, 128, 128, 128}, f[DS];
+#pragma unroll
+                for (int s = 0; s < DS; ++s) f[s] = key(mt, s);
 #pragma unroll
                 for (int s = 0; s < DS; ++s)
-                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[mt][s], qd[ND - 1][s], acc, 0, 0, 0);
-                acc <<= 8;
-#pragma unroll
-                for (int s = 0; s < DS; ++s)
-                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[mt][s], qd[ND - 2][s], acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[s], qd[ND - 1][s], acc, 0, 0, 0);
                 if constexpr (ND == 3) {
 #pragma unroll
                     for (int s = 0; s < DS; ++s)
-                        low = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[mt][s], qd[0][s], low, 0, 0, 0);
+                        low = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[s], qd[0][s], low, 0, 0, 0);
+                    acc = (acc << 8) + (low >> 8);
+                } else {
+                    acc <<= 8;
                 }
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    x[4 * mt + r] = ND == 3 ? fmaf((float)acc[r], 256.f, (float)low[r]) : (float)acc[r];
-                }
+                for (int s = 0; s < DS; ++s)
+                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[s], qd[ND - 2][s], acc, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[4 * mt + r] = (float)acc[r];
             }
-            const int b_now = b;
-            b = b_next;
-            if (more) {
-                load_keys(b);
-                b_next = block_at(i + 2 * kw);
-            }
+            between();
+            // scores in units of 1 / unit: x * unit is the exponent of 2
+            float unit = to_log2 * ks;
             if constexpr (kRules) {
-                const float f = inv * ks;
-                const float per_cap = a.softcap > 0.f ? 1.f / a.softcap : 0.f;
-                const float from = (float)(j0 + 16 * g - pos);   // distance of the lane's first token
+                // slope * distance, from the lane's first token on
+                const float at = slope * (float)(j0 + 16 * g - pos);
+                if (a.softcap > 0.f) {
+                    const float f = inv * ks * per_cap;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    float s = x[e] * f;
-                    if (a.softcap > 0.f) s = a.softcap * tanh_of<ND>(s * per_cap);
-                    x[e] = fmaf(slope, from + (float)e, s) * kLog2e;
+                    for (int e = 0; e < 16; ++e)
+                        x[e] = capped<ND>(x[e], f, cap, fmaf(slope, (float)e, at));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[e] = fmaf(x[e], unit, fmaf(slope, (float)e, at));
                 }
-            } else {
-                const float f = to_log2 * ks;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] *= f;
+                unit = 1.f;
             }
             // some row of the tile does not see the whole block
-            if (!valid(b_now) ||
+            if (!valid(block) ||
                 !((j0 + kKvBlock <= pos_lo + 1 && j0 >= lo_max) || j0 + kKvBlock <= pre)) {
                 const int jl = j0 + 16 * g;
+                const int end = valid(block) ? hi : 0, pre_end = valid(block) ? pre : 0;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int j = jl + e;
-                    const bool seen = valid(b_now) && ((j < hi && j >= lo) || j < pre);
-                    x[e] = seen ? x[e] : -INFINITY;
+                    const bool seen = ((j < end) & (j >= lo)) | (j < pre_end);
+                    x[e] = seen ? x[e] * unit : -INFINITY;
                 }
+                unit = 1.f;   // (a unit of 0 or infinity times -inf is NaN)
             }
             // ---- weights ------------------------------------------------------
             float top = x[0];
 #pragma unroll
             for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
-            top = rows_max(top);
+            top = rows_max(top) * unit;
             const float base = fmaxf(top, kLowest);
+            // p is at most 1 + 2^-24 |base|, which its digits hold up to 2^12
+            const bool far = fabsf(base) > 4096.f;
+            if (__any(far)) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] *= far ? unit : 1.f;
+                unit = far ? 1.f : unit;
+            }
             float sum = 0.f;
             i4 pd[ND];
 #pragma unroll
@@ -374,7 +450,7 @@ __global__ __launch_bounds__(NW * 64, (DT <= 8 ? 2 : 1)) void kv8_attention_kern
                 uint32_t w[4], d[3];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float p = __builtin_amdgcn_exp2f(x[e + r] - base);
+                    const float p = __builtin_amdgcn_exp2f(fmaf(x[e + r], unit, -base));
                     sum += p;
                     // 2^23 + bias + rint(p kTop): the low mantissa bits
                     w[r] = __float_as_uint(fmaf(p, kTop, 8388608.f + (float)Digits<ND>::kBias));
@@ -383,36 +459,87 @@ __global__ __launch_bounds__(NW * 64, (DT <= 8 ? 2 : 1)) void kv8_attention_kern
 #pragma unroll
                 for (int n = 0; n < ND; ++n) pd[n][e / 4] = (int)d[n];
             }
-            const float m_new = fmaxf(m, top), safe = fmaxf(m_new, kLowest);
-            const float beta = __builtin_amdgcn_exp2f(m - safe);
-            const float share = __builtin_amdgcn_exp2f(top - safe);
-            l = fmaf(l, beta, sum * share);
+            // m follows a row's largest score only when that is 2^16 ahead:
+            // shares up to 2^16 cost fp32 sums nothing, scaling O does (by 1 in
+            // the rows that stay: a row's result is its own)
+            const bool ahead = top > m + 16.f;
+            const float m_new = ahead ? top : m;
+            const float beta = ahead ? __builtin_amdgcn_exp2f(m - fmaxf(m_new, kLowest)) : 1.f;
+            const int any_ahead = __builtin_amdgcn_readfirstlane(__any(ahead));
+            l *= beta;
             m = m_new;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) scale_if(any_ahead, beta, o[dt]);
+            const float share = __builtin_amdgcn_exp2f(top - fmaxf(m, kLowest));
+            l = fmaf(sum, share, l);
             // (a row that sees nothing of the block takes nothing of its scale)
-            const float gamma = top == -INFINITY ? 0.f : share * vs * (1.f / kTop);
+            const float gamma =
+                top == -INFINITY ? 0.f : share * vs * (ND == 3 ? 256.f / kTop : 1.f / kTop);
             // ---- O ------------------------------------------------------------
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                i4 acc = {0, 0, 0, 0}, low = {0, 0, 0, 0};
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf[dt], pd[ND - 1], acc, 0, 0, 0);
-                acc <<= 8;
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf[dt], pd[ND - 2], acc, 0, 0, 0);
-                if constexpr (ND == 3)
-                    low = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf[dt], pd[0], low, 0, 0, 0);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float t =
-                        ND == 3 ? fmaf((float)acc[r], 256.f, (float)low[r]) : (float)acc[r];
-                    o[dt][r] = fmaf(gamma, t, o[dt][r] * beta);
+                i4 acc = {0, 0, 0, 0}, low = {128, 128, 128, 128};
+                const i4 f = value(dt);
+                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, pd[ND - 1], acc, 0, 0, 0);
+                if constexpr (ND == 3) {
+                    low = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, pd[0], low, 0, 0, 0);
+                    acc = (acc << 8) + (low >> 8);
+                } else {
+                    acc <<= 8;
                 }
+                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, pd[ND - 2], acc, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[dt][r] = fmaf(gamma, (float)acc[r], o[dt][r]);
             }
-            if (more) load_values(b);
+        };
+        if constexpr (kShared) {
+            const i4* mine = reinterpret_cast<const i4*>(lds);
+            const int swap = key_swap(key_row);   // (the same for all mt)
+            int buffer = 0;
+            for (; i < i_end; ++i, buffer ^= 1) {
+                // this block has arrived, and the other buffer is read, in all waves
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();
+                if (i + 1 < i_end) stage(b_next, buffer ^ 1);
+                const int now = b;
+                b = b_next;
+                b_next = block_at(i + 2);
+                const i4* from = mine + buffer * (2 * kCodes / 16);
+                walk(
+                    now, i,
+                    [&](int mt, int s) {
+                        const int piece = 4 * s + g < per ? 4 * s + g : 0;
+                        return from[(key_row + 4 * mt) * per + (piece ^ swap)];
+                    },
+                    [] {},
+                    [&](int dt) {
+                        return from[kCodes / 16 + (16 * dt + c) * 4 + (g ^ (c >> 1 & 3))];
+                    });
+            }
+            __syncthreads();   // the last block is read
+        } else {
+            // `more`: the next block's loads are issued (a constant, so that every
+            // path to the next block has them in flight and waits for no more)
+            auto direct = [&](auto more) __attribute__((always_inline)) {
+                const int now = b;
+                walk(
+                    now, i, [&](int mt, int s) { return kf[mt][s]; },
+                    [&] {
+                        load_values(now);
+                        b = b_next;
+                        if constexpr (decltype(more)::value) b_next = block_at(i + 2 * kw);
+                    },
+                    [&](int dt) { return vf[dt]; });
+                if constexpr (decltype(more)::value) load_keys(b);
+            };
+            for (; i + kw < i_end; i += kw) direct(std::true_type{});
+            if (i < i_end) direct(std::false_type{});
         }
         l = rows_sum(l);
 
         // ---- the waves of a row joined, halves to halves ----------------------
         for (int half = kw / 2; half > 0; half /= 2) {
-            float* slot = joined + ((wk >= half ? wk - half : wk) * rw + wr) * kSlot + lane;
+            float* slot = reinterpret_cast<float*>(lds) + ((wk >= half ? wk - half : wk) * rw + wr) * kSlot + lane;
             if (wk >= half && wk < 2 * half) {
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
@@ -439,14 +566,14 @@ __global__ __launch_bounds__(NW * 64, (DT <= 8 ? 2 : 1)) void kv8_attention_kern
         }
         if (wk > 0 || tile * 16 + c >= rows) continue;   // (no barrier below)
         if (splits > 1) {
-            const int64_t at = (q_row * a.n_head + head) * splits + split;
+            const int64_t at = ((int64_t)q_row * a.n_head + head) * splits + split;
             float* ml = a.part + (int64_t)a.n_tokens * a.n_head * splits * D + 2 * at;
             if (g == 0) ml[0] = m, ml[1] = l;
             if (l == 0.f) continue;   // nothing seen: the join does not read its dims
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
                 const int d = 16 * dt + 4 * g;
-                if (d < D) *reinterpret_cast<f4*>(a.part + at * D + d) = o[dt];
+                if (d < D) *reinterpret_cast<f4*>(a.part + at * D + d) = f4{o[dt][0], o[dt][1], o[dt][2], o[dt][3]};
             }
             continue;
         }
@@ -456,7 +583,7 @@ __global__ __launch_bounds__(NW * 64, (DT <= 8 ? 2 : 1)) void kv8_attention_kern
         for (int dt = 0; dt < DT; ++dt) {
             const int d = 16 * dt + 4 * g;
             if (d >= D) continue;
-            const f4 v = o[dt] * norm;
+            const f4 v = f4{o[dt][0], o[dt][1], o[dt][2], o[dt][3]} * norm;
             if (a.out_dtype == NB_F32) {
                 float* p = static_cast<float*>(a.out) + to + d;
                 if (a.vec_out) {
@@ -481,31 +608,54 @@ __global__ __launch_bounds__(NW * 64, (DT <= 8 ? 2 : 1)) void kv8_attention_kern
     }
 }
 
-template <int DT, int ND, int NW>
+// kPrompts: chunks of over two tiles of 16 rows share their blocks' codes
+// through LDS, the others of the launch go as without.
+template <int DT, int ND, bool kRules, bool kWhole, bool kPrompts>
+__global__ __launch_bounds__(kWavesKv8 * 64, (DT <= 8 ? 3 : 1)) void kv8_attention_kernel(
+    Kv8AttentionArgs a) {
+    __shared__ __align__(16) char lds[kv8_lds_bytes<DT, kPrompts>()];
+    // Heads vary fastest (neighbouring workgroups, dealt to the XCDs in turn,
+    // then share no keys, and with heads a multiple of 8 an XCD's L2 holds its
+    // own heads only); the last chunks, which see the longest caches, go first.
+    const int h = blockIdx.x % a.n_kv;
+    const Kv8Chunk ch = kv8_chunk(a, a.n_chunks - 1 - blockIdx.x / a.n_kv);
+    if (ch.n == 0) return;
+    if constexpr (kPrompts) {
+        if (ch.n * (a.n_head / a.n_kv) > 32) {
+            kv8_rows<DT, ND, kRules, kWhole, true>(a, ch, h, lds);
+            return;
+        }
+    }
+    kv8_rows<DT, ND, kRules, kWhole, false>(a, ch, h, lds);
+}
+
+template <int DT, int ND, bool kWhole, bool kPrompts>
 void launch_kv8_form(const Kv8AttentionArgs& a, dim3 grid, bool rules, hipStream_t stream) {
     if (rules) {
-        hipLaunchKernelGGL((kv8_attention_kernel<DT, ND, true, NW>), grid, dim3(NW * 64), 0, stream, a);
+        hipLaunchKernelGGL((kv8_attention_kernel<DT, ND, true, kWhole, kPrompts>), grid,
+                           dim3(kWavesKv8 * 64), 0, stream, a);
     } else {
-        hipLaunchKernelGGL((kv8_attention_kernel<DT, ND, false, NW>), grid, dim3(NW * 64), 0, stream, a);
+        hipLaunchKernelGGL((kv8_attention_kernel<DT, ND, false, kWhole, kPrompts>), grid,
+                           dim3(kWavesKv8 * 64), 0, stream, a);
     }
 }
 
-template <int ND>
+// The head dim as a constant where it fills the tiles, else the next tiles' form.
+template <int ND, bool kPrompts>
 void launch_kv8_digits(const Kv8AttentionArgs& a, dim3 grid, bool rules, hipStream_t stream) {
-    if (a.D <= 64) {
-        launch_kv8_form<4, ND, 4>(a, grid, rules, stream);
-    } else if (a.D <= 96) {
-        launch_kv8_form<6, ND, 4>(a, grid, rules, stream);
-    } else if (a.D <= 128) {
-        launch_kv8_form<8, ND, 4>(a, grid, rules, stream);
-    } else {
-        launch_kv8_form<16, ND, 4>(a, grid, rules, stream);
-    }
+    if (a.D == 64) launch_kv8_form<4, ND, true, kPrompts>(a, grid, rules, stream);
+    else if (a.D < 64) launch_kv8_form<4, ND, false, kPrompts>(a, grid, rules, stream);
+    else if (a.D == 96) launch_kv8_form<6, ND, true, kPrompts>(a, grid, rules, stream);
+    else if (a.D == 128) launch_kv8_form<8, ND, true, kPrompts>(a, grid, rules, stream);
+    else if (a.D < 128) launch_kv8_form<8, ND, false, kPrompts>(a, grid, rules, stream);
+    else if (a.D == 256) launch_kv8_form<16, ND, true, kPrompts>(a, grid, rules, stream);
+    else launch_kv8_form<16, ND, false, kPrompts>(a, grid, rules, stream);
 }
 
 }  // namespace
 
-void launch_kv8_attention_2(const Kv8AttentionArgs& a, dim3 grid, bool rules, hipStream_t stream);
-void launch_kv8_attention_3(const Kv8AttentionArgs& a, dim3 grid, bool rules, hipStream_t stream);
+// Two or three digits; with or without chunks that share codes through LDS.
+using Kv8AttentionLaunch = void(const Kv8AttentionArgs& a, dim3 grid, bool rules, hipStream_t stream);
+Kv8AttentionLaunch launch_kv8_tokens_2, launch_kv8_tokens_3, launch_kv8_prompts_2, launch_kv8_prompts_3;
 
 }  // namespace nb

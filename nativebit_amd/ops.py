@@ -6,6 +6,7 @@ torch's current stream and raises NativeBitError on a non-zero status.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple
 
@@ -526,38 +527,47 @@ class KVPlan(NamedTuple):
     state: torch.Tensor
 
 
-def _launch(t: torch.Tensor, fn, *args):
-    """fn(*args, stream) on t's device and torch's current stream there."""
-    stream = _stream(t)
-    device = t.get_device()
-    if device == torch._C._cuda_getDevice():
-        status = fn(*args, stream)
+def _is(t, dtype, shape, dev) -> bool:
+    """t is a contiguous GPU tensor of this type, shape and device: the check
+    of a call's usual arguments.  Where it fails, the slower ones below say
+    what is wrong."""
+    return (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and
+            t.get_device() == dev and t.is_cuda and t.is_contiguous())
+
+
+def _launch(dev: int, fn, *args):
+    """fn(*args, stream) on GPU dev and torch's current stream there."""
+    if dev == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
-        with torch.cuda.device(device):
-            status = fn(*args, stream)
+        with torch.cuda.device(dev):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     if status:
         _lib.check(status)
 
 
-def _int32(name: str, t: torch.Tensor, shape, like: torch.Tensor | None = None):
-    """t is a contiguous int32 GPU tensor of this shape (None: any size)."""
+def _require(name: str, t, dtype, shape, dev):
+    """t is a contiguous GPU tensor of this type, shape (None: any size) and
+    device, or an error that says what it is not."""
     _require_cuda(name, t)
-    if t.dtype != torch.int32 or not t.is_contiguous():
-        raise TypeError(f"{name} must be a contiguous int32 tensor")
+    if t.dtype != dtype or not t.is_contiguous():
+        raise TypeError(f"{name} must be a contiguous {dtype} tensor")
     if t.dim() != len(shape) or any(want is not None and have != want
                                     for have, want in zip(t.shape, shape)):
         raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
-    if like is not None:
-        _same_device(like, t)
+    if t.get_device() != dev:
+        raise ValueError(f"tensors on different devices: {name} on {t.device}, cuda:{dev}")
 
 
 def _table(table: torch.Tensor):
+    """(device, requests, blocks, row stride) of a block table."""
     _require_cuda("table", table)
-    if table.dtype != torch.int32 or table.dim() != 2 or table.numel() == 0 or \
+    if table.dtype is not torch.int32 or table.dim() != 2 or table.numel() == 0 or \
             (table.shape[1] > 1 and table.stride(1) != 1):
         raise TypeError("table must be an int32 (requests, blocks) tensor, rows contiguous")
+    R, width = table.shape
     # (a table of one row may have any row stride)
-    return table.stride(0) if table.shape[0] > 1 else table.shape[1]
+    return table.get_device(), R, width, table.stride(0) if R > 1 else width
 
 
 def kv_plan_chunks(n_tokens: int, n_requests: int) -> int:
@@ -576,30 +586,34 @@ def kv_plan(table: torch.Tensor, lens: torch.Tensor, new: torch.Tensor, free: to
     the rows of the step (the sum of ``new``, or more: the rows behind have no
     slot).  ``lens`` and ``state`` are left as they are; the plan's are those
     after the step.  ``out``: a plan of the same sizes to write."""
-    stride = _table(table)
-    R, width = table.shape
+    dev, R, width, stride = _table(table)
     n_tokens = int(n_tokens)
-    _int32("lens", lens, (R,), table)
-    _int32("new", new, (R,), table)
-    _int32("free", free, (None,), table)
-    _int32("state", state, (2,), table)
+    i32, n_blocks = torch.int32, free.numel()
+    if not (_is(lens, i32, (R,), dev) and _is(new, i32, (R,), dev) and
+            _is(free, i32, (n_blocks,), dev) and _is(state, i32, (2,), dev)):
+        _require("lens", lens, i32, (R,), dev)
+        _require("new", new, i32, (R,), dev)
+        _require("free", free, i32, (None,), dev)
+        _require("state", state, i32, (2,), dev)
     chunks = kv_plan_chunks(n_tokens, R)
     if out is None:
         if n_tokens < 0:
             raise ValueError(f"n_tokens={n_tokens}")
-        buf = torch.empty(4 * chunks + 2 * n_tokens + R + 2, dtype=torch.int32, device=table.device)
+        buf = torch.empty(4 * chunks + 2 * n_tokens + R + 2, dtype=i32, device=table.device)
         c, s, p, l, st = buf.split_with_sizes([4 * chunks, n_tokens, n_tokens, R, 2])
         out = KVPlan(s, p, c.view(chunks, 4), l, st)
+        at = buf.data_ptr()     # the parts' places, in the order of the split
+        c, s, p, l, st = at, at + 16 * chunks, at + 16 * chunks + 4 * n_tokens, \
+            at + 16 * chunks + 8 * n_tokens, at + 16 * chunks + 8 * n_tokens + 4 * R
     else:
         for name, t, shape in (("slots", out.slots, (n_tokens,)),
                                ("positions", out.positions, (n_tokens,)),
                                ("chunks", out.chunks, (chunks, 4)), ("lens", out.lens, (R,)),
                                ("state", out.state, (2,))):
-            _int32(f"out.{name}", t, shape, table)
-    _launch(table, _lib.load().nb_kv_plan, table.data_ptr(), stride, lens.data_ptr(),
-            new.data_ptr(), free.data_ptr(), state.data_ptr(), R, width, free.numel(), n_tokens,
-            out.slots.data_ptr(), out.positions.data_ptr(), out.chunks.data_ptr(),
-            out.lens.data_ptr(), out.state.data_ptr())
+            _require(f"out.{name}", t, i32, shape, dev)
+        s, p, c, l, st = (t.data_ptr() for t in out)
+    _launch(dev, _lib.load().nb_kv_plan, table.data_ptr(), stride, lens.data_ptr(), new.data_ptr(),
+            free.data_ptr(), state.data_ptr(), R, width, n_blocks, n_tokens, s, p, c, l, st)
     return out
 
 
@@ -608,54 +622,49 @@ def kv_release(table: torch.Tensor, lens: torch.Tensor, finished: torch.Tensor,
     """The blocks of the requests with ``finished[r] != 0`` back on the free
     list, their lengths 0 and table entries -1, all in place
     (nb_kv_release)."""
-    stride = _table(table)
-    R, width = table.shape
-    _int32("lens", lens, (R,), table)
-    _int32("finished", finished, (R,), table)
-    _int32("free", free, (None,), table)
-    _int32("state", state, (2,), table)
-    _launch(table, _lib.load().nb_kv_release, table.data_ptr(), stride, lens.data_ptr(),
+    dev, R, width, stride = _table(table)
+    _require("lens", lens, torch.int32, (R,), dev)
+    _require("finished", finished, torch.int32, (R,), dev)
+    _require("free", free, torch.int32, (None,), dev)
+    _require("state", state, torch.int32, (2,), dev)
+    _launch(dev, _lib.load().nb_kv_release, table.data_ptr(), stride, lens.data_ptr(),
             finished.data_ptr(), free.data_ptr(), state.data_ptr(), R, width, free.numel())
 
 
 def _kv8_cache(k, v, k_scale, v_scale):
-    """(blocks, heads, head dim) of an 8-bit cache, its tensors checked."""
-    for name, t in (("k", k), ("v", v), ("k_scale", k_scale), ("v_scale", v_scale)):
-        _require_cuda(name, t)
-        if not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
-    _same_device(k, v, k_scale, v_scale)
-    if k.dtype != torch.int8 or v.dtype != torch.int8 or k.dim() != 4 or k.shape[2] != KV_BLOCK:
-        raise ValueError(f"k must be int8 (blocks, heads, {KV_BLOCK}, head_dim), v int8 "
-                         f"(blocks, heads, head_dim, {KV_BLOCK})")
-    n, h, _, d = k.shape
-    if v.shape != (n, h, d, KV_BLOCK):
-        raise ValueError(f"v must be {(n, h, d, KV_BLOCK)}, got {tuple(v.shape)}")
-    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if t.dtype != torch.float32 or t.shape != (n, h):
-            raise ValueError(f"{name} must be float32 {(n, h)}")
-    return n, h, d
+    """(device, blocks, heads, head dim) of an 8-bit cache, its tensors
+    checked."""
+    _require_cuda("k", k)
+    if k.dim() != 4:
+        raise ValueError(f"k must be (blocks, heads, {KV_BLOCK}, head_dim), got {tuple(k.shape)}")
+    dev = k.get_device()
+    n, h, block, d = k.shape
+    if not (_is(k, torch.int8, (n, h, KV_BLOCK, d), dev) and
+            _is(v, torch.int8, (n, h, d, KV_BLOCK), dev) and
+            _is(k_scale, torch.float32, (n, h), dev) and _is(v_scale, torch.float32, (n, h), dev)):
+        _require("k", k, torch.int8, (None, None, KV_BLOCK, None), dev)
+        _require("v", v, torch.int8, (n, h, d, KV_BLOCK), dev)
+        _require("k_scale", k_scale, torch.float32, (n, h), dev)
+        _require("v_scale", v_scale, torch.float32, (n, h), dev)
+    return dev, n, h, d
 
 
-def _rows(name, t, rows, width, like):
+def _rows(name, t, rows, width, dev):
     """Row stride of a (rows, width) float32 / bfloat16 tensor."""
-    _require_cuda(name, t)
-    _same_device(like, t)
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        _require_cuda(name, t)
+    if t.get_device() != dev:
+        raise ValueError(f"tensors on different devices: {name} on {t.device}, cuda:{dev}")
     if t.dtype not in _DT:
         raise TypeError(f"{name} dtype {t.dtype} not supported (float32 or bfloat16)")
-    if t.dim() != 2 or t.shape[0] != rows or (width is not None and t.shape[1] != width) or \
-            (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name} must be ({rows}, {width}), rows contiguous; got "
-                         f"{tuple(t.shape)}, strides {t.stride()}")
-    if rows > 1 and t.stride(0) < t.shape[1]:
-        raise ValueError(f"{name}: rows overlap")
-    return t.stride(0) if rows > 1 else t.shape[1]
-
-
-def _plan(plan: KVPlan, rows: int, like):
-    _int32("plan.slots", plan.slots, (rows,), like)
-    _int32("plan.positions", plan.positions, (rows,), like)
-    _int32("plan.chunks", plan.chunks, (None, 4), like)
+    if t.shape != (rows, width):
+        raise ValueError(f"{name} must be ({rows}, {width}), got {tuple(t.shape)}")
+    ld, step = t.stride()
+    if rows <= 1:
+        ld = width
+    if (step != 1 and width > 1) or ld < width:
+        raise ValueError(f"{name}: rows must be contiguous and not overlap (strides {t.stride()})")
+    return ld
 
 
 def kv8_append(qkv: torch.Tensor, plan: KVPlan, cos: torch.Tensor, sin: torch.Tensor,
@@ -666,26 +675,31 @@ def kv8_append(qkv: torch.Tensor, plan: KVPlan, cos: torch.Tensor, sin: torch.Te
     float32 or bfloat16, ``cos`` / ``sin`` (positions, head_dim / 2) float32.
     Returns the turned queries times head_dim^-0.5, (rows, n_head head_dim) in
     qkv's dtype (or into ``q``); rows without a slot are not written."""
-    n_blocks, n_kv, D = _kv8_cache(k, v, k_scale, v_scale)
-    n_head = int(n_head)
+    dev, n_blocks, n_kv, D = _kv8_cache(k, v, k_scale, v_scale)
+    n_head, i32 = int(n_head), torch.int32
+    width = (n_head + 2 * n_kv) * D
     if qkv.dim() != 2:
-        raise ValueError(f"qkv must be (rows, {(n_head + 2 * n_kv) * D})")
-    n = qkv.shape[0]
-    ld = _rows("qkv", qkv, n, (n_head + 2 * n_kv) * D, k)
-    _plan(plan, n, k)
-    for name, t in (("cos", cos), ("sin", sin)):
-        _require_cuda(name, t)
-        if t.dtype != torch.float32 or not t.is_contiguous() or t.dim() != 2 or \
-                t.shape[1] * 2 != D or t.shape != cos.shape:
-            raise ValueError(f"{name} must be a contiguous float32 (positions, {D // 2}) tensor")
-        _same_device(k, t)
+        raise ValueError(f"qkv must be (rows, {width})")
+    n, n_pos, chunks = qkv.shape[0], cos.shape[0], plan.chunks
+    ld = _rows("qkv", qkv, n, width, dev)
+    if not (_is(plan.slots, i32, (n,), dev) and _is(plan.positions, i32, (n,), dev) and
+            _is(chunks, i32, (chunks.shape[0], 4), dev) and
+            _is(cos, torch.float32, (n_pos, D // 2), dev) and
+            _is(sin, torch.float32, (n_pos, D // 2), dev)):
+        _require("plan.slots", plan.slots, i32, (n,), dev)
+        _require("plan.positions", plan.positions, i32, (n,), dev)
+        _require("plan.chunks", chunks, i32, (None, 4), dev)
+        _require("cos", cos, torch.float32, (None, D // 2), dev)
+        _require("sin", sin, torch.float32, (n_pos, D // 2), dev)
     if q is None:
         q = torch.empty((n, n_head * D), dtype=qkv.dtype, device=qkv.device)
-    ld_q = _rows("q", q, n, n_head * D, k)
+        ld_q = n_head * D
+    else:
+        ld_q = _rows("q", q, n, n_head * D, dev)
     if n:
-        _launch(k, _lib.load().nb_kv8_append, qkv.data_ptr(), _DT[qkv.dtype], ld,
-                plan.slots.data_ptr(), plan.positions.data_ptr(), plan.chunks.data_ptr(),
-                plan.chunks.shape[0], cos.data_ptr(), sin.data_ptr(), cos.shape[0], k.data_ptr(),
+        _launch(dev, _lib.load().nb_kv8_append, qkv.data_ptr(), _DT[qkv.dtype], ld,
+                plan.slots.data_ptr(), plan.positions.data_ptr(), chunks.data_ptr(),
+                chunks.shape[0], cos.data_ptr(), sin.data_ptr(), n_pos, k.data_ptr(),
                 v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_blocks, q.data_ptr(),
                 _DT[q.dtype], ld_q, n, n_head, n_kv, D)
     return q
@@ -696,15 +710,15 @@ def kv8_read(slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: tor
     """(keys, values), each (n, heads, head_dim), that the cache holds at
     ``slots`` (n,); zeros for slots outside it, -1 among them
     (nb_kv8_read)."""
-    n_blocks, n_kv, D = _kv8_cache(k, v, k_scale, v_scale)
-    _int32("slots", slots, (None,), k)
+    dev, n_blocks, n_kv, D = _kv8_cache(k, v, k_scale, v_scale)
+    _require("slots", slots, torch.int32, (None,), dev)
     if dtype not in _DT:
-        raise TypeError(f"dtype {dtype} not supported")
-    n = slots.numel()
+        raise TypeError(f"dtype {dtype} not supported (float32 or bfloat16)")
+    n = slots.shape[0]
     keys = torch.empty((n, n_kv, D), dtype=dtype, device=k.device)
     values = torch.empty_like(keys)
     if n:
-        _launch(k, _lib.load().nb_kv8_read, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(),
+        _launch(dev, _lib.load().nb_kv8_read, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(),
                 k_scale.data_ptr(), v_scale.data_ptr(), n_blocks, n_kv, D, keys.data_ptr(),
                 values.data_ptr(), _DT[dtype])
     return keys, values
@@ -724,41 +738,55 @@ def kv8_attention(q: torch.Tensor, plan: KVPlan, table: torch.Tensor, k: torch.T
     besides all before prefix[request].  Returns (rows, heads * head_dim) in
     q's dtype or ``out_dtype`` (or into ``out``); rows without a slot are not
     written."""
-    n_blocks, n_kv, D = _kv8_cache(k, v, k_scale, v_scale)
-    stride = _table(table)
-    _same_device(k, table)
-    R, width = table.shape
+    dev, n_blocks, n_kv, D = _kv8_cache(k, v, k_scale, v_scale)
+    table_dev, R, width, stride = _table(table)
     if q.dim() != 2 or q.shape[1] == 0 or q.shape[1] % (n_kv * D):
         raise ValueError(f"q must be (rows, heads * {D}), heads a multiple of {n_kv}")
-    n, n_head = q.shape[0], q.shape[1] // D
-    ld_q = _rows("q", q, n, None, k)
-    _plan(plan, n, k)
-    _int32("plan.lens", plan.lens, (R,), k)
+    n, columns = q.shape
+    n_head, i32, chunks = columns // D, torch.int32, plan.chunks
+    ld_q = _rows("q", q, n, columns, dev)
+    n_chunks = chunks.shape[0]
+    if table_dev != dev or not (_is(chunks, i32, (n_chunks, 4), dev) and
+                                _is(plan.lens, i32, (R,), dev)):
+        _require("table", table, i32, (R, width), dev)
+        _require("plan.chunks", chunks, i32, (None, 4), dev)
+        _require("plan.lens", plan.lens, i32, (R,), dev)
     if slopes is not None:
-        _require_cuda("slopes", slopes)
-        _same_device(k, slopes)
-        if slopes.dtype != torch.float32 or slopes.shape != (n_head,) or not slopes.is_contiguous():
-            raise ValueError(f"slopes must be a contiguous float32 ({n_head},) tensor")
+        _require("slopes", slopes, torch.float32, (n_head,), dev)
     if prefix is not None:
-        _int32("prefix", prefix, (R,), k)
+        _require("prefix", prefix, i32, (R,), dev)
     if out is None:
-        out = torch.empty((n, n_head * D), dtype=out_dtype or q.dtype, device=q.device)
-    elif out_dtype is not None and out.dtype != out_dtype:
-        raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
-    ld_out = _rows("out", out, n, n_head * D, k)
+        out = torch.empty((n, columns), dtype=out_dtype or q.dtype, device=q.device)
+        ld_out = columns
+        if out.dtype not in _DT:
+            raise TypeError(f"out_dtype {out_dtype} not supported (float32 or bfloat16)")
+    else:
+        if out_dtype is not None and out.dtype != out_dtype:
+            raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
+        ld_out = _rows("out", out, n, columns, dev)
     if n:
-        lib = _lib.load()
-        n_chunks = plan.chunks.shape[0]
-        nbytes = lib.nb_kv8_attention_ws_bytes(n, n_chunks, width, n_head, n_kv, D)
+        nbytes = _kv8_attention_bytes(dev, n, n_chunks, width, n_head, n_kv, D)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-        _launch(k, lib.nb_kv8_attention, q.data_ptr(), _DT[q.dtype], ld_q, plan.chunks.data_ptr(),
-                n_chunks, plan.lens.data_ptr(), table.data_ptr(), stride, R, width, k.data_ptr(),
-                v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_blocks, out.data_ptr(),
-                _DT[out.dtype], ld_out, n, n_head, n_kv, D, float(softcap), int(window),
-                slopes.data_ptr() if slopes is not None else None,
+        _launch(dev, _lib.load().nb_kv8_attention, q.data_ptr(), _DT[q.dtype], ld_q,
+                chunks.data_ptr(), n_chunks, plan.lens.data_ptr(), table.data_ptr(), stride, R,
+                width, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                n_blocks, out.data_ptr(), _DT[out.dtype], ld_out, n, n_head, n_kv, D,
+                softcap, window, slopes.data_ptr() if slopes is not None else None,
                 prefix.data_ptr() if prefix is not None else None,
                 ws.data_ptr() if nbytes else None, nbytes)
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _kv8_attention_bytes(dev, *sizes) -> int:
+    """Workspace bytes of nb_kv8_attention on GPU dev (they go by its CUs)."""
+    with torch.cuda.device(dev):
+        return int(_lib.load().nb_kv8_attention_ws_bytes(*sizes))
+
+
+@functools.lru_cache(maxsize=256)
+def _logits_rules_bytes(rows, vocab) -> int:
+    return int(_lib.load().nb_logits_rules_ws_bytes(rows, vocab))
 
 
 def logits_rules(logits: torch.Tensor, *, history: torch.Tensor | None = None,
@@ -781,7 +809,8 @@ def logits_rules(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"logits must be (B, V), got {tuple(logits.shape)}")
     B, V = logits.shape
-    ld = _rows("logits", logits, B, V, logits)
+    dev = logits.get_device()
+    ld = _rows("logits", logits, B, V, dev)
     if (history is None) != (lens is None):
         raise ValueError("history and lens go together")
     if history is None and not (prompt_lens is None and repetition is None and
@@ -789,56 +818,63 @@ def logits_rules(logits: torch.Tensor, *, history: torch.Tensor | None = None,
         raise ValueError("penalties need a history")
     if (bias_ids is None) != (bias is None):
         raise ValueError("bias_ids and bias go together")
-    p = {}
-
-    def matrix(name, t, dtype, columns):
-        if t is None:
-            return 0, 0
-        _require_cuda(name, t)
-        _same_device(logits, t)
-        if t.dtype != dtype or t.dim() != 2 or t.shape[0] != B or t.shape[1] < columns or \
-                (t.shape[1] > 1 and t.stride(1) != 1):
-            raise ValueError(f"{name} must be a {dtype} ({B}, >= {columns}) tensor, rows contiguous")
-        if t.numel():
-            p[name] = t.data_ptr()
-        # (a row stride of 0 gives every row the same entries)
-        return t.stride(0) if B > 1 else t.shape[1], t.shape[1]
-
-    def vector(name, t, dtype):
-        if t is None:
-            return
-        _require_cuda(name, t)
-        _same_device(logits, t)
-        if t.dtype != dtype or t.shape != (B,) or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous {dtype} ({B},) tensor")
-        p[name] = t.data_ptr()
-
-    ld_history, n_history = matrix("history", history, torch.int32, 0)
-    ld_ids, n_bias = matrix("bias_ids", bias_ids, torch.int32, 0)
-    ld_bias, n_values = matrix("bias", bias, torch.float32, 0)
-    ld_mask, _ = matrix("mask", mask, torch.int32, (V + 31) // 32)
+    i32, f32 = torch.int32, torch.float32
+    h, ld_history, n_history = _matrix("history", history, i32, B, 0, dev)
+    ids, ld_ids, n_bias = _matrix("bias_ids", bias_ids, i32, B, 0, dev)
+    values, ld_bias, n_values = _matrix("bias", bias, f32, B, 0, dev)
+    m, ld_mask, _ = _matrix("mask", mask, i32, B, (V + 31) // 32, dev)
     if n_bias != n_values or ld_ids != ld_bias:
         raise ValueError("bias_ids and bias must have the same shape and strides")
-    if n_history:   # (an empty history has no penalties)
-        vector("lens", lens, torch.int32)
-        vector("prompt_lens", prompt_lens, torch.int32)
-        vector("repetition", repetition, torch.float32)
-        vector("frequency", frequency, torch.float32)
-        vector("presence", presence, torch.float32)
+    # (an empty history has no penalties)
+    lens, prompt_lens, repetition, frequency, presence = (
+        _vector(name, t, dtype, B, dev) if h else None for name, t, dtype in (
+            ("lens", lens, i32), ("prompt_lens", prompt_lens, i32),
+            ("repetition", repetition, f32), ("frequency", frequency, f32),
+            ("presence", presence, f32)))
     if out is None:
-        out = torch.empty((B, V), dtype=torch.float32, device=logits.device)
-    ld_out = _rows("out", out, B, V, logits)
-    if out.dtype != torch.float32:
-        raise TypeError("out must be float32")
-    tokens = torch.empty(B, dtype=torch.int32, device=logits.device) if choose else None
+        out = torch.empty((B, V), dtype=f32, device=logits.device)
+        ld_out = V
+    else:
+        ld_out = _rows("out", out, B, V, dev)
+        if out.dtype is not f32:
+            raise TypeError("out must be float32")
+    nbytes = _logits_rules_bytes(B, V) if choose else 0
+    tokens = at = None
+    if choose:
+        # the tokens, behind them the workspace, 8-byte aligned
+        tokens = torch.empty((B + 1) // 2 * 2 + nbytes // 4, dtype=i32, device=logits.device)
+        at = tokens.data_ptr()
+        tokens = tokens[:B]
     if B:
-        lib = _lib.load()
-        nbytes = lib.nb_logits_rules_ws_bytes(B, V) if choose else 0
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
-        g = p.get
-        _launch(logits, lib.nb_logits_rules, logits.data_ptr(), _DT[logits.dtype], ld, B, V,
-                g("history"), ld_history, n_history, g("lens"), g("prompt_lens"),
-                g("repetition"), g("frequency"), g("presence"), g("bias_ids"), g("bias"), ld_bias,
-                n_bias, g("mask"), ld_mask, out.data_ptr(), ld_out,
-                tokens.data_ptr() if choose else None, ws.data_ptr() if nbytes else None, nbytes)
+        _launch(dev, _lib.load().nb_logits_rules, logits.data_ptr(), _DT[logits.dtype], ld, B, V,
+                h, ld_history, n_history, lens, prompt_lens, repetition, frequency, presence,
+                ids, values, ld_bias, n_bias, m, ld_mask, out.data_ptr(), ld_out, at,
+                at + (B + 1) // 2 * 8 if nbytes else None, nbytes)
     return (out, tokens) if choose else out
+
+
+def _matrix(name, t, dtype, rows, columns, dev):
+    """(address, row stride, columns) of a rule's rows of at least `columns`;
+    a row stride of 0 gives all rows the same entries."""
+    if t is None:
+        return None, 0, 0
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == dev and
+            t.dtype is dtype and t.dim() == 2 and t.shape[0] == rows and t.shape[1] >= columns):
+        _require_cuda(name, t)
+        raise ValueError(f"{name} must be a {dtype} ({rows}, >= {columns}) tensor on cuda:{dev}, "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+    n = t.shape[1]
+    ld, step = t.stride()
+    if step != 1 and n > 1:
+        raise ValueError(f"{name}: rows must be contiguous")
+    if not n or not rows:
+        return None, 0, 0
+    return t.data_ptr(), ld if rows > 1 else n, n
+
+
+def _vector(name, t, dtype, rows, dev):
+    if t is None:
+        return None
+    if not _is(t, dtype, (rows,), dev):
+        _require(name, t, dtype, (rows,), dev)
+    return t.data_ptr()

@@ -102,7 +102,7 @@ def append(qkv, slots, positions, chunks, cos, sin, k, v, ks, vs, H):
                 old = np.float32(scale[block, h]) if before else np.float32(0)
                 m = np.abs(new)
                 top = np.float32(np.where(np.isnan(m), np.inf, m).max())
-                grown = np.maximum(old, top / np.float32(127))
+                grown = np.maximum(old, top * (np.float32(1) / np.float32(127)))
                 if before and grown > old:
                     cache[:before] = codes(cache[:before].astype(np.float32) * old, grown)
                 cache[before:before + count] = codes(new, grown)
