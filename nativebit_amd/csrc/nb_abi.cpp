@@ -1260,7 +1260,7 @@ int nb_kv8_append(const void* qkv, int qkv_dtype, int64_t ld_qkv, const int32_t*
     if (st) return st;
     st = check_rows(fn, "q_out", q_out, q_dtype, ld_q, (int64_t)n_head * head_dim);
     if (st) return st;
-    st = check_chunks(fn, chunks, n_chunks, 1);
+    st = check_chunks(fn, chunks, n_chunks, 3 * n_kv_head);
     if (st) return st;
     if (n_pos < 0) return fail(NB_EINVAL, "%s: n_pos=%d", fn, n_pos);
     if (!slots || !positions || !cos_t || !sin_t) return fail(NB_EINVAL, "%s: NULL pointer", fn);
@@ -1285,7 +1285,7 @@ int nb_kv8_read(const int32_t* slots, int64_t n, const int8_t* k, const int8_t* 
     if (st) return st;
     st = check_cache(fn, k, v, k_scale, v_scale, n_blocks, n_kv_head, head_dim);
     if (st || n == 0) return st;
-    if (n >= 1LL << 29) return fail(NB_EUNSUPPORTED, "%s: n=%lld", fn, (long long)n);
+    if (n >= 1LL << 28) return fail(NB_EUNSUPPORTED, "%s: n=%lld", fn, (long long)n);
     st = check_rows(fn, "keys", keys, dtype, 0, 0);
     if (st) return st;
     st = check_rows(fn, "values", values, dtype, 0, 0);
@@ -1358,7 +1358,8 @@ int nb_logits_rules(const void* logits, int dtype, int64_t ld, int rows, int V,
                     int64_t ld_mask, float* out, int64_t ld_out, int32_t* tokens, void* workspace,
                     int64_t ws_bytes, void* stream) {
     const char* fn = "nb_logits_rules";
-    if (rows < 0 || V < 1 || V > 0x7fffffff - 8) return fail(NB_EINVAL, "%s: rows=%d V=%d", fn, rows, V);
+    if (rows < 0 || V < 1) return fail(NB_EINVAL, "%s: rows=%d V=%d", fn, rows, V);
+    if (V > 1 << 30) return fail(NB_EUNSUPPORTED, "%s: V=%d", fn, V);
     if (rows > 65535) return fail(NB_EUNSUPPORTED, "%s: rows=%d (<= 65535)", fn, rows);
     if (rows == 0) return NB_OK;
     int st = check_rows(fn, "logits", logits, dtype, ld, V);

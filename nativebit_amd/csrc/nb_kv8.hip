@@ -78,10 +78,28 @@ __device__ __forceinline__ void store4(void* p, int dtype, int64_t i, f4 v, bool
     for (int e = 0; e < 4; ++e) d[e] = b[e];
 }
 
-// code of x at scale s (> 0, or 0 / +inf: code 0)
-__device__ __forceinline__ int code_of(float x, float s) {
-    if (!(s > 0.f && s < INFINITY)) return 0;
-    return (int)fminf(fmaxf(rintf(x / s), -127.f), 127.f);
+// A block's scale as the codes need it.
+struct Scale {
+    float s, inv;
+    bool usable;   // else (0 or +inf) codes are 0
+};
+__device__ __forceinline__ Scale scale_of(float s) {
+    // (with an infinite reciprocal all quotients divide: where 1 / s or s is no
+    // normal number)
+    const bool usable = s > 0.f && s < INFINITY;
+    return {s, s > 0x1p-120f && s < 0x1p120f ? __builtin_amdgcn_rcpf(s) : INFINITY, usable};
+}
+
+// clamp(rint(x / s), -127, 127).  x times the reciprocal is the quotient to
+// 2^-21 of it, under 2^-13 where it counts, so a product that is further than
+// that from the middle between two whole numbers rounds as the quotient does;
+// the others divide (about one in 10^4).
+__device__ __forceinline__ int code_of(float x, const Scale& s) {
+    if (!s.usable) return 0;
+    float q = x * s.inv;
+    float r = rintf(q);
+    if (!(fabsf(q - r) < 0.4995f)) r = rintf(x / s.s);
+    return (int)fminf(fmaxf(r, -127.f), 127.f);
 }
 
 __device__ __forceinline__ uint32_t pack_codes(const int* c) {
@@ -90,7 +108,7 @@ __device__ __forceinline__ uint32_t pack_codes(const int* c) {
 }
 
 // four codes at scale s again at scale s2
-__device__ __forceinline__ uint32_t rescale4(uint32_t w, float s, float s2) {
+__device__ __forceinline__ uint32_t rescale4(uint32_t w, float s, const Scale& s2) {
     int c[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) c[e] = code_of((float)(int8_t)(w >> (8 * e)) * s, s2);
@@ -99,13 +117,16 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float s, float s2) {
 
 // ---------------------------------------------------------------------------
 // append: a workgroup takes one chunk and, of one key / value head, its keys,
-// its values or the queries that share it.  A thread holds four consecutive
-// dims of every (256 / (D / 4))-th row of the chunk in registers between the
-// maximum and the codes.
+// its values or the queries that share it.  A thread takes four consecutive
+// dims of every (256 / (D / 4))-th row, all of whose loads are issued before
+// the first is used, and holds them in registers between the maximum and the
+// codes.
 // ---------------------------------------------------------------------------
 constexpr int kThreads = 256;
 constexpr int kMaxD = 256;
-constexpr int kMaxPass = kKvBlock * kMaxD / 4 / kThreads;
+// LDS row of a dim's new value codes: 17 dwords, so that the 16 dims that a
+// half row of lanes writes (4 apart) lie in 16 banks.
+constexpr int kVtPitch = kKvBlock + 4;
 
 struct AppendArgs {
     const void* qkv;
@@ -116,185 +137,308 @@ struct AppendArgs {
     float *k_scale, *v_scale;
     void* q_out;
     int64_t ld_q;
-    int qkv_dtype, q_dtype, vec_in, vec_q;
+    int qkv_dtype, q_dtype, vec_in, vec_q, vec_cos;
     int n_pos, n_blocks, n_tokens, n_head, n_kv, D;
     float q_scale;
 };
 
-// Pairs (x0, x1), (x2, x3) turned by the angles of dims d, d + 2 at position
-// pos: each product and sum rounded by itself, as nb_rope_kv_rows rounds them.
-// A position outside the tables has no angle: NaN.
-__device__ __forceinline__ f4 turn4(f4 x, const AppendArgs& a, int pos, int d) {
-    float c[2], s[2];
-    if (pos >= 0 && pos < a.n_pos) {
-        const int64_t o = (int64_t)pos * (a.D / 2) + d / 2;
-        c[0] = a.cos_t[o], c[1] = a.cos_t[o + 1];
-        s[0] = a.sin_t[o], s[1] = a.sin_t[o + 1];
+// Angles of dims d, d + 2 at a position; one outside the tables has none: NaN.
+struct Angles { float c[2], s[2]; };
+__device__ __forceinline__ Angles angles_at(const AppendArgs& a, int pos, int d) {
+    typedef __attribute__((ext_vector_type(2))) float f2;
+    Angles r;
+    const bool in = pos >= 0 && pos < a.n_pos;
+    const int64_t o = (int64_t)(in ? pos : 0) * (a.D / 2) + d / 2;
+    if (!in) {
+        r.c[0] = r.c[1] = r.s[0] = r.s[1] = __builtin_nanf("");
+    } else if (a.vec_cos) {
+        const f2 c = *reinterpret_cast<const f2*>(a.cos_t + o), s = *reinterpret_cast<const f2*>(a.sin_t + o);
+        r.c[0] = c[0], r.c[1] = c[1], r.s[0] = s[0], r.s[1] = s[1];
     } else {
-        c[0] = c[1] = s[0] = s[1] = __builtin_nanf("");
-    }
-    f4 r;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        const float x0 = x[2 * e], x1 = x[2 * e + 1];
-        r[2 * e] = x0 * c[e] - x1 * s[e];
-        r[2 * e + 1] = x1 * c[e] + x0 * s[e];
+        r.c[0] = a.cos_t[o], r.c[1] = a.cos_t[o + 1], r.s[0] = a.sin_t[o], r.s[1] = a.sin_t[o + 1];
     }
     return r;
 }
 
-__global__ __launch_bounds__(kThreads) void kv8_append_kernel(AppendArgs a) {
-    __shared__ float wave_max[kThreads / 64];
-    __shared__ __align__(16) uint8_t vt[kMaxD * kKvBlock];   // new value codes, as a block holds them
-    const int32_t* ch = a.chunks + 4 * (int64_t)blockIdx.x;
-    const int row0 = ch[0], n = ch[1];
-    const int h = blockIdx.y / 3, part = blockIdx.y % 3;   // 0 keys, 1 values, 2 queries
-    if (n <= 0 || row0 < 0 || row0 > a.n_tokens - n) return;
-    const int D = a.D, per = D / 4, rows = kThreads / per;
-    const int tr = threadIdx.x / per, d = 4 * (threadIdx.x - tr * per);
-    const bool on = tr < rows;
-    if (part == 2) {
-        const int G = a.n_head / a.n_kv;
-        if (!on) return;
-        for (int e = tr; e < n * G; e += rows) {
-            const int t = row0 + e / G, head = h * G + e % G;
-            if (a.slots[t] < 0) continue;
-            const f4 x = load4(a.qkv, a.qkv_dtype, t * a.ld_qkv + head * D + d, a.vec_in);
-            const f4 r = turn4(x, a, a.positions[t], d);
+// Pairs (x0, x1), (x2, x3) turned: each product and sum rounded by itself, as
+// nb_rope_kv_rows rounds them.
+__device__ __forceinline__ f4 turn4(f4 x, const Angles& w) {
+    f4 r;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const float x0 = x[2 * e], x1 = x[2 * e + 1];
+        r[2 * e] = x0 * w.c[e] - x1 * w.s[e];
+        r[2 * e + 1] = x1 * w.c[e] + x0 * w.s[e];
+    }
+    return r;
+}
+
+struct AppendChunk { int row0, n, block, before; };
+
+// The queries of a chunk's rows that share key / value head h, kRows of a
+// thread at once.
+template <int kRows>
+__device__ __forceinline__ void append_queries(const AppendArgs& a, const AppendChunk& ch, int h,
+                                               int tr, int d, int rows) {
+    const int G = a.n_head / a.n_kv, total = ch.n * G;
+    for (int e0 = tr; e0 < total; e0 += kRows * rows) {
+        f4 x[kRows];
+        int pos[kRows];
+        Angles w[kRows];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const int e = min(e0 + i * rows, total - 1);   // (past the last: the last again)
+            const int64_t t = ch.row0 + e / G;
+            pos[i] = a.positions[t];
+            x[i] = load4(a.qkv, a.qkv_dtype, t * a.ld_qkv + (h * G + e % G) * a.D + d, a.vec_in);
+        }
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) w[i] = angles_at(a, pos[i], d);
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const int e = e0 + i * rows;
+            if (e >= total) break;
+            const int64_t t = ch.row0 + e / G;
+            const f4 r = turn4(x[i], w[i]);
             f4 q;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) q[i] = r[i] * a.q_scale;
-            store4(a.q_out, a.q_dtype, t * a.ld_q + head * D + d, q, a.vec_q);
+            for (int j = 0; j < 4; ++j) q[j] = r[j] * a.q_scale;
+            store4(a.q_out, a.q_dtype, t * a.ld_q + (h * G + e % G) * a.D + d, q, a.vec_q);
         }
-        return;
     }
-    const int slot = a.slots[row0];
-    const int block = slot / kKvBlock, before = slot % kKvBlock;
-    if (slot < 0 || block >= a.n_blocks || before + n > kKvBlock) return;
-    const int64_t bh = (int64_t)block * a.n_kv + h;
-    const int64_t col = (int64_t)(a.n_head + part * a.n_kv + h) * D + d;
-    f4 x[kMaxPass];
+}
+
+// The keys (kKeys) or values of a chunk, kRows rows a thread.
+template <int kRows, bool kKeys>
+__device__ __forceinline__ void append_codes(const AppendArgs& a, const AppendChunk& ch, int h,
+                                             int tr, int d, int rows, float* wave_max, uint8_t* vt) {
+    const int D = a.D, n = ch.n, before = ch.before;
+    const bool on = tr < rows;
+    const int64_t bh = (int64_t)ch.block * a.n_kv + h;
+    const int64_t col = (int64_t)(a.n_head + (kKeys ? 0 : a.n_kv) + h) * D + d;
+    float* scale = (kKeys ? a.k_scale : a.v_scale) + bh;
+    const float s = before > 0 ? *scale : 0.f;
+    // keys: rows tr, tr + rows, ..; values: kRows consecutive ones, whose codes
+    // go to the transposed block by the dword
+    auto row_of = [&](int p) { return kKeys ? p * rows + tr : tr * kRows + p; };
+    f4 x[kRows];
+    int pos[kRows];
+#pragma unroll
+    for (int p = 0; p < kRows; ++p) {
+        const int64_t t = ch.row0 + min(row_of(p), n - 1);   // (past the last: the last again)
+        if (kKeys) pos[p] = a.positions[t];
+        x[p] = load4(a.qkv, a.qkv_dtype, t * a.ld_qkv + col, a.vec_in);
+    }
+    if (kKeys) {
+        constexpr int kBatch = kRows < 4 ? kRows : 4;
+#pragma unroll
+        for (int p0 = 0; p0 < kRows; p0 += kBatch) {
+            Angles w[kBatch];
+#pragma unroll
+            for (int p = 0; p < kBatch; ++p) w[p] = angles_at(a, pos[p0 + p], d);
+#pragma unroll
+            for (int p = 0; p < kBatch; ++p) x[p0 + p] = turn4(x[p0 + p], w[p]);
+        }
+    }
     float most = 0.f;
 #pragma unroll
-    for (int p = 0; p < kMaxPass; ++p) {
-        if (p * rows >= n) break;
-        const int i = p * rows + tr;
-        if (on && i < n) {
-            const int64_t t = row0 + i;
-            x[p] = load4(a.qkv, a.qkv_dtype, t * a.ld_qkv + col, a.vec_in);
-            if (part == 0) x[p] = turn4(x[p], a, a.positions[t], d);
+    for (int p = 0; p < kRows; ++p) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float m = fabsf(x[p][e]);
-                most = fmaxf(most, m < INFINITY ? m : INFINITY);   // (NaN counts as infinity)
-            }
+        for (int e = 0; e < 4; ++e) {
+            const float m = fabsf(x[p][e]);
+            most = fmaxf(most, m < INFINITY ? m : INFINITY);   // (NaN counts as infinity)
         }
     }
     most = wave64_max(most);
     if ((threadIdx.x & 63) == 0) wave_max[threadIdx.x >> 6] = most;
-    __syncthreads();
+    __syncthreads();   // (and every thread has the old scale)
     most = fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3]));
-    float* scale = (part == 0 ? a.k_scale : a.v_scale) + bh;
-    const float s = before > 0 ? *scale : 0.f;
-    const float s2 = fmaxf(s, most * (1.f / 127.f));
-    const bool again = before > 0 && s2 > s;   // the earlier codes change
-    __syncthreads();   // every thread has the old scale
-    if (threadIdx.x == 0 && (again || before == 0)) *scale = s2;
-    int8_t* codes = (part == 0 ? a.k : a.v) + bh * kKvBlock * D;
-    if (part == 0 && again) {
+    const float grown = fmaxf(s, most * (1.f / 127.f));
+    const bool again = before > 0 && grown > s;   // the earlier codes change
+    const Scale s2 = scale_of(grown);
+    if (threadIdx.x == 0 && (again || before == 0)) *scale = grown;
+    int8_t* codes = (kKeys ? a.k : a.v) + bh * kKvBlock * D;
+    if (kKeys && again) {
         uint32_t* w = reinterpret_cast<uint32_t*>(codes);
-        for (int i = threadIdx.x; i < before * per; i += kThreads) w[i] = rescale4(w[i], s, s2);
+        for (int i = threadIdx.x; i < before * (D / 4); i += kThreads) w[i] = rescale4(w[i], s, s2);
     }
+    if constexpr (kKeys) {
 #pragma unroll
-    for (int p = 0; p < kMaxPass; ++p) {
-        if (p * rows >= n) break;
-        const int i = p * rows + tr;
-        if (on && i < n) {
+        for (int p = 0; p < kRows; ++p) {
+            const int i = row_of(p);
+            if (!on || i >= n) continue;
             int c[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) c[e] = code_of(x[p][e], s2);
-            if (part == 0) {
-                *reinterpret_cast<uint32_t*>(codes + (before + i) * D + d) = pack_codes(c);
-            } else if (n == 1 && !again) {
+            *reinterpret_cast<uint32_t*>(codes + (before + i) * D + d) = pack_codes(c);
+        }
+        return;
+    }
+    if (n == 1 && !again) {   // a column of bytes
+        if (tr == 0) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) codes[(d + e) * kKvBlock + before] = (int8_t)c[e];
-            } else {
+            for (int e = 0; e < 4; ++e) codes[(d + e) * kKvBlock + before] = (int8_t)code_of(x[0][e], s2);
+        }
+        return;
+    }
+    // vt[dim][i]: the code of new row i
 #pragma unroll
-                for (int e = 0; e < 4; ++e) vt[(d + e) * kKvBlock + before + i] = (uint8_t)c[e];
+    for (int e = 0; e < 4; ++e) {
+        if (!on || row_of(0) >= n) break;
+        if constexpr (kRows % 4 == 0) {
+#pragma unroll
+            for (int p = 0; p < kRows; p += 4) {
+                int c[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) c[r] = code_of(x[p + r][e], s2);
+                *reinterpret_cast<uint32_t*>(&vt[(d + e) * kVtPitch + row_of(p)]) = pack_codes(c);
             }
+        } else {
+#pragma unroll
+            for (int p = 0; p < kRows; ++p) vt[(d + e) * kVtPitch + row_of(p)] = (uint8_t)code_of(x[p][e], s2);
         }
     }
-    if (part == 0 || (n == 1 && !again)) return;
-    // Values: 16 tokens of a dim at a time.  The block is this workgroup's
-    // alone, so a piece that is new in part is read, completed and written.
+    // 16 tokens of a dim at a time.  The block is this workgroup's alone, so a
+    // piece that is new in part is read, completed and written.
     __syncthreads();
     const int end = before + n;
     const int first = again ? 0 : before / 16, last = (end + 15) / 16;   // pieces of a dim
     for (int i = threadIdx.x; i < D * (last - first); i += kThreads) {
         const int dim = i / (last - first), j = 16 * (first + i - dim * (last - first));
         uint4* g = reinterpret_cast<uint4*>(codes + dim * kKvBlock + j);
-        const uint4 fresh = *reinterpret_cast<const uint4*>(&vt[dim * kKvBlock + j]);
-        uint32_t w[4] = {fresh.x, fresh.y, fresh.z, fresh.w};
-        if (j < before || j + 16 > end) {
+        const uint8_t* row = &vt[dim * kVtPitch];
+        uint32_t w[4];
+        if (before % 4 == 0 && j >= before && j + 16 <= end) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = *reinterpret_cast<const uint32_t*>(row + j - before + 4 * e);
+        } else {
             const uint4 held = *g;
             const uint32_t o[4] = {held.x, held.y, held.z, held.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                uint32_t fresh_bytes = 0, held_bytes = 0;   // of the new and of the earlier tokens
+                const int at = j + 4 * e;
+                const uint32_t old = again && at < before ? rescale4(o[e], s, s2) : o[e];
+                w[e] = 0;
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    const int at = j + 4 * e + b;
-                    fresh_bytes |= at >= before && at < end ? 255u << (8 * b) : 0u;
-                    held_bytes |= at < before ? 255u << (8 * b) : 0u;
+                    const uint32_t byte = at + b >= end      ? o[e] >> (8 * b)
+                                          : at + b >= before ? row[at + b - before]
+                                                             : old >> (8 * b);
+                    w[e] |= (byte & 255) << (8 * b);
                 }
-                const uint32_t old = again && held_bytes ? rescale4(o[e], s, s2) : o[e];
-                w[e] = (w[e] & fresh_bytes) | (old & held_bytes) | (o[e] & ~(fresh_bytes | held_bytes));
             }
         }
         *g = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
+template <int kRows>
+__device__ __forceinline__ void append_part(const AppendArgs& a, const AppendChunk& ch, int h,
+                                            int part, int tr, int d, int rows, float* wave_max,
+                                            uint8_t* vt) {
+    if (part == 0) append_codes<kRows, true>(a, ch, h, tr, d, rows, wave_max, vt);
+    else append_codes<kRows, false>(a, ch, h, tr, d, rows, wave_max, vt);
+}
+
+// kMost: head dims up to it (the most rows of a thread go by them).
+template <int kMost>
+__global__ __launch_bounds__(kThreads) void kv8_append_kernel(AppendArgs a) {
+    __shared__ float wave_max[kThreads / 64];
+    __shared__ __align__(16) uint8_t vt[kMost * kVtPitch];
+    // the parts and heads of a chunk vary fastest: together they read its rows whole
+    const int parts = 3 * a.n_kv;
+    const int chunk = blockIdx.x / parts, which = blockIdx.x - chunk * parts;
+    const int part = which / a.n_kv, h = which - part * a.n_kv;   // 0 keys, 1 values, 2 queries
+    const auto* c = as_constant(a.chunks) + 4 * (int64_t)chunk;
+    const int row0 = c[0], n = c[1];
+    if (n <= 0 || row0 < 0 || n > kKvBlock || row0 > a.n_tokens - n) return;
+    const int slot = as_constant(a.slots)[row0];
+    const AppendChunk ch{row0, n, slot / kKvBlock, slot % kKvBlock};
+    if (slot < 0 || ch.block >= a.n_blocks || ch.before + n > kKvBlock) return;
+    const int per = a.D / 4, rows = kThreads / per;
+    const int tr = threadIdx.x / per, d = 4 * (threadIdx.x - tr * per);
+    if (part == 2) {
+        if (tr >= rows) return;
+        if (n * (a.n_head / a.n_kv) <= rows) append_queries<1>(a, ch, h, tr, d, rows);
+        else append_queries<4>(a, ch, h, tr, d, rows);
+        return;
+    }
+    // rows of a thread: a single token's, or up to 64 / rows (rows >= 8 up to 128
+    // dims, >= 4 up to 256)
+    if (n <= rows) append_part<1>(a, ch, h, part, tr, d, rows, wave_max, vt);
+    else if (n <= 4 * rows) append_part<4>(a, ch, h, part, tr, d, rows, wave_max, vt);
+    else if (n <= 8 * rows) append_part<8>(a, ch, h, part, tr, d, rows, wave_max, vt);
+    else if constexpr (kMost > 128) append_part<16>(a, ch, h, part, tr, d, rows, wave_max, vt);
+}
+
 // ---------------------------------------------------------------------------
-// read: a workgroup takes 64 slots of one head.  Values pass through LDS: a
-// lane reads one slot's byte of a dim (slots of one block lie side by side),
-// and the rows are written whole.
+// read: a workgroup takes 32 slots of one head.  Values pass through LDS: half
+// a wave's lanes read the slots' bytes of a dim (slots of one block lie side by
+// side), and the rows are written whole.
 // ---------------------------------------------------------------------------
+constexpr int kReadSlots = 32;
+
 __global__ __launch_bounds__(kThreads) void kv8_read_kernel(
     const int32_t* slots, int64_t n, const int8_t* k, const int8_t* v, const float* k_scale,
     const float* v_scale, int n_blocks, int n_kv, int D, void* keys, void* values, int dtype,
     int vec) {
-    __shared__ int8_t vt[64][kMaxD + 4];   // (rows 65 dwords apart: a row a bank)
-    const int64_t i0 = blockIdx.x * 64LL;
+    __shared__ int8_t vt[kReadSlots][kMaxD + 4];   // (rows 65 dwords apart: a row a bank)
+    const int64_t i0 = (int64_t)blockIdx.x * kReadSlots;
     const int h = blockIdx.y;
-    const int count = (int)min((int64_t)64, n - i0);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int count = (int)min((int64_t)kReadSlots, n - i0);
+    const int lane = threadIdx.x % kReadSlots, half = threadIdx.x / kReadSlots;
+    constexpr int kHalves = kThreads / kReadSlots;
     const int mine = lane < count ? slots[i0 + lane] : -1;
-    if (mine >= 0 && mine / kKvBlock < n_blocks) {
-        const int8_t* g = v + ((int64_t)(mine / kKvBlock) * n_kv + h) * kKvBlock * D + mine % kKvBlock;
-        for (int d = wave; d < D; d += kThreads / 64) vt[lane][d] = g[d * kKvBlock];
+    const bool held = mine >= 0 && mine / kKvBlock < n_blocks;
+    const int8_t* g = v + ((int64_t)(held ? mine / kKvBlock : 0) * n_kv + h) * kKvBlock * D +
+                      (held ? mine % kKvBlock : 0);
+    // a thread's first rows of keys and scales, under way with the values
+    const int per = D / 4, rows = kThreads / per;
+    const int tr = threadIdx.x / per, d = 4 * (threadIdx.x - tr * per);
+    constexpr int kRows = 4;
+    uint32_t kw[kRows];
+    float ks[kRows], vs[kRows];
+    bool ok[kRows];
+    auto ask = [&](int t0) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const int slot = slots[i0 + min(t0 + i * rows, count - 1)];
+            ok[i] = slot >= 0 && slot / kKvBlock < n_blocks;
+            const int64_t bh = (int64_t)(ok[i] ? slot / kKvBlock : 0) * n_kv + h;
+            kw[i] = *reinterpret_cast<const uint32_t*>(
+                k + (bh * kKvBlock + (ok[i] ? slot % kKvBlock : 0)) * D + min(d, D - 4));
+            ks[i] = k_scale[bh], vs[i] = v_scale[bh];
+        }
+    };
+    ask(tr);
+    for (int d0 = half; d0 < D; d0 += 16 * kHalves) {   // 16 dims of a lane's slot at once
+        int8_t c[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) c[e] = g[min(d0 + kHalves * e, D - 1) * kKvBlock];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            if (d0 + kHalves * e < D) vt[lane][d0 + kHalves * e] = c[e];
+        }
     }
     __syncthreads();
-    const int per = D / 4;
-    for (int i = threadIdx.x; i < count * per; i += kThreads) {
-        const int t = i / per, d = 4 * (i - t * per);
-        const int slot = slots[i0 + t];
-        f4 kr = {0.f, 0.f, 0.f, 0.f}, vr = kr;
-        if (slot >= 0 && slot / kKvBlock < n_blocks) {
-            const int64_t bh = (int64_t)(slot / kKvBlock) * n_kv + h;
-            const uint32_t kw = *reinterpret_cast<const uint32_t*>(
-                k + (bh * kKvBlock + slot % kKvBlock) * D + d);
+    if (tr >= rows) return;
+    for (int t0 = tr; t0 < count; t0 += kRows * rows) {
+        if (t0 != tr) ask(t0);
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const int t = t0 + i * rows;
+            if (t >= count) break;
             const uint32_t vw = *reinterpret_cast<const uint32_t*>(&vt[t][d]);
-            const float ks = k_scale[bh], vs = v_scale[bh];
+            f4 kr, vr;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                kr[e] = (float)(int8_t)(kw >> (8 * e)) * ks;
-                vr[e] = (float)(int8_t)(vw >> (8 * e)) * vs;
+                kr[e] = ok[i] ? (float)(int8_t)(kw[i] >> (8 * e)) * ks[i] : 0.f;
+                vr[e] = ok[i] ? (float)(int8_t)(vw >> (8 * e)) * vs[i] : 0.f;
             }
+            const int64_t o = ((i0 + t) * n_kv + h) * D + d;
+            store4(keys, dtype, o, kr, vec);
+            store4(values, dtype, o, vr, vec);
         }
-        const int64_t o = ((i0 + t) * n_kv + h) * D + d;
-        store4(keys, dtype, o, kr, vec);
-        store4(values, dtype, o, vr, vec);
     }
 }
 
@@ -316,8 +460,9 @@ int launch_kv8_append(const void* qkv, int qkv_dtype, int64_t ld_qkv, const int3
                  q_out, ld_q, qkv_dtype, q_dtype,
                  four_aligned(qkv, qkv_dtype) && ld_qkv % 4 == 0,
                  four_aligned(q_out, q_dtype) && ld_q % 4 == 0,
+                 (reinterpret_cast<uintptr_t>(cos_t) | reinterpret_cast<uintptr_t>(sin_t)) % 8 == 0,
                  n_pos, n_blocks, n_tokens, n_head, n_kv, D, (float)(1.0 / sqrt((double)D))};
-    hipLaunchKernelGGL(kv8_append_kernel, dim3(n_chunks, 3 * n_kv), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(D <= 128 ? kv8_append_kernel<128> : kv8_append_kernel<kMaxD>, dim3((unsigned)n_chunks * 3 * n_kv), dim3(kThreads), 0, stream, a);
     return check_launch("nb_kv8_append");
 }
 
@@ -325,7 +470,7 @@ int launch_kv8_read(const int32_t* slots, int64_t n, const int8_t* k, const int8
                     const float* k_scale, const float* v_scale, int n_blocks, int n_kv, int D,
                     void* keys, void* values, int dtype, hipStream_t stream) {
     const int vec = four_aligned(keys, dtype) && four_aligned(values, dtype);
-    hipLaunchKernelGGL(kv8_read_kernel, dim3((unsigned)((n + 63) / 64), n_kv), dim3(kThreads), 0,
+    hipLaunchKernelGGL(kv8_read_kernel, dim3((unsigned)((n + kReadSlots - 1) / kReadSlots), n_kv), dim3(kThreads), 0,
                        stream, slots, n, k, v, k_scale, v_scale, n_blocks, n_kv, D, keys, values,
                        dtype, vec);
     return check_launch("nb_kv8_read");

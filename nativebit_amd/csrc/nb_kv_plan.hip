@@ -30,27 +30,36 @@ namespace nb {
 namespace {
 
 constexpr int kMaxRequests = 4096;
-constexpr int kWaves = 16;   // of the largest workgroup
+constexpr int kPlanThreads = 256;
 
-// Inclusive sum over the workgroup's threads; `total` its last value.
+// Inclusive sum over a wave's lanes, by row shifts and row broadcasts.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);   // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast 15 into rows 1, 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);   // row_bcast 31 into rows 2, 3
+    return v;
+}
+
+// Exclusive sum over the workgroup's threads; `total` that of all.
+template <int kWaves>
 __device__ __forceinline__ int block_scan(int v, int* wave_sums, int& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int sum = wave_scan(v);
     __syncthreads();   // the sums of an earlier call are read
-    if (lane == 63) wave_sums[wave] = v;
+    if (lane == 63) wave_sums[wave] = sum;
     __syncthreads();
     int before = 0, all = 0;
-    for (int w = 0; w < waves; ++w) {
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
         const int s = wave_sums[w];
         before += w < wave ? s : 0;
         all += s;
     }
     total = all;
-    return v + before;
+    return before + sum - v;
 }
 
 // The first of n ascending inclusive sums that is over i (n if none is).
@@ -76,51 +85,69 @@ __device__ __forceinline__ int blocks_of(int tokens) {
     return (int)(((int64_t)tokens + kKvBlock - 1) / kKvBlock);
 }
 
-__global__ __launch_bounds__(kWaves * 64) void kv_plan_kernel(PlanArgs a) {
-    __shared__ int rows_upto[kMaxRequests];     // inclusive sums over the requests: rows,
-    __shared__ int need_upto[kMaxRequests];     // blocks they need,
-    __shared__ int chunks_upto[kMaxRequests];   // chunks
+// kItems consecutive requests a thread.
+template <int kItems>
+__global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
+    constexpr int kMost = kItems * kPlanThreads, kWaves = kPlanThreads / 64;
+    __shared__ int rows_upto[kMost];     // inclusive sums over the requests: rows,
+    __shared__ int need_upto[kMost];     // blocks they need,
+    __shared__ int chunks_upto[kMost];   // chunks
     __shared__ int wave_sums[kWaves];
-    __shared__ unsigned long long asked_sum, stored_sum;
-    const int tid = threadIdx.x, nt = blockDim.x;
+    __shared__ long long wave_dropped[kWaves];
+    const int tid = threadIdx.x, nt = kPlanThreads;
     const int cap = a.max_blocks * kKvBlock;
     const int left = min(max(a.state[0], 0), a.n_blocks);
-    if (tid == 0) asked_sum = stored_sum = 0;
-    __syncthreads();
-    int rows = 0, need = 0, chunks = 0;   // of the requests before this strip
-    for (int r0 = 0; r0 < a.R; r0 += nt) {
-        const int r = r0 + tid;
-        const bool in = r < a.R;
-        const int len = in ? min(max(a.lens[r], 0), cap) : 0;
-        const int asked = in ? max(a.asked[r], 0) : 0;
-        int total;
-        // rows: what is asked, up to the rows that exist (clipped to n_tokens
-        // each, which changes no result and keeps the sums in 31 bits)
-        const int clipped = min(asked, a.n_tokens);
-        const int upto = rows + block_scan(clipped, wave_sums, total);
-        const int first = min(upto - clipped, a.n_tokens);
-        const int n = min(clipped, a.n_tokens - first);
-        rows += total;
-        const int have = blocks_of(len);
-        int end = (int)min((int64_t)len + n, (int64_t)cap);
-        const int want = blocks_of(end) - have;
-        const int base = need + block_scan(want, wave_sums, total) - want;
-        need += total;
-        const int got = min(want, max(left - base, 0));
-        end = max(len, min(end, (have + got) * kKvBlock));
-        const int c = end > len ? (end - 1) / kKvBlock - len / kKvBlock + 1 : 0;
-        const int cu = chunks + block_scan(c, wave_sums, total);
-        chunks += total;
-        if (in) {
-            rows_upto[r] = first + n;
-            need_upto[r] = base + want;
-            chunks_upto[r] = cu;
-            if (blockIdx.x == 0) {
-                a.lens_out[r] = end;
-                if (asked) atomicAdd(&asked_sum, (unsigned long long)asked);
-                if (end > len) atomicAdd(&stored_sum, (unsigned long long)(end - len));
-            }
-        }
+    const int r0 = tid * kItems;
+    int len[kItems], asked[kItems], n[kItems], want[kItems], count[kItems];
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+        const bool in = r0 + i < a.R;
+        len[i] = in ? min(max(a.lens[r0 + i], 0), cap) : 0;
+        asked[i] = in ? max(a.asked[r0 + i], 0) : 0;
+    }
+    // rows: what is asked, up to the rows that exist (clipped to n_tokens each,
+    // which changes no result and keeps the sums in 31 bits)
+    int sum = 0, total;
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) sum += min(asked[i], a.n_tokens);
+    int upto = block_scan<kWaves>(sum, wave_sums, total);
+    sum = 0;
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+        const int first = min(upto, a.n_tokens);
+        upto += min(asked[i], a.n_tokens);
+        n[i] = min(upto, a.n_tokens) - first;
+        rows_upto[r0 + i] = first + n[i];
+        want[i] = blocks_of((int)min((int64_t)len[i] + n[i], (int64_t)cap)) - blocks_of(len[i]);
+        sum += want[i];
+    }
+    long long dropped = 0;   // tokens asked for and not stored
+    int need;   // blocks of the step
+    upto = block_scan<kWaves>(sum, wave_sums, need);
+    sum = 0;
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+        const int have = blocks_of(len[i]), got = min(want[i], max(left - upto, 0));
+        upto += want[i];
+        need_upto[r0 + i] = upto;
+        int end = (int)min((int64_t)len[i] + n[i], (int64_t)cap);
+        end = max(len[i], min(end, (have + got) * kKvBlock));
+        count[i] = end > len[i] ? (end - 1) / kKvBlock - len[i] / kKvBlock + 1 : 0;
+        sum += count[i];
+        dropped += (long long)asked[i] - (end - len[i]);
+        if (blockIdx.x == 0 && r0 + i < a.R) a.lens_out[r0 + i] = end;
+    }
+    if (blockIdx.x == 0) {
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) dropped += __shfl_xor(dropped, d);
+        if ((tid & 63) == 0) wave_dropped[tid >> 6] = dropped;
+    }
+    int chunks;   // of the step
+    upto = block_scan<kWaves>(sum, wave_sums, chunks);
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+        upto += count[i];
+        chunks_upto[r0 + i] = upto;
     }
     __syncthreads();
     // what request r has stored after the step: its end, its blocks before it
@@ -178,18 +205,23 @@ __global__ __launch_bounds__(kWaves * 64) void kv_plan_kernel(PlanArgs a) {
     }
     if (id == 0) {
         a.state_out[0] = left - given;
-        a.state_out[1] = (int)min(asked_sum - stored_sum, 0x7fffffffULL);
+        dropped = 0;
+#pragma unroll
+        for (int w = 0; w < kPlanThreads / 64; ++w) dropped += wave_dropped[w];
+        a.state_out[1] = (int)min(dropped, 0x7fffffffLL);
     }
 }
 
+constexpr int kReleaseWaves = 16;
+
 // One workgroup: a wave counts the blocks of a finished request, their sum
 // over the requests says where each one's go, a wave copies them.
-__global__ __launch_bounds__(kWaves * 64) void kv_release_kernel(
+__global__ __launch_bounds__(kReleaseWaves * 64) void kv_release_kernel(
     int32_t* table, int64_t table_stride, int32_t* lens, const int32_t* finished,
     int32_t* free_blocks, int32_t* state, int R, int max_blocks, int n_blocks) {
     __shared__ int upto[kMaxRequests];
-    __shared__ int wave_sums[kWaves];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+    __shared__ int wave_sums[kReleaseWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = kReleaseWaves;
     const int left = min(max(state[0], 0), n_blocks);
     // the valid entries of a row, 64 at a time: f(bit set of valid lanes, entry)
     auto row = [&](int r, auto&& f) {
@@ -206,10 +238,11 @@ __global__ __launch_bounds__(kWaves * 64) void kv_release_kernel(
     }
     __syncthreads();
     int before = 0;
-    for (int r0 = 0; r0 < R; r0 += blockDim.x) {
+    for (int r0 = 0; r0 < R; r0 += kReleaseWaves * 64) {
         const int r = r0 + tid;
+        const int mine = r < R ? upto[r] : 0;
         int total;
-        const int sum = before + block_scan(r < R ? upto[r] : 0, wave_sums, total);
+        const int sum = before + mine + block_scan<kReleaseWaves>(mine, wave_sums, total);
         if (r < R) upto[r] = sum;
         before += total;
     }
@@ -239,16 +272,18 @@ int launch_kv_plan(int32_t* table, int64_t table_stride, const int32_t* lens,
                    hipStream_t stream) {
     const PlanArgs a{table, table_stride, lens, new_tokens, free_blocks, state, R, max_blocks,
                      n_blocks, n_tokens, n_chunks, slots, positions, chunks, lens_out, state_out};
-    const int threads = R <= 256 ? 256 : 1024;
-    const int groups = std::min(64, std::max(1, (n_tokens + 2 * threads - 1) / (2 * threads)));
-    hipLaunchKernelGGL(kv_plan_kernel, dim3(groups), dim3(threads), 0, stream, a);
+    const int groups = std::min(256, std::max(1, (n_tokens + kPlanThreads - 1) / kPlanThreads));
+    auto* kernel = R <= kPlanThreads ? kv_plan_kernel<1>
+                   : R <= 4 * kPlanThreads ? kv_plan_kernel<4>
+                                           : kv_plan_kernel<kMaxRequests / kPlanThreads>;
+    hipLaunchKernelGGL(kernel, dim3(groups), dim3(kPlanThreads), 0, stream, a);
     return check_launch("nb_kv_plan");
 }
 
 int launch_kv_release(int32_t* table, int64_t table_stride, int32_t* lens, const int32_t* finished,
                       int32_t* free_blocks, int32_t* state, int R, int max_blocks, int n_blocks,
                       hipStream_t stream) {
-    hipLaunchKernelGGL(kv_release_kernel, dim3(1), dim3(R <= 16 ? 256 : 1024), 0, stream, table,
+    hipLaunchKernelGGL(kv_release_kernel, dim3(1), dim3(kReleaseWaves * 64), 0, stream, table,
                        table_stride, lens, finished, free_blocks, state, R, max_blocks, n_blocks);
     return check_launch("nb_kv_release");
 }

@@ -10,12 +10,12 @@
 // each operation rounded by itself in fp32, and tokens[b] the lowest v with
 // the largest x (-1 where no x is over -inf; a NaN is never chosen).
 //
-// Bound by memory: one pass over the logits.  A workgroup takes 4096 tokens of
-// a row; it issues the loads of their logits, counts the row's history in an
-// LDS word per token (bit 31: seen, the rest: n) and notes the biases there
+// Bound by memory: one pass over the logits.  A workgroup takes 1024 or 2048
+// tokens of a row; it issues the loads of their logits, counts the row's history in an
+// LDS word per token and notes the biases beside it
 // while they are under way, so that neither counts nor dense biases exist in
 // memory.  Every workgroup of a row walks its whole history, from the L2:
-// against 32 KB of logits read and written, a history of 1000 is 4 KB.  LDS
+// against 16 KB of logits read and written, a history of 1000 is 4 KB.  LDS
 // atomics are on whole numbers (sums, or, maximum): no result depends on their
 // order.
 #include <math.h>
@@ -36,9 +36,15 @@ typedef __attribute__((ext_vector_type(4))) float f4;
 typedef __attribute__((ext_vector_type(4))) uint16_t h4;
 
 constexpr int kThreads = 256;
-constexpr int kLoads = 4;                          // groups of four tokens a thread
-constexpr int kTokens = 4 * kThreads * kLoads;     // of a workgroup
-constexpr uint32_t kSeen = 0x80000000u;
+// Tokens of a workgroup: one group of four for each thread up to 2^20 logits
+// (more workgroups, each sooner done), two above (half as many that walk a
+// history).  With histories of 700 to 1000, in us: 1 row of 50257 6.0 (two 7.0),
+// 8 rows 6.8 (7.7); 16 rows of 131077 10.3 (one 11.3), 160 rows 40.7 (50), with
+// histories of 4000 45 (57; four groups, with 32 KB of LDS, 52).
+constexpr int tokens_of(int loads) { return 4 * kThreads * loads; }
+int loads_of(int rows, int V) { return (int64_t)rows * V <= 1 << 20 ? 1 : 2; }
+// An LDS word per token: seen in the history, has a bias, times in the answer.
+constexpr uint32_t kSeen = 0x80000000u, kBias = 0x40000000u, kTimes = 0x3fffffffu;
 
 struct LogitsArgs {
     const void* logits;
@@ -75,10 +81,11 @@ __device__ __forceinline__ uint64_t wave_max(uint64_t key) {
 
 // kVec: input and output rows begin at the same place of a group of four
 // elements, so that all groups but a row's first and last move as vectors.
-template <bool kVec>
+template <bool kVec, int kLoads>
 __global__ __launch_bounds__(kThreads) void logits_rules_kernel(LogitsArgs a) {
-    __shared__ uint32_t count[kTokens];
-    __shared__ int32_t bias_at[kTokens];   // 1 + the place of the token's bias
+    constexpr int kTokens = tokens_of(kLoads);
+    __shared__ __align__(16) uint32_t count[kTokens];
+    __shared__ int32_t bias_at[kTokens];   // the place of the token's bias, where it has one
     __shared__ uint64_t wave_keys[kThreads / 64];
     const int b = blockIdx.y, tid = threadIdx.x;
     const int esize = a.dtype == NB_F32 ? 4 : 2;
@@ -86,16 +93,32 @@ __global__ __launch_bounds__(kThreads) void logits_rules_kernel(LogitsArgs a) {
     float* out = a.out + b * a.ld_out;
     // group q of four elements holds tokens 4 q - shift ..
     const int shift = kVec ? (int)(reinterpret_cast<uintptr_t>(in) / esize & 3) : 0;
-    const int64_t v0 = (int64_t)blockIdx.x * kTokens - shift;
+    const int v0 = (int)blockIdx.x * kTokens - shift;   // (V <= 2^30)
+    // everything that the row's rules read is asked for before it is used: the
+    // lengths, the first history entries and biases, the logits, the masks
+    const int32_t* hist = a.history ? a.history + b * a.ld_history : nullptr;
+    const int len = hist ? min(max(as_constant(a.lens)[b], 0), a.max_history) : 0;
+    const int prompt = hist && a.prompt_lens ? as_constant(a.prompt_lens)[b] : 0;
+    const float rep = a.repetition ? as_constant(a.repetition)[b] : 1.f;
+    const float freq = a.frequency ? as_constant(a.frequency)[b] : 0.f;
+    const float pres = a.presence ? as_constant(a.presence)[b] : 0.f;
+    constexpr int kBatch = 8;   // history entries of a thread under way at once
+    int ids[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+        ids[j] = a.max_history > 0 && hist ? hist[min(tid + j * kThreads, a.max_history - 1)] : -1;
+    }
+    const int bias_id = tid < a.n_bias ? a.bias_ids[b * a.ld_bias + tid] : -1;
     f4 x[kLoads];
+    uint32_t allowed[kLoads];   // bits of the group's four tokens
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
-        const int64_t v = v0 + 4 * (tid + j * kThreads);
+        const int v = v0 + 4 * (tid + j * kThreads);
         if (kVec && v >= 0 && v + 3 < a.V) {
             if (a.dtype == NB_F32) {
-                x[j] = *reinterpret_cast<const f4*>(in + 4 * v);
+                x[j] = *reinterpret_cast<const f4*>(in + 4 * (int64_t)v);
             } else {
-                const h4 w = *reinterpret_cast<const h4*>(in + 2 * v);
+                const h4 w = *reinterpret_cast<const h4*>(in + 2 * (int64_t)v);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[j][e] = bf16_to_f32(w[e]);
             }
@@ -108,58 +131,86 @@ __global__ __launch_bounds__(kThreads) void logits_rules_kernel(LogitsArgs a) {
                                               : bf16_to_f32(reinterpret_cast<const bf16_bits*>(in)[v + e]);
             }
         }
-    }
-    if (a.history) {
-        for (int i = tid; i < kTokens; i += kThreads) count[i] = 0;
-    }
-    if (a.n_bias) {
-        for (int i = tid; i < kTokens; i += kThreads) bias_at[i] = 0;
-    }
-    __syncthreads();
-    if (a.history) {
-        const int32_t* hist = a.history + b * a.ld_history;
-        const int len = min(max(a.lens[b], 0), a.max_history);
-        const int prompt = a.prompt_lens ? a.prompt_lens[b] : 0;
-        for (int i = tid; i < len; i += kThreads) {
-            const int id = hist[i];
-            const int64_t at = id - v0;
-            if (id >= 0 && id < a.V && at >= 0 && at < kTokens) {
-                if (i >= prompt) atomicAdd(&count[at], 1u);
-                else atomicOr(&count[at], kSeen);
-            }
+        allowed[j] = 15;
+        if (a.mask) {
+            const int32_t* mask = a.mask + b * a.ld_mask;
+            const int last = (a.V - 1) >> 5, w = max(v, 0) >> 5;
+            const uint32_t m0 = mask[min(w, last)];
+            // (a group that is not aligned may reach into the next word, a row's
+            // first may begin before token 0)
+            const uint32_t m1 = kVec ? mask[min(w + 1, last)] : 0;
+            const uint64_t m = (uint64_t)m1 << 32 | m0;
+            allowed[j] = v >= 0 ? (uint32_t)(m >> (v & 31)) : m0 << -v;
         }
     }
-    for (int i = tid; i < a.n_bias; i += kThreads) {
-        const int id = a.bias_ids[b * a.ld_bias + i];
-        const int64_t at = id - v0;
-        if (id >= 0 && id < a.V && at >= 0 && at < kTokens) atomicMax(&bias_at[at], i + 1);
+    const bool marked = hist || a.n_bias;   // whether there are words to look at
+    const uint4 none = make_uint4(0, 0, 0, 0);
+    if (marked) {
+        for (int i = tid; i < kTokens / 4; i += kThreads) reinterpret_cast<uint4*>(count)[i] = none;
     }
     __syncthreads();
-    const float rep = a.repetition ? a.repetition[b] : 1.f;
-    const float freq = a.frequency ? a.frequency[b] : 0.f;
-    const float pres = a.presence ? a.presence[b] : 0.f;
-    const int32_t* mask = a.mask ? a.mask + b * a.ld_mask : nullptr;
-    uint64_t best = 0;
+    // place of a token in this workgroup's, where it is under `span`
+    const int low = max(v0, 0);
+    const uint32_t span = (uint32_t)max(min(a.V, v0 + kTokens) - low, 0);
+    auto is_here = [&](int id) { return (uint32_t)(id - low) < span; };   // (id >= 0: low is)
+    for (int i0 = tid; i0 < len; i0 += kBatch * kThreads) {
+        int next[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {   // (past the end: the last again, unused)
+            next[j] = hist[min(i0 + (kBatch + j) * kThreads, len - 1)];
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const int i = i0 + j * kThreads;
+            if (is_here(ids[j]) && i < len) {
+                if (i >= prompt) atomicAdd(&count[ids[j] - v0], 1u);
+                else atomicOr(&count[ids[j] - v0], kSeen);
+            }
+            ids[j] = next[j];
+        }
+    }
+    auto id_of = [&](int i) { return i == tid ? bias_id : a.bias_ids[b * a.ld_bias + i]; };
+    for (int i = tid; i < a.n_bias; i += kThreads) {
+        const int id = id_of(i);
+        if (is_here(id)) atomicOr(&count[id - v0], kBias), bias_at[id - v0] = 0;
+    }
+    __syncthreads();
+    if (a.n_bias) {   // the last of a token's places
+        for (int i = tid; i < a.n_bias; i += kThreads) {
+            const int id = id_of(i);
+            if (is_here(id)) atomicMax(&bias_at[id - v0], i);
+        }
+        __syncthreads();
+    }
+    float best = -INFINITY;
+    int best_v = -1;
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
         const int at = 4 * (tid + j * kThreads);
-        const int64_t v = v0 + at;
+        const int v = v0 + at;
+        uint4 c4 = none;
+        if (marked) c4 = *reinterpret_cast<const uint4*>(&count[at]);
+        // the marked tokens of the group, one a turn: few lanes have any, hardly
+        // one has two
+        uint32_t left = (c4.x ? 1 : 0) | (c4.y ? 2 : 0) | (c4.z ? 4 : 0) | (c4.w ? 8 : 0);
+        while (left) {
+            const int e = __ffs((int)left) - 1;
+            left &= left - 1;
+            const uint32_t c = e < 2 ? (e ? c4.y : c4.x) : (e == 2 ? c4.z : c4.w);
+            float y = e < 2 ? (e ? x[j][1] : x[j][0]) : (e == 2 ? x[j][2] : x[j][3]);
+            const uint32_t n = c & kTimes;
+            if (n || c & kSeen) y = y > 0.f ? y / rep : y * rep;
+            if (n) y = (y - freq * (float)n) - pres;
+            if (c & kBias) y = y + a.bias[b * a.ld_bias + bias_at[at + e]];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[j][i] = e == i ? y : x[j][i];
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            if (v + e < 0 || v + e >= a.V) continue;
-            float y = x[j][e];
-            const uint32_t c = a.history ? count[at + e] : 0;
-            if (c) {
-                y = y > 0.f ? y / rep : y * rep;
-                const uint32_t n = c & ~kSeen;
-                if (n) y = (y - freq * (float)n) - pres;
-            }
-            const int i = a.n_bias ? bias_at[at + e] : 0;
-            if (i) y = y + a.bias[b * a.ld_bias + i - 1];
-            if (mask && !((uint32_t)mask[(v + e) >> 5] >> ((v + e) & 31) & 1)) y = -INFINITY;
+            const float y = allowed[j] >> e & 1 ? x[j][e] : -INFINITY;
             x[j][e] = y;
-            const uint64_t key = key_of(y, (int)(v + e));
-            best = key > best ? key : best;
+            const bool in_row = v + e >= 0 && v + e < a.V;
+            if (y > best && in_row) best = y, best_v = v + e;   // (a NaN is not over it)
         }
         if (kVec && v >= 0 && v + 3 < a.V) {
             *reinterpret_cast<f4*>(out + v) = x[j];
@@ -171,13 +222,13 @@ __global__ __launch_bounds__(kThreads) void logits_rules_kernel(LogitsArgs a) {
         }
     }
     if (!a.tokens) return;
-    best = wave_max(best);
-    if ((tid & 63) == 0) wave_keys[tid >> 6] = best;
+    uint64_t key = wave_max(key_of(best, best_v));
+    if ((tid & 63) == 0) wave_keys[tid >> 6] = key;
     __syncthreads();
     if (tid == 0) {
-        for (int w = 1; w < kThreads / 64; ++w) best = wave_keys[w] > best ? wave_keys[w] : best;
-        if (gridDim.x == 1) a.tokens[b] = token_of(best);
-        else a.keys[(int64_t)b * gridDim.x + blockIdx.x] = best;
+        for (int w = 1; w < kThreads / 64; ++w) key = wave_keys[w] > key ? wave_keys[w] : key;
+        if (gridDim.x == 1) a.tokens[b] = token_of(key);
+        else a.keys[(int64_t)b * gridDim.x + blockIdx.x] = key;
     }
 }
 
@@ -194,12 +245,15 @@ __global__ __launch_bounds__(64) void logits_choose_kernel(const uint64_t* keys,
 }
 
 // One workgroup more where a row's first group is not whole.
-int parts_of(int V) { return (int)(((int64_t)V + 3 + kTokens - 1) / kTokens); }
+int parts_of(int rows, int V) {
+    const int tokens = tokens_of(loads_of(rows, V));
+    return (int)(((int64_t)V + 3 + tokens - 1) / tokens);
+}
 
 }  // namespace
 
 int64_t logits_rules_bytes(int rows, int V) {
-    const int parts = parts_of(V);
+    const int parts = parts_of(rows, V);
     return parts == 1 ? 0 : (int64_t)rows * parts * 8;
 }
 
@@ -214,11 +268,13 @@ int launch_logits_rules(const void* logits, int dtype, int64_t ld, int rows, int
                        prompt_lens, repetition, frequency, presence, bias_ids, bias, mask, out,
                        static_cast<uint64_t*>(workspace), tokens, dtype, V, max_history, n_bias};
     const int esize = dtype == NB_F32 ? 4 : 2;
-    const int parts = parts_of(V);
+    const int parts = parts_of(rows, V);
     const bool vec = ((reinterpret_cast<uintptr_t>(logits) / esize) & 3) ==
                          ((reinterpret_cast<uintptr_t>(out) / 4) & 3) && (ld - ld_out) % 4 == 0;
-    hipLaunchKernelGGL(vec ? logits_rules_kernel<true> : logits_rules_kernel<false>,
-                       dim3(parts, rows), dim3(kThreads), 0, stream, a);
+    auto* kernel = loads_of(rows, V) == 1
+                       ? (vec ? logits_rules_kernel<true, 1> : logits_rules_kernel<false, 1>)
+                       : (vec ? logits_rules_kernel<true, 2> : logits_rules_kernel<false, 2>);
+    hipLaunchKernelGGL(kernel, dim3(parts, rows), dim3(kThreads), 0, stream, a);
     if (tokens && parts > 1) {
         hipLaunchKernelGGL(logits_choose_kernel, dim3(rows), dim3(64), 0, stream,
                            a.keys, parts, tokens);

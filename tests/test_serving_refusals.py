@@ -169,8 +169,9 @@ def test_workspaces():
     assert lib.nb_kv8_attention_ws_bytes(5, 5, 8, 20, 20, 128) == 0          # short caches
     nbytes = lib.nb_kv8_attention_ws_bytes(6, 6, 626, 32, 8, 128)            # few long ones
     assert nbytes > 0 and nbytes % (6 * 32 * 130 * 4) == 0
-    assert lib.nb_logits_rules_ws_bytes(3, 100) == 0
-    assert lib.nb_logits_rules_ws_bytes(3, 50257) == 3 * 13 * 8
+    assert lib.nb_logits_rules_ws_bytes(3, 1000) == 0
+    assert lib.nb_logits_rules_ws_bytes(300, 50257) == 300 * 25 * 8
+    assert lib.nb_logits_rules_ws_bytes(1, 50257) == 50 * 8
 
 
 def test_wrappers_refuse_host_tensors():
