@@ -29,7 +29,9 @@ ctx) storage -- the layout the attention kernels read, 64 consecutive
 positions per wave load -- so indexing them as the reference does
 (``k_buf[:, :, :n]``) gives positions.  A cache built by the caller in the
 reference's contiguous layout is accepted too: its keys are copied into the
-kernel layout for the call and the new positions written back.
+kernel layout for the call and the new positions written back.  A
+``nativebit_amd.paged.PagedCache`` in their place holds several requests of
+different lengths in 8-bit blocks.
 """
 from __future__ import annotations
 
@@ -43,6 +45,7 @@ import torch.nn as nn
 from . import _lib, formats, synth
 from .linear import PackedLinear
 from .ops import _stream
+from .paged import PagedCache, PagedLayer
 
 
 @dataclass
@@ -175,7 +178,9 @@ class CausalAttention(nn.Module):
     length + T - 1 and attend to the cache, which is extended (pos_offset is
     ignored, as in the reference); without one the T tokens attend causally
     to each other only, rotated at positions pos_offset .. pos_offset + T - 1
-    (the reference's scaled_dot_product_attention branch)."""
+    (the reference's scaled_dot_product_attention branch).  With a layer of a
+    PagedCache the B * T rows are the tokens of its planned step, of several
+    requests (nb_kv8_append, nb_kv8_attention)."""
 
     def __init__(self, n_embd, n_head, context_len, make_linear, rope_theta=10000.0):
         super().__init__()
@@ -198,6 +203,9 @@ class CausalAttention(nn.Module):
         if qkv.shape != (B, T, 3 * C):
             qkv = qkv.reshape(B, T, 3 * C)
         cos, sin = _f32(self.cos.to(dev)), _f32(self.sin.to(dev))
+        if isinstance(kv_cache, PagedLayer):
+            att = kv_cache.attend(qkv.view(B * T, 3 * C), cos, sin, H)
+            return self.out_proj(att.view(B, T, C)), kv_cache
         if kv_cache is not None:
             k_buf, v_buf, pos0 = kv_cache
             pos0 = int(pos0)
@@ -331,19 +339,32 @@ class PackedGPT(nn.Module):
                    make_linear, norm_eps=c.norm_eps, rope_theta=c.rope_theta,
                    block_size=c.block_size, n_entries=c.n_entries, device=device)
 
-    @torch.no_grad()
-    def forward(self, idx, kv_caches=None, pos_offset=0):
-        """Logits (B, T, vocab) fp32 of tokens idx (B, T); with kv_caches
-        (from init_kv_cache) the caches are read and extended and the new
-        caches are returned too."""
+    def hidden(self, idx, kv_caches=None, pos_offset=0):
+        """The blocks' outputs (B, T, n_embd) of tokens idx, before the final
+        norm, and the new caches."""
         x = self.embedding(idx)
         caches = []
         for i, block in enumerate(self.blocks):
             x, c = block(x, kv_caches[i] if kv_caches is not None else None, pos_offset)
             caches.append(c)
+        return x, caches
+
+    def head(self, x):
+        """The final norm and the tied, soft-capped head: fp32 logits."""
         h = self.ln_f(x)
         emb = self.embedding.weight
-        logits = 30.0 * torch.tanh((h.to(emb.dtype) @ emb.T).float() / 30.0)
+        return 30.0 * torch.tanh((h.to(emb.dtype) @ emb.T).float() / 30.0)
+
+    @torch.no_grad()
+    def forward(self, idx, kv_caches=None, pos_offset=0):
+        """Logits (B, T, vocab) fp32 of tokens idx (B, T); with kv_caches
+        (from init_kv_cache) the caches are read and extended and the new
+        caches are returned too.  A PagedCache with a planned step takes the
+        step's tokens, of several requests, for idx (one row of all of them)."""
+        x, caches = self.hidden(idx, kv_caches, pos_offset)
+        logits = self.head(x)
+        if isinstance(kv_caches, PagedCache):
+            return logits, kv_caches
         return (logits, caches) if kv_caches is not None else logits
 
 

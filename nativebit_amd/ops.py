@@ -528,22 +528,20 @@ class KVPlan(NamedTuple):
 
 
 def _is(t, dtype, shape, dev) -> bool:
-    """t is a contiguous GPU tensor of this type, shape and device: the check
-    of a call's usual arguments.  Where it fails, the slower ones below say
-    what is wrong."""
-    return (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and
-            t.get_device() == dev and t.is_cuda and t.is_contiguous())
+    """t is a contiguous GPU tensor of this type, shape and device (>= 0: host
+    tensors are on -1): the check of a call's usual arguments.  Where it fails,
+    ``_require`` says what is wrong."""
+    try:
+        return (t.dtype is dtype and t.shape == shape and t.get_device() == dev and
+                t.is_contiguous())
+    except AttributeError:
+        return False
 
 
-def _launch(dev: int, fn, *args):
-    """fn(*args, stream) on GPU dev and torch's current stream there."""
-    if dev == torch._C._cuda_getDevice():
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    else:
-        with torch.cuda.device(dev):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    if status:
-        _lib.check(status)
+def _here(dev: int) -> bool:
+    """Whether GPU dev is the current device, which the kernels are launched
+    on (a wrapper calls itself again under it where it is not)."""
+    return dev == torch._C._cuda_getDevice()
 
 
 def _require(name: str, t, dtype, shape, dev):
@@ -587,6 +585,9 @@ def kv_plan(table: torch.Tensor, lens: torch.Tensor, new: torch.Tensor, free: to
     slot).  ``lens`` and ``state`` are left as they are; the plan's are those
     after the step.  ``out``: a plan of the same sizes to write."""
     dev, R, width, stride = _table(table)
+    if not _here(dev):
+        with torch.cuda.device(dev):
+            return kv_plan(table, lens, new, free, state, n_tokens, out)
     n_tokens = int(n_tokens)
     i32, n_blocks = torch.int32, free.numel()
     if not (_is(lens, i32, (R,), dev) and _is(new, i32, (R,), dev) and
@@ -602,9 +603,12 @@ def kv_plan(table: torch.Tensor, lens: torch.Tensor, new: torch.Tensor, free: to
         buf = torch.empty(4 * chunks + 2 * n_tokens + R + 2, dtype=i32, device=table.device)
         c, s, p, l, st = buf.split_with_sizes([4 * chunks, n_tokens, n_tokens, R, 2])
         out = KVPlan(s, p, c.view(chunks, 4), l, st)
-        at = buf.data_ptr()     # the parts' places, in the order of the split
-        c, s, p, l, st = at, at + 16 * chunks, at + 16 * chunks + 4 * n_tokens, \
-            at + 16 * chunks + 8 * n_tokens, at + 16 * chunks + 8 * n_tokens + 4 * R
+        # the parts' places, in the order of the split
+        c = buf.data_ptr()
+        s = c + 16 * chunks
+        p = s + 4 * n_tokens
+        l = p + 4 * n_tokens
+        st = l + 4 * R
     else:
         for name, t, shape in (("slots", out.slots, (n_tokens,)),
                                ("positions", out.positions, (n_tokens,)),
@@ -612,8 +616,12 @@ def kv_plan(table: torch.Tensor, lens: torch.Tensor, new: torch.Tensor, free: to
                                ("state", out.state, (2,))):
             _require(f"out.{name}", t, i32, shape, dev)
         s, p, c, l, st = (t.data_ptr() for t in out)
-    _launch(dev, _lib.load().nb_kv_plan, table.data_ptr(), stride, lens.data_ptr(), new.data_ptr(),
-            free.data_ptr(), state.data_ptr(), R, width, n_blocks, n_tokens, s, p, c, l, st)
+    status = _lib.load().nb_kv_plan(
+        table.data_ptr(), stride, lens.data_ptr(), new.data_ptr(), free.data_ptr(),
+        state.data_ptr(), R, width, n_blocks, n_tokens, s, p, c, l, st,
+        torch._C._cuda_getCurrentRawStream(dev))
+    if status:
+        _lib.check(status)
     return out
 
 
@@ -623,12 +631,16 @@ def kv_release(table: torch.Tensor, lens: torch.Tensor, finished: torch.Tensor,
     list, their lengths 0 and table entries -1, all in place
     (nb_kv_release)."""
     dev, R, width, stride = _table(table)
+    if not _here(dev):
+        with torch.cuda.device(dev):
+            return kv_release(table, lens, finished, free, state)
     _require("lens", lens, torch.int32, (R,), dev)
     _require("finished", finished, torch.int32, (R,), dev)
     _require("free", free, torch.int32, (None,), dev)
     _require("state", state, torch.int32, (2,), dev)
-    _launch(dev, _lib.load().nb_kv_release, table.data_ptr(), stride, lens.data_ptr(),
-            finished.data_ptr(), free.data_ptr(), state.data_ptr(), R, width, free.numel())
+    _lib.check(_lib.load().nb_kv_release(
+        table.data_ptr(), stride, lens.data_ptr(), finished.data_ptr(), free.data_ptr(),
+        state.data_ptr(), R, width, free.numel(), torch._C._cuda_getCurrentRawStream(dev)))
 
 
 def _kv8_cache(k, v, k_scale, v_scale):
@@ -638,7 +650,7 @@ def _kv8_cache(k, v, k_scale, v_scale):
     if k.dim() != 4:
         raise ValueError(f"k must be (blocks, heads, {KV_BLOCK}, head_dim), got {tuple(k.shape)}")
     dev = k.get_device()
-    n, h, block, d = k.shape
+    n, h, _, d = k.shape
     if not (_is(k, torch.int8, (n, h, KV_BLOCK, d), dev) and
             _is(v, torch.int8, (n, h, d, KV_BLOCK), dev) and
             _is(k_scale, torch.float32, (n, h), dev) and _is(v_scale, torch.float32, (n, h), dev)):
@@ -676,6 +688,9 @@ def kv8_append(qkv: torch.Tensor, plan: KVPlan, cos: torch.Tensor, sin: torch.Te
     Returns the turned queries times head_dim^-0.5, (rows, n_head head_dim) in
     qkv's dtype (or into ``q``); rows without a slot are not written."""
     dev, n_blocks, n_kv, D = _kv8_cache(k, v, k_scale, v_scale)
+    if not _here(dev):
+        with torch.cuda.device(dev):
+            return kv8_append(qkv, plan, cos, sin, k, v, k_scale, v_scale, n_head, q)
     n_head, i32 = int(n_head), torch.int32
     width = (n_head + 2 * n_kv) * D
     if qkv.dim() != 2:
@@ -697,11 +712,14 @@ def kv8_append(qkv: torch.Tensor, plan: KVPlan, cos: torch.Tensor, sin: torch.Te
     else:
         ld_q = _rows("q", q, n, n_head * D, dev)
     if n:
-        _launch(dev, _lib.load().nb_kv8_append, qkv.data_ptr(), _DT[qkv.dtype], ld,
-                plan.slots.data_ptr(), plan.positions.data_ptr(), chunks.data_ptr(),
-                chunks.shape[0], cos.data_ptr(), sin.data_ptr(), n_pos, k.data_ptr(),
-                v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_blocks, q.data_ptr(),
-                _DT[q.dtype], ld_q, n, n_head, n_kv, D)
+        status = _lib.load().nb_kv8_append(
+            qkv.data_ptr(), _DT[qkv.dtype], ld, plan.slots.data_ptr(), plan.positions.data_ptr(),
+            chunks.data_ptr(), chunks.shape[0], cos.data_ptr(), sin.data_ptr(), n_pos,
+            k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_blocks,
+            q.data_ptr(), _DT[q.dtype], ld_q, n, n_head, n_kv, D,
+            torch._C._cuda_getCurrentRawStream(dev))
+        if status:
+            _lib.check(status)
     return q
 
 
@@ -711,16 +729,23 @@ def kv8_read(slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: tor
     ``slots`` (n,); zeros for slots outside it, -1 among them
     (nb_kv8_read)."""
     dev, n_blocks, n_kv, D = _kv8_cache(k, v, k_scale, v_scale)
-    _require("slots", slots, torch.int32, (None,), dev)
+    if not _here(dev):
+        with torch.cuda.device(dev):
+            return kv8_read(slots, k, v, k_scale, v_scale, dtype)
+    if not _is(slots, torch.int32, (len(slots),), dev):
+        _require("slots", slots, torch.int32, (None,), dev)
     if dtype not in _DT:
         raise TypeError(f"dtype {dtype} not supported (float32 or bfloat16)")
     n = slots.shape[0]
     keys = torch.empty((n, n_kv, D), dtype=dtype, device=k.device)
-    values = torch.empty_like(keys)
+    values = torch.empty((n, n_kv, D), dtype=dtype, device=k.device)
     if n:
-        _launch(dev, _lib.load().nb_kv8_read, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(),
-                k_scale.data_ptr(), v_scale.data_ptr(), n_blocks, n_kv, D, keys.data_ptr(),
-                values.data_ptr(), _DT[dtype])
+        status = _lib.load().nb_kv8_read(
+            slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(),
+            v_scale.data_ptr(), n_blocks, n_kv, D, keys.data_ptr(), values.data_ptr(), _DT[dtype],
+            torch._C._cuda_getCurrentRawStream(dev))
+        if status:
+            _lib.check(status)
     return keys, values
 
 
@@ -739,6 +764,11 @@ def kv8_attention(q: torch.Tensor, plan: KVPlan, table: torch.Tensor, k: torch.T
     q's dtype or ``out_dtype`` (or into ``out``); rows without a slot are not
     written."""
     dev, n_blocks, n_kv, D = _kv8_cache(k, v, k_scale, v_scale)
+    if not _here(dev):
+        with torch.cuda.device(dev):
+            return kv8_attention(q, plan, table, k, v, k_scale, v_scale, softcap=softcap,
+                                 window=window, slopes=slopes, prefix=prefix, out=out,
+                                 out_dtype=out_dtype)
     table_dev, R, width, stride = _table(table)
     if q.dim() != 2 or q.shape[1] == 0 or q.shape[1] % (n_kv * D):
         raise ValueError(f"q must be (rows, heads * {D}), heads a multiple of {n_kv}")
@@ -767,21 +797,23 @@ def kv8_attention(q: torch.Tensor, plan: KVPlan, table: torch.Tensor, k: torch.T
     if n:
         nbytes = _kv8_attention_bytes(dev, n, n_chunks, width, n_head, n_kv, D)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-        _launch(dev, _lib.load().nb_kv8_attention, q.data_ptr(), _DT[q.dtype], ld_q,
-                chunks.data_ptr(), n_chunks, plan.lens.data_ptr(), table.data_ptr(), stride, R,
-                width, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                n_blocks, out.data_ptr(), _DT[out.dtype], ld_out, n, n_head, n_kv, D,
-                softcap, window, slopes.data_ptr() if slopes is not None else None,
-                prefix.data_ptr() if prefix is not None else None,
-                ws.data_ptr() if nbytes else None, nbytes)
+        status = _lib.load().nb_kv8_attention(
+            q.data_ptr(), _DT[q.dtype], ld_q, chunks.data_ptr(), n_chunks, plan.lens.data_ptr(),
+            table.data_ptr(), stride, R, width, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(),
+            v_scale.data_ptr(), n_blocks, out.data_ptr(), _DT[out.dtype], ld_out, n, n_head, n_kv,
+            D, softcap, window, None if slopes is None else slopes.data_ptr(),
+            None if prefix is None else prefix.data_ptr(), ws.data_ptr() if nbytes else None,
+            nbytes, torch._C._cuda_getCurrentRawStream(dev))
+        if status:
+            _lib.check(status)
     return out
 
 
 @functools.lru_cache(maxsize=256)
 def _kv8_attention_bytes(dev, *sizes) -> int:
-    """Workspace bytes of nb_kv8_attention on GPU dev (they go by its CUs)."""
-    with torch.cuda.device(dev):
-        return int(_lib.load().nb_kv8_attention_ws_bytes(*sizes))
+    """Workspace bytes of nb_kv8_attention on GPU dev, the current one (they
+    go by its CUs)."""
+    return int(_lib.load().nb_kv8_attention_ws_bytes(*sizes))
 
 
 @functools.lru_cache(maxsize=256)
@@ -810,6 +842,11 @@ def logits_rules(logits: torch.Tensor, *, history: torch.Tensor | None = None,
         raise ValueError(f"logits must be (B, V), got {tuple(logits.shape)}")
     B, V = logits.shape
     dev = logits.get_device()
+    if not _here(dev):
+        with torch.cuda.device(dev):
+            return logits_rules(logits, history=history, lens=lens, prompt_lens=prompt_lens,
+                                repetition=repetition, frequency=frequency, presence=presence,
+                                bias_ids=bias_ids, bias=bias, mask=mask, out=out, choose=choose)
     ld = _rows("logits", logits, B, V, dev)
     if (history is None) != (lens is None):
         raise ValueError("history and lens go together")
@@ -819,18 +856,24 @@ def logits_rules(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     if (bias_ids is None) != (bias is None):
         raise ValueError("bias_ids and bias go together")
     i32, f32 = torch.int32, torch.float32
-    h, ld_history, n_history = _matrix("history", history, i32, B, 0, dev)
-    ids, ld_ids, n_bias = _matrix("bias_ids", bias_ids, i32, B, 0, dev)
-    values, ld_bias, n_values = _matrix("bias", bias, f32, B, 0, dev)
-    m, ld_mask, _ = _matrix("mask", mask, i32, B, (V + 31) // 32, dev)
-    if n_bias != n_values or ld_ids != ld_bias:
-        raise ValueError("bias_ids and bias must have the same shape and strides")
-    # (an empty history has no penalties)
-    lens, prompt_lens, repetition, frequency, presence = (
-        _vector(name, t, dtype, B, dev) if h else None for name, t, dtype in (
-            ("lens", lens, i32), ("prompt_lens", prompt_lens, i32),
-            ("repetition", repetition, f32), ("frequency", frequency, f32),
-            ("presence", presence, f32)))
+    h = ids = values = m = None
+    ld_history = n_history = ld_bias = n_bias = ld_mask = 0
+    if history is not None:
+        h, ld_history, n_history = _matrix("history", history, i32, B, 0, dev)
+        lens = _vector("lens", lens, i32, B, dev)
+        prompt_lens = _vector("prompt_lens", prompt_lens, i32, B, dev)
+        repetition = _vector("repetition", repetition, f32, B, dev)
+        frequency = _vector("frequency", frequency, f32, B, dev)
+        presence = _vector("presence", presence, f32, B, dev)
+        if not h:   # (an empty history has no penalties)
+            lens = prompt_lens = repetition = frequency = presence = None
+    if bias_ids is not None:
+        ids, ld_bias, n_bias = _matrix("bias_ids", bias_ids, i32, B, 0, dev)
+        values, ld_values, n_values = _matrix("bias", bias, f32, B, 0, dev)
+        if n_bias != n_values or ld_bias != ld_values:
+            raise ValueError("bias_ids and bias must have the same shape and strides")
+    if mask is not None:
+        m, ld_mask, _ = _matrix("mask", mask, i32, B, (V + 31) // 32, dev)
     if out is None:
         out = torch.empty((B, V), dtype=f32, device=logits.device)
         ld_out = V
@@ -838,28 +881,30 @@ def logits_rules(logits: torch.Tensor, *, history: torch.Tensor | None = None,
         ld_out = _rows("out", out, B, V, dev)
         if out.dtype is not f32:
             raise TypeError("out must be float32")
-    nbytes = _logits_rules_bytes(B, V) if choose else 0
-    tokens = at = None
+    tokens = ws = None
+    nbytes = 0
     if choose:
-        # the tokens, behind them the workspace, 8-byte aligned
-        tokens = torch.empty((B + 1) // 2 * 2 + nbytes // 4, dtype=i32, device=logits.device)
-        at = tokens.data_ptr()
-        tokens = tokens[:B]
+        tokens = torch.empty(B, dtype=i32, device=logits.device)
+        nbytes = _logits_rules_bytes(B, V)
+        if nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
     if B:
-        _launch(dev, _lib.load().nb_logits_rules, logits.data_ptr(), _DT[logits.dtype], ld, B, V,
-                h, ld_history, n_history, lens, prompt_lens, repetition, frequency, presence,
-                ids, values, ld_bias, n_bias, m, ld_mask, out.data_ptr(), ld_out, at,
-                at + (B + 1) // 2 * 8 if nbytes else None, nbytes)
+        status = _lib.load().nb_logits_rules(
+            logits.data_ptr(), _DT[logits.dtype], ld, B, V, h, ld_history, n_history, lens,
+            prompt_lens, repetition, frequency, presence, ids, values, ld_bias, n_bias, m, ld_mask,
+            out.data_ptr(), ld_out, None if tokens is None else tokens.data_ptr(),
+            None if ws is None else ws.data_ptr(), nbytes,
+            torch._C._cuda_getCurrentRawStream(dev))
+        if status:
+            _lib.check(status)
     return (out, tokens) if choose else out
 
 
 def _matrix(name, t, dtype, rows, columns, dev):
     """(address, row stride, columns) of a rule's rows of at least `columns`;
     a row stride of 0 gives all rows the same entries."""
-    if t is None:
-        return None, 0, 0
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == dev and
-            t.dtype is dtype and t.dim() == 2 and t.shape[0] == rows and t.shape[1] >= columns):
+    if not (isinstance(t, torch.Tensor) and t.get_device() == dev and t.dtype is dtype and
+            t.dim() == 2 and t.shape[0] == rows and t.shape[1] >= columns):
         _require_cuda(name, t)
         raise ValueError(f"{name} must be a {dtype} ({rows}, >= {columns}) tensor on cuda:{dev}, "
                          f"got {t.dtype} {tuple(t.shape)} on {t.device}")
