@@ -11,22 +11,24 @@ namespace {
 // tables of 32 blocks or more, 8 blocks each at least (two a wave).  One token
 // of six requests of 40000 positions, 8 heads of 128 (48 workgroups unsplit):
 // 16 splits 75.7 us, 10 (two a CU) 78.8, 24 82; of one request of 8000 17 us
-// against 25 in splits of 32 blocks or more.
+// against 25 in splits of 32 blocks or more.  512 prompt tokens after 8000 (180
+// workgroups): 4 splits 114 us, one 229; 300 of two requests after 3000, 2
+// heads of 256: 8 blocks or more 45 us, 16 63, one split 129.  More than fill
+// the CUs cost their partial results: 2048 prompt tokens 60 us, in two splits 95.
 int splits_of(int n_chunks, int n_tokens, int max_blocks, int n_head, int n_kv) {
-    const int64_t groups = (int64_t)n_chunks * n_kv;
+    const int64_t rows = ((int64_t)n_tokens + n_chunks - 1) / n_chunks * (n_head / n_kv);
+    const int64_t groups = (int64_t)n_chunks * n_kv * ((rows + 63) / 64);
     const int64_t want = 3 * device_cu_count();
-    if (groups >= want || max_blocks < 32 || (int64_t)n_tokens * (n_head / n_kv) > 16LL * n_chunks) {
-        return 1;
-    }
+    if (groups >= want || max_blocks < 32) return 1;
     return (int)std::max<int64_t>(1, std::min<int64_t>({want / groups, max_blocks / 8, 64}));
 }
 
-// One wave a row and head: the splits' maxima and sums in its lanes, then
-// the dims.
+// A wave takes a row and head at a time: the splits' maxima and sums in its
+// lanes, then the dims.  blockIdx.z takes every gridDim.z-th token of a chunk.
 __global__ __launch_bounds__(64) void kv8_join_kernel(Kv8AttentionArgs a, int splits) {
     const Kv8Chunk ch = kv8_chunk(a, blockIdx.x);
     const int head = blockIdx.y, lane = threadIdx.x;
-    for (int t = 0; t < ch.n; ++t) {
+    for (int t = blockIdx.z; t < ch.n; t += gridDim.z) {
         const int64_t row = ch.row0 + t, at = (row * a.n_head + head) * splits;
         const float* ml = a.part + (int64_t)a.n_tokens * a.n_head * splits * a.D + 2 * at;
         const float m = lane < splits ? ml[2 * lane] : -INFINITY;
@@ -88,7 +90,8 @@ int launch_kv8_attention(const void* q, int q_dtype, int64_t ld_q, const int32_t
                              : (prompts ? launch_kv8_prompts_3 : launch_kv8_tokens_3);
     launch(a, grid, rules, stream);
     if (splits > 1) {
-        hipLaunchKernelGGL(kv8_join_kernel, dim3(n_chunks, n_head), dim3(64), 0, stream, a, splits);
+        const int per = std::min(kKvBlock, (n_tokens + n_chunks - 1) / n_chunks);
+        hipLaunchKernelGGL(kv8_join_kernel, dim3(n_chunks, n_head, per), dim3(64), 0, stream, a, splits);
     }
     return check_launch("nb_kv8_attention");
 }

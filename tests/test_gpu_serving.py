@@ -665,3 +665,17 @@ def test_step_under_graphs_and_streams(dev):
                 assert torch.equal(a, b)
             for a, b in zip(caches[j], caches[2]):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("rules", ["plain", "all"])
+def test_attention_split_prompts(dev, dt, rules):
+    """Few chunks of many rows, some of few, over wide tables: split and
+    joined row by row."""
+    rng = np.random.default_rng(12)
+    p, t, want, n_blocks, n = step(dev, [2100, 0, 700], [70, 1, 30], 40, 2, rng, rows=103)
+    cache = random_cache(n_blocks, 2, 64, rng)
+    q = torch.from_numpy(rng.standard_normal((n, 4 * 64)).astype(np.float32) * 0.3).to(DT[dt])
+    from nativebit_amd import _lib
+    assert _lib.load().nb_kv8_attention_ws_bytes(n, p.chunks.shape[0], 40, 4, 2, 64) > 0
+    check_attention(dev, p, t, want, q, cache, 4, dt, RULES[rules], rng)
