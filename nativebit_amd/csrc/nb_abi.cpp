@@ -1326,7 +1326,10 @@ int nb_kv8_attention(const void* q, int q_dtype, int64_t ld_q, const int32_t* ch
     if (st) return st;
     st = check_chunks(fn, chunks, n_chunks, n_kv_head);
     if (st) return st;
-    if (!(softcap >= 0.f) || !std::isfinite(softcap)) return fail(NB_EINVAL, "%s: softcap=%g", fn, (double)softcap);
+    // (its reciprocal is a factor of the scores)
+    if (!(softcap >= 0.f) || !std::isfinite(softcap) || (softcap > 0.f && softcap < 1e-20f)) {
+        return fail(NB_EINVAL, "%s: softcap=%g", fn, (double)softcap);
+    }
     if (window < 0) return fail(NB_EINVAL, "%s: window=%d", fn, window);
     if (!lens) return fail(NB_EINVAL, "%s: lens is NULL", fn);
     if (n_chunks == 0) return NB_OK;
@@ -1368,6 +1371,11 @@ int nb_logits_rules(const void* logits, int dtype, int64_t ld, int rows, int V,
     if (st) return st;
     if (out == logits && (dtype != NB_F32 || ld != ld_out)) {
         return fail(NB_EINVAL, "%s: in place only over fp32 logits of the same stride", fn);
+    }
+    const char *in0 = static_cast<const char*>(logits), *out0 = reinterpret_cast<const char*>(out);
+    if (out0 != in0 && out0 < in0 + ((rows - 1) * ld + V) * (int64_t)dtype_size(dtype) &&
+        in0 < out0 + ((rows - 1) * ld_out + V) * 4) {
+        return fail(NB_EINVAL, "%s: out overlaps logits", fn);
     }
     if ((history == nullptr) != (lens == nullptr)) return fail(NB_EINVAL, "%s: history and lens go together", fn);
     if (!history && (prompt_lens || repetition || frequency || presence)) {

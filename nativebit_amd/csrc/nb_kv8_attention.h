@@ -300,8 +300,9 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
         };
         const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
         constexpr int kIns = (DT + NW - 1) / NW;   // loads of a wave for a block's keys
-        auto stage = [&](int b, int buffer) {
-            const int8_t *kp = codes_at(a.k, b), *vp = codes_at(a.v, b);
+        // (keys of two blocks, then the values of two)
+        auto stage_keys = [&](int b, int slot) {
+            const int8_t* p = codes_at(a.k, b);
 #pragma unroll
             for (int n = 0; n < kIns; ++n) {
                 const int ins = wave + NW * n;   // 64 pieces each
@@ -310,18 +311,34 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
                 }
                 const int l = 64 * ins + lane;
                 const int token = l / per, piece = l - token * per;
-                const uint32_t to = lds0 + buffer * 2 * kCodes + 1024 * ins;
-                to_lds16(to, kp + token * D + 16 * (piece ^ key_swap(token)));
-                const int dim = l >> 2;
-                to_lds16(to + kCodes, vp + dim * kKvBlock + 16 * ((l & 3) ^ (dim >> 1 & 3)));
+                to_lds16(lds0 + slot * kCodes + 1024 * ins, p + token * D + 16 * (piece ^ key_swap(token)));
             }
         };
-        int b = 0, b_next = 0;
+        auto stage_values = [&](int b, int slot) {
+            const int8_t* p = codes_at(a.v, b);
+#pragma unroll
+            for (int n = 0; n < kIns; ++n) {
+                const int ins = wave + NW * n;
+                if (DT % NW != 0 || !kWhole) {
+                    if (ins >= per) break;
+                }
+                const int l = 64 * ins + lane, dim = l >> 2;
+                to_lds16(lds0 + (2 + slot) * kCodes + 1024 * ins,
+                         p + dim * kKvBlock + 16 * ((l & 3) ^ (dim >> 1 & 3)));
+            }
+        };
+        // the block, or two, under way and the next
+        constexpr int kAtOnce = kShared ? 2 : 1;
+        int now[kAtOnce], next[kAtOnce];
         if (i < i_end) {
-            b = block_at(i);
-            b_next = block_at(i + kw);
-            if constexpr (kShared) stage(b, 0);
-            else load_keys(b);
+#pragma unroll
+            for (int e = 0; e < kAtOnce; ++e) now[e] = block_at(i + e), next[e] = block_at(i + kAtOnce * kw + e);
+            if constexpr (kShared) {
+                stage_keys(now[0], 0);
+                if (i + 1 < i_end) stage_keys(now[1], 1);
+            } else {
+                load_keys(now[0]);
+            }
         }
 
         // ---- the row's digits -------------------------------------------------
@@ -369,168 +386,212 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
         for (int dt = 0; dt < DT; ++dt) o[dt][0] = o[dt][1] = o[dt][2] = o[dt][3] = 0.f;
         float m = -INFINITY, l = 0.f;   // l: of the lane's own tokens
 
-        // one block: key(mt, s) and value(dt) give the codes; between() runs
-        // after the first product
-        auto walk = [&](int block, int n, auto&& key, auto&& between, auto&& value)
+        // Blocks n .. n + NB - 1 of the walk, one or two, at once: key(e, mt, s) and
+        // value(e, dt) give the codes of the e-th, between() runs after the first
+        // product.  Two share their weights' largest score and one step of O; the
+        // ratio of their value scales is a factor of the weights' digits.
+        auto walk = [&](auto nb, int n, auto&& key, auto&& between, auto&& value)
                         __attribute__((always_inline)) {
-            const int64_t bh = (int64_t)(valid(block) ? block : 0) * a.n_kv + h;
-            const float ks = as_constant(a.k_scale)[bh], vs = as_constant(a.v_scale)[bh];
-            const int j0 = place(n) * kKvBlock;
+            constexpr int NB = decltype(nb)::value;
             // ---- scores -------------------------------------------------------
-            float x[16];
+            float x[NB][16], unit[NB], vs[NB], top[NB];
+            bool there[NB];
 #pragma unroll
-            for (int mt = 0; mt < 4; ++mt) {
-                i4 acc = {0, 0, 0, 0}, low = {128, 128, 128, 128}, f[DS];
+            for (int e = 0; e < NB; ++e) {
+                there[e] = valid(now[e]);
+                const int64_t bh = (int64_t)(there[e] ? now[e] : 0) * a.n_kv + h;
+                // scores in units of 1 / unit: x * unit is the exponent of 2
+                unit[e] = as_constant(a.k_scale)[bh];
+                vs[e] = as_constant(a.v_scale)[bh];
 #pragma unroll
-                for (int s = 0; s < DS; ++s) f[s] = key(mt, s);
+                for (int mt = 0; mt < 4; ++mt) {
+                    i4 acc = {0, 0, 0, 0}, low = {128, 128, 128, 128}, f[DS];
 #pragma unroll
-                for (int s = 0; s < DS; ++s)
-                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[s], qd[ND - 1][s], acc, 0, 0, 0);
-                if constexpr (ND == 3) {
+                    for (int s = 0; s < DS; ++s) f[s] = key(e, mt, s);
 #pragma unroll
                     for (int s = 0; s < DS; ++s)
-                        low = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[s], qd[0][s], low, 0, 0, 0);
-                    acc = (acc << 8) + (low >> 8);
-                } else {
-                    acc <<= 8;
+                        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[s], qd[ND - 1][s], acc, 0, 0, 0);
+                    if constexpr (ND == 3) {
+#pragma unroll
+                        for (int s = 0; s < DS; ++s)
+                            low = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[s], qd[0][s], low, 0, 0, 0);
+                        acc = (acc << 8) + (low >> 8);
+                    } else {
+                        acc <<= 8;
+                    }
+#pragma unroll
+                    for (int s = 0; s < DS; ++s)
+                        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[s], qd[ND - 2][s], acc, 0, 0, 0);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[e][4 * mt + r] = (float)acc[r];
                 }
-#pragma unroll
-                for (int s = 0; s < DS; ++s)
-                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[s], qd[ND - 2][s], acc, 0, 0, 0);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) x[4 * mt + r] = (float)acc[r];
             }
             between();
-            // scores in units of 1 / unit: x * unit is the exponent of 2
-            float unit = to_log2 * ks;
-            if constexpr (kRules) {
-                // slope * distance, from the lane's first token on
-                const float at = slope * (float)(j0 + 16 * g - pos);
-                if (a.softcap > 0.f) {
-                    const float f = inv * ks * per_cap;
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        x[e] = capped<ND>(x[e], f, cap, fmaf(slope, (float)e, at));
+            for (int e = 0; e < NB; ++e) {
+                const int j0 = place(n + e) * kKvBlock, j_lane = j0 + 16 * g;
+                if constexpr (kRules) {
+                    // slope * distance, from the lane's first token on
+                    const float at = slope * (float)(j_lane - pos);
+                    if (a.softcap > 0.f) {
+                        const float f = inv * unit[e] * per_cap;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            x[e][i] = capped<ND>(x[e][i], f, cap, fmaf(slope, (float)i, at));
+                    } else {
+                        const float f = to_log2 * unit[e];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            x[e][i] = fmaf(x[e][i], f, fmaf(slope, (float)i, at));
+                    }
+                    unit[e] = 1.f;
                 } else {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) x[e] = fmaf(x[e], unit, fmaf(slope, (float)e, at));
+                    unit[e] *= to_log2;
                 }
-                unit = 1.f;
-            }
-            // some row of the tile does not see the whole block
-            if (!valid(block) ||
-                !((j0 + kKvBlock <= pos_lo + 1 && j0 >= lo_max) || j0 + kKvBlock <= pre)) {
-                const int jl = j0 + 16 * g;
-                const int end = valid(block) ? hi : 0, pre_end = valid(block) ? pre : 0;
+                // some row of the tile does not see the whole block
+                if (!there[e] ||
+                    !((j0 + kKvBlock <= pos_lo + 1 && j0 >= lo_max) || j0 + kKvBlock <= pre)) {
+                    const int end = there[e] ? hi : 0, pre_end = there[e] ? pre : 0;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int j = jl + e;
-                    const bool seen = ((j < end) & (j >= lo)) | (j < pre_end);
-                    x[e] = seen ? x[e] * unit : -INFINITY;
+                    for (int i = 0; i < 16; ++i) {
+                        const int j = j_lane + i;
+                        const bool seen = ((j < end) & (j >= lo)) | (j < pre_end);
+                        x[e][i] = seen ? x[e][i] * unit[e] : -INFINITY;
+                    }
+                    unit[e] = 1.f;   // (a unit of 0 or infinity times -inf is NaN)
                 }
-                unit = 1.f;   // (a unit of 0 or infinity times -inf is NaN)
+                float most = x[e][0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) most = fmaxf(most, x[e][i]);
+                top[e] = rows_max(most) * unit[e];
             }
             // ---- weights ------------------------------------------------------
-            float top = x[0];
-#pragma unroll
-            for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
-            top = rows_max(top) * unit;
-            const float base = fmaxf(top, kLowest);
+            float all = top[0];
+            if constexpr (NB == 2) all = fmaxf(all, top[1]);
+            const float base = fmaxf(all, kLowest);
             // p is at most 1 + 2^-24 |base|, which its digits hold up to 2^12
             const bool far = fabsf(base) > 4096.f;
             if (__any(far)) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] *= far ? unit : 1.f;
-                unit = far ? 1.f : unit;
+                for (int e = 0; e < NB; ++e) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[e][i] *= far ? unit[e] : 1.f;
+                    unit[e] = far ? 1.f : unit[e];
+                }
+            }
+            // (a row that sees nothing of a block takes nothing of its scale)
+            float v_scale = top[0] == -INFINITY ? 0.f : vs[0];
+            float digits_of_1[NB] = {kTop};
+            if constexpr (NB == 2) {
+                const float v0 = v_scale, v1 = top[1] == -INFINITY ? 0.f : vs[1];
+                v_scale = fmaxf(v0, v1);
+                digits_of_1[0] = v0 == v_scale ? kTop : kTop * (v0 / v_scale);
+                digits_of_1[1] = v1 == v_scale ? kTop : kTop * (v1 / v_scale);
             }
             float sum = 0.f;
-            i4 pd[ND];
+            i4 pd[NB][ND];
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                uint32_t w[4], d[3];
+            for (int e = 0; e < NB; ++e) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(x[e + r], unit, -base));
-                    sum += p;
-                    // 2^23 + bias + rint(p kTop): the low mantissa bits
-                    w[r] = __float_as_uint(fmaf(p, kTop, 8388608.f + (float)Digits<ND>::kBias));
+                for (int i = 0; i < 16; i += 4) {
+                    uint32_t w[4], d[3];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float p = __builtin_amdgcn_exp2f(fmaf(x[e][i + r], unit[e], -base));
+                        sum += p;
+                        // 2^23 + bias + rint(p kTop): the low mantissa bits
+                        w[r] = __float_as_uint(
+                            fmaf(p, digits_of_1[e], 8388608.f + (float)Digits<ND>::kBias));
+                    }
+                    digits4<ND>(w, d);
+#pragma unroll
+                    for (int j = 0; j < ND; ++j) pd[e][j][i / 4] = (int)d[j];
                 }
-                digits4<ND>(w, d);
-#pragma unroll
-                for (int n = 0; n < ND; ++n) pd[n][e / 4] = (int)d[n];
             }
             // m follows a row's largest score only when that is 2^16 ahead:
             // shares up to 2^16 cost fp32 sums nothing, scaling O does (by 1 in
             // the rows that stay: a row's result is its own)
-            const bool ahead = top > m + 16.f;
-            const float m_new = ahead ? top : m;
+            const bool ahead = all > m + 16.f;
+            const float m_new = ahead ? all : m;
             const float beta = ahead ? __builtin_amdgcn_exp2f(m - fmaxf(m_new, kLowest)) : 1.f;
             const int any_ahead = __builtin_amdgcn_readfirstlane(__any(ahead));
             l *= beta;
             m = m_new;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) scale_if(any_ahead, beta, o[dt]);
-            const float share = __builtin_amdgcn_exp2f(top - fmaxf(m, kLowest));
+            const float share = __builtin_amdgcn_exp2f(all - fmaxf(m, kLowest));
             l = fmaf(sum, share, l);
-            // (a row that sees nothing of the block takes nothing of its scale)
-            const float gamma =
-                top == -INFINITY ? 0.f : share * vs * (ND == 3 ? 256.f / kTop : 1.f / kTop);
+            const float gamma = v_scale == 0.f ? 0.f : share * v_scale * (ND == 3 ? 256.f / kTop : 1.f / kTop);
             // ---- O ------------------------------------------------------------
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                i4 acc = {0, 0, 0, 0}, low = {128, 128, 128, 128};
-                const i4 f = value(dt);
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, pd[ND - 1], acc, 0, 0, 0);
+                i4 acc = {0, 0, 0, 0}, low = {128, 128, 128, 128}, f[NB];
+#pragma unroll
+                for (int e = 0; e < NB; ++e) f[e] = value(e, dt);
+#pragma unroll
+                for (int e = 0; e < NB; ++e)
+                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[e], pd[e][ND - 1], acc, 0, 0, 0);
                 if constexpr (ND == 3) {
-                    low = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, pd[0], low, 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < NB; ++e)
+                        low = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[e], pd[e][0], low, 0, 0, 0);
                     acc = (acc << 8) + (low >> 8);
                 } else {
                     acc <<= 8;
                 }
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, pd[ND - 2], acc, 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < NB; ++e)
+                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[e], pd[e][ND - 2], acc, 0, 0, 0);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[dt][r] = fmaf(gamma, (float)acc[r], o[dt][r]);
             }
         };
         if constexpr (kShared) {
+            // Two blocks a turn: their values load during the first product, the
+            // next two's keys during the rest.
             const i4* mine = reinterpret_cast<const i4*>(lds);
             const int swap = key_swap(key_row);   // (the same for all mt)
-            int buffer = 0;
-            for (; i < i_end; ++i, buffer ^= 1) {
-                // this block has arrived, and the other buffer is read, in all waves
+            auto key = [&](int e, int mt, int s) {
+                const int piece = 4 * s + g < per ? 4 * s + g : 0;
+                return mine[e * (kCodes / 16) + (key_row + 4 * mt) * per + (piece ^ swap)];
+            };
+            auto value = [&](int e, int dt) {
+                return mine[(2 + e) * (kCodes / 16) + (16 * dt + c) * 4 + (g ^ (c >> 1 & 3))];
+            };
+            // this wave's loads are there, then everybody's, and what was read
+            // before is free
+            auto arrive = [] {
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 __syncthreads();
-                if (i + 1 < i_end) stage(b_next, buffer ^ 1);
-                const int now = b;
-                b = b_next;
-                b_next = block_at(i + 2);
-                const i4* from = mine + buffer * (2 * kCodes / 16);
-                walk(
-                    now, i,
-                    [&](int mt, int s) {
-                        const int piece = 4 * s + g < per ? 4 * s + g : 0;
-                        return from[(key_row + 4 * mt) * per + (piece ^ swap)];
-                    },
-                    [] {},
-                    [&](int dt) {
-                        return from[kCodes / 16 + (16 * dt + c) * 4 + (g ^ (c >> 1 & 3))];
-                    });
+            };
+            for (; i < i_end; i += 2) {
+                const bool two = i + 1 < i_end;
+                arrive();
+                stage_values(now[0], 0);
+                if (two) stage_values(now[1], 1);
+                auto between = [&] {
+                    arrive();
+                    if (i + 2 < i_end) stage_keys(next[0], 0);
+                    if (i + 3 < i_end) stage_keys(next[1], 1);
+                };
+                if (two) walk(std::integral_constant<int, 2>{}, i, key, between, value);
+                else walk(std::integral_constant<int, 1>{}, i, key, between, value);
+                now[0] = next[0], now[1] = next[1];
+                next[0] = block_at(i + 4), next[1] = block_at(i + 5);
             }
-            __syncthreads();   // the last block is read
+            __syncthreads();   // the last values are read
         } else {
             // `more`: the next block's loads are issued (a constant, so that every
             // path to the next block has them in flight and waits for no more)
             auto direct = [&](auto more) __attribute__((always_inline)) {
-                const int now = b;
                 walk(
-                    now, i, [&](int mt, int s) { return kf[mt][s]; },
-                    [&] {
-                        load_values(now);
-                        b = b_next;
-                        if constexpr (decltype(more)::value) b_next = block_at(i + 2 * kw);
-                    },
-                    [&](int dt) { return vf[dt]; });
-                if constexpr (decltype(more)::value) load_keys(b);
+                    std::integral_constant<int, 1>{}, i, [&](int, int mt, int s) { return kf[mt][s]; },
+                    [&] { load_values(now[0]); }, [&](int, int dt) { return vf[dt]; });
+                if constexpr (decltype(more)::value) {
+                    now[0] = next[0];
+                    next[0] = block_at(i + 2 * kw);
+                    load_keys(now[0]);
+                }
             };
             for (; i + kw < i_end; i += kw) direct(std::true_type{});
             if (i < i_end) direct(std::false_type{});

@@ -579,8 +579,9 @@ def kv_plan(table: torch.Tensor, lens: torch.Tensor, new: torch.Tensor, free: to
             state: torch.Tensor, n_tokens: int, out: KVPlan | None = None) -> KVPlan:
     """The plan of a serving step from the requests' lengths, on the GPU
     (nb_kv_plan): request r has ``lens[r]`` tokens cached and brings ``new[r]``;
-    its new blocks come from the end of ``free[:state[0]]`` and are entered in
-    ``table`` (requests, blocks), which is updated in place.  ``n_tokens`` is
+    its new blocks come from the end of ``free[:state[0]]`` (``free`` has an entry
+    for each block of the cache) and are entered in ``table`` (requests, blocks),
+    which is updated in place.  ``n_tokens`` is
     the rows of the step (the sum of ``new``, or more: the rows behind have no
     slot).  ``lens`` and ``state`` are left as they are; the plan's are those
     after the step.  ``out``: a plan of the same sizes to write."""
@@ -686,7 +687,8 @@ def kv8_append(qkv: torch.Tensor, plan: KVPlan, cos: torch.Tensor, sin: torch.Te
     8-bit cache (nb_kv8_append).  ``qkv`` (rows, (n_head + 2 heads) head_dim)
     float32 or bfloat16, ``cos`` / ``sin`` (positions, head_dim / 2) float32.
     Returns the turned queries times head_dim^-0.5, (rows, n_head head_dim) in
-    qkv's dtype (or into ``q``); rows without a slot are not written."""
+    qkv's dtype (or into ``q``, which may be qkv's own query columns); rows
+    without a slot are not written."""
     dev, n_blocks, n_kv, D = _kv8_cache(k, v, k_scale, v_scale)
     if not _here(dev):
         with torch.cuda.device(dev):
@@ -781,6 +783,8 @@ def kv8_attention(q: torch.Tensor, plan: KVPlan, table: torch.Tensor, k: torch.T
         _require("table", table, i32, (R, width), dev)
         _require("plan.chunks", chunks, i32, (None, 4), dev)
         _require("plan.lens", plan.lens, i32, (R,), dev)
+    if not 0 <= window < 1 << 31:
+        raise ValueError(f"window={window}")
     if slopes is not None:
         _require("slopes", slopes, torch.float32, (n_head,), dev)
     if prefix is not None:

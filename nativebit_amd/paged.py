@@ -106,11 +106,13 @@ class PagedCache:
         request a number of leading tokens that all its queries see."""
         R = self.table.shape[0]
         dev = self.table.device
-        if isinstance(new, torch.Tensor):
-            if n_tokens is None:
-                raise ValueError("a step from a tensor needs n_tokens")
-            self._known, self.whole = None, False
-        else:
+        if prefix is not None:
+            prefix = torch.as_tensor(prefix, dtype=torch.int32).to(dev)
+            if prefix.shape != (R,):
+                raise ValueError(f"prefix must have {R} numbers, got {tuple(prefix.shape)}")
+        whole = not isinstance(new, torch.Tensor)
+        known = left = None
+        if whole:
             new = [int(n) for n in new]
             if len(new) > R or min(new, default=0) < 0:
                 raise ValueError(f"{len(new)} counts for {R} requests, none below 0")
@@ -119,23 +121,24 @@ class PagedCache:
             new += [0] * (R - len(new))
             if self._known is None:     # (lengths that only the GPU knows)
                 self._known, self._left = self.lens.tolist(), int(self.state[0])
-            ends = [a + b for a, b in zip(self._known, new)]
+            known = [a + b for a, b in zip(self._known, new)]
             need = sum(-(-e // ops.KV_BLOCK) - -(-a // ops.KV_BLOCK)
-                       for a, e in zip(self._known, ends))
-            if max(ends) > self.max_len:
-                raise ValueError(f"{max(ends)} tokens of a request exceed max_len {self.max_len}")
+                       for a, e in zip(self._known, known))
+            if max(known) > self.max_len:
+                raise ValueError(f"{max(known)} tokens of a request exceed max_len {self.max_len}")
             if need > self._left:
                 raise ValueError(f"{need} blocks needed, {self._left} free")
-            self._known, self._left, self.whole = ends, self._left - need, True
+            left = self._left - need
             n_tokens = sum(new)
             new = torch.tensor(new, dtype=torch.int32, device=dev)
-        if prefix is not None:
-            prefix = torch.as_tensor(prefix, dtype=torch.int32).to(dev)
-        self.prefix = prefix
-        self.plan = ops.kv_plan(self.table, self.lens, new, self.free, self.state, n_tokens)
-        self.lens.copy_(self.plan.lens)
-        self.state.copy_(self.plan.state)
-        return self.plan
+        elif n_tokens is None:
+            raise ValueError("a step from a tensor needs n_tokens")
+        plan = ops.kv_plan(self.table, self.lens, new, self.free, self.state, n_tokens)
+        self.lens.copy_(plan.lens)
+        self.state.copy_(plan.state)
+        self.plan, self.prefix, self.whole = plan, prefix, whole
+        self._known, self._left = known, left
+        return plan
 
     def release(self, requests) -> None:
         """Ends requests (their numbers): their blocks are free again."""
@@ -191,6 +194,9 @@ def generate(model, prompts, n_generate: int, *, repetition=None, frequency=None
         raise ValueError(f"prompt token outside 0..{V - 1}")
     dev = model.embedding.weight.device
     lengths = [len(p) for p in prompts]
+    room = model.context_len if cache is None else cache.max_len
+    if max(lengths) + n_generate - 1 > room:     # (the last token is not fed)
+        raise ValueError(f"{max(lengths)} prompt tokens and {n_generate} more exceed {room}")
     if cache is None:
         blocks = sum(-(-(length + n_generate) // ops.KV_BLOCK) for length in lengths)
         cache = PagedCache(model, blocks, n, device=dev)

@@ -34,8 +34,11 @@ def test_steps_are_checked_on_the_host():
         c.step([1, 1], n_tokens=3)
     with pytest.raises(ValueError):
         c.step(torch.zeros(2, dtype=torch.int32))
-    with pytest.raises(ValueError):      # fits, but there is no CPU implementation
-        c.step([128, 65])
+    with pytest.raises(ValueError):
+        c.step([1, 1], prefix=[3])
+    for _ in range(2):                   # fits, but there is no CPU implementation: nothing changes
+        with pytest.raises(ValueError):
+            c.step([128, 65])
     with pytest.raises(ValueError):
         c.release([2])
     with pytest.raises(IndexError):
@@ -45,7 +48,11 @@ def test_steps_are_checked_on_the_host():
 
 
 def test_generate_refuses():
-    model = types.SimpleNamespace(embedding=types.SimpleNamespace(weight=torch.zeros(10, 4)))
+    model = types.SimpleNamespace(embedding=types.SimpleNamespace(weight=torch.zeros(10, 4)),
+                                  context_len=20)
+    for n in (20, 100):
+        with pytest.raises(ValueError):
+            paged.generate(model, [[1], [2, 3]], n)
     for prompts in ([], [[]], [[1], []], [[10]], [[-1]]):
         with pytest.raises(ValueError):
             paged.generate(model, prompts, 1)

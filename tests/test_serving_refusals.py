@@ -102,7 +102,7 @@ def attention(**kw):
     (dict(ld_q=255), EINVAL), (dict(ld_out=255), EINVAL), (dict(q_dtype=2), EINVAL),
     (dict(out_dtype=2), EINVAL), (dict(out=None), EINVAL), (dict(q=P + 2), EALIGN),
     (dict(chunks=None), EINVAL), (dict(lens=None), EINVAL), (dict(softcap=-1.0), EINVAL),
-    (dict(softcap=float("nan")), EINVAL), (dict(softcap=float("inf")), EINVAL),
+    (dict(softcap=float("nan")), EINVAL), (dict(softcap=float("inf")), EINVAL), (dict(softcap=1e-25), EINVAL),
     (dict(window=-1), EINVAL), (dict(slopes=P + 2), EALIGN), (dict(prefix=P + 1), EALIGN),
     (dict(n_chunks=1 << 23), EUNSUP), (dict(table=None), EINVAL),
     # few chunks over a long cache need a workspace
@@ -131,6 +131,7 @@ def logits(**kw):
     (dict(tokens=P + 2), EALIGN), (dict(V=50257, ld=50257, ld_out=50257, ld_mask=1571, ws_bytes=8), EINVAL),
     (dict(V=50257, ld=50257, ld_out=50257, ld_mask=1571, ws=None), EINVAL),
     (dict(out=P, dtype=BF16), EINVAL), (dict(out=P, ld_out=101), EINVAL),
+    (dict(out=P + 4), EINVAL), (dict(out=P + 1196), EINVAL), (dict(out=P - 1196), EINVAL),
 ])
 def test_logits_refuses(kw, status):
     assert logits(**kw) == status
