@@ -15,7 +15,10 @@
 // new rows makes s' +inf and the block's codes 0: the block then reads as NaN.
 //
 // What bounds them: memory.  One token writes D bytes of codes a head, and
-// reads the earlier codes of its block only when the scale grows.
+// reads the earlier codes of its block only when the scale grows.  Append, 32
+// query and 8 key / value heads of 128 in bf16, 96 tokens of 96 requests: 8 us;
+// 6001 fp32 prompt tokens, 20 heads of 128: 71 us for 276 MB in and out (3.9
+// TB/s).  Read, fp32 out: 6240 slots of 8 heads 16 us, 6577 of 20 heads 34.
 #include <math.h>
 
 #include <algorithm>
@@ -462,7 +465,8 @@ int launch_kv8_append(const void* qkv, int qkv_dtype, int64_t ld_qkv, const int3
                  four_aligned(q_out, q_dtype) && ld_q % 4 == 0,
                  (reinterpret_cast<uintptr_t>(cos_t) | reinterpret_cast<uintptr_t>(sin_t)) % 8 == 0,
                  n_pos, n_blocks, n_tokens, n_head, n_kv, D, (float)(1.0 / sqrt((double)D))};
-    hipLaunchKernelGGL(D <= 128 ? kv8_append_kernel<128> : kv8_append_kernel<kMaxD>, dim3((unsigned)n_chunks * 3 * n_kv), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(D <= 128 ? kv8_append_kernel<128> : kv8_append_kernel<kMaxD>,
+                       dim3((unsigned)n_chunks * 3 * n_kv), dim3(kThreads), 0, stream, a);
     return check_launch("nb_kv8_append");
 }
 

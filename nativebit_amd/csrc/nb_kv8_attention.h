@@ -15,28 +15,44 @@
 // largest score of the row, are three digits, and V's dims get
 //     O = O + (A 2^8 + B + C / 2^8) / (127 * 2^8) v_scale exp(m - M)
 // with M the row's running reference, its largest score or up to 16 binary
-// orders less (O is scaled when it moves).  Scores, statistics and O are fp32.  Two digits (16 bits of q and of w, each relative to the largest of its row)
+// orders less (O is scaled when it moves).  Scores, statistics and O are fp32.
+// Two digits (16 bits of q and of w, each relative to the largest of its row)
 // serve bf16 outputs, whose own rounding is 2^-9: 2^-17 is lost of q and w.
-// The codes go from memory into the MFMAs as they are.
+// The codes go into the MFMAs as they are.
 //
 // Layout.  Everything is transposed, so that a lane keeps one row from the
-// scores to the output and nothing passes through LDS.  Lane (c, g) = (lane %
-// 16, lane / 16) holds row c of a tile of 16 rows (a row is a query token and
-// a head of those that share the keys).
+// scores to the output and no row's numbers pass through LDS.  Lane (c, g) =
+// (lane % 16, lane / 16) holds row c of a tile of 16 rows (a row is a query
+// token and a head of those that share the keys).
 //   S^T = K Q^T: MFMA mt takes the 16 tokens 16 (i / 4) + 4 mt + i % 4, so that
 //     the lane ends with the scores of tokens 16 g + 4 mt + r, the 16
 //     consecutive ones whose weights, packed to bytes, are its B operand of
 //   O^T = V^T P^T: A = 16 dims x 64 tokens of V's [D][64]; the lane ends with
 //     dims 16 dt + 4 g + r of its row.
-// A wave walks whole blocks; the next block's keys are loaded while the
-// softmax and the second product run, its values during the first.
 //
-// Split.  A workgroup takes one chunk and key / value head.  Up to 16 rows
-// (single tokens) all its waves take the blocks in turn and are joined through
-// LDS at the end; more rows go to the waves 16 each, which then walk the same
-// blocks (one trip through the L1 for all).  Few chunks over long caches are
-// split over workgroups too (gridDim.z), with partial results in a workspace
-// that a second launch joins.
+// Chunks of up to 32 rows (single tokens): a wave takes whole blocks of one or
+// two tiles of rows, codes straight to registers, a block's values on their way
+// during the softmax and the next one's keys during the second product; the
+// waves of a tile take the blocks in turn and are joined through LDS at the end.
+// More rows: the four waves take 16 each and walk the blocks together, two at a
+// time, whose codes each wave brings a quarter of to LDS (directly, with no
+// register between) while the product before runs.  Without LDS every wave
+// fetches all codes through the L1: 8003 prompt tokens of two requests, 20
+// heads of 128, 505 us then; 375 with LDS, scalar loads of tables and scales
+// and the reference that moves seldom; two blocks a turn (one maximum, one step
+// of O) instead of one: 384 to 371 in turn on one card, about 360 on others.
+//
+// Split.  A workgroup takes one chunk and key / value head (and 64 rows of it).
+// Few of them over long caches are split over workgroups too (gridDim.z), with
+// partial results in a workspace that a second launch joins.
+//
+// What bounds it.  Single tokens: the codes, 2 D bytes a cached token and head.
+// 64 requests of 960 positions at most, 20 heads of 128: 45 us, 5.3 TB/s; six of
+// 40000, 8 heads: 75 us with the join, 4.9 TB/s.  Prompts: the issue of vector
+// instructions and MFMAs, which overlap only in part.  16384 tokens, 16 heads
+// on 2: 563 TFLOP/s (of 4 D a score; each takes three int8 MFMA products in
+// fp32, two for bf16 outputs: 744).  Of 360 us for the 8003 tokens 125 go with
+// the second product, 85 with the first, 10 with the exponentials.
 #pragma once
 
 #include <math.h>
@@ -143,10 +159,10 @@ __device__ __forceinline__ void scale_if(int flag, float beta, float (&o)[4]) {
 // exponent.
 template <int ND>
 __device__ __forceinline__ float capped(float x, float f, float cap, float add) {
-    const float t = x * f;
-    const float e = __builtin_amdgcn_exp2f(t * (2.f * kLog2e));
+    const float e = __builtin_amdgcn_exp2f(x * (f * (2.f * kLog2e)));
     const float far = fmaf(__builtin_amdgcn_rcpf(e + 1.f), -2.f * cap, cap + add);
     if constexpr (ND == 2) return far;
+    const float t = x * f;
     const float z = t * t;
     float p = 0.0035921280f;
     p = fmaf(p, z, -0.0088632356f);
@@ -293,6 +309,7 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
         // by its row, so that the 8 lanes that are served together (rows c ..
         // c + 7, one piece) reach all 32 banks: keys of 8 or 16 pieces by c & 7
         // (token bits 0, 1, 4), of 4 by token bits 1, 4; values by dim bits 1, 2.
+        // (No conflicts counted at 128 dims.  Other sizes stay in order.)
         auto key_swap = [&](int token) {
             return per % 8 == 0 ? (token & 3) | (token >> 4 & 1) << 2
                    : per == 4   ? (token >> 1 & 1) | (token >> 4 & 1) << 1
@@ -671,8 +688,11 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
 
 // kPrompts: chunks of over two tiles of 16 rows share their blocks' codes
 // through LDS, the others of the launch go as without.
+// Registers: those of three workgroups a CU, for heads of over 128 dims (O alone
+// is 64 of them) of two.  4096 prompt tokens, 16 heads of 256 on 4: 327 us, 230
+// for bf16 outputs; with all registers, one a CU, 374 and 310.
 template <int DT, int ND, bool kRules, bool kWhole, bool kPrompts>
-__global__ __launch_bounds__(kWavesKv8 * 64, (DT <= 8 ? 3 : 1)) void kv8_attention_kernel(
+__global__ __launch_bounds__(kWavesKv8 * 64, (DT <= 8 ? 3 : 2)) void kv8_attention_kernel(
     Kv8AttentionArgs a) {
     __shared__ __align__(16) char lds[kv8_lds_bytes<DT, kPrompts>()];
     // Heads vary fastest (neighbouring workgroups, dealt to the XCDs in turn,

@@ -7,18 +7,19 @@
 namespace nb {
 namespace {
 
-// Workgroups over a row's blocks: three a CU, what their registers allow, over
-// tables of 32 blocks or more, 8 blocks each at least (two a wave).  One token
-// of six requests of 40000 positions, 8 heads of 128 (48 workgroups unsplit):
-// 16 splits 75.7 us, 10 (two a CU) 78.8, 24 82; of one request of 8000 17 us
-// against 25 in splits of 32 blocks or more.  512 prompt tokens after 8000 (180
-// workgroups): 4 splits 114 us, one 229; 300 of two requests after 3000, 2
+// Workgroups over a row's blocks: three a CU (heads of over 128 dims two), what
+// their registers allow, over tables of 32 blocks or more, 8 blocks each at
+// least (two a wave).  One token of six requests of 40000 positions, 8 heads of
+// 128 (48 workgroups unsplit): 16 splits 75.7 us, 10 (two a CU) 78.8, 24 82; 4
+// heads of 256: 21 splits 85 us, 32 (three a CU) 97; of one request of 8000 17
+// us against 25 in splits of 32 blocks or more.  512 prompt tokens after 8000
+// (180 workgroups): 4 splits 114 us, one 229; 300 of two requests after 3000, 2
 // heads of 256: 8 blocks or more 45 us, 16 63, one split 129.  More than fill
 // the CUs cost their partial results: 2048 prompt tokens 60 us, in two splits 95.
-int splits_of(int n_chunks, int n_tokens, int max_blocks, int n_head, int n_kv) {
+int splits_of(int n_chunks, int n_tokens, int max_blocks, int n_head, int n_kv, int D) {
     const int64_t rows = ((int64_t)n_tokens + n_chunks - 1) / n_chunks * (n_head / n_kv);
     const int64_t groups = (int64_t)n_chunks * n_kv * ((rows + 63) / 64);
-    const int64_t want = 3 * device_cu_count();
+    const int64_t want = (D <= 128 ? 3 : 2) * device_cu_count();
     if (groups >= want || max_blocks < 32) return 1;
     return (int)std::max<int64_t>(1, std::min<int64_t>({want / groups, max_blocks / 8, 64}));
 }
@@ -59,7 +60,7 @@ __global__ __launch_bounds__(64) void kv8_join_kernel(Kv8AttentionArgs a, int sp
 }  // namespace
 
 int64_t kv8_attention_bytes(int n_chunks, int n_tokens, int max_blocks, int n_head, int n_kv, int D) {
-    const int splits = splits_of(n_chunks, n_tokens, max_blocks, n_head, n_kv);
+    const int splits = splits_of(n_chunks, n_tokens, max_blocks, n_head, n_kv, D);
     return splits == 1 ? 0 : (int64_t)n_tokens * n_head * splits * (D + 2) * 4;
 }
 
@@ -73,7 +74,7 @@ int launch_kv8_attention(const void* q, int q_dtype, int64_t ld_q, const int32_t
     auto four = [](const void* p, int dtype, int64_t ld) {
         return reinterpret_cast<uintptr_t>(p) % (dtype == NB_F32 ? 16 : 8) == 0 && ld % 4 == 0;
     };
-    const int splits = splits_of(n_chunks, n_tokens, max_blocks, n_head, n_kv);
+    const int splits = splits_of(n_chunks, n_tokens, max_blocks, n_head, n_kv, D);
     Kv8AttentionArgs a{q, ld_q, chunks, lens, table, table_stride, k, v, k_scale, v_scale, out,
                        ld_out, slopes, prefix, static_cast<float*>(workspace), q_dtype, out_dtype,
                        four(q, q_dtype, ld_q), four(out, out_dtype, ld_out), n_chunks, n_tokens, R,

@@ -11,13 +11,14 @@
 // the largest x (-1 where no x is over -inf; a NaN is never chosen).
 //
 // Bound by memory: one pass over the logits.  A workgroup takes 1024 or 2048
-// tokens of a row; it issues the loads of their logits, counts the row's history in an
-// LDS word per token and notes the biases beside it
-// while they are under way, so that neither counts nor dense biases exist in
-// memory.  Every workgroup of a row walks its whole history, from the L2:
-// against 16 KB of logits read and written, a history of 1000 is 4 KB.  LDS
-// atomics are on whole numbers (sums, or, maximum): no result depends on their
-// order.
+// tokens of a row; it issues the loads of their logits, counts the row's history
+// in an LDS word per token and notes the biases beside it while they are under
+// way, so that neither counts nor dense biases exist in memory.  Every workgroup
+// of a row walks its whole history, from the L2: against 16 KB of logits read
+// and written, a history of 1000 is 4 KB.  LDS atomics are on whole numbers
+// (sums, or, maximum): no result depends on their order.  160 fp32 rows of
+// 131077 with histories of 4000: 45 us, 3.8 TB/s, and 5 us for the second launch
+// that turns the chosen keys into tokens; one row of 50257 4.5 and 1.6.
 #include <math.h>
 
 #include <algorithm>
