@@ -577,8 +577,8 @@ int nb_attention_batch(const float* q, const float* k_cache, const float* v_cach
  *     k        int8 [n_blocks][n_kv_head][NB_KV_BLOCK][head_dim]
  *     v        int8 [n_blocks][n_kv_head][head_dim][NB_KV_BLOCK]
  *     k_scale, v_scale   fp32 [n_blocks][n_kv_head]
- * the key being k * k_scale, the value v * v_scale.  table[r][j] (row stride
- * table_stride) is the block with positions 64 j .. 64 j + 63 of request r,
+ * the key being k * k_scale, the value v * v_scale (scales are not negative;
+ * +inf with codes 0 reads as NaN).  table[r][j] (row stride table_stride) is the block with positions 64 j .. 64 j + 63 of request r,
  * -1 where there is none; slot 64 b + i is token i of block b.  All layers
  * share the tables.
  *
@@ -631,7 +631,9 @@ int nb_kv_release(int32_t* table, int64_t table_stride, int32_t* lens, const int
  * (n_head + 2 n_kv_head) head_dim values q | k | v.  Queries and keys are
  * turned in pairs (2i, 2i + 1) by the angles cos_t / sin_t [n_pos][head_dim /
  * 2] of the row's position (NaN where it is not under n_pos); q_out row =
- * turned q * head_dim^-0.5 (stride ld_q, NB_F32 or NB_BF16).  Keys and values
+ * turned q * head_dim^-0.5 (stride ld_q, NB_F32 or NB_BF16; it may be qkv
+ * itself, of the same type and stride, and else overlaps it in no element;
+ * more than 2^24 workgroups, 3 n_kv_head a chunk, are refused).  Keys and values
  * go to the cache: with s the block's scale (0 before its first token), a
  * chunk's rows x set it to s' = max(s, max|x| * (1 / 127)), their codes to
  * clamp(rint(x / s'), -127, 127) and, where s' > s, the block's earlier codes
@@ -665,10 +667,12 @@ int nb_kv8_read(const int32_t* slots, int64_t n, const int8_t* k, const int8_t* 
  * the request has after the step, lens).  A block whose table entry lies
  * outside the cache is not seen; a row that sees nothing is 0.  q, out:
  * n_tokens rows of n_head * head_dim (strides ld_q, ld_out; NB_F32 or
- * NB_BF16).  Sums and statistics in fp32; with NB_F32 outputs products of 24
- * bits of q and of the softmax weights (each relative to the largest of its row) with the
- * exact codes, with NB_BF16 outputs of 16.  The workspace needs
- * nb_kv8_attention_ws_bytes(...) bytes, 16-byte aligned (0: may be NULL).
+ * NB_BF16; out may be q, of the same type and stride, and else overlaps it in
+ * no element).  softcap: 0, or finite from 1e-20 on.  Sums and statistics in
+ * fp32; with NB_F32 outputs products of 24 bits of q and of the softmax weights
+ * (each relative to the largest of its row) with the exact codes, with NB_BF16
+ * outputs of 16.  The workspace needs nb_kv8_attention_ws_bytes(...) bytes,
+ * 16-byte aligned (0: may be NULL).
  */
 int64_t nb_kv8_attention_ws_bytes(int n_tokens, int n_chunks, int max_blocks, int n_head,
                                   int n_kv_head, int head_dim);
@@ -681,8 +685,9 @@ int nb_kv8_attention(const void* q, int q_dtype, int64_t ld_q, const int32_t* ch
                      const int32_t* prefix, void* workspace, int64_t ws_bytes, void* stream);
 /*
  * Rules on `rows` rows of V logits (NB_F32 or NB_BF16, stride ld) and the
- * greedy choice; out fp32 (stride ld_out; may be logits).  For row b, token v,
- * in this order, each operation rounded by itself:
+ * greedy choice; out fp32 (stride ld_out; may be fp32 logits of the same stride,
+ * and else overlaps them in no element).  rows <= 65535, V <= 2^30.  For row b,
+ * token v, in this order, each operation rounded by itself:
  *     x = logits[b][v]
  *     x = x > 0 ? x / repetition[b] : x * repetition[b]
  *                                   if v is in history[b][0 .. lens[b])

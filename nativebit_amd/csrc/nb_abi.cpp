@@ -1172,6 +1172,22 @@ int check_rows(const char* fn, const char* name, const void* p, int dtype, int64
     return NB_OK;
 }
 
+// Whether `rows` rows written at `out` reach into those read at `in` (widths and
+// strides in elements), but for each row in its own place and type and for other
+// columns of the same array.
+bool rows_overlap(const void* in, int in_dtype, int64_t ld_in, int64_t in_width, const void* out,
+                  int out_dtype, int64_t ld_out, int64_t out_width, int64_t rows) {
+    if (in == out && in_dtype == out_dtype && (ld_in == ld_out || rows == 1)) return false;
+    const int64_t in_size = (int64_t)dtype_size(in_dtype), out_size = (int64_t)dtype_size(out_dtype);
+    const int64_t apart = (int64_t)(reinterpret_cast<uintptr_t>(out) - reinterpret_cast<uintptr_t>(in));
+    if (apart >= ((rows - 1) * ld_in + in_width) * in_size) return false;
+    if (-apart >= ((rows - 1) * ld_out + out_width) * out_size) return false;
+    const int64_t pitch = ld_in * in_size;
+    if (rows == 1 || pitch != ld_out * out_size) return true;
+    const int64_t column = (apart % pitch + pitch) % pitch;
+    return column < in_width * in_size || column + out_width * out_size > pitch;
+}
+
 // Chunks times the workgroups of each in one dimension of a grid of 256
 // threads each (under 2^32 work-items).
 int check_chunks(const char* fn, const void* chunks, int n_chunks, int64_t per_chunk) {
@@ -1267,6 +1283,10 @@ int nb_kv8_append(const void* qkv, int qkv_dtype, int64_t ld_qkv, const int32_t*
     if (!aligned(slots, 4) || !aligned(positions, 4) || !aligned(cos_t, 4) || !aligned(sin_t, 4)) {
         return fail(NB_EALIGN, "%s: misaligned pointer", fn);
     }
+    if (rows_overlap(qkv, qkv_dtype, ld_qkv, (int64_t)(n_head + 2 * n_kv_head) * head_dim, q_out,
+                     q_dtype, ld_q, (int64_t)n_head * head_dim, n_tokens)) {
+        return fail(NB_EINVAL, "%s: q_out overlaps qkv (in place: the same type and stride)", fn);
+    }
     if (n_chunks == 0) return NB_OK;
     st = ensure_device();
     if (st) return st;
@@ -1336,6 +1356,9 @@ int nb_kv8_attention(const void* q, int q_dtype, int64_t ld_q, const int32_t* ch
     if (!aligned(lens, 4) || !aligned(slopes, 4) || !aligned(prefix, 4)) {
         return fail(NB_EALIGN, "%s: misaligned pointer", fn);
     }
+    if (rows_overlap(q, q_dtype, ld_q, width, out, out_dtype, ld_out, width, n_tokens)) {
+        return fail(NB_EINVAL, "%s: out overlaps q (in place: the same type and stride)", fn);
+    }
     const int dev_st = ensure_device();
     const int64_t need = kv8_attention_bytes(n_chunks, n_tokens, max_blocks, n_head, n_kv_head, head_dim);
     if (ws_bytes < need || (need && !workspace)) {
@@ -1369,13 +1392,8 @@ int nb_logits_rules(const void* logits, int dtype, int64_t ld, int rows, int V,
     if (st) return st;
     st = check_rows(fn, "out", out, NB_F32, ld_out, V);
     if (st) return st;
-    if (out == logits && (dtype != NB_F32 || ld != ld_out)) {
-        return fail(NB_EINVAL, "%s: in place only over fp32 logits of the same stride", fn);
-    }
-    const char *in0 = static_cast<const char*>(logits), *out0 = reinterpret_cast<const char*>(out);
-    if (out0 != in0 && out0 < in0 + ((rows - 1) * ld + V) * (int64_t)dtype_size(dtype) &&
-        in0 < out0 + ((rows - 1) * ld_out + V) * 4) {
-        return fail(NB_EINVAL, "%s: out overlaps logits", fn);
+    if (rows_overlap(logits, dtype, ld, V, out, NB_F32, ld_out, V, rows)) {
+        return fail(NB_EINVAL, "%s: out overlaps logits (in place: fp32 of the same stride)", fn);
     }
     if ((history == nullptr) != (lens == nullptr)) return fail(NB_EINVAL, "%s: history and lens go together", fn);
     if (!history && (prompt_lens || repetition || frequency || presence)) {

@@ -581,10 +581,10 @@ def kv_plan(table: torch.Tensor, lens: torch.Tensor, new: torch.Tensor, free: to
     (nb_kv_plan): request r has ``lens[r]`` tokens cached and brings ``new[r]``;
     its new blocks come from the end of ``free[:state[0]]`` (``free`` has an entry
     for each block of the cache) and are entered in ``table`` (requests, blocks),
-    which is updated in place.  ``n_tokens`` is
-    the rows of the step (the sum of ``new``, or more: the rows behind have no
-    slot).  ``lens`` and ``state`` are left as they are; the plan's are those
-    after the step.  ``out``: a plan of the same sizes to write."""
+    which is updated in place.  ``n_tokens`` is the rows of the step (the sum of
+    ``new``, or more: the rows behind have no slot).  ``lens`` and ``state`` are
+    left as they are; the plan's are those after the step.  ``out``: a plan of
+    the same sizes to write."""
     dev, R, width, stride = _table(table)
     if not _here(dev):
         with torch.cuda.device(dev):
@@ -687,8 +687,8 @@ def kv8_append(qkv: torch.Tensor, plan: KVPlan, cos: torch.Tensor, sin: torch.Te
     8-bit cache (nb_kv8_append).  ``qkv`` (rows, (n_head + 2 heads) head_dim)
     float32 or bfloat16, ``cos`` / ``sin`` (positions, head_dim / 2) float32.
     Returns the turned queries times head_dim^-0.5, (rows, n_head head_dim) in
-    qkv's dtype (or into ``q``, which may be qkv's own query columns); rows
-    without a slot are not written."""
+    qkv's dtype (or into ``q``, which may be qkv's own query columns, and
+    overlaps it in no other way); rows without a slot are not written."""
     dev, n_blocks, n_kv, D = _kv8_cache(k, v, k_scale, v_scale)
     if not _here(dev):
         with torch.cuda.device(dev):
@@ -763,8 +763,8 @@ def kv8_attention(q: torch.Tensor, plan: KVPlan, table: torch.Tensor, k: torch.T
     query position); a query sees the positions up to its own, with ``window``
     > 0 only the last ``window`` of them, and with ``prefix`` (requests,)
     besides all before prefix[request].  Returns (rows, heads * head_dim) in
-    q's dtype or ``out_dtype`` (or into ``out``); rows without a slot are not
-    written."""
+    q's dtype or ``out_dtype`` (or into ``out``, which may be ``q``); rows
+    without a slot are not written."""
     dev, n_blocks, n_kv, D = _kv8_cache(k, v, k_scale, v_scale)
     if not _here(dev):
         with torch.cuda.device(dev):

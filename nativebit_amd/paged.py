@@ -197,6 +197,10 @@ def generate(model, prompts, n_generate: int, *, repetition=None, frequency=None
     room = model.context_len if cache is None else cache.max_len
     if max(lengths) + n_generate - 1 > room:     # (the last token is not fed)
         raise ValueError(f"{max(lengths)} prompt tokens and {n_generate} more exceed {room}")
+    if bias is not None and len(bias) != n:
+        raise ValueError(f"{len(bias)} bias dicts for {n} prompts")
+    if cache is not None and bool(cache.lens.any()):
+        raise ValueError("the cache holds requests already")
     if cache is None:
         blocks = sum(-(-(length + n_generate) // ops.KV_BLOCK) for length in lengths)
         cache = PagedCache(model, blocks, n, device=dev)

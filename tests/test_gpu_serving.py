@@ -679,3 +679,43 @@ def test_attention_split_prompts(dev, dt, rules):
     from nativebit_amd import _lib
     assert _lib.load().nb_kv8_attention_ws_bytes(n, p.chunks.shape[0], 40, 4, 2, 64) > 0
     check_attention(dev, p, t, want, q, cache, 4, dt, RULES[rules], rng)
+
+
+@pytest.mark.parametrize("lens,new,width,H,Hk,D", [
+    ([30, 0, 700], [1, 1, 1], 18, 6, 2, 64),            # single tokens
+    ([30, 5, 700], [200, 1, 70], 18, 6, 2, 64),         # prompts, codes shared
+    ([2100, 0, 700], [1, 3, 1], 40, 4, 2, 128),         # split
+    ([2100, 0, 700], [70, 1, 30], 40, 4, 2, 256),       # split prompts
+])
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+def test_attention_in_place(dev, lens, new, width, H, Hk, D, dt):
+    """out may be q, whole or columns of an array, and beside it in its rows."""
+    rng = np.random.default_rng(13)
+    p, t, want, n_blocks, n = step(dev, lens, new, width, 2, rng, rows=sum(new))
+    cache = [torch.from_numpy(a).to(dev) for a in random_cache(n_blocks, Hk, D, rng)]
+    q = torch.from_numpy(rng.standard_normal((n, H * D)).astype(np.float32) * 0.3).to(DT[dt]).to(dev)
+    out = ops.kv8_attention(q, p, t, *cache)
+    both = torch.full((n, 2 * H * D + 8), 3.0, dtype=DT[dt], device=dev)
+    both[:, :H * D] = q
+    ops.kv8_attention(both[:, :H * D], p, t, *cache, out=both[:, H * D + 8:])
+    assert torch.equal(both[:, :H * D], q) and torch.equal(both[:, H * D + 8:], out)
+    ops.kv8_attention(both[:, :H * D], p, t, *cache, out=both[:, :H * D])
+    assert torch.equal(both[:, :H * D], out) and bool((both[:, H * D:H * D + 8] == 3.0).all())
+    assert ops.kv8_attention(q, p, t, *cache, out=q) is q and torch.equal(q, out)
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+def test_append_in_place(dev, dt):
+    """q may be the query columns of qkv; the keys and values stay."""
+    rng = np.random.default_rng(14)
+    p, t, want, n_blocks, n = step(dev, [30, 0, 100], [70, 1, 3], 4, 2, rng, rows=74)
+    H, Hk, D = 4, 2, 64
+    qkv = torch.from_numpy(rng.standard_normal((n, (H + 2 * Hk) * D)).astype(np.float32)).to(DT[dt]).to(dev)
+    a = torch.from_numpy(rng.uniform(0, 6, (256, D // 2)).astype(np.float32)).to(dev)
+    first = [torch.from_numpy(x).to(dev) for x in random_cache(n_blocks, Hk, D, rng)]
+    again, mine = [x.clone() for x in first], qkv.clone()
+    q = ops.kv8_append(qkv, p, a.cos(), a.sin(), *first, H)
+    ops.kv8_append(mine, p, a.cos(), a.sin(), *again, H, q=mine[:, :H * D])
+    assert torch.equal(mine[:, :H * D], q) and torch.equal(mine[:, H * D:], qkv[:, H * D:])
+    for x, y in zip(first, again):
+        assert torch.equal(x, y)

@@ -56,3 +56,9 @@ def test_generate_refuses():
     for prompts in ([], [[]], [[1], []], [[10]], [[-1]]):
         with pytest.raises(ValueError):
             paged.generate(model, prompts, 1)
+    with pytest.raises(ValueError, match="bias"):
+        paged.generate(model, [[1], [2, 3]], 1, bias=[{1: 2.0}])
+    cache = paged.PagedCache(shape(context_len=20), 4, 2, device="cpu")
+    cache.lens[1] = 3
+    with pytest.raises(ValueError, match="holds requests"):
+        paged.generate(model, [[1], [2, 3]], 1, cache=cache)

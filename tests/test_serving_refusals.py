@@ -55,7 +55,7 @@ def test_release_refuses(kw, status):
 
 def append(**kw):
     a = dict(qkv=P, qkv_dtype=F32, ld=4 * 3 * 32, slots=P, positions=P, chunks=P, n_chunks=2, cos=P,
-             sin=P, n_pos=10, k=P, v=P, ks=P, vs=P, n_blocks=5, q=P, q_dtype=F32, ld_q=8 * 32,
+             sin=P, n_pos=10, k=P, v=P, ks=P, vs=P, n_blocks=5, q=P + (1 << 20), q_dtype=F32, ld_q=8 * 32,
              n_tokens=7, n_head=8, n_kv=2, D=32, stream=None)
     return call("nb_kv8_append", **{**a, **kw})
 
@@ -91,7 +91,7 @@ def test_read_refuses(kw, status):
 
 def attention(**kw):
     a = dict(q=P, q_dtype=F32, ld_q=256, chunks=P, n_chunks=2, lens=P, table=P, stride=4, R=3,
-             width=4, k=P, v=P, ks=P, vs=P, n_blocks=5, out=P, out_dtype=BF16, ld_out=256, n_tokens=7,
+             width=4, k=P, v=P, ks=P, vs=P, n_blocks=5, out=P + (1 << 20), out_dtype=BF16, ld_out=256, n_tokens=7,
              n_head=8, n_kv=2, D=32, softcap=0.0, window=0, slopes=None, prefix=None, ws=None,
              ws_bytes=0, stream=None)
     return call("nb_kv8_attention", **{**a, **kw})
@@ -135,6 +135,35 @@ def logits(**kw):
 ])
 def test_logits_refuses(kw, status):
     assert logits(**kw) == status
+
+
+Q_ROW, QKV_ROW = 8 * 32 * 4, 12 * 32 * 4   # bytes
+
+
+@pytest.mark.parametrize("f,kw,fits", [
+    # in place; the same memory in another type or stride, or moved
+    (append, dict(q=P, ld_q=384), True), (append, dict(q=P), False), (append, dict(q=P, n_tokens=1), True),
+    (append, dict(q=P, ld_q=384, q_dtype=BF16), False), (append, dict(q=P + 4, ld_q=384), False),
+    # in front, behind, one element into it
+    (append, dict(q=P - 7 * Q_ROW), True), (append, dict(q=P - 7 * Q_ROW + 4), False),
+    (append, dict(q=P + 7 * QKV_ROW), True), (append, dict(q=P + 7 * QKV_ROW - 4), False),
+    # columns beside it in rows of 640 and 639
+    (append, dict(ld=640, ld_q=640, q=P + QKV_ROW), True),
+    (append, dict(ld=640, ld_q=640, q=P - Q_ROW), True),
+    (append, dict(ld=639, ld_q=639, q=P + QKV_ROW), False),
+    (attention, dict(out=P, out_dtype=F32), True), (attention, dict(out=P), False),
+    (attention, dict(out=P, out_dtype=F32, ld_out=512), False),
+    (attention, dict(out=P - 7 * 512), True), (attention, dict(out=P - 7 * 512 + 2), False),
+    (attention, dict(out=P + 7 * 1024), True), (attention, dict(out=P + 7 * 1024 - 2), False),
+    (attention, dict(out=P + 1024, ld_q=512, ld_out=512, out_dtype=F32), True),
+    (attention, dict(out=P + 1020, ld_q=512, ld_out=512, out_dtype=F32), False),
+    (logits, dict(out=P), True), (logits, dict(out=P + 400, ld=200, ld_out=200), True),
+    (logits, dict(out=P + 396, ld=200, ld_out=200), False),
+])
+def test_outputs_over_inputs(f, kw, fits):
+    if fits and gpu_available():
+        pytest.skip("a GPU is there: the call would run")
+    assert f(**kw) == (_lib.NB_ENODEV if fits else EINVAL)
 
 
 def test_nothing_to_do_is_no_error():
