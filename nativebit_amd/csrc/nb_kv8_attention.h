@@ -131,6 +131,14 @@ __device__ __forceinline__ void digits4(const uint32_t* w, uint32_t* d) {
     }
 }
 
+// The largest of three; as one instruction (fmaxf of a number that came by
+// several ways quiets it first, with an instruction more for each).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
 template <int ND>
 struct Digits {
     static constexpr float kTop = ND == 3 ? 127.f * 65536.f : 127.f * 256.f;   // of |value| = 1
@@ -153,14 +161,14 @@ __device__ __forceinline__ void scale_if(int flag, float beta, float (&o)[4]) {
         : "scc");
 }
 
-// cap * tanh(x f) + add.  The tanh to 3e-7 of its value: the odd series up to
-// 0.3 (next term 1.3e-10 of it), above it 1 - 2 / (e^2t + 1), whose 6e-8 are
-// 2e-7 of 0.29.  For bf16 outputs the latter alone: 6e-8 of the cap in the
-// exponent.
+// cap * tanh(x f) + add, to_cap = add + cap.  The tanh to 3e-7 of its value: the
+// odd series up to 0.3 (next term 1.3e-10 of it), above it 1 - 2 / (e^2t + 1),
+// whose 6e-8 are 2e-7 of 0.29.  For bf16 outputs the latter alone: 6e-8 of the
+// cap in the exponent.
 template <int ND>
-__device__ __forceinline__ float capped(float x, float f, float cap, float add) {
+__device__ __forceinline__ float capped(float x, float f, float cap, float add, float to_cap) {
     const float e = __builtin_amdgcn_exp2f(x * (f * (2.f * kLog2e)));
-    const float far = fmaf(__builtin_amdgcn_rcpf(e + 1.f), -2.f * cap, cap + add);
+    const float far = fmaf(__builtin_amdgcn_rcpf(e + 1.f), -2.f * cap, to_cap);
     if constexpr (ND == 2) return far;
     const float t = x * f;
     const float z = t * t;
@@ -403,6 +411,11 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
         for (int dt = 0; dt < DT; ++dt) o[dt][0] = o[dt][1] = o[dt][2] = o[dt][3] = 0.f;
         float m = -INFINITY, l = 0.f;   // l: of the lane's own tokens
 
+        // Waves at their weights go before those at a product, whose MFMAs run on
+        // meanwhile: four prompts of 500 tokens, 24 heads of 64 on 8: 37.8 to 36.2
+        // us (bf16 outputs 31.5 to 30.1), 4096 tokens, 16 heads of 256 on 4: 326 to
+        // 308.  Not with two digits for longer heads: 233 to 245 there.
+        constexpr bool kAhead = kShared && (DT <= 4 || ND == 3);
         // Blocks n .. n + NB - 1 of the walk, one or two, at once: key(e, mt, s) and
         // value(e, dt) give the codes of the e-th, between() runs after the first
         // product.  Two share their weights' largest score and one step of O; the
@@ -454,7 +467,8 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
                         const float f = inv * unit[e] * per_cap;
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
-                            x[e][i] = capped<ND>(x[e][i], f, cap, fmaf(slope, (float)i, at));
+                            x[e][i] = capped<ND>(x[e][i], f, cap, fmaf(slope, (float)i, at),
+                                                 fmaf(slope, (float)i, at + cap));
                     } else {
                         const float f = to_log2 * unit[e];
 #pragma unroll
@@ -479,9 +493,11 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
                 }
                 float most = x[e][0];
 #pragma unroll
-                for (int i = 1; i < 16; ++i) most = fmaxf(most, x[e][i]);
+                for (int i = 1; i < 15; i += 2) most = max3(most, x[e][i], x[e][i + 1]);
+                most = max3(most, x[e][15], x[e][15]);
                 top[e] = rows_max(most) * unit[e];
             }
+            if constexpr (kAhead) __builtin_amdgcn_s_setprio(1);
             // ---- weights ------------------------------------------------------
             float all = top[0];
             if constexpr (NB == 2) all = fmaxf(all, top[1]);
@@ -539,6 +555,7 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
             const float share = __builtin_amdgcn_exp2f(all - fmaxf(m, kLowest));
             l = fmaf(sum, share, l);
             const float gamma = v_scale == 0.f ? 0.f : share * v_scale * (ND == 3 ? 256.f / kTop : 1.f / kTop);
+            if constexpr (kAhead) __builtin_amdgcn_s_setprio(0);
             // ---- O ------------------------------------------------------------
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
