@@ -39,9 +39,10 @@ typedef __attribute__((ext_vector_type(4))) uint16_t h4;
 constexpr int kThreads = 256;
 // Tokens of a workgroup: one group of four for each thread up to 2^20 logits
 // (more workgroups, each sooner done), two above (half as many that walk a
-// history).  With histories of 700 to 1000, in us: 1 row of 50257 6.0 (two 7.0),
-// 8 rows 6.8 (7.7); 16 rows of 131077 10.3 (one 11.3), 160 rows 40.7 (50), with
-// histories of 4000 45 (57; four groups, with 32 KB of LDS, 52).
+// history).  With histories of 700 to 1000, both launches, in us: 1 row of 50257
+// 5.7 (two 6.8), 8 rows 6.5 (7.5); 16 rows of 131077 9.9 (one 10.8), 160 rows 40
+// (48), with histories of 4000 44 (57; four groups, with 32 KB of LDS, 52).  512
+// threads with two groups: 42 for those, but 10.3 for the 16 rows.
 constexpr int tokens_of(int loads) { return 4 * kThreads * loads; }
 int loads_of(int rows, int V) { return (int64_t)rows * V <= 1 << 20 ? 1 : 2; }
 // An LDS word per token: seen in the history, has a bias, times in the answer.
