@@ -47,12 +47,14 @@
 // partial results in a workspace that a second launch joins.
 //
 // What bounds it.  Single tokens: the codes, 2 D bytes a cached token and head.
-// 64 requests of 960 positions at most, 20 heads of 128: 45 us, 5.3 TB/s; six of
-// 40000, 8 heads: 75 us with the join, 4.9 TB/s.  Prompts: the issue of vector
-// instructions and MFMAs, which overlap only in part.  16384 tokens, 16 heads
-// on 2: 563 TFLOP/s (of 4 D a score; each takes three int8 MFMA products in
-// fp32, two for bf16 outputs: 744).  Of 360 us for the 8003 tokens 125 go with
-// the second product, 85 with the first, 10 with the exponentials.
+// 64 requests of 960 positions at most, 20 heads of 128: 52 us, 4.6 TB/s from
+// memory (44 where they come from the last level cache); 128 of 2000, 8 heads:
+// 79 us, 5.0 TB/s; six of 40000, 8 heads: 78 us with the join, 4.7 TB/s.
+// Prompts: the issue of vector instructions and MFMAs, which overlap only in
+// part.  16384 tokens, 16 heads on 2: 563 TFLOP/s (of 4 D a score; each takes
+// three int8 MFMA products in fp32, two for bf16 outputs: 744).  Of 360 us for
+// the 8003 tokens 125 go with the second product, 85 with the first, 10 with
+// the exponentials.
 #pragma once
 
 #include <math.h>
@@ -190,18 +192,22 @@ __device__ __forceinline__ void to_lds16(uint32_t lds, const void* src) {
                  : "memory", "m0");
 }
 
-constexpr int kWavesKv8 = 4;   // of a workgroup
+// Waves of a workgroup: four where chunks share codes, else two.  Four for single
+// tokens cost their start and end: one of 200 requests of 300 positions, 20
+// heads of 128, 69 us against 57; of 128 of 2000, 8 heads 86 and 80, of 64 of 960,
+// 20 heads 55 and 53 (one wave: 56, 82, 52, but 51 against 39 for 40 of 1000, 8
+// heads of 256).
+constexpr int kv8_waves(bool prompts) { return prompts ? 4 : 2; }
 
 // LDS of a workgroup: the waves' results to join, or two blocks' codes.
 template <int DT, bool kShared>
 constexpr int kv8_lds_bytes() {
-    const int join = kWavesKv8 / 2 * (DT * 4 + 2) * 64 * 4, codes = 4 * 64 * 16 * DT;
+    const int join = kv8_waves(kShared) / 2 * (DT * 4 + 2) * 64 * 4, codes = 4 * 64 * 16 * DT;
     return kShared && codes > join ? codes : join;
 }
 
-template <int DT, int ND, bool kRules, bool kWhole, bool kShared>
+template <int DT, int ND, bool kRules, bool kWhole, int NW, bool kShared>
 __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chunk& ch, int h, char* lds) {
-    constexpr int NW = kWavesKv8;
     constexpr int DS = (DT + 3) / 4;   // steps of 64 dims of the first product
     constexpr float kTop = Digits<ND>::kTop;
     constexpr int kSlot = (DT * 4 + 2) * 64;      // floats of a wave's result
@@ -705,12 +711,13 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
 
 // kPrompts: chunks of over two tiles of 16 rows share their blocks' codes
 // through LDS, the others of the launch go as without.
-// Registers: those of three workgroups a CU, for heads of over 128 dims (O alone
-// is 64 of them) of two.  4096 prompt tokens, 16 heads of 256 on 4: 327 us, 230
-// for bf16 outputs; with all registers, one a CU, 374 and 310.
+// Registers: those of three waves a SIMD, for heads of over 128 dims (O alone is
+// 64 of them) of two.  4096 prompt tokens, 16 heads of 256 on 4: 327 us, 230
+// for bf16 outputs; with all registers, one a SIMD, 374 and 310.
 template <int DT, int ND, bool kRules, bool kWhole, bool kPrompts>
-__global__ __launch_bounds__(kWavesKv8 * 64, (DT <= 8 ? 3 : 2)) void kv8_attention_kernel(
+__global__ __launch_bounds__(kv8_waves(kPrompts) * 64, (DT <= 8 ? 3 : 2)) void kv8_attention_kernel(
     Kv8AttentionArgs a) {
+    constexpr int kWaves = kv8_waves(kPrompts);
     __shared__ __align__(16) char lds[kv8_lds_bytes<DT, kPrompts>()];
     // Heads vary fastest (neighbouring workgroups, dealt to the XCDs in turn,
     // then share no keys, and with heads a multiple of 8 an XCD's L2 holds its
@@ -720,21 +727,21 @@ __global__ __launch_bounds__(kWavesKv8 * 64, (DT <= 8 ? 3 : 2)) void kv8_attenti
     if (ch.n == 0) return;
     if constexpr (kPrompts) {
         if (ch.n * (a.n_head / a.n_kv) > 32) {
-            kv8_rows<DT, ND, kRules, kWhole, true>(a, ch, h, lds);
+            kv8_rows<DT, ND, kRules, kWhole, kWaves, true>(a, ch, h, lds);
             return;
         }
     }
-    kv8_rows<DT, ND, kRules, kWhole, false>(a, ch, h, lds);
+    kv8_rows<DT, ND, kRules, kWhole, kWaves, false>(a, ch, h, lds);
 }
 
 template <int DT, int ND, bool kWhole, bool kPrompts>
 void launch_kv8_form(const Kv8AttentionArgs& a, dim3 grid, bool rules, hipStream_t stream) {
     if (rules) {
         hipLaunchKernelGGL((kv8_attention_kernel<DT, ND, true, kWhole, kPrompts>), grid,
-                           dim3(kWavesKv8 * 64), 0, stream, a);
+                           dim3(kv8_waves(kPrompts) * 64), 0, stream, a);
     } else {
         hipLaunchKernelGGL((kv8_attention_kernel<DT, ND, false, kWhole, kPrompts>), grid,
-                           dim3(kWavesKv8 * 64), 0, stream, a);
+                           dim3(kv8_waves(kPrompts) * 64), 0, stream, a);
     }
 }
 

@@ -7,21 +7,22 @@
 namespace nb {
 namespace {
 
-// Workgroups over a row's blocks: three a CU (heads of over 128 dims two), what
-// their registers allow, over tables of 32 blocks or more, 8 blocks each at
-// least (two a wave).  One token of six requests of 40000 positions, 8 heads of
-// 128 (48 workgroups unsplit): 16 splits 75.7 us, 10 (two a CU) 78.8, 24 82; 4
-// heads of 256: 21 splits 85 us, 32 (three a CU) 97; of one request of 8000 17
-// us against 25 in splits of 32 blocks or more.  512 prompt tokens after 8000
-// (180 workgroups): 4 splits 114 us, one 229; 300 of two requests after 3000, 2
-// heads of 256: 8 blocks or more 45 us, 16 63, one split 129.  More than fill
-// the CUs cost their partial results: 2048 prompt tokens 60 us, in two splits 95.
+// Workgroups over a row's blocks: three a CU (heads of over 128 dims two), over
+// tables of 32 blocks or more, two blocks a wave at least.  One token of six
+// requests of 40000 positions, 8 heads of 128 (48 workgroups unsplit): 16 splits
+// 78 us, 10 (two a CU) 85, 21 (four) 80, 32 (six) 81; of 32 of 4000 50, 52, 49,
+// 51; of one of 8000 16.8 against 18 with four blocks a wave.  512 prompt tokens
+// after 8000 (180 workgroups): 4 splits 114 us, one 229; 300 of two requests
+// after 3000, 2 heads of 256: two blocks a wave 45 us, four 63, one split 129.
+// More than fill the CUs cost their partial results: 2048 prompt tokens 60 us,
+// in two splits 95.
 int splits_of(int n_chunks, int n_tokens, int max_blocks, int n_head, int n_kv, int D) {
+    const int waves = kv8_waves(n_tokens > n_chunks);
     const int64_t rows = ((int64_t)n_tokens + n_chunks - 1) / n_chunks * (n_head / n_kv);
-    const int64_t groups = (int64_t)n_chunks * n_kv * ((rows + 63) / 64);
+    const int64_t groups = (int64_t)n_chunks * n_kv * ((rows + 16 * waves - 1) / (16 * waves));
     const int64_t want = (D <= 128 ? 3 : 2) * device_cu_count();
     if (groups >= want || max_blocks < 32) return 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({want / groups, max_blocks / 8, 64}));
+    return (int)std::max<int64_t>(1, std::min<int64_t>({want / groups, max_blocks / (2 * waves), 64}));
 }
 
 // A wave takes a row and head at a time: the splits' maxima and sums in its
@@ -79,13 +80,14 @@ int launch_kv8_attention(const void* q, int q_dtype, int64_t ld_q, const int32_t
                        ld_out, slopes, prefix, static_cast<float*>(workspace), q_dtype, out_dtype,
                        four(q, q_dtype, ld_q), four(out, out_dtype, ld_out), n_chunks, n_tokens, R,
                        max_blocks, n_blocks, n_head, n_kv, D, window, softcap};
-    // a chunk of 64 tokens makes G groups of 64 rows
-    const int64_t rows = ((int64_t)n_tokens + n_chunks - 1) / n_chunks * (n_head / n_kv);
-    const int groups = (int)std::min<int64_t>(std::max<int64_t>(1, (rows + 63) / 64), 64);
-    const dim3 grid((unsigned)(n_chunks * n_kv), groups, splits);
-    const bool rules = softcap > 0.f || window > 0 || slopes || prefix;
     // whether there may be chunks of over 32 rows, by what the host knows
     const bool prompts = n_tokens > R && (int64_t)std::min(n_tokens, kKvBlock) * (n_head / n_kv) > 32;
+    // a chunk of 64 tokens makes G groups of 64 rows
+    const int64_t rows = ((int64_t)n_tokens + n_chunks - 1) / n_chunks * (n_head / n_kv);
+    const int of = 16 * kv8_waves(prompts);
+    const int groups = (int)std::min<int64_t>(std::max<int64_t>(1, (rows + of - 1) / of), 64);
+    const dim3 grid((unsigned)(n_chunks * n_kv), groups, splits);
+    const bool rules = softcap > 0.f || window > 0 || slopes || prefix;
     Kv8AttentionLaunch* launch =
         out_dtype == NB_BF16 ? (prompts ? launch_kv8_prompts_2 : launch_kv8_tokens_2)
                              : (prompts ? launch_kv8_prompts_3 : launch_kv8_tokens_3);
