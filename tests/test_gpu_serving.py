@@ -682,6 +682,25 @@ def test_attention_split_prompts(dev, dt, rules):
 
 
 @pytest.mark.parametrize("lens,new,width,H,Hk,D", [
+    ([130, 0, 700], [1, 1, 1], 18, 64, 1, 64),              # four tiles of rows a token
+    ([130, 0, 700], [1, 0, 1], 18, 40, 1, 256),             # two and a half
+    ([2100, 900], [1, 1], 40, 64, 1, 80),                   # split as well
+    ([3] * 40 + [100] + [0] * 59, [0] * 40 + [90] + [0] * 59, 18, 4, 2, 128),
+    ([3] * 40 + [2000] + [0] * 59, [1] * 40 + [47] + [0] * 59, 40, 8, 2, 64),
+])
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("rules", ["plain", "all"])
+def test_attention_many_rows_of_few_tokens(dev, lens, new, width, H, Hk, D, dt, rules):
+    """No more tokens than requests, but chunks of many rows: many heads that
+    share keys, one request that brings all tokens."""
+    rng = np.random.default_rng(15)
+    p, t, want, n_blocks, n = step(dev, lens, new, width, 2, rng)
+    assert n <= len(lens)
+    q = torch.from_numpy(rng.standard_normal((n, H * D)).astype(np.float32) * 0.3).to(DT[dt])
+    check_attention(dev, p, t, want, q, random_cache(n_blocks, Hk, D, rng), H, dt, RULES[rules], rng)
+
+
+@pytest.mark.parametrize("lens,new,width,H,Hk,D", [
     ([30, 0, 700], [1, 1, 1], 18, 6, 2, 64),            # single tokens
     ([30, 5, 700], [200, 1, 70], 18, 6, 2, 64),         # prompts, codes shared
     ([2100, 0, 700], [1, 3, 1], 40, 4, 2, 128),         # split
