@@ -17,8 +17,11 @@
 // What bounds them: memory.  One token writes D bytes of codes a head, and
 // reads the earlier codes of its block only when the scale grows.  Append, 32
 // query and 8 key / value heads of 128 in bf16, 96 tokens of 96 requests: 8 us;
-// 6001 fp32 prompt tokens, 20 heads of 128: 71 us for 276 MB in and out (3.9
-// TB/s).  Read, fp32 out: 6240 slots of 8 heads 16 us, 6577 of 20 heads 34.
+// fp32 prompts: 8000 tokens of those heads 68 us for 344 MB in and out (5.1
+// TB/s), 6001 of 20 heads 61 for 276 MB (4.5; from a cache that holds none of
+// them 71).  In bf16 the latter take 63: then the angles, which each head reads
+// again, the codes' arithmetic and the chain of loads are as long.  Read, fp32
+// out: 6240 slots of 8 heads 16 us, 6577 of 20 heads 34.
 #include <math.h>
 
 #include <algorithm>
@@ -142,6 +145,7 @@ struct AppendArgs {
     int64_t ld_q;
     int qkv_dtype, q_dtype, vec_in, vec_q, vec_cos;
     int n_pos, n_blocks, n_tokens, n_head, n_kv, D;
+    int shares;   // workgroups of a chunk's and head's queries
     float q_scale;
 };
 
@@ -176,15 +180,23 @@ __device__ __forceinline__ f4 turn4(f4 x, const Angles& w) {
     return r;
 }
 
-struct AppendChunk { int row0, n, block, before; };
+// The slot is looked at only when the first rows are on their way.
+struct AppendChunk {
+    int row0, n, slot;
+    __device__ __forceinline__ int block() const { return slot / kKvBlock; }
+    __device__ __forceinline__ int before() const { return slot % kKvBlock; }
+    __device__ __forceinline__ bool stored(int n_blocks) const {
+        return slot >= 0 && block() < n_blocks && before() + n <= kKvBlock;
+    }
+};
 
 // The queries of a chunk's rows that share key / value head h, kRows of a
-// thread at once.
+// thread at once; every shares-th batch from the share-th on.
 template <int kRows>
 __device__ __forceinline__ void append_queries(const AppendArgs& a, const AppendChunk& ch, int h,
-                                               int tr, int d, int rows) {
+                                               int share, int tr, int d, int rows) {
     const int G = a.n_head / a.n_kv, total = ch.n * G;
-    for (int e0 = tr; e0 < total; e0 += kRows * rows) {
+    for (int e0 = kRows * rows * share + tr; e0 < total; e0 += kRows * rows * a.shares) {
         f4 x[kRows];
         int pos[kRows];
         Angles w[kRows];
@@ -195,6 +207,7 @@ __device__ __forceinline__ void append_queries(const AppendArgs& a, const Append
             pos[i] = a.positions[t];
             x[i] = load4(a.qkv, a.qkv_dtype, t * a.ld_qkv + (h * G + e % G) * a.D + d, a.vec_in);
         }
+        if (!ch.stored(a.n_blocks)) return;
 #pragma unroll
         for (int i = 0; i < kRows; ++i) w[i] = angles_at(a, pos[i], d);
 #pragma unroll
@@ -215,12 +228,9 @@ __device__ __forceinline__ void append_queries(const AppendArgs& a, const Append
 template <int kRows, bool kKeys>
 __device__ __forceinline__ void append_codes(const AppendArgs& a, const AppendChunk& ch, int h,
                                              int tr, int d, int rows, float* wave_max, uint8_t* vt) {
-    const int D = a.D, n = ch.n, before = ch.before;
+    const int D = a.D, n = ch.n;
     const bool on = tr < rows;
-    const int64_t bh = (int64_t)ch.block * a.n_kv + h;
     const int64_t col = (int64_t)(a.n_head + (kKeys ? 0 : a.n_kv) + h) * D + d;
-    float* scale = (kKeys ? a.k_scale : a.v_scale) + bh;
-    const float s = before > 0 ? *scale : 0.f;
     // keys: rows tr, tr + rows, ..; values: kRows consecutive ones, whose codes
     // go to the transposed block by the dword
     auto row_of = [&](int p) { return kKeys ? p * rows + tr : tr * kRows + p; };
@@ -232,6 +242,11 @@ __device__ __forceinline__ void append_codes(const AppendArgs& a, const AppendCh
         if (kKeys) pos[p] = a.positions[t];
         x[p] = load4(a.qkv, a.qkv_dtype, t * a.ld_qkv + col, a.vec_in);
     }
+    if (!ch.stored(a.n_blocks)) return;
+    const int before = ch.before();
+    const int64_t bh = (int64_t)ch.block() * a.n_kv + h;
+    float* scale = (kKeys ? a.k_scale : a.v_scale) + bh;
+    const float s = before > 0 ? *scale : 0.f;
     if (kKeys) {
         constexpr int kBatch = kRows < 4 ? kRows : 4;
 #pragma unroll
@@ -349,21 +364,19 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(AppendArgs a) {
     __shared__ float wave_max[kThreads / 64];
     __shared__ __align__(16) uint8_t vt[kMost * kVtPitch];
     // the parts and heads of a chunk vary fastest: together they read its rows whole
-    const int parts = 3 * a.n_kv;
+    const int parts = (2 + a.shares) * a.n_kv;
     const int chunk = blockIdx.x / parts, which = blockIdx.x - chunk * parts;
-    const int part = which / a.n_kv, h = which - part * a.n_kv;   // 0 keys, 1 values, 2 queries
+    const int part = which / a.n_kv, h = which - part * a.n_kv;   // 0 keys, 1 values, 2 .. queries
     const auto* c = as_constant(a.chunks) + 4 * (int64_t)chunk;
     const int row0 = c[0], n = c[1];
     if (n <= 0 || row0 < 0 || n > kKvBlock || row0 > a.n_tokens - n) return;
-    const int slot = as_constant(a.slots)[row0];
-    const AppendChunk ch{row0, n, slot / kKvBlock, slot % kKvBlock};
-    if (slot < 0 || ch.block >= a.n_blocks || ch.before + n > kKvBlock) return;
+    const AppendChunk ch{row0, n, as_constant(a.slots)[row0]};
     const int per = a.D / 4, rows = kThreads / per;
     const int tr = threadIdx.x / per, d = 4 * (threadIdx.x - tr * per);
-    if (part == 2) {
+    if (part >= 2) {
         if (tr >= rows) return;
-        if (n * (a.n_head / a.n_kv) <= rows) append_queries<1>(a, ch, h, tr, d, rows);
-        else append_queries<4>(a, ch, h, tr, d, rows);
+        if (n * (a.n_head / a.n_kv) <= rows) append_queries<1>(a, ch, h, part - 2, tr, d, rows);
+        else append_queries<4>(a, ch, h, part - 2, tr, d, rows);
         return;
     }
     // rows of a thread: a single token's, or up to 64 / rows (rows >= 8 up to 128
@@ -453,6 +466,17 @@ bool four_aligned(const void* p, int dtype) {
 
 int kv8_max_head_dim() { return kMaxD; }
 
+// Workgroups of a chunk's queries that share a head's keys: two batches of four
+// rows a thread each (but no more of all than a grid holds).  8000 tokens, 32
+// heads on 8 of 128: 84 us with one for all, 68 so; 6001, 16 on 4 of 256: 80 and
+// 60 (one batch each 64).
+int query_shares(int n_chunks, int n_tokens, int n_head, int n_kv, int D) {
+    const int64_t rows = ((int64_t)n_tokens + n_chunks - 1) / n_chunks * (n_head / n_kv);
+    const int batch = 8 * (kThreads / (D / 4));
+    const int64_t most = ((1LL << 24) - 1) / ((int64_t)n_chunks * n_kv) - 2;
+    return (int)std::max<int64_t>(1, std::min((rows + batch - 1) / batch, most));
+}
+
 int launch_kv8_append(const void* qkv, int qkv_dtype, int64_t ld_qkv, const int32_t* slots,
                       const int32_t* positions, const int32_t* chunks, int n_chunks,
                       const float* cos_t, const float* sin_t, int n_pos, int8_t* k, int8_t* v,
@@ -464,9 +488,10 @@ int launch_kv8_append(const void* qkv, int qkv_dtype, int64_t ld_qkv, const int3
                  four_aligned(qkv, qkv_dtype) && ld_qkv % 4 == 0,
                  four_aligned(q_out, q_dtype) && ld_q % 4 == 0,
                  (reinterpret_cast<uintptr_t>(cos_t) | reinterpret_cast<uintptr_t>(sin_t)) % 8 == 0,
-                 n_pos, n_blocks, n_tokens, n_head, n_kv, D, (float)(1.0 / sqrt((double)D))};
+                 n_pos, n_blocks, n_tokens, n_head, n_kv, D,
+                 query_shares(n_chunks, n_tokens, n_head, n_kv, D), (float)(1.0 / sqrt((double)D))};
     hipLaunchKernelGGL(D <= 128 ? kv8_append_kernel<128> : kv8_append_kernel<kMaxD>,
-                       dim3((unsigned)n_chunks * 3 * n_kv), dim3(kThreads), 0, stream, a);
+                       dim3((unsigned)n_chunks * (2 + a.shares) * n_kv), dim3(kThreads), 0, stream, a);
     return check_launch("nb_kv8_append");
 }
 

@@ -42,7 +42,8 @@
 // and the reference that moves seldom; two blocks a turn (one maximum, one step
 // of O) instead of one: 384 to 371 in turn on one card, about 360 on others.
 //
-// Split.  A workgroup takes one chunk and key / value head (and 64 rows of it).
+// Split.  A workgroup takes one chunk and key / value head (and 64 rows of it, 32
+// of single tokens).
 // Few of them over long caches are split over workgroups too (gridDim.z), with
 // partial results in a workspace that a second launch joins.
 //

@@ -339,6 +339,7 @@ class PackedGPT(nn.Module):
                    make_linear, norm_eps=c.norm_eps, rope_theta=c.rope_theta,
                    block_size=c.block_size, n_entries=c.n_entries, device=device)
 
+    @torch.no_grad()
     def hidden(self, idx, kv_caches=None, pos_offset=0):
         """The blocks' outputs (B, T, n_embd) of tokens idx, before the final
         norm, and the new caches."""
@@ -349,6 +350,7 @@ class PackedGPT(nn.Module):
             caches.append(c)
         return x, caches
 
+    @torch.no_grad()
     def head(self, x):
         """The final norm and the tied, soft-capped head: fp32 logits."""
         h = self.ln_f(x)

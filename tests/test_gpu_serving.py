@@ -172,6 +172,7 @@ APPENDS = [
     ([0], [1], 1, 1, 16), ([5], [1], 2, 1, 64), ([63, 64, 0], [1, 1, 1], 4, 4, 128),
     ([0, 130, 7], [64, 0, 200], 4, 2, 80), ([1, 62], [63, 70], 6, 2, 96), ([30], [300], 3, 3, 256),
     ([10, 20, 90, 0], [3, 33, 1, 128], 8, 1, 48), ([17], [40], 20, 20, 128), ([3, 9], [31, 2], 2, 2, 112),
+    ([10, 0], [150, 33], 8, 1, 256), ([61], [200], 32, 4, 64),
 ]
 
 
