@@ -15,13 +15,12 @@
 // new rows makes s' +inf and the block's codes 0: the block then reads as NaN.
 //
 // What bounds them: memory.  One token writes D bytes of codes a head, and
-// reads the earlier codes of its block only when the scale grows.  Append, 32
-// query and 8 key / value heads of 128 in bf16, 96 tokens of 96 requests: 8 us;
-// fp32 prompts: 8000 tokens of those heads 68 us for 344 MB in and out (5.1
-// TB/s), 6001 of 20 heads 61 for 276 MB (4.5; from a cache that holds none of
-// them 71).  In bf16 the latter take 63: then the angles, which each head reads
-// again, the codes' arithmetic and the chain of loads are as long.  Read, fp32
-// out: 6240 slots of 8 heads 16 us, 6577 of 20 heads 34.
+// reads the earlier codes of its block only when the scale grows.  Append of 96
+// tokens of 96 requests, 32 query and 8 key / value heads of 128 in bf16: 8 us;
+// of 8000 prompt tokens of those heads 68 us in fp32 for 344 MB in and out (5.1
+// TB/s), 50 in bf16; of 6001 of 20 heads 58 in fp32 for 276 MB (4.8), 44 in bf16
+// (one form for both types: 62 and 64, with each bf16 load waited for by its
+// conversion).  Read, fp32 out: 6240 slots of 8 heads 15 us, 6577 of 20 heads 33.
 #include <math.h>
 
 #include <algorithm>
@@ -37,51 +36,36 @@ namespace nb {
 namespace {
 
 typedef __attribute__((ext_vector_type(4))) float f4;
-typedef __attribute__((ext_vector_type(4))) uint16_t h4;
+// (rows at any of their elements' places: one access all the same)
+typedef __attribute__((ext_vector_type(4), aligned(4))) float f4_any;
+typedef __attribute__((ext_vector_type(2), aligned(4))) float f2_any;
+typedef __attribute__((ext_vector_type(2), aligned(2))) uint32_t u2_any;
+typedef __attribute__((ext_vector_type(4), aligned(2))) uint16_t h4_any;
 
-// Four consecutive values from p + i in fp32 (vec: 4-value aligned).
-__device__ __forceinline__ f4 load4(const void* p, int dtype, int64_t i, bool vec) {
-    f4 r;
-    if (dtype == NB_F32) {
-        const float* s = static_cast<const float*>(p) + i;
-        if (vec) return *reinterpret_cast<const f4*>(s);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = s[e];
-        return r;
-    }
-    const bf16_bits* s = static_cast<const bf16_bits*>(p) + i;
-    if (vec) {
-        const h4 v = *reinterpret_cast<const h4*>(s);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = bf16_to_f32(v[e]);
-        return r;
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] = bf16_to_f32(s[e]);
-    return r;
+// The bits of four consecutive values from p + i: fp32, or two pairs of bf16 in
+// the first two.  values4 makes fp32 of them, when all loads are out (a
+// conversion beside its load would wait for each).
+__device__ __forceinline__ f4 load4(const void* p, int dtype, int64_t i) {
+    if (dtype == NB_F32) return *reinterpret_cast<const f4_any*>(static_cast<const float*>(p) + i);
+    const u2_any w = *reinterpret_cast<const u2_any*>(static_cast<const bf16_bits*>(p) + i);
+    return f4{__uint_as_float(w[0]), __uint_as_float(w[1]), 0.f, 0.f};
+}
+__device__ __forceinline__ f4 values4(f4 r, int dtype) {
+    if (dtype == NB_F32) return r;
+    const uint32_t a = __float_as_uint(r[0]), b = __float_as_uint(r[1]);
+    return f4{__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u), __uint_as_float(b << 16),
+              __uint_as_float(b & 0xffff0000u)};
 }
 
-__device__ __forceinline__ void store4(void* p, int dtype, int64_t i, f4 v, bool vec) {
+__device__ __forceinline__ void store4(void* p, int dtype, int64_t i, f4 v) {
     if (dtype == NB_F32) {
-        float* d = static_cast<float*>(p) + i;
-        if (vec) {
-            *reinterpret_cast<f4*>(d) = v;
-            return;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) d[e] = v[e];
+        *reinterpret_cast<f4_any*>(static_cast<float*>(p) + i) = v;
         return;
     }
-    bf16_bits* d = static_cast<bf16_bits*>(p) + i;
-    h4 b;
+    h4_any b;
 #pragma unroll
     for (int e = 0; e < 4; ++e) b[e] = f32_to_bf16_rne(v[e]);
-    if (vec) {
-        *reinterpret_cast<h4*>(d) = b;
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) d[e] = b[e];
+    *reinterpret_cast<h4_any*>(static_cast<bf16_bits*>(p) + i) = b;
 }
 
 // A block's scale as the codes need it.
@@ -143,7 +127,7 @@ struct AppendArgs {
     float *k_scale, *v_scale;
     void* q_out;
     int64_t ld_q;
-    int qkv_dtype, q_dtype, vec_in, vec_q, vec_cos;
+    int q_dtype;
     int n_pos, n_blocks, n_tokens, n_head, n_kv, D;
     int shares;   // workgroups of a chunk's and head's queries
     float q_scale;
@@ -152,17 +136,15 @@ struct AppendArgs {
 // Angles of dims d, d + 2 at a position; one outside the tables has none: NaN.
 struct Angles { float c[2], s[2]; };
 __device__ __forceinline__ Angles angles_at(const AppendArgs& a, int pos, int d) {
-    typedef __attribute__((ext_vector_type(2))) float f2;
     Angles r;
     const bool in = pos >= 0 && pos < a.n_pos;
     const int64_t o = (int64_t)(in ? pos : 0) * (a.D / 2) + d / 2;
     if (!in) {
         r.c[0] = r.c[1] = r.s[0] = r.s[1] = __builtin_nanf("");
-    } else if (a.vec_cos) {
-        const f2 c = *reinterpret_cast<const f2*>(a.cos_t + o), s = *reinterpret_cast<const f2*>(a.sin_t + o);
-        r.c[0] = c[0], r.c[1] = c[1], r.s[0] = s[0], r.s[1] = s[1];
     } else {
-        r.c[0] = a.cos_t[o], r.c[1] = a.cos_t[o + 1], r.s[0] = a.sin_t[o], r.s[1] = a.sin_t[o + 1];
+        const f2_any c = *reinterpret_cast<const f2_any*>(a.cos_t + o);
+        const f2_any s = *reinterpret_cast<const f2_any*>(a.sin_t + o);
+        r.c[0] = c[0], r.c[1] = c[1], r.s[0] = s[0], r.s[1] = s[1];
     }
     return r;
 }
@@ -192,40 +174,46 @@ struct AppendChunk {
 
 // The queries of a chunk's rows that share key / value head h, kRows of a
 // thread at once; every shares-th batch from the share-th on.
-template <int kRows>
+template <int kDtype, int kRows>
 __device__ __forceinline__ void append_queries(const AppendArgs& a, const AppendChunk& ch, int h,
                                                int share, int tr, int d, int rows) {
+    // row e of the n G: token e / G, head e % G of theirs; e goes on by `rows`
     const int G = a.n_head / a.n_kv, total = ch.n * G;
+    const int by_t = rows / G, by_g = rows - by_t * G;
     for (int e0 = kRows * rows * share + tr; e0 < total; e0 += kRows * rows * a.shares) {
         f4 x[kRows];
-        int pos[kRows];
+        int t[kRows], g[kRows], pos[kRows];
         Angles w[kRows];
+        t[0] = e0 / G, g[0] = e0 - t[0] * G;
+#pragma unroll
+        for (int i = 1; i < kRows; ++i) {
+            const bool wraps = g[i - 1] + by_g >= G;
+            t[i] = t[i - 1] + by_t + (wraps ? 1 : 0);
+            g[i] = g[i - 1] + by_g - (wraps ? G : 0);
+        }
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            const int e = min(e0 + i * rows, total - 1);   // (past the last: the last again)
-            const int64_t t = ch.row0 + e / G;
-            pos[i] = a.positions[t];
-            x[i] = load4(a.qkv, a.qkv_dtype, t * a.ld_qkv + (h * G + e % G) * a.D + d, a.vec_in);
+            const int64_t row = ch.row0 + min(t[i], ch.n - 1);   // (past the last: unused)
+            pos[i] = a.positions[row];
+            x[i] = load4(a.qkv, kDtype, row * a.ld_qkv + (h * G + g[i]) * a.D + d);
         }
         if (!ch.stored(a.n_blocks)) return;
 #pragma unroll
         for (int i = 0; i < kRows; ++i) w[i] = angles_at(a, pos[i], d);
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            const int e = e0 + i * rows;
-            if (e >= total) break;
-            const int64_t t = ch.row0 + e / G;
-            const f4 r = turn4(x[i], w[i]);
+            if (t[i] >= ch.n) break;
+            const f4 r = turn4(values4(x[i], kDtype), w[i]);
             f4 q;
 #pragma unroll
             for (int j = 0; j < 4; ++j) q[j] = r[j] * a.q_scale;
-            store4(a.q_out, a.q_dtype, t * a.ld_q + (h * G + e % G) * a.D + d, q, a.vec_q);
+            store4(a.q_out, a.q_dtype, (ch.row0 + (int64_t)t[i]) * a.ld_q + (h * G + g[i]) * a.D + d, q);
         }
     }
 }
 
 // The keys (kKeys) or values of a chunk, kRows rows a thread.
-template <int kRows, bool kKeys>
+template <int kDtype, int kRows, bool kKeys>
 __device__ __forceinline__ void append_codes(const AppendArgs& a, const AppendChunk& ch, int h,
                                              int tr, int d, int rows, float* wave_max, uint8_t* vt) {
     const int D = a.D, n = ch.n;
@@ -240,13 +228,15 @@ __device__ __forceinline__ void append_codes(const AppendArgs& a, const AppendCh
     for (int p = 0; p < kRows; ++p) {
         const int64_t t = ch.row0 + min(row_of(p), n - 1);   // (past the last: the last again)
         if (kKeys) pos[p] = a.positions[t];
-        x[p] = load4(a.qkv, a.qkv_dtype, t * a.ld_qkv + col, a.vec_in);
+        x[p] = load4(a.qkv, kDtype, t * a.ld_qkv + col);
     }
     if (!ch.stored(a.n_blocks)) return;
     const int before = ch.before();
     const int64_t bh = (int64_t)ch.block() * a.n_kv + h;
     float* scale = (kKeys ? a.k_scale : a.v_scale) + bh;
     const float s = before > 0 ? *scale : 0.f;
+#pragma unroll
+    for (int p = 0; p < kRows; ++p) x[p] = values4(x[p], kDtype);
     if (kKeys) {
         constexpr int kBatch = kRows < 4 ? kRows : 4;
 #pragma unroll
@@ -350,16 +340,17 @@ __device__ __forceinline__ void append_codes(const AppendArgs& a, const AppendCh
     }
 }
 
-template <int kRows>
+template <int kDtype, int kRows>
 __device__ __forceinline__ void append_part(const AppendArgs& a, const AppendChunk& ch, int h,
                                             int part, int tr, int d, int rows, float* wave_max,
                                             uint8_t* vt) {
-    if (part == 0) append_codes<kRows, true>(a, ch, h, tr, d, rows, wave_max, vt);
-    else append_codes<kRows, false>(a, ch, h, tr, d, rows, wave_max, vt);
+    if (part == 0) append_codes<kDtype, kRows, true>(a, ch, h, tr, d, rows, wave_max, vt);
+    else append_codes<kDtype, kRows, false>(a, ch, h, tr, d, rows, wave_max, vt);
 }
 
-// kMost: head dims up to it (the most rows of a thread go by them).
-template <int kMost>
+// kDtype: qkv's type.  kMost: head dims up to it (the most rows of a thread go by
+// them).
+template <int kDtype, int kMost>
 __global__ __launch_bounds__(kThreads) void kv8_append_kernel(AppendArgs a) {
     __shared__ float wave_max[kThreads / 64];
     __shared__ __align__(16) uint8_t vt[kMost * kVtPitch];
@@ -375,16 +366,16 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(AppendArgs a) {
     const int tr = threadIdx.x / per, d = 4 * (threadIdx.x - tr * per);
     if (part >= 2) {
         if (tr >= rows) return;
-        if (n * (a.n_head / a.n_kv) <= rows) append_queries<1>(a, ch, h, part - 2, tr, d, rows);
-        else append_queries<4>(a, ch, h, part - 2, tr, d, rows);
+        if (n * (a.n_head / a.n_kv) <= rows) append_queries<kDtype, 1>(a, ch, h, part - 2, tr, d, rows);
+        else append_queries<kDtype, 4>(a, ch, h, part - 2, tr, d, rows);
         return;
     }
     // rows of a thread: a single token's, or up to 64 / rows (rows >= 8 up to 128
     // dims, >= 4 up to 256)
-    if (n <= rows) append_part<1>(a, ch, h, part, tr, d, rows, wave_max, vt);
-    else if (n <= 4 * rows) append_part<4>(a, ch, h, part, tr, d, rows, wave_max, vt);
-    else if (n <= 8 * rows) append_part<8>(a, ch, h, part, tr, d, rows, wave_max, vt);
-    else if constexpr (kMost > 128) append_part<16>(a, ch, h, part, tr, d, rows, wave_max, vt);
+    if (n <= rows) append_part<kDtype, 1>(a, ch, h, part, tr, d, rows, wave_max, vt);
+    else if (n <= 4 * rows) append_part<kDtype, 4>(a, ch, h, part, tr, d, rows, wave_max, vt);
+    else if (n <= 8 * rows) append_part<kDtype, 8>(a, ch, h, part, tr, d, rows, wave_max, vt);
+    else if constexpr (kMost > 128) append_part<kDtype, 16>(a, ch, h, part, tr, d, rows, wave_max, vt);
 }
 
 // ---------------------------------------------------------------------------
@@ -396,8 +387,7 @@ constexpr int kReadSlots = 32;
 
 __global__ __launch_bounds__(kThreads) void kv8_read_kernel(
     const int32_t* slots, int64_t n, const int8_t* k, const int8_t* v, const float* k_scale,
-    const float* v_scale, int n_blocks, int n_kv, int D, void* keys, void* values, int dtype,
-    int vec) {
+    const float* v_scale, int n_blocks, int n_kv, int D, void* keys, void* values, int dtype) {
     __shared__ int8_t vt[kReadSlots][kMaxD + 4];   // (rows 65 dwords apart: a row a bank)
     const int64_t i0 = (int64_t)blockIdx.x * kReadSlots;
     const int h = blockIdx.y;
@@ -452,14 +442,10 @@ __global__ __launch_bounds__(kThreads) void kv8_read_kernel(
                 vr[e] = ok[i] ? (float)(int8_t)(vw >> (8 * e)) * vs[i] : 0.f;
             }
             const int64_t o = ((i0 + t) * n_kv + h) * D + d;
-            store4(keys, dtype, o, kr, vec);
-            store4(values, dtype, o, vr, vec);
+            store4(keys, dtype, o, kr);
+            store4(values, dtype, o, vr);
         }
     }
-}
-
-bool four_aligned(const void* p, int dtype) {
-    return reinterpret_cast<uintptr_t>(p) % (dtype == NB_F32 ? 16 : 8) == 0;
 }
 
 }  // namespace
@@ -467,9 +453,9 @@ bool four_aligned(const void* p, int dtype) {
 int kv8_max_head_dim() { return kMaxD; }
 
 // Workgroups of a chunk's queries that share a head's keys: two batches of four
-// rows a thread each (but no more of all than a grid holds).  8000 tokens, 32
-// heads on 8 of 128: 84 us with one for all, 68 so; 6001, 16 on 4 of 256: 80 and
-// 60 (one batch each 64).
+// rows a thread each (but no more of all than a grid holds).  8000 bf16 tokens,
+// 32 heads on 8 of 128: 84 us with one for all, 68 so; 6001 fp32, 16 on 4 of
+// 256: 80 and 60 (one batch each 64).
 int query_shares(int n_chunks, int n_tokens, int n_head, int n_kv, int D) {
     const int64_t rows = ((int64_t)n_tokens + n_chunks - 1) / n_chunks * (n_head / n_kv);
     const int batch = 8 * (kThreads / (D / 4));
@@ -484,24 +470,23 @@ int launch_kv8_append(const void* qkv, int qkv_dtype, int64_t ld_qkv, const int3
                       int64_t ld_q, int n_tokens, int n_head, int n_kv, int D,
                       hipStream_t stream) {
     AppendArgs a{qkv, ld_qkv, slots, positions, chunks, cos_t, sin_t, k, v, k_scale, v_scale,
-                 q_out, ld_q, qkv_dtype, q_dtype,
-                 four_aligned(qkv, qkv_dtype) && ld_qkv % 4 == 0,
-                 four_aligned(q_out, q_dtype) && ld_q % 4 == 0,
-                 (reinterpret_cast<uintptr_t>(cos_t) | reinterpret_cast<uintptr_t>(sin_t)) % 8 == 0,
+                 q_out, ld_q, q_dtype,
                  n_pos, n_blocks, n_tokens, n_head, n_kv, D,
                  query_shares(n_chunks, n_tokens, n_head, n_kv, D), (float)(1.0 / sqrt((double)D))};
-    hipLaunchKernelGGL(D <= 128 ? kv8_append_kernel<128> : kv8_append_kernel<kMaxD>,
-                       dim3((unsigned)n_chunks * (2 + a.shares) * n_kv), dim3(kThreads), 0, stream, a);
+    auto* kernel = qkv_dtype == NB_F32
+                       ? (D <= 128 ? kv8_append_kernel<NB_F32, 128> : kv8_append_kernel<NB_F32, kMaxD>)
+                       : (D <= 128 ? kv8_append_kernel<NB_BF16, 128> : kv8_append_kernel<NB_BF16, kMaxD>);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)n_chunks * (2 + a.shares) * n_kv), dim3(kThreads), 0,
+                       stream, a);
     return check_launch("nb_kv8_append");
 }
 
 int launch_kv8_read(const int32_t* slots, int64_t n, const int8_t* k, const int8_t* v,
                     const float* k_scale, const float* v_scale, int n_blocks, int n_kv, int D,
                     void* keys, void* values, int dtype, hipStream_t stream) {
-    const int vec = four_aligned(keys, dtype) && four_aligned(values, dtype);
     hipLaunchKernelGGL(kv8_read_kernel, dim3((unsigned)((n + kReadSlots - 1) / kReadSlots), n_kv), dim3(kThreads), 0,
                        stream, slots, n, k, v, k_scale, v_scale, n_blocks, n_kv, D, keys, values,
-                       dtype, vec);
+                       dtype);
     return check_launch("nb_kv8_read");
 }
 

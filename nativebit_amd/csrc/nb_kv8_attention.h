@@ -79,7 +79,7 @@ struct Kv8AttentionArgs {
     const float* slopes;
     const int32_t* prefix;
     float* part;        // split results: [rows][heads][splits][D], then (m, l) pairs
-    int q_dtype, out_dtype, vec_q, vec_out;
+    int q_dtype, out_dtype;
     int n_chunks, n_tokens, R, max_blocks, n_blocks, n_head, n_kv, D, window;
     float softcap;
 };
@@ -100,7 +100,10 @@ namespace {
 
 typedef __attribute__((ext_vector_type(4))) int i4;
 typedef __attribute__((ext_vector_type(4))) float f4;
-typedef __attribute__((ext_vector_type(4))) uint16_t h4;
+// (rows of q and out at any of their elements' places: one access all the same)
+typedef __attribute__((ext_vector_type(4), aligned(4))) float f4_any;
+typedef __attribute__((ext_vector_type(2), aligned(2))) uint32_t u2_any;
+typedef __attribute__((ext_vector_type(4), aligned(2))) uint16_t h4_any;
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLowest = -3.0e38f;   // stands for a maximum of -inf in differences
@@ -253,39 +256,30 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
         int i = (int)((int64_t)count * split / splits) + wk;
 
         // ---- the row of q, and the first block on its way -----------------------
+        // (its bits: pairs of bf16 stay as they are until the block's loads are
+        // out, and dims past D are read at the head's start)
         float x[DS][16];
+        if (a.q_dtype == NB_F32) {
+            const float* p = static_cast<const float*>(a.q) + q_row * a.ld_q + head * D;
 #pragma unroll
-        for (int s = 0; s < DS; ++s) {
-            const int d0 = 64 * s + 16 * g;
-            const int64_t at = q_row * a.ld_q + head * D + d0;
+            for (int s = 0; s < DS; ++s) {
+                const int d0 = 64 * s + 16 * g, at = d0 < D ? d0 : 0;   // (D is a multiple of 16)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[s][e] = 0.f;
-            if (d0 < D) {   // (D is a multiple of 16)
-                if (a.q_dtype == NB_F32) {
-                    const float* p = static_cast<const float*>(a.q) + at;
+                for (int e = 0; e < 16; e += 4) {
+                    const f4 v = *reinterpret_cast<const f4_any*>(p + at + e);
+                    x[s][e] = v[0], x[s][e + 1] = v[1], x[s][e + 2] = v[2], x[s][e + 3] = v[3];
+                }
+            }
+        } else {
+            const bf16_bits* p = static_cast<const bf16_bits*>(a.q) + q_row * a.ld_q + head * D;
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4) {
-                        if (a.vec_q) {
-                            const f4 v = *reinterpret_cast<const f4*>(p + e);
-                            x[s][e] = v[0], x[s][e + 1] = v[1], x[s][e + 2] = v[2], x[s][e + 3] = v[3];
-                        } else {
+            for (int s = 0; s < DS; ++s) {
+                const int d0 = 64 * s + 16 * g, at = d0 < D ? d0 : 0;
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) x[s][e + r] = p[e + r];
-                        }
-                    }
-                } else {
-                    const bf16_bits* p = static_cast<const bf16_bits*>(a.q) + at;
-#pragma unroll
-                    for (int e = 0; e < 16; e += 4) {
-                        if (a.vec_q) {
-                            const h4 v = *reinterpret_cast<const h4*>(p + e);
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) x[s][e + r] = bf16_to_f32(v[r]);
-                        } else {
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) x[s][e + r] = bf16_to_f32(p[e + r]);
-                        }
-                    }
+                for (int e = 0; e < 16; e += 4) {
+                    const u2_any v = *reinterpret_cast<const u2_any*>(p + at + e);
+                    x[s][e] = __uint_as_float(v[0]), x[s][e + 2] = __uint_as_float(v[1]);
+                    x[s][e + 1] = x[s][e + 3] = 0.f;
                 }
             }
         }
@@ -377,9 +371,24 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
         i4 qd[ND][DS];
         float inv;
         {
+            if (a.q_dtype != NB_F32) {
+#pragma unroll
+                for (int s = 0; s < DS; ++s) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        const uint32_t w = __float_as_uint(x[s][e]);
+                        x[s][e] = __uint_as_float(w << 16);
+                        x[s][e + 1] = __uint_as_float(w & 0xffff0000u);
+                    }
+                }
+            }
             float most = 0.f, odd = 0.f;
 #pragma unroll
             for (int s = 0; s < DS; ++s) {
+                if (64 * s + 16 * g >= D) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[s][e] = 0.f;
+                }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     most = fmaxf(most, fabsf(x[s][e]));
@@ -687,24 +696,12 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
             if (d >= D) continue;
             const f4 v = f4{o[dt][0], o[dt][1], o[dt][2], o[dt][3]} * norm;
             if (a.out_dtype == NB_F32) {
-                float* p = static_cast<float*>(a.out) + to + d;
-                if (a.vec_out) {
-                    *reinterpret_cast<f4*>(p) = v;
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) p[r] = v[r];
-                }
+                *reinterpret_cast<f4_any*>(static_cast<float*>(a.out) + to + d) = v;
             } else {
-                bf16_bits* p = static_cast<bf16_bits*>(a.out) + to + d;
-                h4 w;
+                h4_any w;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) w[r] = f32_to_bf16_rne(v[r]);
-                if (a.vec_out) {
-                    *reinterpret_cast<h4*>(p) = w;
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) p[r] = w[r];
-                }
+                *reinterpret_cast<h4_any*>(static_cast<bf16_bits*>(a.out) + to + d) = w;
             }
         }
     }

@@ -72,14 +72,10 @@ int launch_kv8_attention(const void* q, int q_dtype, int64_t ld_q, const int32_t
                          void* out, int out_dtype, int64_t ld_out, int n_tokens, int n_head,
                          int n_kv, int D, float softcap, int window, const float* slopes,
                          const int32_t* prefix, void* workspace, hipStream_t stream) {
-    auto four = [](const void* p, int dtype, int64_t ld) {
-        return reinterpret_cast<uintptr_t>(p) % (dtype == NB_F32 ? 16 : 8) == 0 && ld % 4 == 0;
-    };
     const int splits = splits_of(n_chunks, n_tokens, max_blocks, n_head, n_kv, D);
     Kv8AttentionArgs a{q, ld_q, chunks, lens, table, table_stride, k, v, k_scale, v_scale, out,
                        ld_out, slopes, prefix, static_cast<float*>(workspace), q_dtype, out_dtype,
-                       four(q, q_dtype, ld_q), four(out, out_dtype, ld_out), n_chunks, n_tokens, R,
-                       max_blocks, n_blocks, n_head, n_kv, D, window, softcap};
+                       n_chunks, n_tokens, R, max_blocks, n_blocks, n_head, n_kv, D, window, softcap};
     // whether there may be chunks of over 32 rows, by what the host knows
     const bool prompts = n_tokens > R && (int64_t)std::min(n_tokens, kKvBlock) * (n_head / n_kv) > 32;
     // a chunk of 64 tokens makes G groups of 64 rows
