@@ -17,11 +17,13 @@
 // of a row walks its whole history, from the L2: against 16 KB of logits read
 // and written, a history of 1000 is 4 KB.  LDS atomics are on whole numbers
 // (sums, or, maximum): no result depends on their order.  160 fp32 rows of
-// 131077 with histories of 4000: 45 us, 3.8 TB/s, and 5 us for the second launch
-// that turns the chosen keys into tokens; one row of 50257 4.5 and 1.6.
+// 131077, both launches: 37 us with histories of 1000 (4.6 TB/s), 42 with 4000
+// (40 and 44 with the masks' bits made beside their loads, which waited for
+// each); one row of 50257 5.6.
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "nb_device.h"
 #include "nb_internal.h"
@@ -34,7 +36,9 @@ namespace nb {
 namespace {
 
 typedef __attribute__((ext_vector_type(4))) float f4;
-typedef __attribute__((ext_vector_type(4))) uint16_t h4;
+// (logits at any of their elements' places: one access all the same)
+typedef __attribute__((ext_vector_type(4), aligned(4))) float f4_any;
+typedef __attribute__((ext_vector_type(2), aligned(2))) uint32_t u2_any;
 
 constexpr int kThreads = 256;
 // Tokens of a workgroup: one group of four for each thread up to 2^20 logits
@@ -42,7 +46,8 @@ constexpr int kThreads = 256;
 // history).  With histories of 700 to 1000, both launches, in us: 1 row of 50257
 // 5.7 (two 6.8), 8 rows 6.5 (7.5); 16 rows of 131077 9.9 (one 10.8), 160 rows 40
 // (48), with histories of 4000 44 (57; four groups, with 32 KB of LDS, 52).  512
-// threads with two groups: 42 for those, but 10.3 for the 16 rows.
+// threads with two groups: 42 for those, but 10.3 for the 16 rows.  (Both sides
+// of an earlier step, 3 to 7 % slower than now.)
 constexpr int tokens_of(int loads) { return 4 * kThreads * loads; }
 int loads_of(int rows, int V) { return (int64_t)rows * V <= 1 << 20 ? 1 : 2; }
 // An LDS word per token: seen in the history, has a bias, times in the answer.
@@ -59,7 +64,7 @@ struct LogitsArgs {
     float* out;
     uint64_t* keys;
     int32_t* tokens;
-    int dtype, V, max_history, n_bias;
+    int V, max_history, n_bias;
 };
 
 // Larger for larger values, and for the lower of equal tokens; 0 for -inf and NaN.
@@ -81,20 +86,20 @@ __device__ __forceinline__ uint64_t wave_max(uint64_t key) {
     return key;
 }
 
-// kVec: input and output rows begin at the same place of a group of four
-// elements, so that all groups but a row's first and last move as vectors.
-template <bool kVec, int kLoads>
+// kDtype: the logits' type.  Groups of four begin at 16-byte places of the
+// output's row: all but its first and last move as vectors.
+template <int kDtype, int kLoads>
 __global__ __launch_bounds__(kThreads) void logits_rules_kernel(LogitsArgs a) {
     constexpr int kTokens = tokens_of(kLoads);
     __shared__ __align__(16) uint32_t count[kTokens];
     __shared__ int32_t bias_at[kTokens];   // the place of the token's bias, where it has one
     __shared__ uint64_t wave_keys[kThreads / 64];
     const int b = blockIdx.y, tid = threadIdx.x;
-    const int esize = a.dtype == NB_F32 ? 4 : 2;
-    const char* in = static_cast<const char*>(a.logits) + b * a.ld * esize;
+    using In = std::conditional_t<kDtype == NB_F32, float, bf16_bits>;
+    const In* in = static_cast<const In*>(a.logits) + b * a.ld;
     float* out = a.out + b * a.ld_out;
     // group q of four elements holds tokens 4 q - shift ..
-    const int shift = kVec ? (int)(reinterpret_cast<uintptr_t>(in) / esize & 3) : 0;
+    const int shift = (int)(reinterpret_cast<uintptr_t>(out) / 4 & 3);
     const int v0 = (int)blockIdx.x * kTokens - shift;   // (V <= 2^30)
     // everything that the row's rules read is asked for before it is used: the
     // lengths, the first history entries and biases, the logits, the masks
@@ -112,37 +117,35 @@ __global__ __launch_bounds__(kThreads) void logits_rules_kernel(LogitsArgs a) {
     }
     const int bias_id = tid < a.n_bias ? a.bias_ids[b * a.ld_bias + tid] : -1;
     f4 x[kLoads];
-    uint32_t allowed[kLoads];   // bits of the group's four tokens
+    uint32_t m0[kLoads], m1[kLoads];   // the mask's words from the group's first token on
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
         const int v = v0 + 4 * (tid + j * kThreads);
-        if (kVec && v >= 0 && v + 3 < a.V) {
-            if (a.dtype == NB_F32) {
-                x[j] = *reinterpret_cast<const f4*>(in + 4 * (int64_t)v);
+        // (bf16 stay pairs until they are needed, so that no load is waited for here)
+        if (v >= 0 && v + 3 < a.V) {
+            if constexpr (kDtype == NB_F32) {
+                x[j] = *reinterpret_cast<const f4_any*>(in + v);
             } else {
-                const h4 w = *reinterpret_cast<const h4*>(in + 2 * (int64_t)v);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[j][e] = bf16_to_f32(w[e]);
+                const u2_any w = *reinterpret_cast<const u2_any*>(in + v);
+                x[j] = f4{__uint_as_float(w[0]), __uint_as_float(w[1]), 0.f, 0.f};
             }
         } else {
+            In e4[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const bool ok = v + e >= 0 && v + e < a.V;
-                x[j][e] = !ok ? 0.f
-                          : a.dtype == NB_F32 ? reinterpret_cast<const float*>(in)[v + e]
-                                              : bf16_to_f32(reinterpret_cast<const bf16_bits*>(in)[v + e]);
+            for (int e = 0; e < 4; ++e) e4[e] = v + e >= 0 && v + e < a.V ? in[v + e] : In{};
+            if constexpr (kDtype == NB_F32) {
+                x[j] = f4{e4[0], e4[1], e4[2], e4[3]};
+            } else {
+                x[j] = f4{__uint_as_float(e4[0] | (uint32_t)e4[1] << 16),
+                          __uint_as_float(e4[2] | (uint32_t)e4[3] << 16), 0.f, 0.f};
             }
         }
-        allowed[j] = 15;
-        if (a.mask) {
+        m0[j] = m1[j] = 0xffffffffu;
+        if (a.mask) {   // (a group that is not aligned may reach into the next word)
             const int32_t* mask = a.mask + b * a.ld_mask;
             const int last = (a.V - 1) >> 5, w = max(v, 0) >> 5;
-            const uint32_t m0 = mask[min(w, last)];
-            // (a group that is not aligned may reach into the next word, a row's
-            // first may begin before token 0)
-            const uint32_t m1 = kVec ? mask[min(w + 1, last)] : 0;
-            const uint64_t m = (uint64_t)m1 << 32 | m0;
-            allowed[j] = v >= 0 ? (uint32_t)(m >> (v & 31)) : m0 << -v;
+            m0[j] = mask[min(w, last)];
+            m1[j] = mask[min(w + 1, last)];
         }
     }
     const bool marked = hist || a.n_bias;   // whether there are words to look at
@@ -190,6 +193,14 @@ __global__ __launch_bounds__(kThreads) void logits_rules_kernel(LogitsArgs a) {
     for (int j = 0; j < kLoads; ++j) {
         const int at = 4 * (tid + j * kThreads);
         const int v = v0 + at;
+        if constexpr (kDtype == NB_BF16) {
+            const uint32_t w0 = __float_as_uint(x[j][0]), w1 = __float_as_uint(x[j][1]);
+            x[j] = f4{__uint_as_float(w0 << 16), __uint_as_float(w0 & 0xffff0000u),
+                      __uint_as_float(w1 << 16), __uint_as_float(w1 & 0xffff0000u)};
+        }
+        // bits of the group's four tokens (a row's first may begin before token 0)
+        const uint64_t m = (uint64_t)m1[j] << 32 | m0[j];
+        const uint32_t allowed = v >= 0 ? (uint32_t)(m >> (v & 31)) : m0[j] << -v;
         uint4 c4 = none;
         if (marked) c4 = *reinterpret_cast<const uint4*>(&count[at]);
         // the marked tokens of the group, one a turn: few lanes have any, hardly
@@ -209,12 +220,12 @@ __global__ __launch_bounds__(kThreads) void logits_rules_kernel(LogitsArgs a) {
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float y = allowed[j] >> e & 1 ? x[j][e] : -INFINITY;
+            const float y = allowed >> e & 1 ? x[j][e] : -INFINITY;
             x[j][e] = y;
             const bool in_row = v + e >= 0 && v + e < a.V;
             if (y > best && in_row) best = y, best_v = v + e;   // (a NaN is not over it)
         }
-        if (kVec && v >= 0 && v + 3 < a.V) {
+        if (v >= 0 && v + 3 < a.V) {
             *reinterpret_cast<f4*>(out + v) = x[j];
         } else {
 #pragma unroll
@@ -268,14 +279,12 @@ int launch_logits_rules(const void* logits, int dtype, int64_t ld, int rows, int
                         void* workspace, hipStream_t stream) {
     const LogitsArgs a{logits, ld, ld_out, ld_history, ld_bias, ld_mask, history, lens,
                        prompt_lens, repetition, frequency, presence, bias_ids, bias, mask, out,
-                       static_cast<uint64_t*>(workspace), tokens, dtype, V, max_history, n_bias};
-    const int esize = dtype == NB_F32 ? 4 : 2;
+                       static_cast<uint64_t*>(workspace), tokens, V, max_history, n_bias};
     const int parts = parts_of(rows, V);
-    const bool vec = ((reinterpret_cast<uintptr_t>(logits) / esize) & 3) ==
-                         ((reinterpret_cast<uintptr_t>(out) / 4) & 3) && (ld - ld_out) % 4 == 0;
-    auto* kernel = loads_of(rows, V) == 1
-                       ? (vec ? logits_rules_kernel<true, 1> : logits_rules_kernel<false, 1>)
-                       : (vec ? logits_rules_kernel<true, 2> : logits_rules_kernel<false, 2>);
+    const bool one = loads_of(rows, V) == 1;
+    auto* kernel = dtype == NB_F32
+                       ? (one ? logits_rules_kernel<NB_F32, 1> : logits_rules_kernel<NB_F32, 2>)
+                       : (one ? logits_rules_kernel<NB_BF16, 1> : logits_rules_kernel<NB_BF16, 2>);
     hipLaunchKernelGGL(kernel, dim3(parts, rows), dim3(kThreads), 0, stream, a);
     if (tokens && parts > 1) {
         hipLaunchKernelGGL(logits_choose_kernel, dim3(rows), dim3(64), 0, stream,
