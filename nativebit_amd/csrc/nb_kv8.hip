@@ -456,7 +456,7 @@ int kv8_max_head_dim() { return kMaxD; }
 // rows a thread each (but no more of all than a grid holds).  8000 bf16 tokens,
 // 32 heads on 8 of 128: 84 us with one for all, 68 so; 6001 fp32, 16 on 4 of
 // 256: 80 and 60 (one batch each 64).
-int query_shares(int n_chunks, int n_tokens, int n_head, int n_kv, int D) {
+static int query_shares(int n_chunks, int n_tokens, int n_head, int n_kv, int D) {
     const int64_t rows = ((int64_t)n_tokens + n_chunks - 1) / n_chunks * (n_head / n_kv);
     const int batch = 8 * (kThreads / (D / 4));
     const int64_t most = ((1LL << 24) - 1) / ((int64_t)n_chunks * n_kv) - 2;

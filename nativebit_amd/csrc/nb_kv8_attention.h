@@ -48,9 +48,9 @@
 // partial results in a workspace that a second launch joins.
 //
 // What bounds it.  Single tokens: the codes, 2 D bytes a cached token and head.
-// 64 requests of 960 positions at most, 20 heads of 128: 52 us, 4.6 TB/s from
+// 64 requests of 960 positions at most, 20 heads of 128: 51 us, 4.8 TB/s from
 // memory (44 where they come from the last level cache); 128 of 2000, 8 heads:
-// 79 us, 5.0 TB/s; six of 40000, 8 heads: 78 us with the join, 4.7 TB/s.
+// 77 us, 5.1 TB/s; six of 40000, 8 heads: 77 us with the join, 4.8 TB/s.
 // Prompts: the issue of vector instructions and MFMAs, which overlap only in
 // part.  16384 tokens, 16 heads on 2: 563 TFLOP/s (of 4 D a score; each takes
 // three int8 MFMA products in fp32, two for bf16 outputs: 744).  Of 360 us for
