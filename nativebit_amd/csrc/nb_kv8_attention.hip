@@ -78,10 +78,12 @@ int launch_kv8_attention(const void* q, int q_dtype, int64_t ld_q, const int32_t
                        n_chunks, n_tokens, R, max_blocks, n_blocks, n_head, n_kv, D, window, softcap};
     // whether there may be chunks of over 32 rows, by what the host knows
     const bool prompts = n_tokens > R && (int64_t)std::min(n_tokens, kKvBlock) * (n_head / n_kv) > 32;
-    // a chunk of 64 tokens makes G groups of 64 rows
-    const int64_t rows = ((int64_t)n_tokens + n_chunks - 1) / n_chunks * (n_head / n_kv);
-    const int of = 16 * kv8_waves(prompts);
-    const int groups = (int)std::min<int64_t>(std::max<int64_t>(1, (rows + of - 1) / of), 64);
+    // groups of rows of a chunk: the most that one may have (those of a prompt
+    // beside single tokens would else go one after the other), or, without
+    // prompts, the mean
+    const int64_t tokens = prompts ? std::min(n_tokens, kKvBlock) : (n_tokens + n_chunks - 1) / n_chunks;
+    const int64_t rows = tokens * (n_head / n_kv), of = 16 * kv8_waves(prompts);
+    const int groups = (int)std::min<int64_t>((rows + of - 1) / of, 64);
     const dim3 grid((unsigned)(n_chunks * n_kv), groups, splits);
     const bool rules = softcap > 0.f || window > 0 || slopes || prefix;
     Kv8AttentionLaunch* launch =
