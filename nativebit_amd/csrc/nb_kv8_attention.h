@@ -43,9 +43,8 @@
 // of O) instead of one: 384 to 371 in turn on one card, about 360 on others.
 //
 // Split.  A workgroup takes one chunk and key / value head (and 64 rows of it, 32
-// of single tokens).
-// Few of them over long caches are split over workgroups too (gridDim.z), with
-// partial results in a workspace that a second launch joins.
+// of single tokens).  Few of them over long caches are split over workgroups too
+// (gridDim.y), with partial results in a workspace that a second launch joins.
 //
 // What bounds it.  Single tokens: the codes, 2 D bytes a cached token and head.
 // 64 requests of 960 positions at most, 20 heads of 128: 51 us, 4.8 TB/s from
@@ -225,13 +224,13 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
     // waves of a row group (rw) and of a row's blocks (kw)
     const int rw = kShared || tiles > 2 ? NW : tiles, kw = NW / rw;
     const int wr = wave & (rw - 1), wk = wave / rw;
-    const int split = blockIdx.z, splits = gridDim.z;
+    const int split = blockIdx.y, splits = gridDim.y;
     const auto* blocks = as_constant(a.table) + ch.request * a.table_stride;
     const int cached = min(max(as_constant(a.lens)[ch.request], 0), a.max_blocks * kKvBlock);
     const int pre = kRules && a.prefix ? min(max(as_constant(a.prefix)[ch.request], 0), cached) : 0;
     const bool windowed = kRules && a.window > 0;
 
-    for (int group = blockIdx.y; group * rw < tiles; group += gridDim.y) {
+    for (int group = blockIdx.z; group * rw < tiles; group += gridDim.z) {
         const int tile = group * rw + wr;
         const int row = min(tile * 16 + c, rows - 1);   // (rows past the last repeat it)
         const int tok = row / G, head = h * G + row - tok * G;

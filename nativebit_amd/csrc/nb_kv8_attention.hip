@@ -25,12 +25,15 @@ int splits_of(int n_chunks, int n_tokens, int max_blocks, int n_head, int n_kv, 
     return (int)std::max<int64_t>(1, std::min<int64_t>({want / groups, max_blocks / (2 * waves), 64}));
 }
 
+constexpr int kJoinWaves = 4;
+
 // A wave takes a row and head at a time: the splits' maxima and sums in its
-// lanes, then the dims.  blockIdx.z takes every gridDim.z-th token of a chunk.
-__global__ __launch_bounds__(64) void kv8_join_kernel(Kv8AttentionArgs a, int splits) {
+// lanes, then the dims.  A chunk's tokens go to the waves of gridDim.z workgroups.
+__global__ __launch_bounds__(kJoinWaves * 64) void kv8_join_kernel(Kv8AttentionArgs a, int splits) {
     const Kv8Chunk ch = kv8_chunk(a, blockIdx.x);
-    const int head = blockIdx.y, lane = threadIdx.x;
-    for (int t = blockIdx.z; t < ch.n; t += gridDim.z) {
+    const int head = blockIdx.y, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int t = blockIdx.z * kJoinWaves + wave; t < ch.n; t += gridDim.z * kJoinWaves) {
         const int64_t row = ch.row0 + t, at = (row * a.n_head + head) * splits;
         const float* ml = a.part + (int64_t)a.n_tokens * a.n_head * splits * a.D + 2 * at;
         const float m = lane < splits ? ml[2 * lane] : -INFINITY;
@@ -78,21 +81,24 @@ int launch_kv8_attention(const void* q, int q_dtype, int64_t ld_q, const int32_t
                        n_chunks, n_tokens, R, max_blocks, n_blocks, n_head, n_kv, D, window, softcap};
     // whether there may be chunks of over 32 rows, by what the host knows
     const bool prompts = n_tokens > R && (int64_t)std::min(n_tokens, kKvBlock) * (n_head / n_kv) > 32;
-    // groups of rows of a chunk: the most that one may have (those of a prompt
-    // beside single tokens would else go one after the other), or, without
-    // prompts, the mean
-    const int64_t tokens = prompts ? std::min(n_tokens, kKvBlock) : (n_tokens + n_chunks - 1) / n_chunks;
-    const int64_t rows = tokens * (n_head / n_kv), of = 16 * kv8_waves(prompts);
+    // groups of rows of a chunk: the most that one may have (a prompt's beside
+    // single tokens would else go one after the other; those that a chunk does not
+    // have end at once, and come last in the grid: 32 tokens of 4000 positions 49
+    // us with them, 54 between the splits)
+    const int64_t rows = (int64_t)std::min(n_tokens, kKvBlock) * (n_head / n_kv);
+    const int of = 16 * kv8_waves(prompts);
     const int groups = (int)std::min<int64_t>((rows + of - 1) / of, 64);
-    const dim3 grid((unsigned)(n_chunks * n_kv), groups, splits);
+    const dim3 grid((unsigned)(n_chunks * n_kv), splits, groups);
     const bool rules = softcap > 0.f || window > 0 || slopes || prefix;
     Kv8AttentionLaunch* launch =
         out_dtype == NB_BF16 ? (prompts ? launch_kv8_prompts_2 : launch_kv8_tokens_2)
                              : (prompts ? launch_kv8_prompts_3 : launch_kv8_tokens_3);
     launch(a, grid, rules, stream);
     if (splits > 1) {
-        const int per = std::min(kKvBlock, (n_tokens + n_chunks - 1) / n_chunks);
-        hipLaunchKernelGGL(kv8_join_kernel, dim3(n_chunks, n_head, per), dim3(64), 0, stream, a, splits);
+        const int mean = std::min(kKvBlock, (n_tokens + n_chunks - 1) / n_chunks);
+        hipLaunchKernelGGL(kv8_join_kernel,
+                           dim3(n_chunks, n_head, (mean + kJoinWaves - 1) / kJoinWaves),
+                           dim3(kJoinWaves * 64), 0, stream, a, splits);
     }
     return check_launch("nb_kv8_attention");
 }
