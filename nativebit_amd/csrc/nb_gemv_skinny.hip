@@ -216,9 +216,10 @@ __device__ __forceinline__ void mfma_units_tile(const uint32_t (&d)[12], uint32_
 // global_load_lds_dwordx4: 16 bytes per lane from `src` to
 // LDS address m0 + 16 * lane (m0 = the wave-uniform `lds`).  Completion is
 // tracked by vmcnt only; the compiler does not see the LDS write, so the
-// waits below are explicit.
+// waits below are explicit; so is the wait state (s_nop) between a scalar write
+// of m0 and a load to LDS.
 __device__ __forceinline__ void dma16(uint32_t lds, const void* src) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                  :
                  : "s"(lds), "v"(src)
                  : "memory", "m0");
@@ -226,7 +227,7 @@ __device__ __forceinline__ void dma16(uint32_t lds, const void* src) {
 
 // The same load marked non-temporal: weights are read once per launch.
 __device__ __forceinline__ void dma16_nt(uint32_t lds, const void* src) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off nt"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt"
                  :
                  : "s"(lds), "v"(src)
                  : "memory", "m0");

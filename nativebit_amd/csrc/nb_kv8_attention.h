@@ -187,9 +187,10 @@ __device__ __forceinline__ float capped(float x, float f, float cap, float add, 
 }
 
 // 16 bytes a lane from `src` to LDS at m0 + 16 * lane, m0 = `lds`; counted by
-// vmcnt, unseen by the compiler.
+// vmcnt, unseen by the compiler.  (s_nop: the wait state between a scalar write
+// of m0 and a load to LDS.)
 __device__ __forceinline__ void to_lds16(uint32_t lds, const void* src) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                  :
                  : "s"(lds), "v"(src)
                  : "memory", "m0");

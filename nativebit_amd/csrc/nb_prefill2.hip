@@ -86,8 +86,9 @@ __device__ __forceinline__ uint32_t swz(int r, int c) {
     return (uint32_t)(r * kRowBytes + ((c ^ (r & 7)) << 4));
 }
 
+// (s_nop: the wait state between a scalar write of m0 and a load to LDS)
 __device__ __forceinline__ void dma16(uint32_t lds, const void* src) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                  :
                  : "s"(lds), "v"(src)
                  : "memory", "m0");

@@ -131,13 +131,14 @@ __device__ __forceinline__ T* uniform_ptr(T* p) {
 
 // One direct-to-LDS load: every lane reads 16 bytes at src + OFF, and lane
 // i's bytes land at LDS byte address lds + OFF + 16 i (the instruction
-// offset applies to both addresses).  Issued as inline asm so the compiler
+// offset applies to both addresses; the s_nop is the wait state between a
+// scalar write of m0 and a load to LDS).  Issued as inline asm so the compiler
 // does not track it: it would otherwise make every later LDS access wait
 // for all ring loads, draining the prefetch at each chunk.  Reads of the
 // destination are ordered after the load by wait_vm.
 template <int OFF>
 __device__ __forceinline__ void dma16(uint32_t lds, const void* src) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off offset:%2 nt"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%2 nt"
                  :
                  : "s"(lds), "v"(src), "n"(OFF)
                  : "memory", "m0");
