@@ -434,8 +434,8 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
         constexpr bool kAhead = kShared && (DT <= 4 || ND == 3);
         // Blocks n .. n + NB - 1 of the walk, one or two, at once: key(e, mt, s) and
         // value(e, dt) give the codes of the e-th, between() runs after the first
-        // product.  Two share their weights' largest score and one step of O; the
-        // ratio of their value scales is a factor of the weights' digits.
+        // product.  Two share their weights' largest score and one step of O; their
+        // value scales are factors of the weights' digits.
         auto walk = [&](auto nb, int n, auto&& key, auto&& between, auto&& value)
                         __attribute__((always_inline)) {
             constexpr int NB = decltype(nb)::value;
@@ -532,10 +532,18 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
             float v_scale = top[0] == -INFINITY ? 0.f : vs[0];
             float digits_of_1[NB] = {kTop};
             if constexpr (NB == 2) {
+                // v_scale: what the largest weights of a block bring at most, of
+                // the block that brings more, so that p * digits_of_1 is up to
+                // kTop (the larger scale alone would cost the other block's weights
+                // the scales' ratio where the row hardly weighs its block).  A
+                // scale that is NaN or infinite makes it NaN.
                 const float v0 = v_scale, v1 = top[1] == -INFINITY ? 0.f : vs[1];
-                v_scale = fmaxf(v0, v1);
-                digits_of_1[0] = v0 == v_scale ? kTop : kTop * (v0 / v_scale);
-                digits_of_1[1] = v1 == v_scale ? kTop : kTop * (v1 / v_scale);
+                const float c0 = v0 * __builtin_amdgcn_exp2f(top[0] - base);
+                const float c1 = v1 * __builtin_amdgcn_exp2f(top[1] - base);
+                v_scale = fmaxf(c0, c1) + (c0 + c1) * 0.f;
+                // (a ratio over 2^100 has weights under 2^-100)
+                digits_of_1[0] = kTop * fminf(v0 / v_scale, 0x1p100f);
+                digits_of_1[1] = kTop * fminf(v1 / v_scale, 0x1p100f);
             }
             float sum = 0.f;
             i4 pd[NB][ND];
