@@ -668,9 +668,9 @@ int nb_kv8_read(const int32_t* slots, int64_t n, const int8_t* k, const int8_t* 
  * outside the cache is not seen; a row that sees nothing is 0.  q, out:
  * n_tokens rows of n_head * head_dim (strides ld_q, ld_out; NB_F32 or
  * NB_BF16; out may be q, of the same type and stride, and else overlaps it in
- * no element).  softcap: 0, or finite from 1e-20 on.  Sums and statistics in
- * fp32; with NB_F32 outputs products of 24 bits of q and of the softmax weights
- * (each relative to the largest of its row) with the exact codes, with NB_BF16
+ * no element).  softcap: 0, or 1e-20 to 1e20.  Sums and statistics in fp32;
+ * with NB_F32 outputs products of 24 bits of q and of the softmax weights (each
+ * relative to the largest of its row) with the exact codes, with NB_BF16
  * outputs of 16.  The workspace needs nb_kv8_attention_ws_bytes(...) bytes,
  * 16-byte aligned (0: may be NULL).
  */

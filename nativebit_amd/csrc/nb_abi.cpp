@@ -1346,8 +1346,8 @@ int nb_kv8_attention(const void* q, int q_dtype, int64_t ld_q, const int32_t* ch
     if (st) return st;
     st = check_chunks(fn, chunks, n_chunks, n_kv_head);
     if (st) return st;
-    // (its reciprocal is a factor of the scores)
-    if (!(softcap >= 0.f) || !std::isfinite(softcap) || (softcap > 0.f && softcap < 1e-20f)) {
+    // (it and its reciprocal are factors of the scores)
+    if (!(softcap >= 0.f && softcap <= 1e20f) || (softcap > 0.f && softcap < 1e-20f)) {
         return fail(NB_EINVAL, "%s: softcap=%g", fn, (double)softcap);
     }
     if (window < 0) return fail(NB_EINVAL, "%s: window=%d", fn, window);

@@ -168,13 +168,14 @@ __device__ __forceinline__ void scale_if(int flag, float beta, float (&o)[4]) {
 
 // cap * tanh(x f) + add, to_cap = add + cap.  The tanh to 3e-7 of its value: the
 // odd series up to 0.3 (next term 1.3e-10 of it), above it 1 - 2 / (e^2t + 1),
-// whose 6e-8 are 2e-7 of 0.29.  For bf16 outputs the latter alone: 6e-8 of the
-// cap in the exponent.
-template <int ND>
+// whose 6e-8 are 2e-7 of 0.29.  Without the series (bf16 outputs, caps up to
+// kNearCap) the latter alone: 2^-22 of the cap in the exponent, 2^-14 at most.
+constexpr float kNearCap = 256.f;
+template <bool kSeries>
 __device__ __forceinline__ float capped(float x, float f, float cap, float add, float to_cap) {
     const float e = __builtin_amdgcn_exp2f(x * (f * (2.f * kLog2e)));
     const float far = fmaf(__builtin_amdgcn_rcpf(e + 1.f), -2.f * cap, to_cap);
-    if constexpr (ND == 2) return far;
+    if constexpr (!kSeries) return far;
     const float t = x * f;
     const float z = t * t;
     float p = 0.0035921280f;
@@ -481,10 +482,15 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
                     const float at = slope * (float)(j_lane - pos);
                     if (a.softcap > 0.f) {
                         const float f = inv * unit[e] * per_cap;
+                        auto cap_all = [&](auto series) __attribute__((always_inline)) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            x[e][i] = capped<ND>(x[e][i], f, cap, fmaf(slope, (float)i, at),
-                                                 fmaf(slope, (float)i, at + cap));
+                            for (int i = 0; i < 16; ++i)
+                                x[e][i] = capped<decltype(series)::value>(
+                                    x[e][i], f, cap, fmaf(slope, (float)i, at),
+                                    fmaf(slope, (float)i, at + cap));
+                        };
+                        if (ND == 2 && a.softcap <= kNearCap) cap_all(std::false_type{});
+                        else cap_all(std::true_type{});
                     } else {
                         const float f = to_log2 * unit[e];
 #pragma unroll

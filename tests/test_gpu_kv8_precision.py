@@ -124,3 +124,28 @@ def test_blocks_of_infinite_scale_are_nan_in_pairs(dev):
                 assert torch.isnan(out[:, D:]).all()
                 if not weigh:
                     assert torch.equal(out[:, :D], clean[:, :D])
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("cap", [3.0, 255.0, 257.0, 1e4, 1e6, 1e8, 1e20])
+@pytest.mark.parametrize("lens,new", [([70, 200], [60, 1]), ([70, 200, 3], [1, 1, 1])])
+def test_caps_far_above_the_scores(dev, dt, cap, lens, new):
+    """A cap's error goes by the score, not by the cap: 4e-7 of it (the tanh), for
+    bf16 outputs and caps up to 256 2^-14 in the exponent besides."""
+    rng = np.random.default_rng(4)
+    H, Hk, D = 4, 2, 64
+    p, t, want, n_blocks, n = step(dev, lens, new, 5, 1, rng)
+    cache = random_cache(n_blocks, Hk, D, rng)
+    q = torch.from_numpy(rng.standard_normal((n, H * D)).astype(np.float32) * 0.4).to(DT[dt])
+    gpu = [torch.from_numpy(a).to(dev) for a in cache]
+    out = host(ops.kv8_attention(q.to(dev), p, t, *gpu, softcap=cap).float()).reshape(n, H, D)
+    args = (q.float().numpy(), want[3], want[0], *cache, want[4])
+    exact, _, top = ref.attention(*args, softcap=cap)
+    _, loss, _ = ref.attention(*args)       # (the scores' sizes, without the cap's own term)
+    u = U if dt == "fp32" else 2.0 ** -16
+    blocks = 1 + int(want[4].max()) // 64
+    rel = 2 * ((u + 17 * U) * loss + (2.0 ** -14 if dt == "bf16" and cap <= 256 else 0))
+    rel = rel + 64 * u + (14 + 3 * blocks) * U
+    bound = (rel * top)[..., None] + (2.0 ** -8 * np.abs(exact) if dt == "bf16" else 0)
+    worst = (np.abs(out - exact) / bound).max()
+    assert worst <= 1, worst
