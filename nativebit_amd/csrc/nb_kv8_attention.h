@@ -168,14 +168,14 @@ __device__ __forceinline__ void scale_if(int flag, float beta, float (&o)[4]) {
 
 // cap * tanh(x f) + add, to_cap = add + cap.  The tanh to 3e-7 of its value: the
 // odd series up to 0.3 (next term 1.3e-10 of it), above it 1 - 2 / (e^2t + 1),
-// whose 6e-8 are 2e-7 of 0.29.  Without the series (bf16 outputs, caps up to
-// kNearCap) the latter alone: 2^-22 of the cap in the exponent, 2^-14 at most.
+// whose 6e-8 are 2e-7 of 0.29.  For bf16 outputs and caps up to kNearCap the
+// latter alone: 2^-22 of the cap in the exponent, 2^-14 at most.
 constexpr float kNearCap = 256.f;
-template <bool kSeries>
+template <int ND>
 __device__ __forceinline__ float capped(float x, float f, float cap, float add, float to_cap) {
     const float e = __builtin_amdgcn_exp2f(x * (f * (2.f * kLog2e)));
     const float far = fmaf(__builtin_amdgcn_rcpf(e + 1.f), -2.f * cap, to_cap);
-    if constexpr (!kSeries) return far;
+    if constexpr (ND == 2) return far;
     const float t = x * f;
     const float z = t * t;
     float p = 0.0035921280f;
@@ -185,6 +185,15 @@ __device__ __forceinline__ float capped(float x, float f, float cap, float add, 
     p = fmaf(p, z, 0.1333333333f);
     p = fmaf(p, z, -0.3333333333f);
     return z < 0.09f ? fmaf(fmaf(t * z, p, t), cap, add) : far;
+}
+
+// The same for bf16 outputs and larger caps, to 2^-16 of its value: t - t^3 / 3 up
+// to 2^-6.
+__device__ __forceinline__ float capped_wide(float x, float f, float cap) {
+    const float t = x * f, z = t * t;
+    const float e = __builtin_amdgcn_exp2f(t * (2.f * kLog2e));
+    const float far = fmaf(__builtin_amdgcn_rcpf(e + 1.f), -2.f * cap, cap);
+    return z < 0x1p-12f ? t * cap * fmaf(z, -0.33333333f, 1.f) : far;
 }
 
 // 16 bytes a lane from `src` to LDS at m0 + 16 * lane, m0 = `lds`; counted by
@@ -482,15 +491,16 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
                     const float at = slope * (float)(j_lane - pos);
                     if (a.softcap > 0.f) {
                         const float f = inv * unit[e] * per_cap;
-                        auto cap_all = [&](auto series) __attribute__((always_inline)) {
+                        if (ND == 2 && a.softcap > kNearCap) {
 #pragma unroll
                             for (int i = 0; i < 16; ++i)
-                                x[e][i] = capped<decltype(series)::value>(
-                                    x[e][i], f, cap, fmaf(slope, (float)i, at),
-                                    fmaf(slope, (float)i, at + cap));
-                        };
-                        if (ND == 2 && a.softcap <= kNearCap) cap_all(std::false_type{});
-                        else cap_all(std::true_type{});
+                                x[e][i] = fmaf(slope, (float)i, capped_wide(x[e][i], f, cap) + at);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                x[e][i] = capped<ND>(x[e][i], f, cap, fmaf(slope, (float)i, at),
+                                                     fmaf(slope, (float)i, at + cap));
+                        }
                     } else {
                         const float f = to_log2 * unit[e];
 #pragma unroll
