@@ -671,7 +671,8 @@ int nb_kv8_read(const int32_t* slots, int64_t n, const int8_t* k, const int8_t* 
  * no element).  softcap: 0, or 1e-20 to 1e20.  Sums and statistics in fp32;
  * with NB_F32 outputs products of 24 bits of q and of the softmax weights (each
  * relative to the largest of its row) with the exact codes, with NB_BF16
- * outputs of 16.  The workspace needs nb_kv8_attention_ws_bytes(...) bytes,
+ * outputs of 16; 8 more of q in rows whose largest value is over 8 times their
+ * mean one.  The workspace needs nb_kv8_attention_ws_bytes(...) bytes,
  * 16-byte aligned (0: may be NULL).
  */
 int64_t nb_kv8_attention_ws_bytes(int n_tokens, int n_chunks, int max_blocks, int n_head,

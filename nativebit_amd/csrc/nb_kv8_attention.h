@@ -18,7 +18,13 @@
 // orders less (O is scaled when it moves).  Scores, statistics and O are fp32.
 // Two digits (16 bits of q and of w, each relative to the largest of its row)
 // serve bf16 outputs, whose own rounding is 2^-9: 2^-17 is lost of q and w.
-// The codes go into the MFMAs as they are.
+// Rows of q with a few large dims need more: where the largest value is over
+// kEven times the mean one, q has a digit more (32 bits, bf16 outputs 24), and
+// with 32 the sum's halves A 2^8 + B and C 2^8 + E are added in fp32.  One dim 3000
+// times the others, keys small there: errors of 9e-5 without it and 3e-7 with
+// (bf16 outputs 3e-2 and 2e-3).  The rule is a row's own and so is its result; a
+// tile without such rows skips the digit.  8003 prompt tokens, 20 heads of 128: 365
+// us, 409 with the digit in all rows.  The codes go into the MFMAs as they are.
 //
 // Layout.  Everything is transposed, so that a lane keeps one row from the
 // scores to the output and no row's numbers pass through LDS.  Lane (c, g) =
@@ -105,6 +111,9 @@ typedef __attribute__((ext_vector_type(2), aligned(2))) uint32_t u2_any;
 typedef __attribute__((ext_vector_type(4), aligned(2))) uint16_t h4_any;
 
 constexpr float kLog2e = 1.44269504088896340736f;
+// Rows of q whose largest value is over this many times their mean one have a
+// digit more (of 128 normal ones it is 3.5 times).
+constexpr float kEven = 8.f;
 constexpr float kLowest = -3.0e38f;   // stands for a maximum of -inf in differences
 
 // The maximum / sum over the four lanes (c, 0 .. 3) of a row.
@@ -121,18 +130,24 @@ __device__ __forceinline__ float rows_sum(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// Four numbers I + 0x8080 (three digits) or I + 0x80 (two), the digits' bytes
-// gathered by digit: d[0] the lowest.
+// Four numbers I + 0x808080 (four digits), I + 0x8080 (three) or I + 0x80 (two),
+// the digits' bytes gathered by digit: d[0] the lowest.
 template <int ND>
 __device__ __forceinline__ void digits4(const uint32_t* w, uint32_t* d) {
     const uint32_t lo = __builtin_amdgcn_perm(w[1], w[0], 0x05010400);   // w0.0 w1.0 w0.1 w1.1
     const uint32_t hi = __builtin_amdgcn_perm(w[3], w[2], 0x05010400);
     d[0] = __builtin_amdgcn_perm(hi, lo, 0x05040100) ^ 0x80808080u;
     d[1] = __builtin_amdgcn_perm(hi, lo, 0x07060302);
+    if constexpr (ND >= 3) d[1] ^= 0x80808080u;
     if constexpr (ND == 3) {
-        d[1] ^= 0x80808080u;
         d[2] = __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0602) |
                __builtin_amdgcn_perm(w[3], w[2], 0x06020c0c);
+    }
+    if constexpr (ND == 4) {
+        const uint32_t lo2 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602);   // w0.2 w1.2 w0.3 w1.3
+        const uint32_t hi2 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602);
+        d[2] = __builtin_amdgcn_perm(hi2, lo2, 0x05040100) ^ 0x80808080u;
+        d[3] = __builtin_amdgcn_perm(hi2, lo2, 0x07060302);
     }
 }
 
@@ -146,8 +161,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 template <int ND>
 struct Digits {
-    static constexpr float kTop = ND == 3 ? 127.f * 65536.f : 127.f * 256.f;   // of |value| = 1
-    static constexpr int kBias = ND == 3 ? 0x8080 : 0x80;
+    // (of |value| = 1)
+    static constexpr float kTop = ND == 4 ? 127.f * 16777216.f : ND == 3 ? 127.f * 65536.f : 127.f * 256.f;
+    static constexpr int kBias = ND == 4 ? 0x808080 : ND == 3 ? 0x8080 : 0x80;
 };
 
 // o *= beta where flag (the same in all lanes) is not 0.  One instruction to
@@ -220,10 +236,22 @@ constexpr int kv8_lds_bytes() {
     return kShared && codes > join ? codes : join;
 }
 
+// Behind it the waves' lowest digits of q, each lane its own, read back by the
+// first products that need them.  In registers (4 for 64 dims) they cost the
+// others: 4096 prompt tokens, 16 heads of 256 on 4, 218 us so and 235; 1500 with
+// every rule, 20 heads of 128, 162 and 176.
+template <int DT, bool kShared>
+constexpr int kv8_low_bytes() {
+    return kv8_waves(kShared) * ((DT + 3) / 4) * 64 * 16;
+}
+
+// ND: digits of the weights and of most rows of q, NQ of the others.
 template <int DT, int ND, bool kRules, bool kWhole, int NW, bool kShared>
-__device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chunk& ch, int h, char* lds) {
+__device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chunk& ch, int h, char* lds,
+                                         char* low_lds) {
     constexpr int DS = (DT + 3) / 4;   // steps of 64 dims of the first product
-    constexpr float kTop = Digits<ND>::kTop;
+    constexpr int NQ = ND + 1;
+    constexpr float kTop = Digits<ND>::kTop, kTopQ = Digits<NQ>::kTop;
     constexpr int kSlot = (DT * 4 + 2) * 64;      // floats of a wave's result
     constexpr int kCodes = 64 * 16 * DT;          // bytes of a block's keys or values
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
@@ -378,8 +406,10 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
         }
 
         // ---- the row's digits -------------------------------------------------
-        i4 qd[ND][DS];
+        i4 qd[ND][DS];   // but the lowest digit
+        volatile i4* low_q = reinterpret_cast<volatile i4*>(low_lds) + wave * DS * 64 + lane;
         float inv;
+        bool fine;   // the row has a lowest digit
         {
             if (a.q_dtype != NB_F32) {
 #pragma unroll
@@ -392,7 +422,7 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
                     }
                 }
             }
-            float most = 0.f, odd = 0.f;
+            float most = 0.f, odd = 0.f, size = 0.f;
 #pragma unroll
             for (int s = 0; s < DS; ++s) {
                 if (64 * s + 16 * g >= D) {
@@ -402,31 +432,40 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     most = fmaxf(most, fabsf(x[s][e]));
+                    size += fabsf(x[s][e]);
                     odd += x[s][e] * 0.f;   // NaN if any is NaN or infinite
                 }
             }
-            // (rows below 2^-100 keep their size: 127 * 2^16 / most stays finite)
-            most = fmaxf(rows_max(most), 0x1p-100f);
+            most = rows_max(most);
+            fine = most * (float)D > kEven * rows_sum(size);
+            // (rows below 2^-90 keep their size: 127 * 2^24 / most stays finite)
+            most = fmaxf(most, 0x1p-90f);
             odd = rows_sum(odd);
-            const float f = kTop / most;
-            inv = most / kTop + odd;
-            if constexpr (ND == 3) inv *= 256.f;   // (the first product is in units of 2^8)
+            const float top = fine ? kTopQ : kTopQ / 256.f;
+            const int shift = fine ? 0 : 8;
+            const float f = top / most;
+            inv = most / kTopQ + odd;
+            inv *= NQ == 4 ? 65536.f : 256.f;   // (the first product's units)
 #pragma unroll
             for (int s = 0; s < DS; ++s) {
+                i4 low;
 #pragma unroll
                 for (int e = 0; e < 16; e += 4) {
-                    uint32_t w[4], d[3];
+                    uint32_t w[4], d[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float y = fminf(fmaxf(rintf(x[s][e + r] * f), -kTop), kTop);
-                        w[r] = (uint32_t)((int)y + Digits<ND>::kBias);
+                        const float y = fminf(fmaxf(rintf(x[s][e + r] * f), -top), top);
+                        w[r] = ((uint32_t)(int)y << shift) + (uint32_t)Digits<NQ>::kBias;
                     }
-                    digits4<ND>(w, d);
+                    digits4<NQ>(w, d);
+                    low[e / 4] = (int)d[0];
 #pragma unroll
-                    for (int n = 0; n < ND; ++n) qd[n][s][e / 4] = (int)d[n];
+                    for (int n = 0; n < ND; ++n) qd[n][s][e / 4] = (int)d[n + 1];
                 }
+                low_q[64 * s] = low;
             }
         }
+        const int any_fine = __builtin_amdgcn_readfirstlane(__any(fine));
         const float to_log2 = inv * kLog2e;
         // (for exponents of 2)
         const float slope = kRules && a.slopes ? a.slopes[head] * kLog2e : 0.f;
@@ -459,29 +498,51 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a, const Kv8Chu
                 // scores in units of 1 / unit: x * unit is the exponent of 2
                 unit[e] = as_constant(a.k_scale)[bh];
                 vs[e] = as_constant(a.v_scale)[bh];
-#pragma unroll
-                for (int mt = 0; mt < 4; ++mt) {
-                    i4 acc = {0, 0, 0, 0}, low = {128, 128, 128, 128}, f[DS];
-#pragma unroll
-                    for (int s = 0; s < DS; ++s) f[s] = key(e, mt, s);
-#pragma unroll
-                    for (int s = 0; s < DS; ++s)
-                        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[s], qd[ND - 1][s], acc, 0, 0, 0);
-                    if constexpr (ND == 3) {
-#pragma unroll
-                        for (int s = 0; s < DS; ++s)
-                            low = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[s], qd[0][s], low, 0, 0, 0);
-                        acc = (acc << 8) + (low >> 8);
-                    } else {
-                        acc <<= 8;
-                    }
-#pragma unroll
-                    for (int s = 0; s < DS; ++s)
-                        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[s], qd[ND - 2][s], acc, 0, 0, 0);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) x[e][4 * mt + r] = (float)acc[r];
-                }
             }
+            auto product = [&](auto lowest) __attribute__((always_inline)) {
+                i4 q0[DS];
+                if constexpr (lowest.value) {
+#pragma unroll
+                    for (int s = 0; s < DS; ++s) q0[s] = low_q[64 * s];
+                }
+#pragma unroll
+                for (int e = 0; e < NB; ++e) {
+#pragma unroll
+                    for (int mt = 0; mt < 4; ++mt) {
+                        i4 acc = {0, 0, 0, 0}, low = {0, 0, 0, 0}, f[DS];
+                        auto sum = [&](i4 to, const i4* q) {
+#pragma unroll
+                            for (int s = 0; s < DS; ++s)
+                                to = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[s], q[s], to, 0, 0, 0);
+                            return to;
+                        };
+#pragma unroll
+                        for (int s = 0; s < DS; ++s) f[s] = key(e, mt, s);
+                        float* y = &x[e][4 * mt];
+                        acc = sum(acc, qd[ND - 1]) << 8;
+                        if constexpr (ND == 3) low = sum(low, qd[0]);
+                        if constexpr (!lowest.value) {
+                            if constexpr (ND == 3) acc += (low + 128) >> 8;
+                            acc = sum(acc, qd[ND - 2]);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) y[r] = (float)acc[r];
+                        } else {
+                            low = sum(low << 8, q0);
+                            if constexpr (ND == 2) acc += (low + 128) >> 8;
+                            acc = sum(acc, qd[ND - 2]);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                y[r] = (float)acc[r];
+                                if constexpr (ND == 3)   // (the others as without)
+                                    y[r] = fine ? fmaf((float)low[r], 0x1p-16f, y[r])
+                                                : (float)(acc[r] + ((low[r] + 32768) >> 16));
+                            }
+                        }
+                    }
+                }
+            };
+            if (any_fine) product(std::true_type{});
+            else product(std::false_type{});
             between();
 #pragma unroll
             for (int e = 0; e < NB; ++e) {
@@ -740,7 +801,9 @@ template <int DT, int ND, bool kRules, bool kWhole, bool kPrompts>
 __global__ __launch_bounds__(kv8_waves(kPrompts) * 64, (DT <= 8 ? 3 : 2)) void kv8_attention_kernel(
     Kv8AttentionArgs a) {
     constexpr int kWaves = kv8_waves(kPrompts);
-    __shared__ __align__(16) char lds[kv8_lds_bytes<DT, kPrompts>()];
+    // (the codes first: loads to LDS take addresses of 16 bits)
+    constexpr int kBytes = kv8_lds_bytes<DT, kPrompts>();
+    __shared__ __align__(16) char lds[kBytes + kv8_low_bytes<DT, kPrompts>()];
     // Heads vary fastest (neighbouring workgroups, dealt to the XCDs in turn,
     // then share no keys, and with heads a multiple of 8 an XCD's L2 holds its
     // own heads only); the last chunks, which see the longest caches, go first.
@@ -749,11 +812,11 @@ __global__ __launch_bounds__(kv8_waves(kPrompts) * 64, (DT <= 8 ? 3 : 2)) void k
     if (ch.n == 0) return;
     if constexpr (kPrompts) {
         if (ch.n * (a.n_head / a.n_kv) > 32) {
-            kv8_rows<DT, ND, kRules, kWhole, kWaves, true>(a, ch, h, lds);
+            kv8_rows<DT, ND, kRules, kWhole, kWaves, true>(a, ch, h, lds, lds + kBytes);
             return;
         }
     }
-    kv8_rows<DT, ND, kRules, kWhole, kWaves, false>(a, ch, h, lds);
+    kv8_rows<DT, ND, kRules, kWhole, kWaves, false>(a, ch, h, lds, lds + kBytes);
 }
 
 template <int DT, int ND, bool kWhole, bool kPrompts>

@@ -149,3 +149,66 @@ def test_caps_far_above_the_scores(dev, dt, cap, lens, new):
     bound = (rel * top)[..., None] + (2.0 ** -8 * np.abs(exact) if dt == "bf16" else 0)
     worst = (np.abs(out - exact) / bound).max()
     assert worst <= 1, worst
+
+
+@pytest.mark.parametrize("dt,out_dt", [("fp32", "fp32"), ("bf16", "bf16"), ("fp32", "bf16"), ("bf16", "fp32")])
+@pytest.mark.parametrize("large", [1.0, 30.0, 300.0, 3000.0, 1e5])
+@pytest.mark.parametrize("lens,new,H,Hk,D", [([300], [70], 2, 2, 128), ([300, 40], [1, 1], 8, 2, 64),
+                                             ([130], [40], 2, 1, 256), ([70], [1], 3, 3, 80)])
+def test_rows_with_a_large_dim(dev, dt, out_dt, large, lens, new, H, Hk, D):
+    """One dim of q far above the others, whose keys are small there: the others
+    keep the bits that their scores need.  In rows whose largest value is over 8
+    times their mean one an element loses 2^-32 of it (bf16 outputs 2^-24) beside
+    its own rounding, in the others 2^-24 (2^-16); sums half a unit of 2^-15 of it
+    but with 32 bits."""
+    rng = np.random.default_rng(5)
+    p, t, want, n_blocks, n = step(dev, lens, new, 7, 1, rng)
+    cache = random_cache(n_blocks, Hk, D, rng)
+    cache[0][:, :, :, 7] = rng.integers(-1, 2, cache[0].shape[:3])
+    cache[2][:] = 0.02
+    q = rng.standard_normal((n, H, D)).astype(np.float32) * np.float32(D ** -0.5)
+    q[:, :, 7] *= np.float32(large)
+    q = torch.from_numpy(q.reshape(n, H * D)).to(DT[dt])
+    x = q.float().numpy().reshape(n, H, D).astype(np.float64)
+    gpu = [torch.from_numpy(a).to(dev) for a in cache]
+    out = host(ops.kv8_attention(q.to(dev), p, t, *gpu, out_dtype=DT[out_dt]).float()).reshape(n, H, D)
+    exact, _, top = ref.attention(q.float().numpy(), want[3], want[0], *cache, want[4])
+    table, blocks = want[0], 1 + int(want[4].max()) // 64
+    fine = out_dt == "fp32"
+    loss = np.zeros((n, H))
+    for row0, count, r, pos0 in want[3]:
+        for tok in range(row0, row0 + count):
+            end = pos0 + tok - row0 + 1
+            for h in range(H):
+                g = h // (H // Hk)
+                ids = table[r, :-(-end // 64)]
+                k = np.abs(cache[0][ids, g].astype(np.float64) * 0.02).reshape(-1, D)[:end]
+                peak = np.abs(x[tok, h]).max()
+                spread = peak * D > 8.01 * np.abs(x[tok, h]).sum()
+                # (a unit of the product's lower half, rounded to fp32: 2^-25)
+                unit = peak * 0.02 * (2.0 ** -25 if fine and spread else 2.0 ** -16)
+                digit = (2.0 ** -24 if fine else 2.0 ** -16) * (2.0 ** -8 if spread else 1)
+                loss[tok, h] = (11 * U * k @ np.abs(x[tok, h]) + digit * peak * k.sum(1) + unit).max()
+    u = U if fine else 2.0 ** -16
+    rel = 2 * loss + 64 * u + (14 + 3 * blocks) * U
+    bound = (rel * top)[..., None] + (0 if fine else 2.0 ** -8 * np.abs(exact))
+    worst = (np.abs(out - exact) / bound).max()
+    assert worst <= 1, worst
+
+
+def test_rows_keep_their_result_beside_others(dev):
+    """A row's result does not depend on what the rows of its tile need."""
+    rng = np.random.default_rng(6)
+    for lens, new, H, D in (([200], [70], 2, 128), ([200, 9], [1, 1], 16, 64)):
+        p, t, want, n_blocks, n = step(dev, lens, new, 5, 1, rng)
+        cache = [torch.from_numpy(a).to(dev) for a in random_cache(n_blocks, 1, D, rng)]
+        q = torch.from_numpy(rng.standard_normal((n, H, D)).astype(np.float32)).to(dev)
+        for out_dt in (torch.float32, torch.bfloat16):
+            even = ops.kv8_attention(q.view(n, -1), p, t, *cache, out_dtype=out_dt).view(n, H, D)
+            other = q.clone()
+            other[0, 0, 3] = other[-1, 1, 5] = 1e4
+            out = ops.kv8_attention(other.view(n, -1), p, t, *cache, out_dtype=out_dt).view(n, H, D)
+            same = torch.ones(n, H, dtype=torch.bool, device=dev)
+            same[0, 0] = same[-1, 1] = False
+            assert torch.equal(out[same], even[same])
+            assert not torch.equal(out, even)
