@@ -618,6 +618,16 @@ int nb_kv_plan(int32_t* table, int64_t table_stride, const int32_t* lens,
                int32_t* positions, int32_t* chunks, int32_t* lens_out, int32_t* state_out,
                void* stream);
 /*
+ * The same where no request may grow past max_len tokens, a model's context for
+ * one: its further tokens have no slot and count in state_out[1], as where the
+ * table ends (max_len is not a multiple of NB_KV_BLOCK then).
+ */
+int nb_kv_plan_max_len(int32_t* table, int64_t table_stride, const int32_t* lens,
+                       const int32_t* new_tokens, const int32_t* free_blocks, const int32_t* state,
+                       int n_requests, int max_blocks, int n_blocks, int n_tokens, int max_len,
+                       int32_t* slots, int32_t* positions, int32_t* chunks, int32_t* lens_out,
+                       int32_t* state_out, void* stream);
+/*
  * The blocks of every request r with finished[r] != 0 go to the end of the
  * free list (in place, with state[0], its count), its table entries become -1
  * and its length 0.  A block that several tables hold must be in one finished

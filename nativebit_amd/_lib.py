@@ -97,6 +97,8 @@ SIGNATURES = {
                                        _I, _P]),
     "nb_kv_plan_chunks": (_L, [_I, _I]),
     "nb_kv_plan": (_I, [_P, _L, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P]),
+    "nb_kv_plan_max_len": (_I, [_P, _L, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P,
+                                _P]),
     "nb_kv_release": (_I, [_P, _L, _P, _P, _P, _P, _I, _I, _I, _P]),
     "nb_kv8_append": (_I, [_P, _I, _L, _P, _P, _P, _I, _P, _P, _I, _P, _P, _P, _P, _I, _P, _I, _L,
                            _I, _I, _I, _I, _P]),

@@ -1203,15 +1203,15 @@ extern "C" {
 
 int64_t nb_kv_plan_chunks(int n_tokens, int n_requests) { return plan_chunks(n_tokens, n_requests); }
 
-int nb_kv_plan(int32_t* table, int64_t table_stride, const int32_t* lens,
-               const int32_t* new_tokens, const int32_t* free_blocks, const int32_t* state,
-               int n_requests, int max_blocks, int n_blocks, int n_tokens, int32_t* slots,
-               int32_t* positions, int32_t* chunks, int32_t* lens_out, int32_t* state_out,
-               void* stream) {
-    const char* fn = "nb_kv_plan";
+static int plan(const char* fn, int32_t* table, int64_t table_stride, const int32_t* lens,
+                const int32_t* new_tokens, const int32_t* free_blocks, const int32_t* state,
+                int n_requests, int max_blocks, int n_blocks, int n_tokens, int max_len,
+                int32_t* slots, int32_t* positions, int32_t* chunks, int32_t* lens_out,
+                int32_t* state_out, void* stream) {
     int st = check_tables(fn, table, table_stride, n_requests, max_blocks, n_blocks);
     if (st) return st;
     if (n_tokens < 0) return fail(NB_EINVAL, "%s: n_tokens=%d", fn, n_tokens);
+    if (max_len < 0) return fail(NB_EINVAL, "%s: max_len=%d", fn, max_len);
     if (n_requests > kv_plan_max_requests()) {
         return fail(NB_EUNSUPPORTED, "%s: n_requests=%d (<= %d)", fn, n_requests, kv_plan_max_requests());
     }
@@ -1235,8 +1235,28 @@ int nb_kv_plan(int32_t* table, int64_t table_stride, const int32_t* lens,
     if (st) return st;
     return launch_kv_plan(table, table_stride, lens, new_tokens, free_blocks, state, n_requests,
                           max_blocks, n_blocks, n_tokens, (int)plan_chunks(n_tokens, n_requests),
-                          slots, positions, chunks, lens_out, state_out,
+                          max_len, slots, positions, chunks, lens_out, state_out,
                           static_cast<hipStream_t>(stream));
+}
+
+int nb_kv_plan(int32_t* table, int64_t table_stride, const int32_t* lens,
+               const int32_t* new_tokens, const int32_t* free_blocks, const int32_t* state,
+               int n_requests, int max_blocks, int n_blocks, int n_tokens, int32_t* slots,
+               int32_t* positions, int32_t* chunks, int32_t* lens_out, int32_t* state_out,
+               void* stream) {
+    return plan("nb_kv_plan", table, table_stride, lens, new_tokens, free_blocks, state, n_requests,
+                max_blocks, n_blocks, n_tokens, 0x7fffffff, slots, positions, chunks, lens_out,
+                state_out, stream);
+}
+
+int nb_kv_plan_max_len(int32_t* table, int64_t table_stride, const int32_t* lens,
+                       const int32_t* new_tokens, const int32_t* free_blocks, const int32_t* state,
+                       int n_requests, int max_blocks, int n_blocks, int n_tokens, int max_len,
+                       int32_t* slots, int32_t* positions, int32_t* chunks, int32_t* lens_out,
+                       int32_t* state_out, void* stream) {
+    return plan("nb_kv_plan_max_len", table, table_stride, lens, new_tokens, free_blocks, state,
+                n_requests, max_blocks, n_blocks, n_tokens, max_len, slots, positions, chunks,
+                lens_out, state_out, stream);
 }
 
 int nb_kv_release(int32_t* table, int64_t table_stride, int32_t* lens, const int32_t* finished,

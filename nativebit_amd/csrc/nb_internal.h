@@ -221,9 +221,9 @@ constexpr int kKvBlock = NB_KV_BLOCK;   // tokens of a cache block
 int kv_plan_max_requests();
 int launch_kv_plan(int32_t* table, int64_t table_stride, const int32_t* lens,
                    const int32_t* new_tokens, const int32_t* free_blocks, const int32_t* state,
-                   int R, int max_blocks, int n_blocks, int n_tokens, int n_chunks, int32_t* slots,
-                   int32_t* positions, int32_t* chunks, int32_t* lens_out, int32_t* state_out,
-                   hipStream_t stream);
+                   int R, int max_blocks, int n_blocks, int n_tokens, int n_chunks, int max_len,
+                   int32_t* slots, int32_t* positions, int32_t* chunks, int32_t* lens_out,
+                   int32_t* state_out, hipStream_t stream);
 int launch_kv_release(int32_t* table, int64_t table_stride, int32_t* lens, const int32_t* finished,
                       int32_t* free_blocks, int32_t* state, int R, int max_blocks, int n_blocks,
                       hipStream_t stream);

@@ -3,7 +3,8 @@
 //
 //   nb_kv_plan      request r has lens[r] tokens cached and brings new[r].  The
 //                   rows of the step are the requests' new tokens in order;
-//                   with L = lens, N = new (clipped to the rows that exist)
+//                   with L = lens, N = new (clipped to the rows that exist and
+//                   to the length that a request may have)
 //                     first[r] = sum N[< r]             row of its first token
 //                     need[r]  = ceil((L + N) / 64) - ceil(L / 64)
 //                     base[r]  = sum need[< r]
@@ -79,7 +80,7 @@ struct PlanArgs {
     int32_t* table;
     int64_t table_stride;
     const int32_t *lens, *asked, *free_blocks, *state;
-    int R, max_blocks, n_blocks, n_tokens, n_chunks;
+    int R, max_blocks, n_blocks, n_tokens, n_chunks, max_len;
     int32_t *slots, *positions, *chunks, *lens_out, *state_out;
 };
 
@@ -98,6 +99,11 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
     __shared__ long long wave_dropped[kWaves];
     const int tid = threadIdx.x, nt = kPlanThreads;
     const int cap = a.max_blocks * kKvBlock;
+    // where a request of len tokens and n new ones ends, blocks allowing (one that
+    // is longer than it may be stays as it is)
+    auto end_of = [&](int len, int n) {
+        return max(len, (int)min((int64_t)len + n, (int64_t)min(cap, a.max_len)));
+    };
     const int left = min(max(a.state[0], 0), a.n_blocks);
     const int r0 = tid * kItems;
     int len[kItems], asked[kItems], n[kItems], want[kItems], count[kItems];
@@ -120,7 +126,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
         upto += min(asked[i], a.n_tokens);
         n[i] = min(upto, a.n_tokens) - first;
         rows_upto[r0 + i] = first + n[i];
-        want[i] = blocks_of((int)min((int64_t)len[i] + n[i], (int64_t)cap)) - blocks_of(len[i]);
+        want[i] = blocks_of(end_of(len[i], n[i])) - blocks_of(len[i]);
         sum += want[i];
     }
     long long dropped = 0;   // tokens asked for and not stored
@@ -132,8 +138,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
         const int have = blocks_of(len[i]), got = min(want[i], max(left - upto, 0));
         upto += want[i];
         need_upto[r0 + i] = upto;
-        int end = (int)min((int64_t)len[i] + n[i], (int64_t)cap);
-        end = max(len[i], min(end, (have + got) * kKvBlock));
+        const int end = max(len[i], min(end_of(len[i], n[i]), (have + got) * kKvBlock));
         count[i] = end > len[i] ? (end - 1) / kKvBlock - len[i] / kKvBlock + 1 : 0;
         sum += count[i];
         dropped += (long long)asked[i] - (end - len[i]);
@@ -163,8 +168,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
         q.have = blocks_of(q.len);
         const int want = need_upto[r] - q.base;
         const int got = min(want, max(left - q.base, 0));
-        const int end = (int)min((int64_t)q.len + rows_upto[r] - q.first, (int64_t)cap);
-        q.end = max(q.len, min(end, (q.have + got) * kKvBlock));
+        q.end = max(q.len, min(end_of(q.len, rows_upto[r] - q.first), (q.have + got) * kKvBlock));
         return q;
     };
     auto new_block = [&](int rank) { return a.free_blocks[left - 1 - rank]; };   // rank < left
@@ -269,11 +273,11 @@ int kv_plan_max_requests() { return kMaxRequests; }
 
 int launch_kv_plan(int32_t* table, int64_t table_stride, const int32_t* lens,
                    const int32_t* new_tokens, const int32_t* free_blocks, const int32_t* state,
-                   int R, int max_blocks, int n_blocks, int n_tokens, int n_chunks, int32_t* slots,
-                   int32_t* positions, int32_t* chunks, int32_t* lens_out, int32_t* state_out,
-                   hipStream_t stream) {
+                   int R, int max_blocks, int n_blocks, int n_tokens, int n_chunks, int max_len,
+                   int32_t* slots, int32_t* positions, int32_t* chunks, int32_t* lens_out,
+                   int32_t* state_out, hipStream_t stream) {
     const PlanArgs a{table, table_stride, lens, new_tokens, free_blocks, state, R, max_blocks,
-                     n_blocks, n_tokens, n_chunks, slots, positions, chunks, lens_out, state_out};
+                     n_blocks, n_tokens, n_chunks, max_len, slots, positions, chunks, lens_out, state_out};
     const int groups = std::min(256, std::max(1, (n_tokens + kPlanThreads - 1) / kPlanThreads));
     auto* kernel = R <= kPlanThreads ? kv_plan_kernel<1>
                    : R <= 4 * kPlanThreads ? kv_plan_kernel<4>

@@ -576,20 +576,23 @@ def kv_plan_chunks(n_tokens: int, n_requests: int) -> int:
 
 
 def kv_plan(table: torch.Tensor, lens: torch.Tensor, new: torch.Tensor, free: torch.Tensor,
-            state: torch.Tensor, n_tokens: int, out: KVPlan | None = None) -> KVPlan:
+            state: torch.Tensor, n_tokens: int, out: KVPlan | None = None,
+            max_len: int | None = None) -> KVPlan:
     """The plan of a serving step from the requests' lengths, on the GPU
-    (nb_kv_plan): request r has ``lens[r]`` tokens cached and brings ``new[r]``;
+    (nb_kv_plan_max_len): request r has ``lens[r]`` tokens cached and brings ``new[r]``;
     its new blocks come from the end of ``free[:state[0]]`` (``free`` has an entry
     for each block of the cache) and are entered in ``table`` (requests, blocks),
     which is updated in place.  ``n_tokens`` is the rows of the step (the sum of
     ``new``, or more: the rows behind have no slot).  ``lens`` and ``state`` are
     left as they are; the plan's are those after the step.  ``out``: a plan of
-    the same sizes to write."""
+    the same sizes to write.  ``max_len``: the tokens that a request may have
+    (the table's, by default); those past it have no slot."""
     dev, R, width, stride = _table(table)
     if not _here(dev):
         with torch.cuda.device(dev):
-            return kv_plan(table, lens, new, free, state, n_tokens, out)
+            return kv_plan(table, lens, new, free, state, n_tokens, out, max_len)
     n_tokens = int(n_tokens)
+    max_len = 0x7fffffff if max_len is None else min(int(max_len), 0x7fffffff)
     i32, n_blocks = torch.int32, free.numel()
     if not (_is(lens, i32, (R,), dev) and _is(new, i32, (R,), dev) and
             _is(free, i32, (n_blocks,), dev) and _is(state, i32, (2,), dev)):
@@ -617,9 +620,9 @@ def kv_plan(table: torch.Tensor, lens: torch.Tensor, new: torch.Tensor, free: to
                                ("state", out.state, (2,))):
             _require(f"out.{name}", t, i32, shape, dev)
         s, p, c, l, st = (t.data_ptr() for t in out)
-    status = _lib.load().nb_kv_plan(
+    status = _lib.load().nb_kv_plan_max_len(
         table.data_ptr(), stride, lens.data_ptr(), new.data_ptr(), free.data_ptr(),
-        state.data_ptr(), R, width, n_blocks, n_tokens, s, p, c, l, st,
+        state.data_ptr(), R, width, n_blocks, n_tokens, max_len, s, p, c, l, st,
         torch._C._cuda_getCurrentRawStream(dev))
     if status:
         _lib.check(status)

@@ -133,7 +133,8 @@ class PagedCache:
             new = torch.tensor(new, dtype=torch.int32, device=dev)
         elif n_tokens is None:
             raise ValueError("a step from a tensor needs n_tokens")
-        plan = ops.kv_plan(self.table, self.lens, new, self.free, self.state, n_tokens)
+        plan = ops.kv_plan(self.table, self.lens, new, self.free, self.state, n_tokens,
+                           max_len=self.max_len)
         self.lens.copy_(plan.lens)
         self.state.copy_(plan.state)
         self.plan, self.prefix, self.whole = plan, prefix, whole
