@@ -86,6 +86,7 @@ class PagedCache:
         self.whole = True           # every row of the step has a slot
         self._known = [0] * max_requests    # the lengths, where the host knows them
         self._left = n_blocks
+        self._captured = False      # whether replays may change them unseen
 
     def __len__(self):
         return self.n_layers
@@ -119,7 +120,7 @@ class PagedCache:
             if n_tokens is not None and n_tokens != sum(new):
                 raise ValueError(f"n_tokens={n_tokens}, {sum(new)} tokens")
             new += [0] * (R - len(new))
-            if self._known is None:     # (lengths that only the GPU knows)
+            if self._known is None or self._captured:   # (lengths that only the GPU knows)
                 self._known, self._left = self.lens.tolist(), int(self.state[0])
             known = [a + b for a, b in zip(self._known, new)]
             need = sum(-(-e // ops.KV_BLOCK) - -(-a // ops.KV_BLOCK)
@@ -133,6 +134,8 @@ class PagedCache:
             new = torch.tensor(new, dtype=torch.int32, device=dev)
         elif n_tokens is None:
             raise ValueError("a step from a tensor needs n_tokens")
+        elif self.table.is_cuda and torch.cuda.is_current_stream_capturing():
+            self._captured = True
         plan = ops.kv_plan(self.table, self.lens, new, self.free, self.state, n_tokens,
                            max_len=self.max_len)
         self.lens.copy_(plan.lens)
@@ -151,6 +154,8 @@ class PagedCache:
         finished[requests] = 1
         ops.kv_release(self.table, self.lens, finished.to(self.table.device), self.free, self.state)
         self.plan = None    # (its lengths and slots are the ended requests' too)
+        if self._captured:
+            self._known = None
         if self._known is not None:
             for r in requests:
                 self._left += -(-self._known[r] // ops.KV_BLOCK)
