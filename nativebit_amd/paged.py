@@ -189,8 +189,8 @@ def generate(model, prompts, n_generate: int, *, repetition=None, frequency=None
     ``presence``: a number or one for each request; ``bias``: a dict token ->
     bias for each request; ``mask``: int32 (requests, vocabulary / 32) bit
     masks of the allowed tokens.  A request whose mask and biases leave no
-    token gets -1 (fed as token 0).  ``cache``: an empty cache to use; the
-    requests stay in it."""
+    token gets -1 (fed as token 0).  ``cache``: an empty cache to use, with room
+    for all requests to their ends; they stay in it."""
     prompts = [[int(t) for t in p] for p in prompts]
     n = len(prompts)
     if not n or not all(prompts) or n_generate < 0:
@@ -207,6 +207,11 @@ def generate(model, prompts, n_generate: int, *, repetition=None, frequency=None
         raise ValueError(f"{len(bias)} bias dicts for {n} prompts")
     if cache is not None and bool(cache.lens.any()):
         raise ValueError("the cache holds requests already")
+    if cache is not None and n_generate:
+        blocks = sum(-(-(length + n_generate - 1) // ops.KV_BLOCK) for length in lengths)
+        if n > cache.table.shape[0] or blocks > int(cache.state[0]):
+            raise ValueError(f"{n} requests of {blocks} blocks, the cache is for "
+                             f"{cache.table.shape[0]} and has {int(cache.state[0])} free")
     if cache is None:
         blocks = sum(-(-(length + n_generate) // ops.KV_BLOCK) for length in lengths)
         cache = PagedCache(model, blocks, n, device=dev)
