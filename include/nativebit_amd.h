@@ -670,7 +670,8 @@ int nb_kv8_read(const int32_t* slots, int64_t n, const int8_t* k, const int8_t* 
  * n_kv_head):
  *     s(j)  = q[t][h] . k(j)                       (q scaled, as q_out above)
  *     s(j)  = softcap * tanh(s(j) / softcap)       if softcap > 0
- *     s(j) += slopes[h] * (j - i)                  if slopes
+ *     s(j) += slopes[h] * (j - i)                  if slopes (for j > i too, in
+ *                                                  a prefix: it grows there)
  *     out[t][h] = sum_j softmax_j(s) v(j)
  * over the cached positions j that it sees: j <= i, with window > 0 only
  * i - window < j, and with prefix all j < prefix[r] besides (of those that

@@ -103,14 +103,23 @@ class PagedCache:
         suffice, and the step's rows are its sum.  An int32 GPU tensor
         (max_requests,) is not read on the host (a step of ``n_tokens`` rows,
         which may be captured in a graph); tokens that no room is left for have
-        no slot then, and ``state[1]`` counts them.  ``prefix``: for each
-        request a number of leading tokens that all its queries see."""
+        no slot then, and ``state[1]`` counts them.  (After a captured step
+        lists read the lengths back from the GPU: replays change them.)
+        ``prefix``: for each request a number of leading tokens that all its
+        queries see.  With slopes it takes a list, and no new token may have
+        others behind it in its prefix: their bias would grow with the distance."""
         R = self.table.shape[0]
         dev = self.table.device
+        ahead = None
         if prefix is not None:
             prefix = torch.as_tensor(prefix, dtype=torch.int32).to(dev)
             if prefix.shape != (R,):
                 raise ValueError(f"prefix must have {R} numbers, got {tuple(prefix.shape)}")
+            if self.slopes is not None:
+                if isinstance(new, torch.Tensor):
+                    raise ValueError("slopes and a prefix take a step from a list (which tokens lie "
+                                     "inside a prefix is checked on the host)")
+                ahead = prefix.tolist()
         whole = not isinstance(new, torch.Tensor)
         known = left = None
         if whole:
@@ -129,6 +138,11 @@ class PagedCache:
                 raise ValueError(f"{max(known)} tokens of a request exceed max_len {self.max_len}")
             if need > self._left:
                 raise ValueError(f"{need} blocks needed, {self._left} free")
+            if ahead is not None:
+                for r, (a, e, p) in enumerate(zip(self._known, known, ahead)):
+                    if e > a and min(p, e) > a + 1:   # its first token sees others behind it
+                        raise ValueError(f"slopes with tokens of request {r} inside its prefix: "
+                                         "their bias would grow past the query")
             left = self._left - need
             n_tokens = sum(new)
             new = torch.tensor(new, dtype=torch.int32, device=dev)
