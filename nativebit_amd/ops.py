@@ -620,6 +620,14 @@ def kv_plan(table: torch.Tensor, lens: torch.Tensor, new: torch.Tensor, free: to
                                ("state", out.state, (2,))):
             _require(f"out.{name}", t, i32, shape, dev)
         s, p, c, l, st = (t.data_ptr() for t in out)
+        # the parts are memory of their own: every workgroup reads the inputs
+        ends = [0, 0]       # of the inputs, of the parts, in the order of addresses
+        for at, n, part in sorted([(table.data_ptr(), (R - 1) * stride + width, 0),
+                                   *((t.data_ptr(), t.numel(), 0) for t in (lens, new, free, state)),
+                                   *((t.data_ptr(), t.numel(), 1) for t in out)]):
+            if n and (at < ends[1] or (part and at < ends[0])):
+                raise ValueError("out overlaps an input or itself")
+            ends[part] = max(ends[part], at + 4 * n if n else 0)
     status = _lib.load().nb_kv_plan_max_len(
         table.data_ptr(), stride, lens.data_ptr(), new.data_ptr(), free.data_ptr(),
         state.data_ptr(), R, width, n_blocks, n_tokens, max_len, s, p, c, l, st,
