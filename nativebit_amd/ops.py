@@ -792,7 +792,8 @@ def kv8_attention(q: torch.Tensor, plan: KVPlan, table: torch.Tensor, k: torch.T
     n_chunks = chunks.shape[0]
     if table_dev != dev or not (_is(chunks, i32, (n_chunks, 4), dev) and
                                 _is(plan.lens, i32, (R,), dev)):
-        _require("table", table, i32, (R, width), dev)
+        if table_dev != dev:
+            raise ValueError(f"tensors on different devices: table on {table.device}, cuda:{dev}")
         _require("plan.chunks", chunks, i32, (None, 4), dev)
         _require("plan.lens", plan.lens, i32, (R,), dev)
     if not 0 <= window < 1 << 31:

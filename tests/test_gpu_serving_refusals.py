@@ -36,3 +36,18 @@ def test_plan_into_memory_of_its_inputs(dev):
     assert (table == -1).all() and (both == 0).all()
     # inputs may share memory
     ops.kv_plan(table, new, new, free, state, n, out=out())
+
+
+def test_attention_names_the_argument(dev):
+    """A plan of the wrong size beside a table whose rows lie apart (which is
+    taken)."""
+    k = torch.zeros(3, 1, 64, 16, dtype=torch.int8, device=dev)
+    v, s = k.view(3, 1, 16, 64), torch.zeros(3, 1, device=dev)
+    wide = torch.full((2, 5), -1, dtype=torch.int32, device=dev)
+    z = torch.zeros(2, dtype=torch.int32, device=dev)
+    plan = ops.KVPlan(z, z, torch.zeros(2, 4, dtype=torch.int32, device=dev), z, z)
+    q = torch.zeros(2, 16, device=dev)
+    assert ops.kv8_attention(q, plan, wide[:, :2], k, v, s, s).shape == (2, 16)
+    for bad, name in ((plan._replace(chunks=z), "plan.chunks"), (plan._replace(lens=z[:1]), "plan.lens")):
+        with pytest.raises(ValueError, match=name):
+            ops.kv8_attention(q, bad, wide[:, :2], k, v, s, s)
