@@ -388,7 +388,8 @@ constexpr int kReadSlots = 32;
 __global__ __launch_bounds__(kThreads) void kv8_read_kernel(
     const int32_t* slots, int64_t n, const int8_t* k, const int8_t* v, const float* k_scale,
     const float* v_scale, int n_blocks, int n_kv, int D, void* keys, void* values, int dtype) {
-    __shared__ int8_t vt[kReadSlots][kMaxD + 4];   // (rows 65 dwords apart: a row a bank)
+    // (rows 65 dwords apart: a row a bank; read by the dword)
+    __shared__ __align__(4) int8_t vt[kReadSlots][kMaxD + 4];
     const int64_t i0 = (int64_t)blockIdx.x * kReadSlots;
     const int h = blockIdx.y;
     const int count = (int)min((int64_t)kReadSlots, n - i0);
