@@ -15,12 +15,14 @@
 // new rows makes s' +inf and the block's codes 0: the block then reads as NaN.
 //
 // What bounds them: memory.  One token writes D bytes of codes a head, and
-// reads the earlier codes of its block only when the scale grows.  Append of 96
-// tokens of 96 requests, 32 query and 8 key / value heads of 128 in bf16: 8 us;
-// of 8000 prompt tokens of those heads 68 us in fp32 for 344 MB in and out (5.1
-// TB/s), 50 in bf16; of 6001 of 20 heads 58 in fp32 for 276 MB (4.8), 44 in bf16
-// (one form for both types: 62 and 64, with each bf16 load waited for by its
-// conversion).  Read, fp32 out: 6240 slots of 8 heads 15 us, 6577 of 20 heads 33.
+// reads the earlier codes of its block only when the scale grows.  Over three
+// inputs in turn: append of 96 tokens of 96 requests, 32 query and 8 key / value
+// heads of 128 in bf16: 6.5 us; of 8000 prompt tokens of those heads 71 us in fp32
+// for 344 MB in and out (4.9 TB/s), 48 in bf16; of 6001 of 20 heads 69 in fp32 for
+// 276 MB (4.0), 47 in bf16.  The latter on one input, part of it in the last level
+// cache: 58 and 44 (one form for both types: 62 and 64, with each bf16 load waited
+// for by its conversion).  Read, fp32 out: 6240 slots of 8 heads 15 us, 6577 of 20
+// heads 33.
 #include <math.h>
 
 #include <algorithm>
@@ -454,8 +456,10 @@ __global__ __launch_bounds__(kThreads) void kv8_read_kernel(
 int kv8_max_head_dim() { return kMaxD; }
 
 // Workgroups of a chunk's queries that share a head's keys: two batches of four
-// rows a thread each, for the most rows that a chunk may have where some have
-// more than a token (but no more of all than a grid holds).  8000 bf16 tokens,
+// rows a thread each, for the most rows that a chunk may have where some must have
+// more than a token (but no more of all than a grid holds).  The list's length is a
+// plan's bound, so that is not seen of a prompt of up to about twice as many tokens
+// as there are requests: one workgroup takes its chunks' queries.  8000 bf16 tokens,
 // 32 heads on 8 of 128: 84 us with one for all, 68 so; 6001 fp32, 16 on 4 of
 // 256: 80 and 60 (one batch each 64).  64 single tokens and a prompt of 1000, 32
 // heads on 8: 15.7 us, for the mean rows 22.1; the 64 alone 5.4, for the most

@@ -21,10 +21,11 @@
 // Rows of q with a few large dims need more: where the largest value is over
 // kEven times the mean one, q has a digit more (32 bits, bf16 outputs 24), and
 // with 32 the sum's halves A 2^8 + B and C 2^8 + E are added in fp32.  One dim 3000
-// times the others, keys small there: errors of 9e-5 without it and 3e-7 with
-// (bf16 outputs 3e-2 and 2e-3).  The rule is a row's own and so is its result; a
-// tile without such rows skips the digit.  8003 prompt tokens, 20 heads of 128: 365
-// us, 409 with the digit in all rows.  The codes go into the MFMAs as they are.
+// times the others, keys small there, 512 tokens: errors of 1.9e-5 without it and
+// 1.1e-7 with (products in fp32 2.6e-7), with bf16 outputs 4.1e-3 and 4.8e-4 (their
+// rounding).  The rule is a row's own and so is its result; a tile without such
+// rows skips the digit.  8003 prompt tokens, 20 heads of 128: 365 us, 409 with the
+// digit in all rows.  The codes go into the MFMAs as they are.
 //
 // Layout.  Everything is transposed, so that a lane keeps one row from the
 // scores to the output and no row's numbers pass through LDS.  Lane (c, g) =
@@ -46,7 +47,8 @@
 // fetches all codes through the L1: 8003 prompt tokens of two requests, 20
 // heads of 128, 505 us then; 375 with LDS, scalar loads of tables and scales
 // and the reference that moves seldom; two blocks a turn (one maximum, one step
-// of O) instead of one: 384 to 371 in turn on one card, about 360 on others.
+// of O) instead of one: 384 to 371 in turn on one card.  Now 337 to 389 by the drawn
+// lengths.
 //
 // Split.  A workgroup takes one chunk and key / value head (and 64 rows of it, 32
 // of single tokens).  Few of them over long caches are split over workgroups too
@@ -55,12 +57,12 @@
 // What bounds it.  Single tokens: the codes, 2 D bytes a cached token and head.
 // 64 requests of 960 positions at most, 20 heads of 128: 51 us, 4.8 TB/s from
 // memory (44 where they come from the last level cache); 128 of 2000, 8 heads:
-// 77 us, 5.1 TB/s; six of 40000, 8 heads: 77 us with the join, 4.8 TB/s.
+// 77 us, 5.1 TB/s; six of 40000, 8 heads: 74 us with the join, 5.0 TB/s.
 // Prompts: the issue of vector instructions and MFMAs, which overlap only in
-// part.  16384 tokens, 16 heads on 2: 563 TFLOP/s (of 4 D a score; each takes
-// three int8 MFMA products in fp32, two for bf16 outputs: 744).  Of 360 us for
-// the 8003 tokens 125 go with the second product, 85 with the first, 10 with
-// the exponentials.
+// part.  16384 tokens, 16 heads on 2: 546 TFLOP/s (of 4 D a score; each takes
+// three int8 MFMA products in fp32, two for bf16 outputs: 729).  Of 360 us for
+// 8003 tokens 125 go with the second product, 85 with the first, 10 with the
+// exponentials.
 #pragma once
 
 #include <math.h>

@@ -7,6 +7,9 @@
 namespace nb {
 namespace {
 
+// (Waves of a workgroup and rows of a chunk by the list's length, a plan's bound:
+// with up to about twice as many tokens as requests the launch below may start
+// prompts' workgroups of twice the waves, with half the blocks for each.)
 // Workgroups over a row's blocks: three a CU (heads of over 128 dims two), over
 // tables of 32 blocks or more, two blocks a wave at least.  One token of six
 // requests of 40000 positions, 8 heads of 128 (48 workgroups unsplit): 16 splits

@@ -17,9 +17,10 @@
 // of a row walks its whole history, from the L2: against 16 KB of logits read
 // and written, a history of 1000 is 4 KB.  LDS atomics are on whole numbers
 // (sums, or, maximum): no result depends on their order.  160 fp32 rows of
-// 131077, both launches: 37 us with histories of 1000 (4.6 TB/s), 42 with 4000
+// 131077, three inputs in turn, both launches: 42 us with histories of 1000 (4.1
+// TB/s), 49 with 4000; on one input, part of it in the last level cache, 37 and 42
 // (40 and 44 with the masks' bits made beside their loads, which waited for
-// each); one row of 50257 5.6.
+// each); one row of 50257 6.2.
 #include <math.h>
 
 #include <algorithm>
