@@ -578,8 +578,9 @@ int nb_attention_batch(const float* q, const float* k_cache, const float* v_cach
  *     v        int8 [n_blocks][n_kv_head][head_dim][NB_KV_BLOCK]
  *     k_scale, v_scale   fp32 [n_blocks][n_kv_head]
  * the key being k * k_scale, the value v * v_scale (scales are not negative;
- * +inf with codes 0 reads as NaN).  table[r][j] (row stride table_stride) is the block with positions 64 j .. 64 j + 63 of request r,
- * -1 where there is none; slot 64 b + i is token i of block b.  All layers
+ * +inf with codes 0 reads as NaN).  table[r][j] (row stride table_stride) is
+ * the block with positions 64 j .. 64 j + 63 of request r, -1 where there is
+ * none; slot 64 b + i is token i of block b.  All layers
  * share the tables.
  *
  * A step brings new tokens of some requests, their rows one after the other

@@ -3,10 +3,10 @@
 //
 //   nb_kv_plan      request r has lens[r] tokens cached and brings new[r].  The
 //                   rows of the step are the requests' new tokens in order;
-//                   with L = lens, N = new (clipped to the rows that exist and
-//                   to the length that a request may have)
+//                   with L = lens, N = new (clipped to the rows that exist), E =
+//                   L + N (clipped to the table and the longest request)
 //                     first[r] = sum N[< r]             row of its first token
-//                     need[r]  = ceil((L + N) / 64) - ceil(L / 64)
+//                     need[r]  = ceil(E / 64) - ceil(L / 64)
 //                     base[r]  = sum need[< r]
 //                   and new block number k of the step (k < free count) is the
 //                   free list's entry free count - 1 - k.  Row first[r] + i

@@ -772,9 +772,9 @@ def kv8_attention(q: torch.Tensor, plan: KVPlan, table: torch.Tensor, k: torch.T
     step's own among them (nb_kv8_attention).  Scores s become softcap *
     tanh(s / softcap) (softcap > 0), then get slopes[head] * (key position -
     query position), past the query too (where a prefix shows it keys behind it,
-    positive slopes favour the farther ones); a query sees the positions up to its own, with ``window``
-    > 0 only the last ``window`` of them, and with ``prefix`` (requests,)
-    besides all before prefix[request].  Returns (rows, heads * head_dim) in
+    positive slopes favour the farther ones); a query sees the positions up to its
+    own, with ``window`` > 0 only the last ``window`` of them, and with ``prefix``
+    (requests,) besides all before prefix[request].  Returns (rows, heads * head_dim) in
     q's dtype or ``out_dtype`` (or into ``out``, which may be ``q``); rows
     without a slot are not written."""
     dev, n_blocks, n_kv, D = _kv8_cache(k, v, k_scale, v_scale)
