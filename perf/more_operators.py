@@ -173,14 +173,15 @@ def _tiles(index, codes):
     64 units (of 32 indices in 12 bytes) of its 4 x 16 (quarter, output)s, then
     the outputs' 8 codes.  Four indices are the bytes of a selector; byte b of
     a unit's three words holds those of selectors 0 and 1, 2 and 3, 4 and 5 in
-    its low six bits, 6 and 7 in the upper two of all three."""
+    its low six bits; the upper two hold the low bits of selectors 6 and of 7,
+    in the third word the high bit of each."""
     N, K = index.shape
     blocks, tiles = K // BLOCK, (N + 15) // 16
     index = torch.nn.functional.pad(index, (0, 0, 0, tiles * 16 - N))
     codes = torch.nn.functional.pad(codes.view(N, -1), (0, 0, 0, tiles * 16 - N))
     s = index.view(tiles, 16, blocks, 4, 8, 4).permute(0, 2, 3, 1, 4, 5)   # (.., selector, byte)
-    high = torch.stack([s[..., 6, :] & 3, s[..., 6, :] >> 2 | (s[..., 7, :] & 1) << 1,
-                        s[..., 7, :] >> 1], -2)
+    high = torch.stack([s[..., 6, :] & 3, s[..., 7, :] & 3,
+                        s[..., 6, :] >> 2 | s[..., 7, :] >> 2 << 1], -2)
     units = s[..., 0:6:2, :] | s[..., 1:6:2, :] << 3 | high << 6
     codes = codes.view(tiles, 16, blocks, ENTRIES).transpose(1, 2).reshape(tiles, blocks, 128)
     return torch.cat([units.reshape(tiles, blocks, 768), codes.view(torch.uint8)], -1).contiguous()
