@@ -727,6 +727,99 @@ int nb_logits_rules(const void* logits, int dtype, int64_t ld, int rows, int V,
                     int64_t ld_mask, float* out, int64_t ld_out, int32_t* tokens, void* workspace,
                     int64_t ws_bytes, void* stream);
 
+/*
+ * Tokens drawn from `rows` rows of V logits (NB_F32 or NB_BF16, stride ld).
+ * rows <= 65535, V <= 2^24.  For row b with its largest logit m, in the order
+ * "larger first, of equal logits the lower token first":
+ *     w(v)  = exp((logits[b][v] - m) / temperature[b])   (0 for -inf and NaN;
+ *             where m is +inf, 1 for those that are too and 0 for the others)
+ *     kept  = the first top_k[b] tokens of the order (all where it is <= 0),
+ *             of those the shortest beginning whose w sum to top_p[b] of
+ *             theirs or more (all where it is not < 1; at least one token),
+ *             of those the ones with w >= min_p[b] (all where it is not > 0;
+ *             w = 1 always)
+ *     tokens[b]   = the lowest v with sum of kept w up to v > u[b] * their sum
+ *     logprobs[b] = log(w / sum of kept w) of that token       (if logprobs)
+ * A temperature that is not > 0 takes the first token of the order (logprob 0).
+ * u is clamped to [0, 1).  A row of nothing but -inf and NaN gives -1 and -inf.
+ * u, temperature, top_k, top_p and min_p have an entry a row; but for u, NULL is
+ * a temperature of 1 and rules that keep all.  Weights are whole multiples of
+ * 2^-45 (2^-38 at the largest V), their sums exact, so the same call gives the
+ * same tokens.  The workspace needs nb_sample_ws_bytes(rows, V) bytes, 16-byte
+ * aligned (0: may be NULL).
+ */
+int64_t nb_sample_ws_bytes(int rows, int V);
+int nb_sample(const void* logits, int dtype, int64_t ld, int rows, int V, const float* u,
+              const float* temperature, const int32_t* top_k, const float* top_p,
+              const float* min_p, int32_t* tokens, float* logprobs, void* workspace,
+              int64_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Rows in 8 bits through the packed layers.  No counterpart in the reference
+ * (its layers multiply fp32 or bf16 activations, inference/triton_kernel.py:
+ * 240-275); the layers' indices are its own, their codebooks rounded once.
+ * ------------------------------------------------------------------------ */
+/*
+ * Rows in 8 bits with a scale each: codes int8 [rows][width] and scale fp32
+ * [rows] of x's rows (NB_F32 or NB_BF16, stride ld).  With a = max |x| of the
+ * row, in 64 bits: code = rint(x * (127 / a)), ties to even, scale = a / 127
+ * rounded to fp32; 0 where a is 0.  A NaN or infinity in a row gives it scale
+ * NaN and codes 0.
+ */
+int nb_quantize8(const void* x, int dtype, int64_t ld, int rows, int width, int8_t* codes,
+                 float* scale, void* stream);
+/*
+ * The same of the rows v = h * weight / rms, rms = sqrt(mean h^2 + eps), h = x or,
+ * with a residual (of x's type, stride ld_residual), x + residual rounded to
+ * that type; h is written to sum if it is not NULL (of x's type, stride ld_sum;
+ * it may be x or residual itself, of the same stride, and else overlaps them in
+ * no element).  The codes are those of h * weight (rms cancels), the scale its
+ * largest magnitude / (127 rms); in 64 bits.
+ * (RMSNorm, inference/generate_torch.py:29-38, 128-132.)
+ */
+int nb_rmsnorm8(const void* x, int dtype, int64_t ld_x, const void* residual, int64_t ld_residual,
+                void* sum, int64_t ld_sum, const float* weight, float eps, int rows, int width,
+                int8_t* codes, float* scale, void* stream);
+/*
+ * A 3-bit / 8-entry / block-128 layer (packed as above, K % 128 == 0, K <=
+ * 2^17) for nb_linear8, once at load: for output n, a = the largest magnitude
+ * among its blocks' entries, scale[n] = a / 127 (fp32 [N]), each entry's code
+ * rint(entry * (127 / a)) (in 64 bits, ties to even).  tiles:
+ * nb_linear8_tiles_bytes(N, K) = ceil(N / 16) * (K / 128) * 896 bytes, 16-byte
+ * aligned; tile (t, j) holds inputs 128 j .. 128 j + 127 of outputs 16 t .. 16 t
+ * + 15 (zeros past N): bytes 12 (16 g + r) .. the selector-ordered unit of the 32
+ * indices of output r's inputs 32 g .., selector s those of inputs 4 s .. 4 s + 3
+ * of them; bytes 768 + 8 r .. the block's 8 codes of output r.  An output with
+ * a NaN or infinity among its entries has scale NaN and codes 0.
+ */
+int64_t nb_linear8_tiles_bytes(int N, int K);
+int nb_linear8_layout(const uint8_t* packed, const float* codebook, int N, int K, uint8_t* tiles,
+                      float* scale, void* stream);
+enum nb_activation {
+    NB_ACT_NONE = 0,
+    NB_ACT_SILU = 1,    /* v / (1 + exp(-v))                                   */
+    NB_ACT_GELU = 2,    /* v (1 + erf(v / sqrt 2)) / 2                         */
+    NB_ACT_SWIGLU = 3   /* silu(v[2i]) * v[2i + 1]: N / 2 outputs, N even       */
+};
+/*
+ * M rows in 8 bits times such a layer:
+ *     v[m][n] = x_scale[m] * scale[n] * sum_k x[m][k] * code[n][k] + bias[n]
+ *     y[m][n] = activation(v[m])[n] + residual[m][n]
+ * x: codes of M rows of K (stride ld_x, a multiple of 16; 16-byte aligned).
+ * bias fp32 [N] and residual (of y's type, stride ld_residual) may be NULL; y
+ * NB_F32 or NB_BF16, stride ld_y; it may be the residual itself, of the same
+ * stride, and else overlaps it in no element.  The sums over k are whole numbers
+ * and exact, the rest is fp32, rounded to y's type once.  The workspace needs
+ * nb_linear8_ws_bytes(M, N, K) bytes, 16-byte aligned (0: may be NULL).
+ * (PackedLinear.forward, inference/triton_kernel.py:240-275, and what follows
+ * it in a block, inference/generate_torch.py:109-132.)
+ */
+int64_t nb_linear8_ws_bytes(int M, int N, int K);
+int nb_linear8(const int8_t* x, int64_t ld_x, const float* x_scale, const uint8_t* tiles,
+               const float* scale, const float* bias, int activation, const void* residual,
+               int64_t ld_residual, void* y, int y_dtype, int64_t ld_y, int M, int N, int K,
+               void* workspace, int64_t ws_bytes, void* stream);
+
 /* ------------------------------------------------------------------------
  * Persistent decode: many greedy tokens of the whole packed decoder in one
  * cooperative launch (one workgroup per CU), the phases of a token separated

@@ -41,6 +41,12 @@ NB_Y_STORE = 0
 NB_Y_ADD = 1
 NB_Y_SILU_PAIRS = 2
 
+# nb_activation
+NB_ACT_NONE = 0
+NB_ACT_SILU = 1
+NB_ACT_GELU = 2
+NB_ACT_SWIGLU = 3
+
 ABI_VERSION = 2
 
 # Every symbol include/nativebit_amd.h declares: (name, restype, argtypes).
@@ -109,6 +115,14 @@ SIGNATURES = {
     "nb_logits_rules_ws_bytes": (_L, [_I, _I]),
     "nb_logits_rules": (_I, [_P, _I, _L, _I, _I, _P, _L, _I, _P, _P, _P, _P, _P, _P, _P, _L, _I,
                              _P, _L, _P, _L, _P, _P, _L, _P]),
+    "nb_sample_ws_bytes": (_L, [_I, _I]),
+    "nb_sample": (_I, [_P, _I, _L, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _L, _P]),
+    "nb_quantize8": (_I, [_P, _I, _L, _I, _I, _P, _P, _P]),
+    "nb_rmsnorm8": (_I, [_P, _I, _L, _P, _L, _P, _L, _P, ctypes.c_float, _I, _I, _P, _P, _P]),
+    "nb_linear8_tiles_bytes": (_L, [_I, _I]),
+    "nb_linear8_layout": (_I, [_P, _P, _I, _I, _P, _P, _P]),
+    "nb_linear8_ws_bytes": (_L, [_I, _I, _I]),
+    "nb_linear8": (_I, [_P, _L, _P, _P, _P, _P, _I, _P, _L, _P, _I, _L, _I, _I, _I, _P, _L, _P]),
     "nb_decode_workspace_bytes": (_L, [_P]),
     "nb_decode_persistent": (_I, [_P, _P, _L, _P, _P, _P, _I, _P, _I, _I, _I, _P]),
 }

@@ -1446,4 +1446,170 @@ int nb_logits_rules(const void* logits, int dtype, int64_t ld, int rows, int V,
                                static_cast<hipStream_t>(stream));
 }
 
+int64_t nb_sample_ws_bytes(int rows, int V) {
+    return rows < 1 || V < 1 ? 0 : sample_bytes(rows, V);
+}
+
+int nb_sample(const void* logits, int dtype, int64_t ld, int rows, int V, const float* u,
+              const float* temperature, const int32_t* top_k, const float* top_p,
+              const float* min_p, int32_t* tokens, float* logprobs, void* workspace,
+              int64_t ws_bytes, void* stream) {
+    const char* fn = "nb_sample";
+    if (rows < 0 || V < 1) return fail(NB_EINVAL, "%s: rows=%d V=%d", fn, rows, V);
+    if (V > 1 << 24) return fail(NB_EUNSUPPORTED, "%s: V=%d (<= 2^24)", fn, V);
+    if (rows > 65535) return fail(NB_EUNSUPPORTED, "%s: rows=%d (<= 65535)", fn, rows);
+    if (rows == 0) return NB_OK;
+    int st = check_rows(fn, "logits", logits, dtype, ld, V);
+    if (st) return st;
+    if (!u || !tokens) return fail(NB_EINVAL, "%s: %s is NULL", fn, u ? "tokens" : "u");
+    const void* four[] = {u, temperature, top_k, top_p, min_p, tokens, logprobs};
+    for (const void* p : four) {
+        if (!aligned(p, 4)) return fail(NB_EALIGN, "%s: misaligned pointer", fn);
+    }
+    const int64_t need = sample_bytes(rows, V);
+    if (ws_bytes < need || (need && !workspace)) {
+        return fail(NB_EINVAL, "%s: workspace of %lld bytes < %lld", fn, (long long)ws_bytes, (long long)need);
+    }
+    if (!aligned(workspace, 16)) return fail(NB_EALIGN, "%s: workspace not 16-byte aligned", fn);
+    st = ensure_device();
+    if (st) return st;
+    return launch_sample(logits, dtype, ld, rows, V, u, temperature, top_k, top_p, min_p, tokens,
+                         logprobs, workspace, static_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// rows in 8 bits through the packed layers
+// ---------------------------------------------------------------------------
+namespace {
+int check_rows8(const char* fn, const void* x, int dtype, int64_t ld, int rows, int width,
+                const void* codes, const void* scale) {
+    if (rows < 0 || width < 1) return fail(NB_EINVAL, "%s: rows=%d width=%d", fn, rows, width);
+    if (width > 1 << 24) return fail(NB_EUNSUPPORTED, "%s: width=%d (<= 2^24)", fn, width);
+    if (rows >= 1 << 22) return fail(NB_EUNSUPPORTED, "%s: rows=%d (< 2^22)", fn, rows);
+    if (rows == 0) return NB_OK;
+    const int st = check_rows(fn, "x", x, dtype, ld, width);
+    if (st) return st;
+    if (!codes || !scale) return fail(NB_EINVAL, "%s: %s is NULL", fn, codes ? "scale" : "codes");
+    if (!aligned(scale, 4)) return fail(NB_EALIGN, "%s: scale misaligned", fn);
+    return NB_OK;
+}
+
+int check_layer8(const char* fn, int N, int K) {
+    if (N < 0 || K < 128 || K % 128) {
+        return fail(NB_EINVAL, "%s: N=%d K=%d (needs N >= 0, K > 0, K %% 128 == 0)", fn, N, K);
+    }
+    if (K > 1 << 17) return fail(NB_EUNSUPPORTED, "%s: K=%d (<= 2^17)", fn, K);
+    if (((int64_t)N + 15) / 16 * (K / 128) >= 1LL << 24) {
+        return fail(NB_EUNSUPPORTED, "%s: N=%d K=%d, too large a layer", fn, N, K);
+    }
+    return NB_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int nb_quantize8(const void* x, int dtype, int64_t ld, int rows, int width, int8_t* codes,
+                 float* scale, void* stream) {
+    int st = check_rows8("nb_quantize8", x, dtype, ld, rows, width, codes, scale);
+    if (st || rows == 0) return st;
+    st = ensure_device();
+    if (st) return st;
+    return launch_quantize8(x, dtype, ld, rows, width, codes, scale, static_cast<hipStream_t>(stream));
+}
+
+int nb_rmsnorm8(const void* x, int dtype, int64_t ld_x, const void* residual, int64_t ld_residual,
+                void* sum, int64_t ld_sum, const float* weight, float eps, int rows, int width,
+                int8_t* codes, float* scale, void* stream) {
+    const char* fn = "nb_rmsnorm8";
+    if (!(eps >= 0.f) || !std::isfinite(eps)) return fail(NB_EINVAL, "%s: eps=%g", fn, (double)eps);
+    int st = check_rows8(fn, x, dtype, ld_x, rows, width, codes, scale);
+    if (st || rows == 0) return st;
+    if (!weight) return fail(NB_EINVAL, "%s: weight is NULL", fn);
+    if (!aligned(weight, 4)) return fail(NB_EALIGN, "%s: weight misaligned", fn);
+    if (sum && !residual) return fail(NB_EINVAL, "%s: a sum needs a residual", fn);
+    if (residual) {
+        st = check_rows(fn, "residual", residual, dtype, ld_residual, width);
+        if (st) return st;
+    }
+    if (sum) {
+        st = check_rows(fn, "sum", sum, dtype, ld_sum, width);
+        if (st) return st;
+        if (rows_overlap(x, dtype, ld_x, width, sum, dtype, ld_sum, width, rows) ||
+            rows_overlap(residual, dtype, ld_residual, width, sum, dtype, ld_sum, width, rows)) {
+            return fail(NB_EINVAL, "%s: sum overlaps x or residual (in place: of the same stride)", fn);
+        }
+    }
+    st = ensure_device();
+    if (st) return st;
+    return launch_rmsnorm8(x, dtype, ld_x, residual, ld_residual, sum, ld_sum, weight, eps, rows,
+                           width, codes, scale, static_cast<hipStream_t>(stream));
+}
+
+int64_t nb_linear8_tiles_bytes(int N, int K) {
+    return N < 0 || K < 0 || K % 128 ? 0 : linear8_tiles_bytes(N, K);
+}
+
+int nb_linear8_layout(const uint8_t* packed, const float* codebook, int N, int K, uint8_t* tiles,
+                      float* scale, void* stream) {
+    const char* fn = "nb_linear8_layout";
+    int st = check_layer8(fn, N, K);
+    if (st || N == 0) return st;
+    if (!packed || !codebook || !tiles || !scale) return fail(NB_EINVAL, "%s: NULL pointer", fn);
+    if (!aligned(packed, 4) || !aligned(codebook, 4) || !aligned(tiles, 16) || !aligned(scale, 4)) {
+        return fail(NB_EALIGN, "%s: tiles 16-byte, the others 4-byte alignment", fn);
+    }
+    st = ensure_device();
+    if (st) return st;
+    return launch_linear8_layout(packed, codebook, N, K, tiles, scale, static_cast<hipStream_t>(stream));
+}
+
+int64_t nb_linear8_ws_bytes(int M, int N, int K) {
+    if (M < 1 || N < 1 || K < 128 || K % 128 || K > 1 << 17) return 0;
+    if (ensure_device() != NB_OK) g_last_error[0] = '\0';   // (256 CUs without a device)
+    return linear8_bytes(M, N, K);
+}
+
+int nb_linear8(const int8_t* x, int64_t ld_x, const float* x_scale, const uint8_t* tiles,
+               const float* scale, const float* bias, int activation, const void* residual,
+               int64_t ld_residual, void* y, int y_dtype, int64_t ld_y, int M, int N, int K,
+               void* workspace, int64_t ws_bytes, void* stream) {
+    const char* fn = "nb_linear8";
+    int st = check_layer8(fn, N, K);
+    if (st) return st;
+    if (M < 0) return fail(NB_EINVAL, "%s: M=%d", fn, M);
+    if (M > 1 << 20) return fail(NB_EUNSUPPORTED, "%s: M=%d (<= 2^20)", fn, M);
+    if (activation < NB_ACT_NONE || activation > NB_ACT_SWIGLU) {
+        return fail(NB_EINVAL, "%s: activation=%d", fn, activation);
+    }
+    if (activation == NB_ACT_SWIGLU && N % 2) return fail(NB_EINVAL, "%s: N=%d is odd", fn, N);
+    if (M == 0 || N == 0) return NB_OK;
+    const int64_t out = activation == NB_ACT_SWIGLU ? N / 2 : N;
+    st = check_rows(fn, "y", y, y_dtype, ld_y, out);
+    if (st) return st;
+    if (!x || !x_scale || !tiles || !scale) return fail(NB_EINVAL, "%s: NULL pointer", fn);
+    if (ld_x < K || ld_x % 16) return fail(NB_EINVAL, "%s: ld_x=%lld (>= K, a multiple of 16)", fn, (long long)ld_x);
+    if (!aligned(x, 16) || !aligned(tiles, 16)) return fail(NB_EALIGN, "%s: x and tiles need 16-byte alignment", fn);
+    if (!aligned(x_scale, 4) || !aligned(scale, 4) || !aligned(bias, 4)) {
+        return fail(NB_EALIGN, "%s: misaligned pointer", fn);
+    }
+    if (residual) {
+        st = check_rows(fn, "residual", residual, y_dtype, ld_residual, out);
+        if (st) return st;
+        if (rows_overlap(residual, y_dtype, ld_residual, out, y, y_dtype, ld_y, out, M)) {
+            return fail(NB_EINVAL, "%s: y overlaps residual (in place: of the same stride)", fn);
+        }
+    }
+    const int dev_st = ensure_device();
+    const int64_t need = linear8_bytes(M, N, K);
+    if (ws_bytes < need || (need && !workspace)) {
+        return fail(NB_EINVAL, "%s: workspace of %lld bytes < %lld", fn, (long long)ws_bytes, (long long)need);
+    }
+    if (!aligned(workspace, 16)) return fail(NB_EALIGN, "%s: workspace not 16-byte aligned", fn);
+    if (dev_st) return dev_st;
+    return launch_linear8(x, ld_x, x_scale, tiles, scale, bias, activation, residual, ld_residual, y,
+                          y_dtype, ld_y, M, N, K, workspace, static_cast<hipStream_t>(stream));
+}
+
 }  // extern "C"

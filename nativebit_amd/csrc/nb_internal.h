@@ -258,6 +258,28 @@ int launch_logits_rules(const void* logits, int dtype, int64_t ld, int rows, int
                         int64_t ld_mask, float* out, int64_t ld_out, int32_t* tokens,
                         void* workspace, hipStream_t stream);
 
+// nb_rows8.hip
+int launch_quantize8(const void* x, int dtype, int64_t ld_x, int rows, int width, int8_t* codes,
+                     float* scale, hipStream_t stream);
+int launch_rmsnorm8(const void* x, int dtype, int64_t ld_x, const void* residual,
+                    int64_t ld_residual, void* sum, int64_t ld_sum, const float* weight, float eps,
+                    int rows, int width, int8_t* codes, float* scale, hipStream_t stream);
+// nb_linear8.hip
+int64_t linear8_tiles_bytes(int N, int K);
+int launch_linear8_layout(const uint8_t* packed, const float* codebook, int N, int K,
+                          uint8_t* tiles, float* scale, hipStream_t stream);
+int launch_linear8(const int8_t* x, int64_t ld_x, const float* x_scale, const uint8_t* tiles,
+                   const float* scale, const float* bias, int activation, const void* residual,
+                   int64_t ld_residual, void* y, int y_dtype, int64_t ld_y, int M, int N, int K,
+                   void* workspace, hipStream_t stream);
+int64_t linear8_bytes(int M, int N, int K);   // its workspace (0: none)
+// nb_sample.hip
+int64_t sample_bytes(int rows, int V);   // its workspace (0: none)
+int launch_sample(const void* logits, int dtype, int64_t ld, int rows, int V, const float* u,
+                  const float* temperature, const int32_t* top_k, const float* top_p,
+                  const float* min_p, int32_t* tokens, float* logprobs, void* workspace,
+                  hipStream_t stream);
+
 // Persistent decode (nb_decode_persistent.hip); arguments validated.
 int64_t decode_persistent_workspace_bytes(int C, int H, int F);
 int decode_persistent_limits(int* max_c, int* max_f, int* max_d, int* max_ctx, int* max_heads,

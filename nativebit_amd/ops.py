@@ -940,3 +940,259 @@ def _vector(name, t, dtype, rows, dev):
     if not _is(t, dtype, (rows,), dev):
         _require(name, t, dtype, (rows,), dev)
     return t.data_ptr()
+
+
+@functools.lru_cache(maxsize=256)
+def _sample_bytes(rows, vocab) -> int:
+    return int(_lib.load().nb_sample_ws_bytes(rows, vocab))
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: torch.Tensor | None = None,
+           top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None,
+           min_p: torch.Tensor | None = None, logprobs: bool = False):
+    """Tokens drawn from a batch of logits (B, V), float32 or bfloat16, by the
+    numbers ``u`` (B,) in [0, 1) (nb_sample).  Of the weights exp((logit -
+    largest) / ``temperature[b]``), in the order of the logits (the lower token
+    first where they are equal), the first ``top_k[b]`` are kept, of those the
+    shortest beginning that makes up ``top_p[b]`` of their sum, of those the ones
+    that are ``min_p[b]`` or more; the token is the lowest whose running sum of
+    kept weights is over ``u[b]`` of their total.  Each rule is a (B,) tensor,
+    float32 (top_k int32), or None; 0 tokens, a share of 1 and a least weight of
+    0 keep all; a temperature of 0 takes the first of the order.  Returns int32
+    (B,) tokens, -1 where a row has nothing but -inf and NaN, and with
+    ``logprobs`` also their float32 log-probabilities among the kept ones."""
+    _require_cuda("logits", logits)
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError(f"logits must be (B, V), got {tuple(logits.shape)}")
+    B, V = logits.shape
+    dev = logits.get_device()
+    if not _here(dev):
+        with torch.cuda.device(dev):
+            return sample(logits, u, temperature=temperature, top_k=top_k, top_p=top_p,
+                          min_p=min_p, logprobs=logprobs)
+    ld = _rows("logits", logits, B, V, dev)
+    f32 = torch.float32
+    if u is None:
+        raise TypeError("u must be a torch.Tensor")
+    u = _vector("u", u, f32, B, dev)
+    temperature = _vector("temperature", temperature, f32, B, dev)
+    top_k = _vector("top_k", top_k, torch.int32, B, dev)
+    top_p = _vector("top_p", top_p, f32, B, dev)
+    min_p = _vector("min_p", min_p, f32, B, dev)
+    tokens = torch.empty(B, dtype=torch.int32, device=logits.device)
+    logp = torch.empty(B, dtype=f32, device=logits.device) if logprobs else None
+    if B:
+        nbytes = _sample_bytes(B, V)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
+        status = _lib.load().nb_sample(
+            logits.data_ptr(), _DT[logits.dtype], ld, B, V, u, temperature, top_k, top_p, min_p,
+            tokens.data_ptr(), None if logp is None else logp.data_ptr(),
+            None if ws is None else ws.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(dev))
+        if status:
+            _lib.check(status)
+    return (tokens, logp) if logprobs else tokens
+
+
+# ---------------------------------------------------------------------------
+# rows in 8 bits through the packed layers
+# ---------------------------------------------------------------------------
+class Rows8(NamedTuple):
+    """Rows in 8 bits (``quantize8``, ``rmsnorm8``): row m stands for
+    ``codes[m] * scale[m]``.  int8 (rows, width) and float32 (rows,) on the
+    GPU."""
+    codes: torch.Tensor
+    scale: torch.Tensor
+
+    def values(self) -> torch.Tensor:
+        """The float32 values that they stand for."""
+        return self.codes * self.scale[:, None]
+
+
+class Weights8(NamedTuple):
+    """A packed layer (N, K) with its codebooks in 8 bits (``linear8_layout``):
+    uint8 ``tiles`` and a float32 (N,) ``scale`` on the GPU."""
+    tiles: torch.Tensor
+    scale: torch.Tensor
+    N: int
+    K: int
+
+
+_ACTIVATIONS = {None: _lib.NB_ACT_NONE, "silu": _lib.NB_ACT_SILU, "gelu": _lib.NB_ACT_GELU,
+                "swiglu": _lib.NB_ACT_SWIGLU}
+
+
+def _rows8_out(x):
+    """(device, rows, width, codes, scale) for rows x."""
+    _require_cuda("x", x)
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"x must be (rows, width), got {tuple(x.shape)}")
+    return x.get_device(), *x.shape
+
+
+def quantize8(x: torch.Tensor) -> Rows8:
+    """Rows of x (rows, width), float32 or bfloat16, in 8 bits with one scale
+    each (nb_quantize8): with a = max |x| of a row its codes are rint(x * (127 /
+    a)), its scale a / 127.  A NaN or an infinity makes its row's scale NaN."""
+    dev, rows, width = _rows8_out(x)
+    if not _here(dev):
+        with torch.cuda.device(dev):
+            return quantize8(x)
+    ld = _rows("x", x, rows, width, dev)
+    codes = torch.empty((rows, width), dtype=torch.int8, device=x.device)
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    if rows:
+        status = _lib.load().nb_quantize8(
+            x.data_ptr(), _DT[x.dtype], ld, rows, width, codes.data_ptr(), scale.data_ptr(),
+            torch._C._cuda_getCurrentRawStream(dev))
+        if status:
+            _lib.check(status)
+    return Rows8(codes, scale)
+
+
+def rmsnorm8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
+             residual: torch.Tensor | None = None, out: torch.Tensor | None = None):
+    """The root-mean-square norm of the rows of x (rows, width), float32 or
+    bfloat16, times ``weight`` (width,) float32, in 8 bits with one scale each
+    (nb_rmsnorm8).  With a ``residual`` (of x's shape and dtype) the norm is that
+    of x + residual as x's dtype holds it, which is returned too (in ``out`` if
+    given, which may be x or residual): (Rows8, sum) then, else Rows8."""
+    dev, rows, width = _rows8_out(x)
+    if not _here(dev):
+        with torch.cuda.device(dev):
+            return rmsnorm8(x, weight, eps, residual=residual, out=out)
+    ld = _rows("x", x, rows, width, dev)
+    weight = _vector("weight", weight, torch.float32, width, dev)
+    if weight is None:
+        raise TypeError("weight must be a torch.Tensor")
+    ld_residual = ld_out = 0
+    if residual is None:
+        if out is not None:
+            raise ValueError("out is the sum with a residual: there is none")
+    else:
+        ld_residual = _rows("residual", residual, rows, width, dev)
+        if out is None:
+            out = torch.empty((rows, width), dtype=x.dtype, device=x.device)
+            ld_out = width
+        else:
+            ld_out = _rows("out", out, rows, width, dev)
+        if residual.dtype != x.dtype or out.dtype != x.dtype:
+            raise TypeError(f"x is {x.dtype}, residual {residual.dtype}, out {out.dtype}")
+    codes = torch.empty((rows, width), dtype=torch.int8, device=x.device)
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    if rows:
+        status = _lib.load().nb_rmsnorm8(
+            x.data_ptr(), _DT[x.dtype], ld, None if residual is None else residual.data_ptr(),
+            ld_residual, None if out is None else out.data_ptr(), ld_out, weight, eps, rows, width,
+            codes.data_ptr(), scale.data_ptr(), torch._C._cuda_getCurrentRawStream(dev))
+        if status:
+            _lib.check(status)
+    rows8 = Rows8(codes, scale)
+    return rows8 if residual is None else (rows8, out)
+
+
+def linear8_layout(packed: torch.Tensor, codebook: torch.Tensor, N: int, K: int) -> Weights8:
+    """A 3-bit / 8-entry / block-128 N x K layer for ``linear8``
+    (nb_linear8_layout), made once: its codebooks in 8 bits with one scale for
+    each output, its indices in tiles of 16 outputs x 128 inputs."""
+    for name, t in (("packed", packed), ("codebook", codebook)):
+        _require_cuda(name, t)
+    _same_device(packed, codebook)
+    if packed.dtype != torch.uint8 or codebook.dtype != torch.float32:
+        raise TypeError("packed must be uint8 and codebook float32")
+    if N < 1 or K < 128 or K % 128 or codebook.shape != (N * K // 128, 8) or \
+            packed.numel() < packed_nbytes(N * K, 3):
+        raise ValueError(f"not a 3-bit / 8-entry / block-128 {N}x{K} layer")
+    if not packed.is_contiguous() or not codebook.is_contiguous():
+        raise ValueError("packed and codebook must be contiguous")
+    if not _here(packed.get_device()):
+        with torch.cuda.device(packed.get_device()):
+            return linear8_layout(packed, codebook, N, K)
+    lib = _lib.load()
+    tiles = torch.empty(int(lib.nb_linear8_tiles_bytes(N, K)), dtype=torch.uint8,
+                        device=packed.device)
+    scale = torch.empty(N, dtype=torch.float32, device=packed.device)
+    _lib.check(lib.nb_linear8_layout(packed.data_ptr(), codebook.data_ptr(), N, K,
+                                     tiles.data_ptr(), scale.data_ptr(), _stream(packed)))
+    return Weights8(tiles, scale, N, K)
+
+
+@functools.lru_cache(maxsize=1024)
+def _linear8_bytes(dev, *sizes) -> int:
+    """Workspace bytes of nb_linear8 on GPU dev, the current one (they go by its
+    CUs)."""
+    return int(_lib.load().nb_linear8_ws_bytes(*sizes))
+
+
+def linear8(x: Rows8, weights: Weights8, *, bias: torch.Tensor | None = None,
+            activation: str | None = None, residual: torch.Tensor | None = None,
+            out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """Rows in 8 bits (rows, K) times a packed layer with 8-bit codebooks
+    (nb_linear8): activation(x @ W.T + bias) + residual, the products exact,
+    the sums whole numbers.  ``activation``: None, "silu", "gelu" or "swiglu"
+    (silu(y[:, 0::2]) * y[:, 1::2], half as many outputs).  ``bias`` (N,) float32;
+    ``residual`` of the outputs' shape and dtype.  Returns (rows, N) in
+    ``out_dtype`` (default: the residual's, else float32), or into ``out``, which
+    may be the residual."""
+    codes, x_scale = x
+    tiles, scale, N, K = weights
+    _require_cuda("x.codes", codes)
+    dev = codes.get_device()
+    if not _here(dev):
+        with torch.cuda.device(dev):
+            return linear8(x, weights, bias=bias, activation=activation, residual=residual, out=out,
+                           out_dtype=out_dtype)
+    if codes.dtype is not torch.int8 or codes.dim() != 2 or codes.shape[1] != K:
+        raise ValueError(f"x.codes must be (rows, {K}) int8, got {codes.dtype} {tuple(codes.shape)}")
+    rows = codes.shape[0]
+    ld = codes.stride(0) if rows > 1 else K
+    if codes.stride(1) != 1 or ld % 16 or ld < K or codes.data_ptr() % 16:
+        codes = codes.contiguous()
+        if codes.data_ptr() % 16:
+            codes = codes.clone()
+        ld = K
+    f32 = torch.float32
+    nbytes = (N + 15) // 16 * (K // 128) * 896
+    if tiles.dtype is not torch.uint8 or not tiles.is_contiguous() or tiles.numel() < nbytes:
+        _require_cuda("tiles", tiles)
+        raise ValueError(f"tiles must be {nbytes} contiguous bytes for a {N}x{K} layer")
+    if tiles.get_device() != dev:
+        raise ValueError(f"tensors on different devices: tiles on {tiles.device}, cuda:{dev}")
+    if not (_is(x_scale, f32, (rows,), dev) and _is(scale, f32, (N,), dev)):
+        _require("x.scale", x_scale, f32, (rows,), dev)
+        _require("scale", scale, f32, (N,), dev)
+    if bias is not None:
+        _require("bias", bias, f32, (N,), dev)
+    act = _ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"unknown activation {activation!r}")
+    if activation == "swiglu" and N % 2:
+        raise ValueError(f"swiglu takes pairs of outputs, {N} is odd")
+    columns = N // 2 if activation == "swiglu" else N
+    if out is None:
+        if out_dtype is None:
+            out_dtype = f32 if residual is None else residual.dtype
+        if out_dtype not in _DT:
+            raise TypeError(f"out_dtype {out_dtype} not supported (float32 or bfloat16)")
+        out = torch.empty((rows, columns), dtype=out_dtype, device=codes.device)
+        ld_out = columns
+    else:
+        if out_dtype is not None and out.dtype != out_dtype:
+            raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
+        ld_out = _rows("out", out, rows, columns, dev)
+    ld_residual = 0
+    if residual is not None:
+        ld_residual = _rows("residual", residual, rows, columns, dev)
+        if residual.dtype != out.dtype:
+            raise TypeError(f"residual is {residual.dtype}, the outputs {out.dtype}")
+    if rows:
+        nbytes = _linear8_bytes(dev, rows, N, K)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=codes.device) if nbytes else None
+        status = _lib.load().nb_linear8(
+            codes.data_ptr(), ld, x_scale.data_ptr(), tiles.data_ptr(), scale.data_ptr(),
+            None if bias is None else bias.data_ptr(), act,
+            None if residual is None else residual.data_ptr(), ld_residual, out.data_ptr(),
+            _DT[out.dtype], ld_out, rows, N, K, None if ws is None else ws.data_ptr(), nbytes,
+            torch._C._cuda_getCurrentRawStream(dev))
+        if status:
+            _lib.check(status)
+    return out
