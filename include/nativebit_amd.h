@@ -782,7 +782,7 @@ int nb_rmsnorm8(const void* x, int dtype, int64_t ld_x, const void* residual, in
                 int8_t* codes, float* scale, void* stream);
 /*
  * A 3-bit / 8-entry / block-128 layer (packed as above, K % 128 == 0, K <=
- * 2^17) for nb_linear8, once at load: for output n, a = the largest magnitude
+ * 2^17, N <= 2^24) for nb_linear8, once at load: for output n, a = the largest magnitude
  * among its blocks' entries, scale[n] = a / 127 (fp32 [N]), each entry's code
  * rint(entry * (127 / a)) (in 64 bits, ties to even).  tiles:
  * nb_linear8_tiles_bytes(N, K) = ceil(N / 16) * (K / 128) * 896 bytes, 16-byte
@@ -809,16 +809,15 @@ enum nb_activation {
  * bias fp32 [N] and residual (of y's type, stride ld_residual) may be NULL; y
  * NB_F32 or NB_BF16, stride ld_y; it may be the residual itself, of the same
  * stride, and else overlaps it in no element.  The sums over k are whole numbers
- * and exact, the rest is fp32, rounded to y's type once.  The workspace needs
- * nb_linear8_ws_bytes(M, N, K) bytes, 16-byte aligned (0: may be NULL).
+ * and exact, the rest is fp32, rounded to y's type once.  M <= 2^20, M N < 2^36,
+ * ld_x <= 2^22.
  * (PackedLinear.forward, inference/triton_kernel.py:240-275, and what follows
  * it in a block, inference/generate_torch.py:109-132.)
  */
-int64_t nb_linear8_ws_bytes(int M, int N, int K);
 int nb_linear8(const int8_t* x, int64_t ld_x, const float* x_scale, const uint8_t* tiles,
                const float* scale, const float* bias, int activation, const void* residual,
                int64_t ld_residual, void* y, int y_dtype, int64_t ld_y, int M, int N, int K,
-               void* workspace, int64_t ws_bytes, void* stream);
+               void* stream);
 
 /* ------------------------------------------------------------------------
  * Persistent decode: many greedy tokens of the whole packed decoder in one

@@ -121,8 +121,7 @@ SIGNATURES = {
     "nb_rmsnorm8": (_I, [_P, _I, _L, _P, _L, _P, _L, _P, ctypes.c_float, _I, _I, _P, _P, _P]),
     "nb_linear8_tiles_bytes": (_L, [_I, _I]),
     "nb_linear8_layout": (_I, [_P, _P, _I, _I, _P, _P, _P]),
-    "nb_linear8_ws_bytes": (_L, [_I, _I, _I]),
-    "nb_linear8": (_I, [_P, _L, _P, _P, _P, _P, _I, _P, _L, _P, _I, _L, _I, _I, _I, _P, _L, _P]),
+    "nb_linear8": (_I, [_P, _L, _P, _P, _P, _P, _I, _P, _L, _P, _I, _L, _I, _I, _I, _P]),
     "nb_decode_workspace_bytes": (_L, [_P]),
     "nb_decode_persistent": (_I, [_P, _P, _L, _P, _P, _P, _I, _P, _I, _I, _I, _P]),
 }

@@ -1500,7 +1500,9 @@ int check_layer8(const char* fn, int N, int K) {
     if (N < 0 || K < 128 || K % 128) {
         return fail(NB_EINVAL, "%s: N=%d K=%d (needs N >= 0, K > 0, K %% 128 == 0)", fn, N, K);
     }
-    if (K > 1 << 17) return fail(NB_EUNSUPPORTED, "%s: K=%d (<= 2^17)", fn, K);
+    if (K > 1 << 17 || N > 1 << 24) {
+        return fail(NB_EUNSUPPORTED, "%s: N=%d (<= 2^24) K=%d (<= 2^17)", fn, N, K);
+    }
     if (((int64_t)N + 15) / 16 * (K / 128) >= 1LL << 24) {
         return fail(NB_EUNSUPPORTED, "%s: N=%d K=%d, too large a layer", fn, N, K);
     }
@@ -1565,21 +1567,17 @@ int nb_linear8_layout(const uint8_t* packed, const float* codebook, int N, int K
     return launch_linear8_layout(packed, codebook, N, K, tiles, scale, static_cast<hipStream_t>(stream));
 }
 
-int64_t nb_linear8_ws_bytes(int M, int N, int K) {
-    if (M < 1 || N < 1 || K < 128 || K % 128 || K > 1 << 17) return 0;
-    if (ensure_device() != NB_OK) g_last_error[0] = '\0';   // (256 CUs without a device)
-    return linear8_bytes(M, N, K);
-}
-
 int nb_linear8(const int8_t* x, int64_t ld_x, const float* x_scale, const uint8_t* tiles,
                const float* scale, const float* bias, int activation, const void* residual,
                int64_t ld_residual, void* y, int y_dtype, int64_t ld_y, int M, int N, int K,
-               void* workspace, int64_t ws_bytes, void* stream) {
+               void* stream) {
     const char* fn = "nb_linear8";
     int st = check_layer8(fn, N, K);
     if (st) return st;
     if (M < 0) return fail(NB_EINVAL, "%s: M=%d", fn, M);
-    if (M > 1 << 20) return fail(NB_EUNSUPPORTED, "%s: M=%d (<= 2^20)", fn, M);
+    if (M > 1 << 20 || (int64_t)M * N >= 1LL << 36) {
+        return fail(NB_EUNSUPPORTED, "%s: M=%d N=%d (M <= 2^20, M N < 2^36)", fn, M, N);
+    }
     if (activation < NB_ACT_NONE || activation > NB_ACT_SWIGLU) {
         return fail(NB_EINVAL, "%s: activation=%d", fn, activation);
     }
@@ -1590,6 +1588,7 @@ int nb_linear8(const int8_t* x, int64_t ld_x, const float* x_scale, const uint8_
     if (st) return st;
     if (!x || !x_scale || !tiles || !scale) return fail(NB_EINVAL, "%s: NULL pointer", fn);
     if (ld_x < K || ld_x % 16) return fail(NB_EINVAL, "%s: ld_x=%lld (>= K, a multiple of 16)", fn, (long long)ld_x);
+    if (ld_x > 1 << 22) return fail(NB_EUNSUPPORTED, "%s: ld_x=%lld (<= 2^22)", fn, (long long)ld_x);
     if (!aligned(x, 16) || !aligned(tiles, 16)) return fail(NB_EALIGN, "%s: x and tiles need 16-byte alignment", fn);
     if (!aligned(x_scale, 4) || !aligned(scale, 4) || !aligned(bias, 4)) {
         return fail(NB_EALIGN, "%s: misaligned pointer", fn);
@@ -1601,15 +1600,10 @@ int nb_linear8(const int8_t* x, int64_t ld_x, const float* x_scale, const uint8_
             return fail(NB_EINVAL, "%s: y overlaps residual (in place: of the same stride)", fn);
         }
     }
-    const int dev_st = ensure_device();
-    const int64_t need = linear8_bytes(M, N, K);
-    if (ws_bytes < need || (need && !workspace)) {
-        return fail(NB_EINVAL, "%s: workspace of %lld bytes < %lld", fn, (long long)ws_bytes, (long long)need);
-    }
-    if (!aligned(workspace, 16)) return fail(NB_EALIGN, "%s: workspace not 16-byte aligned", fn);
-    if (dev_st) return dev_st;
+    st = ensure_device();
+    if (st) return st;
     return launch_linear8(x, ld_x, x_scale, tiles, scale, bias, activation, residual, ld_residual, y,
-                          y_dtype, ld_y, M, N, K, workspace, static_cast<hipStream_t>(stream));
+                          y_dtype, ld_y, M, N, K, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -271,8 +271,7 @@ int launch_linear8_layout(const uint8_t* packed, const float* codebook, int N, i
 int launch_linear8(const int8_t* x, int64_t ld_x, const float* x_scale, const uint8_t* tiles,
                    const float* scale, const float* bias, int activation, const void* residual,
                    int64_t ld_residual, void* y, int y_dtype, int64_t ld_y, int M, int N, int K,
-                   void* workspace, hipStream_t stream);
-int64_t linear8_bytes(int M, int N, int K);   // its workspace (0: none)
+                   hipStream_t stream);
 // nb_sample.hip
 int64_t sample_bytes(int rows, int V);   // its workspace (0: none)
 int launch_sample(const void* logits, int dtype, int64_t ld, int rows, int V, const float* u,

@@ -21,6 +21,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "nb_device.h"
 #include "nb_internal.h"
 #include "nb_stream_common.h"
@@ -48,7 +50,6 @@ struct Args {
     int64_t ld_y;
     int M, N, K;
     int activation;   // nb_activation
-    int y_dtype;
 };
 
 // A lane's unit of a tile and the codes of its output.
@@ -77,84 +78,144 @@ __device__ __forceinline__ i4 mfma(i4 w, i4 x, i4 sum) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(w, x, sum, 0, 0, 0);
 }
 
-__device__ __forceinline__ float silu(float v) { return v / (1.f + __expf(-v)); }
-
-__device__ __forceinline__ float read_as(const void* p, int dtype, int64_t i) {
-    return dtype == NB_BF16 ? bf16_to_f32(static_cast<const bf16_bits*>(p)[i])
-                            : static_cast<const float*>(p)[i];
+// (the reciprocal within a step: an IEEE quotient takes a dozen instructions, in
+// an epilogue whose instructions are a third of a prompt's time)
+__device__ __forceinline__ float silu(float v) {
+    return v * __builtin_amdgcn_rcpf(1.f + __expf(-v));
 }
 
-// `count` (4 or 2) neighbouring values of a row from element `at` on, `left` of
-// them in the row.
-template <int kCount>
-__device__ __forceinline__ void finish_row(const Args& a, int m, int n, int left, float (&v)[kCount]) {
-    if (a.residual) {
-        const int64_t at = m * a.ld_residual + n;
-#pragma unroll
-        for (int e = 0; e < kCount; ++e) {
-            if (e < left) v[e] += read_as(a.residual, a.y_dtype, at + e);
-        }
-    }
-    const int64_t at = m * a.ld_y + n;
-    if (a.y_dtype == NB_BF16) {
-        bf16_bits* y = static_cast<bf16_bits*>(a.y) + at;
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+    typedef __attribute__((ext_vector_type(2))) __bf16 pair;
+    return __builtin_bit_cast(uint32_t, pair{(__bf16)lo, (__bf16)hi});
+}
+
+// f(the activation as a constant): its code has no branches inside loops.
+template <typename F>
+__device__ __forceinline__ void by_activation(int activation, F f) {
+    if (activation == NB_ACT_NONE) f(std::integral_constant<int, NB_ACT_NONE>{});
+    else if (activation == NB_ACT_SWIGLU) f(std::integral_constant<int, NB_ACT_SWIGLU>{});
+    else if (activation == NB_ACT_SILU) f(std::integral_constant<int, NB_ACT_SILU>{});
+    else f(std::integral_constant<int, NB_ACT_GELU>{});
+}
+
+// kCount (4 or 2) neighbouring values of a row, `left` of them in the row.
+template <int kCount, bool kBf16>
+__device__ __forceinline__ void load_some(const void* row, int64_t at, int left, float (&v)[kCount]) {
+    if constexpr (kBf16) {
+        const bf16_bits* p = static_cast<const bf16_bits*>(row) + at;
         typedef __attribute__((ext_vector_type(kCount / 2), aligned(2))) uint32_t any;
         if (left >= kCount) {
-            any p;
+            const any w = *reinterpret_cast<const any*>(p);
 #pragma unroll
             for (int e = 0; e < kCount; e += 2) {
-                p[e / 2] = f32_to_bf16_rne(v[e]) | (uint32_t)f32_to_bf16_rne(v[e + 1]) << 16;
+                const uint32_t u = reinterpret_cast<const uint32_t*>(&w)[e / 2];
+                v[e] = __uint_as_float(u << 16);
+                v[e + 1] = __uint_as_float(u & 0xffff0000u);
             }
-            *reinterpret_cast<any*>(y) = p;
+        } else {
+#pragma unroll
+            for (int e = 0; e < kCount; ++e) v[e] = e < left ? bf16_to_f32(p[e]) : 0.f;
+        }
+    } else {
+        const float* p = static_cast<const float*>(row) + at;
+        typedef __attribute__((ext_vector_type(kCount), aligned(4))) float any;
+        if (left >= kCount) {
+            const any w = *reinterpret_cast<const any*>(p);
+#pragma unroll
+            for (int e = 0; e < kCount; ++e) v[e] = w[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < kCount; ++e) v[e] = e < left ? p[e] : 0.f;
+        }
+    }
+}
+
+template <int kCount, bool kBf16>
+__device__ __forceinline__ void store_some(void* row, int64_t at, int left, const float (&v)[kCount]) {
+    if constexpr (kBf16) {
+        bf16_bits* p = static_cast<bf16_bits*>(row) + at;
+        typedef __attribute__((ext_vector_type(kCount / 2), aligned(2))) uint32_t any;
+        if (left >= kCount) {
+            uint32_t w[kCount / 2];
+#pragma unroll
+            for (int e = 0; e < kCount; e += 2) {
+                w[e / 2] = bf16_pair(v[e], v[e + 1]);
+            }
+            *reinterpret_cast<any*>(p) = *reinterpret_cast<const any*>(w);
         } else {
 #pragma unroll
             for (int e = 0; e < kCount; ++e) {
-                if (e < left) y[e] = f32_to_bf16_rne(v[e]);
+                if (e < left) p[e] = f32_to_bf16_rne(v[e]);
             }
         }
     } else {
-        float* y = static_cast<float*>(a.y) + at;
+        float* p = static_cast<float*>(row) + at;
         typedef __attribute__((ext_vector_type(kCount), aligned(4))) float any;
         if (left >= kCount) {
-            any p;
-#pragma unroll
-            for (int e = 0; e < kCount; ++e) p[e] = v[e];
-            *reinterpret_cast<any*>(y) = p;
+            *reinterpret_cast<any*>(p) = *reinterpret_cast<const any*>(v);
         } else {
 #pragma unroll
             for (int e = 0; e < kCount; ++e) {
-                if (e < left) y[e] = v[e];
+                if (e < left) p[e] = v[e];
             }
         }
     }
 }
 
-// The outputs of four sums: of row m, layer outputs n .. n + 3 (n a multiple of 4).
-__device__ __forceinline__ void finish(const Args& a, int m, int n, i4 sum) {
-    if (m >= a.M || n >= a.N) return;
-    const float xs = a.x_scale[m];
-    const int left = a.N - n;
-    float v[4];
+// Scales and biases of layer outputs n .. n + 3 (n a multiple of 4), the last
+// output's past the layer.
+struct Column {
+    float scale[4], bias[4];
+};
+__device__ __forceinline__ Column column(const Args& a, int n) {
+    Column c;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const int at = n + min(e, left - 1);
-        v[e] = (float)sum[e] * (xs * a.scale[at]);
-        if (a.bias) v[e] += a.bias[at];
+        const int at = min(n + e, a.N - 1);
+        c.scale[e] = a.scale[at];
+        c.bias[e] = a.bias ? a.bias[at] : 0.f;
     }
-    if (a.activation == NB_ACT_SWIGLU) {   // (N is even)
-        float g[2] = {silu(v[0]) * v[1], silu(v[2]) * v[3]};
-        return finish_row<2>(a, m, n / 2, left / 2, g);
-    }
-    if (a.activation == NB_ACT_SILU) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = silu(v[e]);
-    } else if (a.activation == NB_ACT_GELU) {
-        // v Phi(v) by erfc: no cancellation for negative v
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = 0.5f * v[e] * erfcf(-0.70710678f * v[e]);
-    }
-    finish_row<4>(a, m, n, left, v);
+    return c;
 }
+
+// The outputs of four sums: row m, layer outputs n .. n + 3.  Loads, arithmetic and
+// stores are apart, so that a loop can put several in flight (stores count among
+// the loads that a wait is for).
+template <int kAct>
+struct Finished {
+    static constexpr int kCount = kAct == NB_ACT_SWIGLU ? 2 : 4;   // (swiglu: N is even)
+    float v[kCount];
+
+    template <bool kBf16>
+    __device__ __forceinline__ void load_residual(const Args& a, int m, int n) {
+        if (m < a.M && n < a.N) {
+            load_some<kCount, kBf16>(a.residual, m * a.ld_residual + n * kCount / 4,
+                                     (a.N - n) * kCount / 4, v);
+        }
+    }
+    // xs: the row's scale; kResidual: v holds the residual
+    template <bool kResidual>
+    __device__ __forceinline__ void finish(const Column& c, float xs, i4 sum) {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = (float)sum[e] * (xs * c.scale[e]) + c.bias[e];
+#pragma unroll
+        for (int e = 0; e < kCount; ++e) {
+            float out = y[e];
+            if constexpr (kAct == NB_ACT_SWIGLU) out = silu(y[2 * e]) * y[2 * e + 1];
+            else if constexpr (kAct == NB_ACT_SILU) out = silu(y[e]);
+            // v Phi(v) by erfc: no cancellation for negative v
+            else if constexpr (kAct == NB_ACT_GELU) out = 0.5f * y[e] * erfcf(-0.70710678f * y[e]);
+            v[e] = kResidual ? out + v[e] : out;
+        }
+    }
+    template <bool kBf16>
+    __device__ __forceinline__ void store(const Args& a, int m, int n) const {
+        if (m < a.M && n < a.N) {
+            store_some<kCount, kBf16>(a.y, m * a.ld_y + n * kCount / 4, (a.N - n) * kCount / 4, v);
+        }
+    }
+};
 
 }  // namespace linear8
 }  // namespace nb

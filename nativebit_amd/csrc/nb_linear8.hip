@@ -1,6 +1,15 @@
 // Rows in 8 bits times packed 3-bit weights with 8-bit codebooks (gfx950):
-// nb_linear8_layout, and nb_linear8 for few rows.  Formulas and layout:
-// nb_linear8.h.
+// nb_linear8_layout and nb_linear8.  Formulas and layout: nb_linear8.h.
+//
+// Few rows: bound by latency (a launch, one trip to the weights, the sum over the
+// waves; 2560 x 2560 at one row 3.9 us, 13824 x 2560 5.1 for 15.5 MB).  Many rows: bound
+// by the LDS reads of rows and units beside the products (about 1700 of the 2048
+// cycles that a 256 x 256 x 128 step's products take, in a step of 3000; without
+// barriers 2600, without operands made 2400, loads alone 100), and at the ends by
+// whole rounds of tiles and the epilogue: 13824 x 2560 at 2048 rows 79 us, 1830
+// TOP/s.  Measured and not faster there: units straight to registers (88 us against
+// 82 with 128 x 128 tiles: 12 and 8 bytes a lane are many small requests), waits a block
+// later, tiles of an XCD in the other order.
 #include <math.h>
 
 #include <algorithm>
@@ -90,45 +99,385 @@ __global__ __launch_bounds__(64) void linear8_layout_kernel(const uint8_t* packe
 // ---------------------------------------------------------------------------
 // few rows
 // ---------------------------------------------------------------------------
-// A workgroup takes 16 outputs and 16 kT rows; its waves take the blocks of K in
-// turn and add their sums through LDS.
-template <int kWaves, int kT>
-__global__ __launch_bounds__(64 * kWaves) void linear8_rows_kernel(Args a) {
-    __shared__ i4 part[kWaves][kT][64];
+// A workgroup takes 16 kI outputs and 16 kJ rows; its waves take the blocks of K
+// in turn, each all outputs and rows, and add their sums through LDS.  Units and
+// rows come straight from memory, the next block's ahead of this one's products.
+template <int kWaves, int kI, int kJ, bool kBf16>
+__global__ __launch_bounds__(64 * kWaves, 2) void linear8_rows_kernel(Args a) {
+    extern __shared__ __align__(16) i4 part[];   // [kWaves][kI][kJ][64]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * kT;
-    const int bpr = a.K / 128;
-    const uint8_t* tiles = a.tiles + (int64_t)blockIdx.x * bpr * kTileBytes;
-    const int8_t* x[kT];
+    const int bpr = a.K / 128, last = (a.N + 15) / 16 - 1;
+    const int n0 = blockIdx.x * 16 * kI, m0 = blockIdx.y * 16 * kJ;
+    const uint8_t* tiles[kI];
 #pragma unroll
-    for (int t = 0; t < kT; ++t) {
-        const int m = min(m0 + 16 * t + (lane & 15), a.M - 1);
-        x[t] = a.x + m * a.ld_x + (lane >> 4) * 32;
+    for (int i = 0; i < kI; ++i) {
+        tiles[i] = a.tiles + (int64_t)min((int)blockIdx.x * kI + i, last) * bpr * kTileBytes;
     }
-    i4 sum[kT];
+    const int8_t* x[kJ];
 #pragma unroll
-    for (int t = 0; t < kT; ++t) sum[t] = i4{0, 0, 0, 0};
-    for (int kb = wave; kb < bpr; kb += kWaves) {
-        const Unit u = load_unit(tiles + (int64_t)kb * kTileBytes, lane);
-        i4 w[2];
-        unit_weights(u, w);
+    for (int j = 0; j < kJ; ++j) {
+        x[j] = a.x + min(m0 + 16 * j + (lane & 15), a.M - 1) * a.ld_x + (lane >> 4) * 32;
+    }
+    struct Block {
+        Unit u[kI];
+        i4 x[kJ][2];
+    };
+    auto load = [&](int kb, Block& b) {
 #pragma unroll
-        for (int t = 0; t < kT; ++t) {
-            const i4* p = reinterpret_cast<const i4*>(x[t] + kb * 128);
-            sum[t] = mfma(w[0], p[0], sum[t]);
-            sum[t] = mfma(w[1], p[1], sum[t]);
+        for (int i = 0; i < kI; ++i) b.u[i] = load_unit(tiles[i] + (int64_t)kb * kTileBytes, lane);
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) {
+            const i4* p = reinterpret_cast<const i4*>(x[j] + kb * 128);
+            b.x[j][0] = p[0], b.x[j][1] = p[1];
         }
+    };
+    i4 sum[kI][kJ];
+#pragma unroll
+    for (int i = 0; i < kI; ++i)
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) sum[i][j] = i4{0, 0, 0, 0};
+    auto multiply = [&](const Block& b) {
+#pragma unroll
+        for (int i = 0; i < kI; ++i) {
+            i4 w[2];
+            unit_weights(b.u[i], w);
+#pragma unroll
+            for (int j = 0; j < kJ; ++j) {
+                sum[i][j] = mfma(w[0], b.x[j][0], sum[i][j]);
+                sum[i][j] = mfma(w[1], b.x[j][1], sum[i][j]);
+            }
+        }
+    };
+    Block b0, b1;
+    if (wave < bpr) load(wave, b0);
+    for (int kb = wave; kb < bpr; kb += 2 * kWaves) {
+        if (kb + kWaves < bpr) load(kb + kWaves, b1);
+        multiply(b0);
+        if (kb + kWaves >= bpr) break;
+        if (kb + 2 * kWaves < bpr) load(kb + 2 * kWaves, b0);
+        multiply(b1);
     }
 #pragma unroll
-    for (int t = 0; t < kT; ++t) part[wave][t][lane] = sum[t];
+    for (int i = 0; i < kI; ++i)
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) part[((wave * kI + i) * kJ + j) * 64 + lane] = sum[i][j];
     __syncthreads();
-    for (int i = tid; i < kT * 64; i += 64 * kWaves) {
-        const int t = i >> 6, l = i & 63;
-        i4 s = part[0][t][l];
+    for (int at = tid; at < kI * kJ * 64; at += 64 * kWaves) {
+        const int i = at / (kJ * 64), j = at / 64 % kJ, l = at & 63;
+        const int m = m0 + 16 * j + (l & 15), n = n0 + 16 * i + (l >> 4) * 4;
+        const Column c = column(a, n);
+        const float xs = a.x_scale[min(m, a.M - 1)];
+        i4 s = part[at];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) s += part[w][t][l];
-        finish(a, m0 + 16 * t + (l & 15), n0 + (l >> 4) * 4, s);
+        for (int w = 1; w < kWaves; ++w) s += part[w * kI * kJ * 64 + at];
+        by_activation(a.activation, [&](auto act) {
+            Finished<decltype(act)::value> f;
+            if (a.residual) {
+                f.template load_residual<kBf16>(a, m, n);
+                f.template finish<true>(c, xs, s);
+            } else {
+                f.template finish<false>(c, xs, s);
+            }
+            f.template store<kBf16>(a, m, n);
+        });
     }
+}
+
+// ---------------------------------------------------------------------------
+// many rows
+// ---------------------------------------------------------------------------
+// (s_nop: the wait state between a scalar write of m0 and a load to LDS)
+__device__ __forceinline__ void load_to_lds(uint32_t lds, const void* base, uint32_t offset) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(lds), "v"(offset), "s"(base)
+                 : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t lds_address(void* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)p;
+}
+
+// A lane's unit of a tile in LDS.
+__device__ __forceinline__ Unit read_unit(const unsigned char* tile, int lane) {
+    const uint32_t* d = reinterpret_cast<const uint32_t*>(tile + lane * 12);
+    const u2 c = *reinterpret_cast<const u2*>(tile + kTileCodes + (lane & 15) * 8);
+    return Unit{d[0], d[1], d[2], c[0], c[1]};
+}
+// Half h of its weights (10 and 15 instructions).
+template <int kHalf>
+__device__ __forceinline__ i4 half_weights(const Unit& u) {
+    i4 w[2];
+    unit_weights(u, w);
+    return w[kHalf];
+}
+
+constexpr int kAhead = 2;   // reads of rows under way in front of the products
+
+// Sizes of a workgroup of kN x kM waves with kI x kJ products of 16 x 16 each and
+// kStages blocks in LDS, kSplit times.
+template <int kI, int kJ, int kN, int kM, int kStages, int kSplit>
+struct Tile {
+    static constexpr int kWaves = kN * kM, kOutputs = 16 * kI * kN, kRows = 16 * kJ * kM;
+    static constexpr int kRowLoads = kRows / (8 * kWaves);   // of a wave, 1 KB each: eight rows
+    static constexpr int kTileLoads = (kI * kN * kTileBytes + 1024 * kWaves - 1) / (1024 * kWaves);
+    static constexpr int kStage = kRows * 128 + kTileLoads * kWaves * 1024;
+    static constexpr int kHalf = kJ < 4 ? kJ : 4;            // groups of 16 rows that leave at once
+    static constexpr int kPitch = 16 * kI + 4;
+    static constexpr int kSums = kWaves * 16 * kHalf * kPitch * 4;
+    static constexpr int kLds = kSplit * (kStages * kStage > kSums ? kStages * kStage : kSums);
+    static constexpr int kThreads = 64 * kWaves * kSplit;
+    static constexpr int kLoads = kRowLoads + kTileLoads;    // of a wave and block
+    static_assert(kRows % (8 * kWaves) == 0, "rows of a wave's loads");
+    static_assert(kStages >= 3 && (kStages - 2) * kLoads < 64, "loads under way");
+};
+
+// All but the last kLoads loads of the wave are there.  (The compiler does not track
+// those to LDS.)
+template <int kLoads>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kLoads) : "memory");
+}
+
+// A workgroup of kN x kM waves takes 16 kI kN outputs and 16 kJ kM rows and walks K
+// a block at a time, wave (n, m) with kI x kJ products of 16 x 16.  Rows and tiles
+// are loaded straight to LDS, kStages blocks of them, 16-byte chunk c of row r in place
+// c ^ (r & 7), so that eight rows' reads of a chunk hit eight groups of banks.
+// In the middle of a block the next one is waited for, and one is asked for into the
+// place of the last one, which the barrier there says all waves have left: kStages
+// - 1 blocks ahead, past the end the last block again (every wave has the same
+// number of loads under way at every wait).  While a half block's products run, the
+// next half's operands are made.
+// kSplit > 1: so many groups of waves take the blocks of K in turn, each with LDS of
+// its own; their sums are added as they leave.
+template <int kI, int kJ, int kN, int kM, int kStages, int kSplit, bool kBf16>
+__global__ __launch_bounds__(64 * kN * kM * kSplit, 2) void linear8_tiles_kernel(Args a) {
+    using T = Tile<kI, kJ, kN, kM, kStages, kSplit>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, all = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = all % T::kWaves, group = all / T::kWaves;
+    const int fr = lane & 15, fq = lane >> 4;
+    const int bpr = a.K / 128, last = (a.N + 15) / 16 - 1;
+    // workgroups are dealt to the 8 XCDs in turn; an XCD takes a contiguous run of
+    // tiles, so that its L2 holds the rows of one or two of them
+    const int columns = (a.N + T::kOutputs - 1) / T::kOutputs;
+    const int total = gridDim.x, g = blockIdx.x, xcd = g % 8;
+    const int tile = xcd * (total / 8) + min(xcd, total % 8) + g / 8;
+    const int n0 = tile % columns * T::kOutputs, m0 = tile / columns * T::kRows;
+    const int wn = wave % kN, wm = wave / kN;
+
+    // what the wave loads of a block, as offsets that every block shares (under
+    // 2^31: ld_x is at most 2^22); rows and tiles past the last one are that again
+    const int8_t* rows = a.x + m0 * a.ld_x;
+    const uint8_t* tiles = a.tiles + (int64_t)(n0 / 16) * bpr * kTileBytes;
+    uint32_t row_at[T::kRowLoads], tile_at[T::kTileLoads];
+#pragma unroll
+    for (int i = 0; i < T::kRowLoads; ++i) {
+        const int r = (wave * T::kRowLoads + i) * 8 + (lane >> 3);
+        row_at[i] = (uint32_t)(min(r, a.M - 1 - m0) * (int)a.ld_x) + (((lane & 7) ^ (r & 7)) << 4);
+    }
+#pragma unroll
+    for (int i = 0; i < T::kTileLoads; ++i) {
+        const int at = (wave * T::kTileLoads + i) * 1024 + lane * 16;
+        tile_at[i] = (uint32_t)(min(at / kTileBytes, last - n0 / 16) * bpr * kTileBytes + at % kTileBytes);
+    }
+    unsigned char* lds = smem + group * kStages * T::kStage;
+    const uint32_t lds_rows = lds_address(lds) + wave * T::kRowLoads * 1024;
+    const uint32_t lds_tiles = lds_address(lds) + T::kRows * 128 + wave * T::kTileLoads * 1024;
+    auto load = [&](int turn, int stage) {
+        const int kb = min(turn * kSplit + group, bpr - 1);
+#pragma unroll
+        for (int i = 0; i < T::kRowLoads; ++i) {
+            load_to_lds(__builtin_amdgcn_readfirstlane(lds_rows + stage * T::kStage + i * 1024),
+                        rows + kb * 128, row_at[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < T::kTileLoads; ++i) {
+            load_to_lds(__builtin_amdgcn_readfirstlane(lds_tiles + stage * T::kStage + i * 1024),
+                        tiles + kb * kTileBytes, tile_at[i]);
+        }
+    };
+    i4 sum[kI][kJ];
+#pragma unroll
+    for (int i = 0; i < kI; ++i)
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) sum[i][j] = i4{0, 0, 0, 0};
+    const unsigned char* own_rows = lds + (wm * 16 * kJ + fr) * 128;
+    const unsigned char* own_tiles = lds + T::kRows * 128 + wn * kI * kTileBytes;
+    // The products of half h of the block in `stage`.  The next half's operands are
+    // made meanwhile: after half 0 those of half 1, of the units in registers; after
+    // half 1 those of half 0 of the block in `after`, whose units are read first.
+    // (Left alone, the compiler puts all operands in front of the products that use
+    // them, and reads next to their use.)
+    Unit u[kI];
+    auto half = [&](auto h_, int stage, int after, const i4 (&w)[kI], i4 (&next)[kI]) {
+        constexpr int h = decltype(h_)::value;
+        const unsigned char* s = own_rows + stage * T::kStage + (((2 * fq + h) ^ (fr & 7)) << 4);
+        const unsigned char* t = own_tiles + after * T::kStage;
+        i4 x[kJ];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) x[j] = *reinterpret_cast<const i4*>(s + j * 2048);
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) {
+            if (j + kAhead < kJ) x[j + kAhead] = *reinterpret_cast<const i4*>(s + (j + kAhead) * 2048);
+#pragma unroll
+            for (int i = 0; i < kI; ++i) {
+                if (h == 1 && i * kJ / kI == j) u[i] = read_unit(t + i * kTileBytes, lane);
+            }
+#pragma unroll
+            for (int i = 0; i < kI; ++i) sum[i][j] = mfma(w[i], x[j], sum[i][j]);
+#pragma unroll
+            for (int i = 0; i < kI; ++i) {
+                if ((i + 1) * kJ / kI - 1 == j) next[i] = half_weights<1 - h>(u[i]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int i = 0; i < kI; ++i) asm volatile("" : "+v"(next[i]));   // (made here, not later)
+    };
+    using zero = std::integral_constant<int, 0>;
+    using one = std::integral_constant<int, 1>;
+    i4 w0[kI], w1[kI];
+#pragma unroll
+    for (int turn = 0; turn < kStages - 1; ++turn) load(turn, turn);
+    wait_loads<(kStages - 2) * T::kLoads>();
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kI; ++i) {
+        u[i] = read_unit(own_tiles + i * kTileBytes, lane);
+        w0[i] = half_weights<0>(u[i]);
+    }
+    int stage = 0;
+    for (int turn = 0; turn * kSplit < bpr; ++turn) {
+        const int after = stage == kStages - 1 ? 0 : stage + 1;
+        const bool mine = kSplit == 1 || turn * kSplit + group < bpr;
+        if (mine) half(zero{}, stage, after, w0, w1);
+        wait_loads<(kStages - 3) * T::kLoads>();
+        __syncthreads();
+        load(turn + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
+        // (past the last block: operands that nothing uses)
+        if (mine) half(one{}, stage, after, w1, w0);
+        stage = after;
+    }
+    wait_loads<0>();
+    __syncthreads();
+    // The sums go through LDS, kHalf of the wave's 16-row groups at a time, so that a
+    // row's outputs leave side by side, in a loop that is not unrolled over them
+    // (sums in registers have no index).
+    constexpr int kLanes = 4 * kI, kRegion = 16 * T::kHalf * T::kPitch;
+    int* sums = reinterpret_cast<int*>(smem);
+    const int n = n0 + wn * 16 * kI + lane % kLanes * 4;
+    const Column c = column(a, n);
+#pragma unroll
+    for (int j0 = 0; j0 < kJ; j0 += T::kHalf) {
+        const int first = m0 + (wm * kJ + j0) * 16;
+        const float xs = a.x_scale[min(first + lane, a.M - 1)];   // of 16 kHalf <= 64 rows
+        if (kSplit > 1 && j0) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kI; ++i)
+#pragma unroll
+            for (int j = 0; j < T::kHalf; ++j) {
+                *reinterpret_cast<i4*>(sums + all * kRegion + (j * 16 + fr) * T::kPitch + i * 16 +
+                                       fq * 4) = sum[i][j0 + j];
+            }
+        if (kSplit > 1) __syncthreads();   // (else read by the wave itself, in order)
+        by_activation(a.activation, [&](auto act) {
+            constexpr int kAct = decltype(act)::value;
+            auto leave = [&](auto residual) {
+                constexpr int kStep = 64 / kLanes, kTurns = T::kHalf * 16 / kStep / kSplit;
+                constexpr int kAtOnce = kTurns < 4 ? kTurns : 4;
+                static_assert(kTurns > 0 && kTurns % kAtOnce == 0, "turns of the epilogue");
+                const int r0 = group * kTurns * kStep + lane / kLanes;
+#pragma unroll 1
+                for (int turn = 0; turn < kTurns; turn += kAtOnce) {
+                    Finished<kAct> f[kAtOnce];
+#pragma unroll
+                    for (int i = 0; i < kAtOnce; ++i) {
+                        if constexpr (decltype(residual)::value) {
+                            f[i].template load_residual<kBf16>(a, first + r0 + (turn + i) * kStep, n);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < kAtOnce; ++i) {
+                        const int r = r0 + (turn + i) * kStep;
+                        const int* at = sums + wave * kRegion + r * T::kPitch + lane % kLanes * 4;
+                        i4 v = *reinterpret_cast<const i4*>(at);
+#pragma unroll
+                        for (int k = 1; k < kSplit; ++k) {
+                            v += *reinterpret_cast<const i4*>(at + k * T::kWaves * kRegion);
+                        }
+                        f[i].template finish<decltype(residual)::value>(c, __shfl(xs, r), v);
+                    }
+#pragma unroll
+                    for (int i = 0; i < kAtOnce; ++i) {
+                        f[i].template store<kBf16>(a, first + r0 + (turn + i) * kStep, n);
+                    }
+                }
+            };
+            if (a.residual) leave(std::true_type{});
+            else leave(std::false_type{});
+        });
+    }
+}
+
+template <int kWaves, int kI, int kJ>
+void launch_rows(const Args& a, bool bf16, hipStream_t stream) {
+    const dim3 grid((unsigned)((a.N + 16 * kI - 1) / (16 * kI)), (unsigned)((a.M + 16 * kJ - 1) / (16 * kJ)));
+    constexpr size_t lds = (size_t)kWaves * kI * kJ * 64 * 16;
+    auto* kernel = bf16 ? linear8_rows_kernel<kWaves, kI, kJ, true> : linear8_rows_kernel<kWaves, kI, kJ, false>;
+    hipLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), lds, stream, a);
+}
+
+template <int kI, int kJ, int kN, int kM, int kStages, int kSplit>
+void launch_tiles(const Args& a, bool bf16, hipStream_t stream) {
+    using T = Tile<kI, kJ, kN, kM, kStages, kSplit>;
+    const int64_t grid = (int64_t)((a.N + T::kOutputs - 1) / T::kOutputs) * ((a.M + T::kRows - 1) / T::kRows);
+    auto* kernel = bf16 ? linear8_tiles_kernel<kI, kJ, kN, kM, kStages, kSplit, true>
+                        : linear8_tiles_kernel<kI, kJ, kN, kM, kStages, kSplit, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(T::kThreads), T::kLds, stream, a);
+}
+
+// The forms, and what each costs in microseconds: `launch` once, `start` for the
+// workgroups that a CU holds at once, `step[c - 1]` for a block of K (of `split`) with c of
+// them.  Fitted to 413 shapes (1 to 2500 rows, 64 to 16000 outputs, K of 128 to 8192)
+// times 10 forms on MI355X; the form of least estimated time is 2 % slower than
+// the fastest one on the mean, half as long again at worst (long K, few outputs,
+// hundreds of rows).  What the other forms lose where each is taken: 9 rows of 7680 x 2560
+// 4.4 us by 32 x 32 (rows), 5.2 by 16 x 16, 6.4 by 64 x 32; 129 of 2560 x 6912 13.0 by 64 x
+// 32, 14.4 by 64 x 64, 18.3 by rows; 512 of 2560 x 6912 20.2 by 128 x 64 of two
+// groups, 27.3 of one, 27.9 by 64 x 64; 1500 of it 30.7 by 128 x 128 of two groups, 36.0 by
+// 128 x 64, 36.8 of one; 1500 of 13824 x 2560 67 by 128 x 128 of one, 85 of two, 75 by 256
+// x 256; 2048 of it 79.5 by 256 x 256, 85 by 128 x 128.
+struct Form {
+    int outputs, rows, split, resident;
+    float launch, start, step[2];
+    void (*run)(const Args&, bool, hipStream_t);
+};
+const Form kForms[] = {
+    {16, 16, 8, 1, 3.11f, 0.f, {0.276f}, launch_rows<8, 1, 1>},
+    {32, 32, 8, 2, 3.0f, 0.f, {0.58f, 1.21f}, launch_rows<8, 2, 2>},
+    {64, 32, 2, 2, 1.65f, 1.98f, {0.287f, 0.516f}, launch_tiles<1, 2, 4, 1, 4, 2>},
+    {64, 64, 2, 1, 1.03f, 2.46f, {0.397f}, launch_tiles<1, 4, 4, 1, 4, 2>},
+    {128, 64, 2, 1, 0.38f, 3.25f, {0.603f}, launch_tiles<2, 4, 4, 1, 3, 2>},
+    {128, 64, 1, 2, 1.25f, 2.36f, {0.392f, 0.546f}, launch_tiles<2, 4, 4, 1, 3, 1>},
+    {128, 128, 2, 1, 0.f, 4.53f, {0.919f}, launch_tiles<2, 8, 4, 1, 3, 2>},
+    {128, 128, 1, 1, 2.12f, 2.32f, {0.497f}, launch_tiles<2, 8, 4, 1, 3, 1>},
+    {256, 256, 1, 1, 0.f, 6.93f, {1.446f}, launch_tiles<4, 8, 4, 2, 3, 1>},
+};
+
+const Form& form_of(int M, int N, int K) {
+    const int64_t cus = device_cu_count();
+    const Form* best = &kForms[0];
+    float least = INFINITY;
+    for (const Form& f : kForms) {
+        const int64_t grid = ((int64_t)N + f.outputs - 1) / f.outputs * (((int64_t)M + f.rows - 1) / f.rows);
+        if (grid >= 1 << 22) continue;   // (a launch is under 2^32 threads; M N < 2^36: 256 x 256 fits)
+        const int64_t each = (grid + cus - 1) / cus, rest = each % f.resident;
+        const float steps = (float)((K / 128 + f.split - 1) / f.split);
+        float t = f.launch + (float)(each / f.resident) * (f.start + steps * f.step[f.resident - 1]);
+        if (rest) t += f.start + steps * f.step[rest - 1];
+        if (t < least) least = t, best = &f;
+    }
+    return *best;
 }
 
 }  // namespace
@@ -146,21 +495,13 @@ int launch_linear8_layout(const uint8_t* packed, const float* codebook, int N, i
     return check_launch("nb_linear8_layout");
 }
 
-int64_t linear8_bytes(int, int, int) { return 0; }
-
 int launch_linear8(const int8_t* x, int64_t ld_x, const float* x_scale, const uint8_t* tiles,
                    const float* scale, const float* bias, int activation, const void* residual,
                    int64_t ld_residual, void* y, int y_dtype, int64_t ld_y, int M, int N, int K,
-                   void*, hipStream_t stream) {
+                   hipStream_t stream) {
     const Args a{x, ld_x, x_scale, tiles, scale, bias, residual, ld_residual, y, ld_y, M, N, K,
-                 activation, y_dtype};
-    const unsigned columns = ((unsigned)N + 15) / 16;
-    if (M <= 16) {
-        hipLaunchKernelGGL((linear8_rows_kernel<8, 1>), dim3(columns, 1), dim3(512), 0, stream, a);
-    } else {
-        hipLaunchKernelGGL((linear8_rows_kernel<8, 4>), dim3(columns, ((unsigned)M + 63) / 64),
-                           dim3(512), 0, stream, a);
-    }
+                 activation};
+    form_of(M, N, K).run(a, y_dtype == NB_BF16, stream);
     return check_launch("nb_linear8");
 }
 

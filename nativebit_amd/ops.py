@@ -1116,13 +1116,6 @@ def linear8_layout(packed: torch.Tensor, codebook: torch.Tensor, N: int, K: int)
     return Weights8(tiles, scale, N, K)
 
 
-@functools.lru_cache(maxsize=1024)
-def _linear8_bytes(dev, *sizes) -> int:
-    """Workspace bytes of nb_linear8 on GPU dev, the current one (they go by its
-    CUs)."""
-    return int(_lib.load().nb_linear8_ws_bytes(*sizes))
-
-
 def linear8(x: Rows8, weights: Weights8, *, bias: torch.Tensor | None = None,
             activation: str | None = None, residual: torch.Tensor | None = None,
             out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -1145,7 +1138,7 @@ def linear8(x: Rows8, weights: Weights8, *, bias: torch.Tensor | None = None,
         raise ValueError(f"x.codes must be (rows, {K}) int8, got {codes.dtype} {tuple(codes.shape)}")
     rows = codes.shape[0]
     ld = codes.stride(0) if rows > 1 else K
-    if codes.stride(1) != 1 or ld % 16 or ld < K or codes.data_ptr() % 16:
+    if codes.stride(1) != 1 or ld % 16 or not K <= ld <= 1 << 22 or codes.data_ptr() % 16:
         codes = codes.contiguous()
         if codes.data_ptr() % 16:
             codes = codes.clone()
@@ -1185,14 +1178,11 @@ def linear8(x: Rows8, weights: Weights8, *, bias: torch.Tensor | None = None,
         if residual.dtype != out.dtype:
             raise TypeError(f"residual is {residual.dtype}, the outputs {out.dtype}")
     if rows:
-        nbytes = _linear8_bytes(dev, rows, N, K)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=codes.device) if nbytes else None
         status = _lib.load().nb_linear8(
             codes.data_ptr(), ld, x_scale.data_ptr(), tiles.data_ptr(), scale.data_ptr(),
             None if bias is None else bias.data_ptr(), act,
             None if residual is None else residual.data_ptr(), ld_residual, out.data_ptr(),
-            _DT[out.dtype], ld_out, rows, N, K, None if ws is None else ws.data_ptr(), nbytes,
-            torch._C._cuda_getCurrentRawStream(dev))
+            _DT[out.dtype], ld_out, rows, N, K, torch._C._cuda_getCurrentRawStream(dev))
         if status:
             _lib.check(status)
     return out

@@ -60,11 +60,14 @@ def tiles(index, q):
     return out.reshape(-1)
 
 
-def linear8(x, x_scale, index, q, scale, bias, activation, residual, dtype):
-    """(outputs in 64 bits, how far fp32 steps may be off) on the host."""
+def linear8(x, x_scale, index, q, scale, bias, activation, residual, dtype, dev="cpu"):
+    """(outputs in 64 bits, how far fp32 steps may be off) on the host; the
+    products on `dev`."""
     N, K = index.shape
     w = np.take_along_axis(q, index.reshape(N, K // 128, 128).astype(np.int64), 2).reshape(N, K)
-    sums = x.astype(np.float64) @ w.astype(np.float64).T     # whole numbers under 2^31: exact
+    # whole numbers under 2^31: exact in 64 bits, in any order
+    sums = torch.matmul(torch.from_numpy(x).to(dev).double(),
+                        torch.from_numpy(w).to(dev).double().T.contiguous()).cpu().numpy()
     v = sums * x_scale.astype(np.float64)[:, None] * scale.astype(np.float64)
     h = 2.0 ** -24                                           # half a step of fp32
     # the sum as fp32, the scales' product, their product
@@ -80,7 +83,7 @@ def linear8(x, x_scale, index, q, scale, bias, activation, residual, dtype):
     if activation == "silu":
         v, off = silu(v, off)
     elif activation == "gelu":
-        s = np.array([0.5 * z * math.erfc(-z / math.sqrt(2)) for z in v.ravel()]).reshape(v.shape)
+        s = 0.5 * v * torch.special.erfc(torch.from_numpy(-v / math.sqrt(2))).numpy()
         # |gelu'| <= 1.13; erfc within 16 steps, its argument's two roundings times
         # its condition (under 2 + v^2)
         v, off = s, 1.13 * off + np.abs(s) * (16 + 2 * (2 + v * v) + 2) * 2 * h

@@ -61,7 +61,7 @@ def check(dev, M, N, K, dtype, bias=False, activation=None, residual=False, seed
     b = (rng.standard_normal(N) * 0.3).astype(np.float32) if bias else None
     r = torch.from_numpy(rng.standard_normal((M, out)).astype(np.float32)).to(DT[dtype]) if residual else None
     want, off = ref.linear8(x, xs, index, q, scale, b, activation,
-                            None if r is None else r.float().numpy(), DT[dtype])
+                            None if r is None else r.float().numpy(), DT[dtype], dev)
     rows8 = ops.Rows8(torch.from_numpy(x).to(dev), torch.from_numpy(xs).to(dev))
     kw = dict(bias=None if b is None else torch.from_numpy(b).to(dev), activation=activation,
               residual=None if r is None else r.to(dev), out_dtype=DT[dtype])
@@ -95,6 +95,28 @@ def test_layers(dev, M, N, K):
 def test_epilogues(dev, activation, residual, bias, dtype):
     for M, N, K in ((1, 34, 256), (20, 70, 128), (150, 258, 384), (300, 518, 256)):
         check(dev, M, N, K, dtype, bias, activation, residual, seed=M)
+
+
+# (rows, outputs, K) where each form of the product is the fastest, with whole and
+# uneven shares of K, and rows and outputs that end inside its tiles
+FORMS = [(2, 11, 256), (1, 14, 896), (1, 4110, 128), (2, 4099, 256), (1, 4104, 1152),          # rows
+         (1, 12291, 384), (65, 8363, 256), (65, 8261, 640), (17, 8206, 1408),                  # 64 x 32
+         (1, 8199, 128), (33, 8474, 384), (33, 12344, 896),                                    # 64 x 64
+         (65, 10907, 256), (65, 10977, 1152),                                                  # 128 x 64
+         (65, 8198, 128), (129, 10935, 256), (129, 11078, 640),
+         (1024, 2560, 2560), (385, 14049, 1152),                                               # 128 x 128
+         (518, 14693, 128), (517, 14490, 256), (516, 14875, 384)]                              # 256 x 256
+
+
+@pytest.mark.parametrize("M,N,K", FORMS)
+def test_forms(dev, M, N, K):
+    w = layer(N, K, 5, dev)
+    check(dev, M, N, K, "fp32", seed=5, w=w)
+    check(dev, M, N, K, "bf16", True, "silu", True, seed=5, w=w)
+    check(dev, M, N, K, "fp32", True, "gelu", seed=5, w=w)
+    if N % 2 == 0:
+        check(dev, M, N, K, "fp32", True, "swiglu", True, seed=5, w=w)
+        check(dev, M, N, K, "bf16", False, "swiglu", seed=5, w=w)
 
 
 def test_largest_sums(dev):

@@ -69,7 +69,7 @@ LAYOUT = dict(packed=P, codebook=P, N=40, K=256, tiles=P, scale=P, stream=None)
 
 @pytest.mark.parametrize("kw,status", [
     (dict(N=-1), EINVAL), (dict(K=0), EINVAL), (dict(K=200), EINVAL), (dict(K=(1 << 17) + 128), EUNSUP),
-    (dict(N=1 << 20, K=1 << 16), EUNSUP), (dict(packed=None), EINVAL), (dict(codebook=None), EINVAL),
+    (dict(N=1 << 20, K=1 << 16), EUNSUP), (dict(N=(1 << 24) + 1, K=128), EUNSUP), (dict(packed=None), EINVAL), (dict(codebook=None), EINVAL),
     (dict(tiles=None), EINVAL), (dict(scale=None), EINVAL), (dict(tiles=P + 8), EALIGN),
     (dict(packed=P + 2), EALIGN), (dict(scale=P + 1), EALIGN), (dict(codebook=P + 2), EALIGN),
 ])
@@ -81,13 +81,12 @@ def test_sizes():
     lib = _lib.load()
     assert lib.nb_linear8_tiles_bytes(17, 256) == 2 * 2 * 896
     assert lib.nb_linear8_tiles_bytes(16, 128) == 896 and lib.nb_linear8_tiles_bytes(16, 100) == 0
-    assert lib.nb_linear8_ws_bytes(0, 16, 128) == 0 and lib.nb_linear8_ws_bytes(4, 16, 100) == 0
     assert lib.nb_sample_ws_bytes(0, 100) == 0
 
 
 LINEAR = dict(x=P, ld_x=256, x_scale=P, tiles=P, scale=P, bias=P, activation=0,
               residual=P + (1 << 20), ld_residual=40, y=P + (2 << 20), y_dtype=F32, ld_y=40, M=3, N=40,
-              K=256, ws=P, ws_bytes=1 << 40, stream=None)
+              K=256, stream=None)
 
 
 @pytest.mark.parametrize("kw,status", [
@@ -99,7 +98,8 @@ LINEAR = dict(x=P, ld_x=256, x_scale=P, tiles=P, scale=P, bias=P, activation=0,
     (dict(ld_x=128), EINVAL), (dict(x=P + 8), EALIGN), (dict(tiles=P + 8), EALIGN),
     (dict(bias=P + 2), EALIGN), (dict(x_scale=P + 2), EALIGN), (dict(ld_y=39), EINVAL),
     (dict(y_dtype=_lib.NB_U8), EINVAL), (dict(ld_residual=39), EINVAL), (dict(y=P + (1 << 20) + 4), EINVAL),
-    (dict(y=P + (1 << 20), ld_y=48), EINVAL), (dict(y=P + 2), EALIGN), (dict(ws=P + 8), EALIGN),
+    (dict(y=P + (1 << 20), ld_y=48), EINVAL), (dict(y=P + 2), EALIGN), (dict(ld_x=(1 << 22) + 16), EUNSUP),
+    (dict(M=1 << 20, N=1 << 17), EUNSUP), (dict(N=(1 << 24) + 1), EUNSUP),
 ])
 def test_linear_refuses(kw, status):
     assert call("nb_linear8", LINEAR, kw) == status and _lib.last_error()
