@@ -11,6 +11,20 @@
 // Sums decide which token it is, so they are exact: weights are whole numbers of
 // 2^-S (S = 45 for V up to 2^17), exp in 64 bits rounded once, and every sum of
 // them is a 64-bit integer, the same in any order.
+//
+// A row is cut into slices, one workgroup each:
+//   1. sample_max_kernel     each slice's first token of the order
+//   2. sample_bins_kernel    each slice's weights, summed and counted in bins of an
+//                            eighth of an octave of w (257: the last holds all
+//                            under 2^-32)
+//   3. sample_list_kernel    the row's bins say where the rules cut; the tokens of
+//                            the bins that they cut through are listed
+//   4. sample_finish_kernel  one workgroup a row: the listed tokens, sorted, give
+//                            the cuts; bins and list each slice's sum of kept
+//                            weights, u the slice, the slice read again the token
+// (without rules 1, 2 without bins, 4).  A row with more than kMostListed tokens in
+// the cut bins (equal logits, mostly) is worked out by its last workgroup alone:
+// radix selection over the row.
 #include <math.h>
 
 #include <algorithm>
@@ -22,15 +36,32 @@
 namespace nb {
 namespace {
 
+typedef __attribute__((ext_vector_type(4), aligned(4))) float f4_any;
+typedef __attribute__((ext_vector_type(2), aligned(2))) uint32_t u2_any;
+
+constexpr int kBins = 256;          // of an eighth of an octave; one more below them
+constexpr int kListed = 2048;       // listed tokens of a slice
+constexpr int kMostListed = 4096;   // and of a row (a power of two)
+constexpr int kSliceThreads = 512;
+constexpr int kMostSlices = 128;
+
 struct SampleArgs {
     const void* logits;
     int64_t ld;
-    int dtype, V, shift;   // shift: S
+    int V, shift;          // shift: S
+    int slices, length;    // of a row; tokens of a slice
     const float *u, *temperature;
     const int32_t* top_k;
     const float *top_p, *min_p;
     int32_t* tokens;
     float* logprobs;
+    // workspace, for each row and slice
+    uint64_t* first;       // the slice's first token of the order (place_of)
+    uint64_t* sums;        // [kBins + 1] with rules, else one
+    uint32_t* counts;      // [kBins + 1]
+    uint32_t* listed;      // how many are listed (more than kListed: not all are)
+    uint64_t* list;        // [kListed] places
+    __device__ __forceinline__ bool rules() const { return top_k || top_p || min_p; }
 };
 
 // Larger for larger logits; 0 for -inf and NaN.
@@ -43,11 +74,64 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
+// A token's place in the order (larger: earlier); 0 for -inf and NaN.
+__device__ __forceinline__ uint64_t place_of(uint32_t key, int v) {
+    return key ? (uint64_t)key << 32 | (0xffffffffu - (uint32_t)v) : 0;
+}
+__device__ __forceinline__ uint32_t key_of_place(uint64_t place) { return (uint32_t)(place >> 32); }
+__device__ __forceinline__ int token_of_place(uint64_t place) {
+    return (int)(0xffffffffu - (uint32_t)place);
+}
+
+template <int kDtype>
 __device__ __forceinline__ uint32_t key_at(const SampleArgs& a, int64_t b, int v) {
     const int64_t at = b * a.ld + v;
-    return key_of(a.dtype == NB_F32 ? static_cast<const float*>(a.logits)[at]
-                                    : bf16_to_f32(static_cast<const bf16_bits*>(a.logits)[at]));
+    return key_of(kDtype == NB_F32 ? static_cast<const float*>(a.logits)[at]
+                                   : bf16_to_f32(static_cast<const bf16_bits*>(a.logits)[at]));
 }
+
+// f(token, key) for the tokens lo .. hi - 1 of row b, by the kThreads threads of
+// a workgroup: groups of four, kBatch of them asked for at once.
+template <int kDtype, int kThreads, typename F>
+__device__ __forceinline__ void for_tokens(const SampleArgs& a, int64_t b, int lo, int hi, F f) {
+    constexpr int kBatch = 4;
+    const char* row = static_cast<const char*>(a.logits) + b * a.ld * (kDtype == NB_F32 ? 4 : 2);
+    for (int v0 = lo + 4 * (int)threadIdx.x; v0 < hi; v0 += 4 * kThreads * kBatch) {
+        float x[kBatch][4];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const int v = v0 + j * 4 * kThreads;
+            if (v + 3 < hi) {
+                if constexpr (kDtype == NB_F32) {
+                    const f4_any w = *reinterpret_cast<const f4_any*>(row + (int64_t)v * 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[j][e] = w[e];
+                } else {
+                    const u2_any w = *reinterpret_cast<const u2_any*>(row + (int64_t)v * 2);
+                    x[j][0] = __uint_as_float(w[0] << 16), x[j][1] = __uint_as_float(w[0] & 0xffff0000u);
+                    x[j][2] = __uint_as_float(w[1] << 16), x[j][3] = __uint_as_float(w[1] & 0xffff0000u);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[j][e] = -INFINITY;
+                    if (v + e < hi) {
+                        x[j][e] = kDtype == NB_F32 ? reinterpret_cast<const float*>(row)[v + e]
+                                                   : bf16_to_f32(reinterpret_cast<const bf16_bits*>(row)[v + e]);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f(v0 + j * 4 * kThreads + e, key_of(x[j][e]));
+        }
+    }
+}
+
+// The bin of a weight by its log2.
+__device__ __forceinline__ int bin_of(double z) { return z > -kBins / 8 ? (int)(z * -8.0) : kBins; }
 
 constexpr int kFractions = 32;   // entries of 2^(i / 32)
 
@@ -63,8 +147,9 @@ struct Weights {
     // 2^(n + f): the table's entry by f's upper bits, a polynomial of the rest
     // (|r| <= 1/64: its next term is 2e-15)
     __device__ __forceinline__ uint64_t of(uint32_t key) const {
-        if (key == 0) return 0;
-        const double z = log2_of(key);
+        return key ? of_log2(log2_of(key)) : 0;
+    }
+    __device__ __forceinline__ uint64_t of_log2(double z) const {
         constexpr double kMagic = 6755399441055744.0;   // 1.5 * 2^52: rounds to a whole number
         const double y = z * kFractions + kMagic;
         const int n = __double2loint(y);
@@ -80,23 +165,259 @@ struct Weights {
     }
 };
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64, kBins = 2048;
-
-struct Shared {
-    double table[kFractions];
-    uint64_t bins[kBins];
-    uint64_t part[kWaves], ties[kWaves];
-    uint64_t found[3];
-};
-
-__device__ __forceinline__ uint64_t lesser(uint64_t x, uint64_t y) { return x < y ? x : y; }
+__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint64_t o = __shfl_xor((unsigned long long)v, d);
+        v = o > v ? o : v;
+    }
+    return v;
+}
 __device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) v += __shfl_xor((unsigned long long)v, d);
     return v;
 }
-// The sum over the workgroup, in all threads.
-__device__ uint64_t block_sum(Shared& s, uint64_t v) {
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v, int lane) {   // sum of lanes 0 .. lane
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint64_t o = __shfl_up((unsigned long long)v, d);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+__device__ __forceinline__ uint64_t lesser(uint64_t x, uint64_t y) { return x < y ? x : y; }
+
+// A row's rules.  (Weights of a greedy row are those of T = 1: nothing uses them.)
+struct Rules {
+    bool greedy;       // the first of the order: T is not over 0, or one token is kept
+    int64_t k;         // 0: all
+    float p;           // 1: all
+    uint64_t least;    // of a kept weight
+    double least_high, least_low;   // log2s around it
+    uint64_t first;    // of the row's order; 0: nothing is left
+    Weights w;
+    __device__ __forceinline__ Rules(const SampleArgs& a, int64_t b, const double* table) {
+        const float t = a.temperature ? as_constant(a.temperature)[b] : 1.f;
+        k = a.top_k ? as_constant(a.top_k)[b] : 0;
+        if (k <= 0 || k >= a.V) k = 0;
+        greedy = !(t > 0.f) || k == 1;
+        p = a.top_p ? as_constant(a.top_p)[b] : 1.f;
+        if (!(p < 1.f)) p = 1.f;
+        const float mp = a.min_p ? as_constant(a.min_p)[b] : 0.f;
+        const double m = mp > 0.f ? fmin((double)mp, 1.0) : 0.0;
+        least = (uint64_t)ceil(m * (double)(1ull << a.shift));
+        if (least <= 1) least = 0;   // (weights of 0 are never drawn)
+        if (least) {
+            // around it: a unit of the weights' rounding, and of the logarithms'
+            const double unit = 1e-9 + 2.0 / (double)least, z = log2(m);
+            least_high = fmin(z + unit, 0.0), least_low = z - unit;
+        }
+        const int lane = threadIdx.x & 63;
+        static_assert(kMostSlices <= 128, "two slices a lane");
+        const uint64_t o0 = lane < a.slices ? a.first[b * a.slices + lane] : 0;
+        const uint64_t o1 = lane + 64 < a.slices ? a.first[b * a.slices + lane + 64] : 0;
+        first = wave_max(o0 > o1 ? o0 : o1);
+        w.most = (double)logit_of(key_of_place(first));
+        w.turn = 1.4426950408889634 / (t > 0.f ? (double)t : 1.0);
+        w.table = table;
+        w.shift = a.shift;
+    }
+};
+__device__ __forceinline__ void make_table(double* table) {
+    if (threadIdx.x < kFractions) table[threadIdx.x] = exp2((double)threadIdx.x / kFractions);
+}
+
+// ---------------------------------------------------------------------------
+// slices
+// ---------------------------------------------------------------------------
+template <int kDtype>
+__global__ __launch_bounds__(kSliceThreads) void sample_max_kernel(SampleArgs a) {
+    __shared__ uint64_t part[kSliceThreads / 64];
+    const int64_t b = blockIdx.y;
+    const int lo = blockIdx.x * a.length, hi = min(lo + a.length, a.V), tid = threadIdx.x;
+    uint64_t first = 0;
+    for_tokens<kDtype, kSliceThreads>(a, b, lo, hi, [&](int v, uint32_t key) {
+        const uint64_t place = place_of(key, v);
+        first = place > first ? place : first;
+    });
+    first = wave_max(first);
+    if ((tid & 63) == 0) part[tid >> 6] = first;
+    __syncthreads();
+    if (tid) return;
+    for (int i = 1; i < kSliceThreads / 64; ++i) first = part[i] > first ? part[i] : first;
+    a.first[b * a.slices + blockIdx.x] = first;
+}
+
+template <int kDtype, bool kRules>
+__global__ __launch_bounds__(kSliceThreads) void sample_bins_kernel(SampleArgs a) {
+    __shared__ double table[kFractions];
+    __shared__ unsigned long long sums[kBins + 1];
+    __shared__ uint32_t counts[kBins + 1];
+    const int64_t b = blockIdx.y, slice = b * a.slices + blockIdx.x;
+    const int lo = blockIdx.x * a.length, hi = min(lo + a.length, a.V), tid = threadIdx.x;
+    make_table(table);
+    const Rules r(a, b, table);
+    if (r.greedy || r.first == 0) return;   // (nothing reads the row's bins)
+    if (kRules) {
+        for (int i = tid; i <= kBins; i += kSliceThreads) sums[i] = 0, counts[i] = 0;
+    }
+    __syncthreads();
+    uint64_t sum = 0;       // without bins of all, else of the last bin
+    uint32_t count = 0;
+    for_tokens<kDtype, kSliceThreads>(a, b, lo, hi, [&](int, uint32_t key) {
+        if (!key) return;
+        const double z = r.w.log2_of(key);
+        const uint64_t w = r.w.of_log2(z);
+        const int bin = kRules ? bin_of(z) : kBins;
+        if (bin < kBins) {
+            atomicAdd(&sums[bin], (unsigned long long)w);
+            atomicAdd(&counts[bin], 1u);
+        } else {
+            sum += w, ++count;
+        }
+    });
+    if (kRules) {
+        sum = wave_sum(sum), count = (uint32_t)wave_sum(count);
+        if ((tid & 63) == 0) atomicAdd(&sums[kBins], (unsigned long long)sum), atomicAdd(&counts[kBins], count);
+        __syncthreads();
+        for (int i = tid; i <= kBins; i += kSliceThreads) {
+            a.sums[slice * (kBins + 1) + i] = sums[i];
+            a.counts[slice * (kBins + 1) + i] = counts[i];
+        }
+    } else {
+        sum = wave_sum(sum);
+        if ((tid & 63) == 0) sums[tid >> 6] = sum;
+        __syncthreads();
+        if (tid) return;
+        for (int i = 1; i < kSliceThreads / 64; ++i) sum += sums[i];
+        a.sums[slice] = sum;
+    }
+}
+
+// Where the rules cut a row, from its bins.
+struct Cuts {
+    int k;               // the bin that top_k ends in; past the last: none
+    int p_low, p_high;   // those that top_p may end in (what top_k keeps of its bin
+                         // is not known yet)
+    int m_low, m_high;   // those around min_p
+    uint64_t above_k, sum_k, above_p;   // tokens and weights over bin k, weights over p_low
+    __device__ __forceinline__ bool listed(int bin) const {
+        return bin == k || (bin >= p_low && bin <= p_high) || (bin >= m_low && bin <= m_high);
+    }
+    // all tokens of the bins before it are kept, of those after it only listed ones
+    __device__ __forceinline__ int sure() const { return min(k, min(p_low, m_low)); }
+};
+// The least sum of a beginning that makes up p of `total`: at least one unit.
+__device__ __forceinline__ uint64_t share_of(float p, uint64_t total) {
+    if (!(p > 0.f)) return 1;
+    const double s = fmax(ceil((double)p * (double)total), 1.0);
+    return s < (double)total ? (uint64_t)s : total;
+}
+struct CutShared {
+    uint64_t sum[kBins + 2], above[kBins + 2];   // of a bin; of those before it
+    uint32_t count[kBins + 2], before[kBins + 2];
+    int found[4];
+};
+// By all threads of a workgroup of over kBins + 1.
+__device__ Cuts find_cuts(const SampleArgs& a, int64_t b, const Rules& r, CutShared& s) {
+    const int tid = threadIdx.x;
+    constexpr int kAll = kBins + 1, kNone = kBins + 1;
+    if (tid < kAll) {
+        uint64_t sum = 0;
+        uint32_t count = 0;
+#pragma unroll 8
+        for (int i = 0; i < a.slices; ++i) {
+            sum += a.sums[(b * a.slices + i) * kAll + tid];
+            count += a.counts[(b * a.slices + i) * kAll + tid];
+        }
+        s.sum[tid] = sum, s.count[tid] = count;
+    }
+    if (tid < 4) s.found[tid] = kNone;
+    __syncthreads();
+    if (tid < 64) {   // a wave: five bins a lane
+        constexpr int kEach = (kAll + 63) / 64;
+        uint64_t sum = 0, count = 0;
+        for (int i = tid * kEach; i < min((tid + 1) * kEach, kAll); ++i) sum += s.sum[i], count += s.count[i];
+        uint64_t above = wave_scan(sum, tid) - sum, before = wave_scan(count, tid) - count;
+        for (int i = tid * kEach; i < min((tid + 1) * kEach, kAll); ++i) {
+            s.above[i] = above, s.before[i] = (uint32_t)before;
+            above += s.sum[i], before += s.count[i];
+        }
+        if (tid == 63) s.above[kNone] = above, s.sum[kNone] = 0, s.before[kNone] = (uint32_t)before;
+    }
+    __syncthreads();
+    if (r.k && tid < kAll && s.before[tid] < r.k && s.before[tid] + (uint64_t)s.count[tid] >= (uint64_t)r.k) {
+        s.found[0] = tid;
+    }
+    __syncthreads();
+    Cuts c;
+    c.k = s.found[0];
+    c.above_k = s.before[c.k], c.sum_k = s.above[c.k];
+    if (r.p < 1.f && tid < kAll) {
+        const uint64_t low = share_of(r.p, max(s.above[c.k], (uint64_t)1));
+        const uint64_t high = share_of(r.p, s.above[c.k] + s.sum[c.k]);
+        if (s.above[tid] < low && s.above[tid] + s.sum[tid] >= low) s.found[1] = tid;
+        if (s.above[tid] < high && s.above[tid] + s.sum[tid] >= high) s.found[2] = tid;
+    }
+    __syncthreads();
+    c.p_low = s.found[1], c.p_high = s.found[2];
+    c.above_p = s.above[c.p_low];
+    c.m_low = c.m_high = kNone;
+    if (r.least) {
+        c.m_low = bin_of(r.least_high);
+        c.m_high = bin_of(r.least_low);
+    }
+    return c;
+}
+
+template <int kDtype>
+__global__ __launch_bounds__(kSliceThreads) void sample_list_kernel(SampleArgs a) {
+    __shared__ CutShared shared;
+    __shared__ uint32_t count;
+    const int64_t b = blockIdx.y, slice = b * a.slices + blockIdx.x;
+    const int lo = blockIdx.x * a.length, hi = min(lo + a.length, a.V);
+    const Rules r(a, b, nullptr);   // (no weights here, only their bins)
+    if (r.greedy || r.first == 0) return;
+    if (threadIdx.x == 0) count = 0;
+    const Cuts c = find_cuts(a, b, r, shared);
+    for_tokens<kDtype, kSliceThreads>(a, b, lo, hi, [&](int v, uint32_t key) {
+        if (!key || !c.listed(bin_of(r.w.log2_of(key)))) return;
+        const uint32_t at = atomicAdd(&count, 1u);
+        if (at < kListed) a.list[slice * kListed + at] = place_of(key, v);
+    });
+    __syncthreads();
+    if (threadIdx.x == 0) a.listed[slice] = count;
+}
+
+// ---------------------------------------------------------------------------
+// rows
+// ---------------------------------------------------------------------------
+constexpr int kThreads = 1024, kWaves = kThreads / 64, kDigits = 2048;
+
+struct Shared {
+    double table[kFractions];
+    union {
+        uint64_t digits[kDigits];        // radix selection
+        uint64_t list[kMostListed];      // the listed tokens
+    };
+    CutShared cuts;
+    uint64_t part[kWaves], ties[kWaves];
+    uint64_t found[2];
+};
+
+// What is kept: tokens up to `last` in the order, of weights of `least` or more.
+// (0: all of the order.)
+struct Kept {
+    uint64_t last, least;
+    __device__ __forceinline__ uint64_t weight(const Weights& w, uint32_t key, int v) const {
+        if (!key || place_of(key, v) < last) return 0;
+        const uint64_t n = w.of(key);
+        return n >= least ? n : 0;
+    }
+};
+
+__device__ uint64_t block_sum(Shared& s, uint64_t v) {   // in all threads
     v = wave_sum(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) s.part[threadIdx.x >> 6] = v;
@@ -113,18 +434,13 @@ struct Crossing {
     uint64_t above;
 };
 __device__ Crossing cross(Shared& s, uint64_t bound) {
-    constexpr int kEach = kBins / kThreads;
+    constexpr int kEach = kDigits / kThreads;
     const int tid = threadIdx.x, lane = tid & 63;
     // thread t takes the bins from the t-th largest pair on
     uint64_t mine = 0;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) mine += s.bins[kBins - 1 - (tid * kEach + i)];
-    uint64_t upto = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = __shfl_up((unsigned long long)upto, d);
-        if (lane >= d) upto += o;
-    }
+    for (int i = 0; i < kEach; ++i) mine += s.digits[kDigits - 1 - (tid * kEach + i)];
+    const uint64_t upto = wave_scan(mine, lane);
     __syncthreads();
     if (lane == 63) s.part[tid >> 6] = upto;
     if (tid == 0) s.found[0] = 0, s.found[1] = 0;
@@ -133,8 +449,8 @@ __device__ Crossing cross(Shared& s, uint64_t bound) {
     for (int i = 0; i < (tid >> 6); ++i) above += s.part[i];
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-        const int bin = kBins - 1 - (tid * kEach + i);
-        const uint64_t n = s.bins[bin];
+        const int bin = kDigits - 1 - (tid * kEach + i);
+        const uint64_t n = s.digits[bin];
         if (above < bound && above + n >= bound) {
             s.found[0] = (uint64_t)bin, s.found[1] = above;
         }
@@ -146,7 +462,7 @@ __device__ Crossing cross(Shared& s, uint64_t bound) {
 
 // The key at which the order's sum of `value(key)` over keys >= least first
 // reaches `bound` (> 0, at most the sum of all), and the sum above that key.
-template <typename Value>
+template <int kDtype, typename Value>
 __device__ uint64_t select(const SampleArgs& a, int64_t b, Shared& s, uint32_t least, uint64_t bound,
                            Value value, uint32_t& at) {
     uint64_t above = 0;
@@ -154,15 +470,14 @@ __device__ uint64_t select(const SampleArgs& a, int64_t b, Shared& s, uint32_t l
     for (int shift = 21; shift >= -1; shift -= 11) {   // 11, 11 and 10 bits
         const int low = max(shift, 0), bits = shift < 0 ? 10 : 11;
         __syncthreads();
-        for (int i = threadIdx.x; i < kBins; i += kThreads) s.bins[i] = 0;
+        for (int i = threadIdx.x; i < kDigits; i += kThreads) s.digits[i] = 0;
         __syncthreads();
-        for (int v = threadIdx.x; v < a.V; v += kThreads) {
-            const uint32_t key = key_at(a, b, v);
+        for_tokens<kDtype, kThreads>(a, b, 0, a.V, [&](int, uint32_t key) {
             if (key && key >= least && (key & mask) == prefix) {
-                atomicAdd((unsigned long long*)&s.bins[key >> low & ((1u << bits) - 1)],
+                atomicAdd((unsigned long long*)&s.digits[key >> low & ((1u << bits) - 1)],
                           (unsigned long long)value(key));
             }
-        }
+        });
         __syncthreads();
         const Crossing c = cross(s, bound - above);
         above += c.above;
@@ -173,156 +488,309 @@ __device__ uint64_t select(const SampleArgs& a, int64_t b, Shared& s, uint32_t l
     return above;
 }
 
-// One row.
-__global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
-    __shared__ Shared s;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t b = blockIdx.x;
-    const float t = a.temperature ? a.temperature[b] : 1.f;
-    const bool greedy = !(t > 0.f);
-    if (tid < kFractions) s.table[tid] = exp2((double)tid / kFractions);
-    // the maximum
-    uint32_t top = 0;
-    for (int v = tid; v < a.V; v += kThreads) top = max(top, key_at(a, b, v));
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-    if (lane == 0) s.part[wave] = top;
-    __syncthreads();
-    for (int i = 0; i < kWaves; ++i) top = max(top, (uint32_t)s.part[i]);
-    if (top == 0) {   // nothing is left
-        if (tid == 0) {
-            a.tokens[b] = -1;
-            if (a.logprobs) a.logprobs[b] = -INFINITY;
-        }
-        return;
-    }
-    Weights w;
-    w.most = (double)logit_of(top);
-    w.turn = 1.4426950408889634 / (greedy ? 1.0 : (double)t);
-    w.table = s.table;
-    w.shift = a.shift;
+// The last kept token of the row (its place), of what top_k and top_p keep, by
+// selection over the whole row: any number of tokens in a bin.
+template <int kDtype>
+__device__ uint64_t last_of_row(const SampleArgs& a, int64_t b, const Rules& r, Shared& s) {
     // kept: keys over `edge`, and the first `edge_ties` of those that equal it
     uint32_t edge = 1;
     uint64_t edge_ties = ~0ull;
-    const int64_t k = greedy ? 1 : a.top_k ? a.top_k[b] : 0;
-    if (k > 0 && k < a.V) {
+    if (r.k) {
         uint64_t some = 0;
-        for (int v = tid; v < a.V; v += kThreads) some += key_at(a, b, v) != 0;
-        some = block_sum(s, some);
-        if ((uint64_t)k < some) {
-            const uint64_t above = select(a, b, s, 1, (uint64_t)k, [](uint32_t) { return 1ull; }, edge);
-            edge_ties = (uint64_t)k - above;
+        for_tokens<kDtype, kThreads>(a, b, 0, a.V, [&](int, uint32_t key) { some += key != 0; });
+        if ((uint64_t)r.k < block_sum(s, some)) {
+            edge_ties = (uint64_t)r.k -
+                        select<kDtype>(a, b, s, 1, (uint64_t)r.k, [](uint32_t) { return 1ull; }, edge);
         }
     }
-    const float p = a.top_p ? a.top_p[b] : 1.f;
-    if (p < 1.f) {
-        uint64_t total = 0, ties = 0;
-        for (int v = tid; v < a.V; v += kThreads) {
-            const uint32_t key = key_at(a, b, v);
-            if (key > edge) total += w.of(key);
+    uint64_t ties = 0;
+    if (r.p < 1.f) {
+        uint64_t total = 0;
+        for_tokens<kDtype, kThreads>(a, b, 0, a.V, [&](int, uint32_t key) {
+            if (key > edge) total += r.w.of(key);
             ties += key == edge;
-        }
+        });
         total = block_sum(s, total);
         ties = block_sum(s, ties);
-        total += lesser(ties, edge_ties) * w.of(edge);
-        // (at least the first of the order)
-        const uint64_t bound = p > 0.f ? lesser((uint64_t)fmax(ceil((double)p * (double)total), 1.0), total) : 1;
+        total += lesser(ties, edge_ties) * r.w.of(edge);
+        const uint64_t bound = share_of(r.p, total);
         uint32_t at = 0;
-        const uint64_t above = select(a, b, s, edge, bound, [&](uint32_t key) { return w.of(key); }, at);
-        const uint64_t each = w.of(at);   // (not 0: the sum reached the bound with it)
+        const uint64_t above = select<kDtype>(a, b, s, edge, bound, [&](uint32_t key) { return r.w.of(key); }, at);
+        const uint64_t each = r.w.of(at);   // (not 0: the sum reached the bound with it)
         const uint64_t need = (bound - above + each - 1) / each;
         edge_ties = at == edge ? lesser(edge_ties, need) : need;
         edge = at;
     }
-    const float mp = a.min_p ? a.min_p[b] : 0.f;
-    const uint64_t one = 1ull << a.shift;
-    const uint64_t least = mp > 0.f ? (uint64_t)ceil(fmin((double)mp, 1.0) * (double)one) : 0;
-    const uint64_t edge_weight = w.of(edge);
-    // the sum of kept weights by index: a range is split over the waves, the part
-    // with the token split again
-    int lo = 0, hi = a.V;
-    uint64_t ties_before = 0, rest = 0, total = 0;
-    bool first = true;
-    while (hi - lo > 64 || first) {
-        const int each = max(((hi - lo + kWaves - 1) / kWaves + 63) / 64 * 64, 64);
+    if (edge == 1) return 0;
+    // the token of the last tie: waves count those of their part of the row
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int each = ((a.V + kWaves - 1) / kWaves + 63) / 64 * 64;
+    const int begin = min(wave * each, a.V), end = min(begin + each, a.V);
+    ties = 0;
+    for (int v = begin + lane; v < end; v += 64) ties += key_at<kDtype>(a, b, v) == edge;
+    ties = wave_sum(ties);
+    __syncthreads();
+    if (lane == 0) s.ties[wave] = ties;
+    if (tid == 0) s.found[0] = 0xffffffffu;   // (all ties are kept)
+    __syncthreads();
+    uint64_t before = 0;
+    for (int i = 0; i < wave; ++i) before += s.ties[i];
+    if (before < edge_ties && before + ties >= edge_ties) {   // one wave
+        for (int v0 = begin; v0 < end; v0 += 64) {
+            const int v = v0 + lane;
+            const uint64_t tied = __ballot(v < end && key_at<kDtype>(a, b, min(v, end - 1)) == edge);
+            const uint64_t rank = before + __popcll(tied & ((1ull << lane) - 1));
+            if ((tied >> lane & 1) && rank + 1 == edge_ties) s.found[0] = (uint64_t)v;
+            before += __popcll(tied);
+            if (before >= edge_ties) break;
+        }
+    }
+    __syncthreads();
+    const uint64_t v = s.found[0];
+    return v == 0xffffffffu ? (uint64_t)edge << 32 : place_of(edge, (int)v);
+}
+
+// The same by the listed tokens; their kept weights are added to s.digits' place
+// of their slices' sums, `slice_sums`.
+__device__ uint64_t last_of_list(const SampleArgs& a, const Rules& r, const Cuts& c, Shared& s, int n,
+                                 unsigned long long* slice_sums) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int size = 64;
+    while (size < n) size *= 2;
+    for (int i = n + tid; i < size; i += kThreads) s.list[i] = 0;
+    // sorted into the order, largest place first
+    for (int k = 2; k <= size; k *= 2) {
+        for (int j = k / 2; j > 0; j /= 2) {
+            __syncthreads();
+            for (int i = tid; i < size / 2; i += kThreads) {
+                const int x = (i & ~(j - 1)) << 1 | (i & (j - 1)), y = x + j;   // (j: a power of two)
+                const uint64_t p = s.list[x], q = s.list[y];
+                if ((p < q) == ((x & k) == 0)) s.list[x] = q, s.list[y] = p;
+            }
+        }
+    }
+    __syncthreads();
+    // thread t has the tokens 4 t .. 4 t + 3
+    constexpr int kEach = kMostListed / kThreads;
+    uint64_t place[kEach], weight[kEach];
+    int bin[kEach];
+    uint64_t first_k = 0, in_p = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const int i = tid * kEach + e;
+        place[e] = i < n ? s.list[i] : 0;
+        const uint32_t key = key_of_place(place[e]);
+        const double z = key ? r.w.log2_of(key) : 0.0;
+        weight[e] = key ? r.w.of_log2(z) : 0;
+        bin[e] = key ? bin_of(z) : kBins + 2;
+        first_k += bin[e] < c.k;   // listed tokens before bin k
+        if (bin[e] >= c.p_low && bin[e] <= c.p_high) in_p += weight[e];
+    }
+    uint64_t kept_k = 0;
+    if (c.k <= kBins) {
+        first_k = block_sum(s, first_k);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const uint64_t rank = c.above_k + (uint64_t)(tid * kEach + e) - first_k;
+            if (bin[e] == c.k && rank < (uint64_t)r.k) kept_k += weight[e];
+        }
+    }
+    kept_k = block_sum(s, kept_k);
+    const uint64_t bound = r.p < 1.f ? share_of(r.p, c.sum_k + kept_k) : 0;
+    // weights of the order before a token, over p_low's bin
+    uint64_t upto = wave_scan(in_p, lane);
+    __syncthreads();
+    if (lane == 63) s.part[wave] = upto;
+    __syncthreads();
+    uint64_t before = c.above_p + upto - in_p;
+    for (int i = 0; i < wave; ++i) before += s.part[i];
+    uint64_t last = 0;    // the largest number of a token that top_k and top_p keep
+    bool kept[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const uint64_t i = (uint64_t)(tid * kEach + e), rank = c.above_k + i - first_k;
+        kept[e] = place[e] && (bin[e] < c.k || (bin[e] == c.k && rank < (uint64_t)r.k));
+        if (r.p < 1.f) {
+            const bool inside = bin[e] >= c.p_low && bin[e] <= c.p_high;
+            kept[e] = kept[e] && (bin[e] < c.p_low || (inside && before < bound));
+            if (inside) before += weight[e];
+        }
+        if (kept[e]) last = i + 1;
+        if (kept[e] && weight[e] >= r.least && bin[e] >= c.sure()) {
+            atomicAdd(&slice_sums[token_of_place(place[e]) / a.length], (unsigned long long)weight[e]);
+        }
+    }
+    if (c.k > kBins && !(r.p < 1.f)) return 0;   // (min_p alone)
+    last = wave_max(last);
+    __syncthreads();
+    if (lane == 0) s.part[wave] = last;
+    __syncthreads();
+    for (int i = 0; i < kWaves; ++i) last = s.part[i] > last ? s.part[i] : last;
+    return s.list[last - 1];
+}
+
+template <int kDtype>
+__global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
+    __shared__ Shared s;
+    __shared__ unsigned long long slice_sums[kMostSlices];
+    __shared__ int list_at[kMostSlices + 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t b = blockIdx.x, slice0 = b * a.slices;
+    make_table(s.table);
+    const Rules r(a, b, s.table);
+    if (r.first == 0 || r.greedy) {
+        if (tid == 0) {
+            a.tokens[b] = r.first ? token_of_place(r.first) : -1;
+            if (a.logprobs) a.logprobs[b] = r.first ? 0.f : -INFINITY;
+        }
+        return;
+    }
+    __syncthreads();
+    Kept kept{0, r.least};
+    bool known = true;   // slice_sums are those of kept weights
+    if (!a.rules()) {
+        if (tid < a.slices) slice_sums[tid] = a.sums[slice0 + tid];
+    } else {
+        const Cuts c = find_cuts(a, b, r, s.cuts);
+        // listed tokens: two slices a lane, their places one after the other
+        const uint32_t l0 = 2 * lane < a.slices ? a.listed[slice0 + 2 * lane] : 0;
+        const uint32_t l1 = 2 * lane + 1 < a.slices ? a.listed[slice0 + 2 * lane + 1] : 0;
+        const uint64_t upto = wave_scan((uint64_t)l0 + l1, lane);
+        const uint64_t listed = __shfl((unsigned long long)upto, 63);
+        known = __ballot(l0 > kListed || l1 > kListed) == 0 && listed <= kMostListed;
+        const int n = known ? (int)listed : 0;
+        if (known) {
+            if (wave == 0) {
+                list_at[2 * lane] = (int)(upto - l0 - l1);
+                list_at[2 * lane + 1] = (int)(upto - l1);
+                if (lane == 63) list_at[kMostSlices] = n;
+            }
+            // sums of the bins that are kept whole, a wave a slice
+            for (int i = wave; i < a.slices; i += kWaves) {
+                uint64_t sum = 0;
+                for (int bin = lane; bin < c.sure() && bin <= kBins; bin += 64) {
+                    sum += a.sums[(slice0 + i) * (kBins + 1) + bin];
+                }
+                sum = wave_sum(sum);
+                if (lane == 0) slice_sums[i] = sum;
+            }
+            __syncthreads();
+            for (int i = wave; i < a.slices; i += kWaves) {
+                const int at = list_at[i], count = list_at[i + 1] - at;
+                for (int e = lane; e < count; e += 64) s.list[at + e] = a.list[(slice0 + i) * kListed + e];
+            }
+            __syncthreads();
+            kept.last = last_of_list(a, r, c, s, n, slice_sums);
+        } else {
+            kept.last = last_of_row<kDtype>(a, b, r, s);
+        }
+    }
+    __syncthreads();
+    if (!known) {   // the slices' sums, a wave a slice
+        for (int i = wave; i < a.slices; i += kWaves) {
+            const int lo = i * a.length, hi = min(lo + a.length, a.V);
+            uint64_t sum = 0;
+            for (int v = lo + lane; v < hi; v += 64) sum += kept.weight(r.w, key_at<kDtype>(a, b, v), v);
+            sum = wave_sum(sum);
+            if (lane == 0) slice_sums[i] = sum;
+        }
+        __syncthreads();
+    }
+    // the slice that u falls in: two slices a lane, every wave by itself
+    const uint64_t s0 = 2 * lane < a.slices ? slice_sums[2 * lane] : 0;
+    const uint64_t s1 = 2 * lane + 1 < a.slices ? slice_sums[2 * lane + 1] : 0;
+    const uint64_t sums = wave_scan(s0 + s1, lane), total = __shfl((unsigned long long)sums, 63);
+    // u of it, rounded down: u in 64 bits of fraction, exact
+    const float u = as_constant(a.u)[b];
+    const uint64_t fraction = u >= 1.f ? ~0ull : u > 0.f ? (uint64_t)((double)u * 18446744073709551616.0) : 0;
+    uint64_t rest = __umul64hi(fraction, total);
+    const int pair = __popcll(__ballot(sums <= rest));   // (under 64: rest is under the total)
+    const uint64_t before = __shfl((unsigned long long)(sums - s0 - s1), pair);
+    const uint64_t first = __shfl((unsigned long long)s0, pair);
+    rest -= before;
+    int part = 2 * pair;
+    if (rest >= first) rest -= first, ++part;
+    // the slice is split over the waves, the part with the token split again
+    int lo = part * a.length, hi = min(lo + a.length, a.V);
+    while (hi - lo > 64) {
+        const int each = ((hi - lo + kWaves - 1) / kWaves + 63) / 64 * 64;
         const int begin = min(lo + wave * each, hi), end = min(begin + each, hi);
-        uint64_t sum = 0, ties = 0;
-        for (int v = begin + lane; v < end; v += 64) {
-            const uint32_t key = key_at(a, b, v);
-            if (key > edge) {
-                const uint64_t n = w.of(key);
-                sum += n >= least ? n : 0;
-            }
-            ties += key == edge;
-        }
+        uint64_t sum = 0;
+#pragma unroll 4
+        for (int v = begin + lane; v < end; v += 64) sum += kept.weight(r.w, key_at<kDtype>(a, b, v), v);
         sum = wave_sum(sum);
-        ties = wave_sum(ties);
         __syncthreads();
-        if (lane == 0) s.part[wave] = sum, s.ties[wave] = ties;
+        if (lane == 0) s.part[wave] = sum;
         __syncthreads();
-        auto kept_ties = [&](uint64_t before, uint64_t n) {   // of n after `before`
-            return edge_weight < least || before >= edge_ties ? 0 : lesser(n, edge_ties - before);
-        };
-        if (first) {
-            uint64_t before = 0;
-            for (int i = 0; i < kWaves; ++i) {
-                total += s.part[i] + kept_ties(before, s.ties[i]) * edge_weight;
-                before += s.ties[i];
-            }
-            // u of it, rounded down: u in 64 bits of fraction, exact
-            const float u = a.u[b];
-            const uint64_t fraction = u >= 1.f ? ~0ull : u > 0.f ? (uint64_t)((double)u * 18446744073709551616.0) : 0;
-            rest = __umul64hi(fraction, total);
-            first = false;
-        }
-        int part = 0;
-        for (;; ++part) {
-            const uint64_t n = s.part[part] + kept_ties(ties_before, s.ties[part]) * edge_weight;
-            if (rest < n || part == kWaves - 1) break;
-            rest -= n;
-            ties_before += s.ties[part];
-        }
+        for (part = 0; part < kWaves - 1 && rest >= s.part[part]; ++part) rest -= s.part[part];
         lo = min(lo + part * each, hi);
         hi = min(lo + each, hi);
     }
     if (wave) return;
     const int v = lo + lane;
-    const uint32_t key = v < hi ? key_at(a, b, v) : 0;
-    const uint64_t tied = __ballot(key == edge);
-    const uint64_t rank = ties_before + __popcll(tied & ((1ull << lane) - 1));
-    uint64_t mine = key > edge || (key == edge && rank < edge_ties) ? w.of(key) : 0;
-    if (mine < least) mine = 0;
-    uint64_t upto = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = __shfl_up((unsigned long long)upto, d);
-        if (lane >= d) upto += o;
-    }
+    const uint32_t key = v < hi ? key_at<kDtype>(a, b, v) : 0;
+    const uint64_t mine = kept.weight(r.w, key, v), upto = wave_scan(mine, lane);
     if (upto > rest && upto - mine <= rest) {   // one lane
         a.tokens[b] = v;
         if (a.logprobs) {
-            a.logprobs[b] = (float)(w.log2_of(key) * 0.6931471805599453 -
-                                    log((double)total / (double)one));
+            a.logprobs[b] = (float)(r.w.log2_of(key) * 0.6931471805599453 -
+                                    log((double)total / (double)(1ull << a.shift)));
         }
     }
 }
 
-}  // namespace
+// Slices of a row.  About 1024 workgroups, each of at least 2048 tokens (one
+// batch of loads is 8192).
+struct Slices {
+    int count, length;
+};
+Slices slices_of(int rows, int V) {
+    const int64_t each = ((int64_t)rows * V + 1023) / 1024;
+    int64_t length = std::max<int64_t>((each + 2047) / 2048 * 2048, 2048);
+    while (((int64_t)V + length - 1) / length > kMostSlices) length *= 2;
+    return {(int)(((int64_t)V + length - 1) / length), (int)length};
+}
 
-int sample_shift(int V) {   // a row's sum stays under 2^63
+int shift_of(int V) {   // a row's sum stays under 2^63
     int bits = 0;
     while ((int64_t)1 << bits < V) ++bits;
     return std::min(45, 62 - bits);
 }
 
-int64_t sample_bytes(int, int) { return 0; }
+}  // namespace
+
+int64_t sample_bytes(int rows, int V) {
+    const int64_t slices = (int64_t)rows * slices_of(rows, V).count;
+    return slices * (8 + (kBins + 1) * 8 + kListed * 8 + (kBins + 1) * 4 + 4);
+}
 
 int launch_sample(const void* logits, int dtype, int64_t ld, int rows, int V, const float* u,
                   const float* temperature, const int32_t* top_k, const float* top_p,
-                  const float* min_p, int32_t* tokens, float* logprobs, void*, hipStream_t stream) {
-    const SampleArgs a{logits, ld, dtype, V, sample_shift(V), u, temperature, top_k, top_p, min_p,
-                       tokens, logprobs};
-    hipLaunchKernelGGL(sample_kernel, dim3(rows), dim3(kThreads), 0, stream, a);
+                  const float* min_p, int32_t* tokens, float* logprobs, void* workspace,
+                  hipStream_t stream) {
+    const Slices cut = slices_of(rows, V);
+    const int64_t slices = (int64_t)rows * cut.count;
+    SampleArgs a{logits, ld, V, shift_of(V), cut.count, cut.length, u, temperature, top_k, top_p, min_p,
+                 tokens, logprobs};
+    a.first = static_cast<uint64_t*>(workspace);
+    a.sums = a.first + slices;
+    a.list = a.sums + slices * (kBins + 1);
+    a.counts = reinterpret_cast<uint32_t*>(a.list + slices * kListed);
+    a.listed = a.counts + slices * (kBins + 1);
+    const dim3 grid(cut.count, rows);
+    auto run = [&](auto type) {
+        constexpr int kDtype = decltype(type)::value;
+        hipLaunchKernelGGL(sample_max_kernel<kDtype>, grid, dim3(kSliceThreads), 0, stream, a);
+        if (top_k || top_p || min_p) {
+            hipLaunchKernelGGL((sample_bins_kernel<kDtype, true>), grid, dim3(kSliceThreads), 0, stream, a);
+            hipLaunchKernelGGL(sample_list_kernel<kDtype>, grid, dim3(kSliceThreads), 0, stream, a);
+        } else {
+            hipLaunchKernelGGL((sample_bins_kernel<kDtype, false>), grid, dim3(kSliceThreads), 0, stream, a);
+        }
+        hipLaunchKernelGGL(sample_finish_kernel<kDtype>, dim3(rows), dim3(kThreads), 0, stream, a);
+    };
+    if (dtype == NB_F32) run(std::integral_constant<int, NB_F32>{});
+    else run(std::integral_constant<int, NB_BF16>{});
     return check_launch("nb_sample");
 }
 
