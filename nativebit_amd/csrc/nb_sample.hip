@@ -16,15 +16,14 @@
 //   1. sample_max_kernel     each slice's first token of the order
 //   2. sample_bins_kernel    each slice's weights, summed and counted in bins of an
 //                            eighth of an octave of w (257: the last holds all
-//                            under 2^-32)
-//   3. sample_list_kernel    the row's bins say where the rules cut; the tokens of
-//                            the bins that they cut through are listed
+//                            under 2^-32); without rules one sum
+//   3. sample_list_kernel    (with rules) the row's bins say where the rules cut; each
+//                            slice's tokens of the bins that they cut through are listed
 //   4. sample_finish_kernel  one workgroup a row: the listed tokens, sorted, give
 //                            the cuts; bins and list each slice's sum of kept
 //                            weights, u the slice, the slice read again the token
-// (without rules 1, 2 without bins, 4).  A row with more than kMostListed tokens in
-// the cut bins (equal logits, mostly) is worked out by its last workgroup alone:
-// radix selection over the row.
+// A row with over kMostListed listed tokens (equal logits, mostly) is worked out by
+// its last workgroup alone: radix selection over the row.
 #include <math.h>
 
 #include <algorithm>
@@ -61,7 +60,9 @@ struct SampleArgs {
     uint32_t* counts;      // [kBins + 1]
     uint32_t* listed;      // how many are listed (more than kListed: not all are)
     uint64_t* list;        // [kListed] places
-    __device__ __forceinline__ bool rules() const { return top_k || top_p || min_p; }
+    uint64_t* whole;       // the sum of the bins that are kept whole
+    struct Cuts* cuts;     // of a row
+    __host__ __device__ __forceinline__ bool rules() const { return top_k || top_p || min_p; }
 };
 
 // Larger for larger logits; 0 for -inf and NaN.
@@ -90,50 +91,76 @@ __device__ __forceinline__ uint32_t key_at(const SampleArgs& a, int64_t b, int v
                                    : bf16_to_f32(static_cast<const bf16_bits*>(a.logits)[at]));
 }
 
-// f(token, key) for the tokens lo .. hi - 1 of row b, by the kThreads threads of
-// a workgroup: groups of four, kBatch of them asked for at once.
-template <int kDtype, int kThreads, typename F>
-__device__ __forceinline__ void for_tokens(const SampleArgs& a, int64_t b, int lo, int hi, F f) {
-    constexpr int kBatch = 4;
-    const char* row = static_cast<const char*>(a.logits) + b * a.ld * (kDtype == NB_F32 ? 4 : 2);
-    for (int v0 = lo + 4 * (int)threadIdx.x; v0 < hi; v0 += 4 * kThreads * kBatch) {
-        float x[kBatch][4];
+// The tokens lo .. hi - 1 of a row by the kThreads threads of a workgroup, groups of
+// four, kBatch groups of a thread at once and as many asked for ahead of them.
+template <int kDtype, int kThreads>
+struct Tokens {
+    static constexpr int kBatch = 4, kStep = 4 * kThreads * kBatch;
+    using Four = std::conditional_t<kDtype == NB_F32, f4_any, u2_any>;
+    const char* row;
+    int v0, hi;
+    Four x[kBatch];
+
+    __device__ __forceinline__ Tokens(const SampleArgs& a, int64_t b, int lo, int hi_)
+        : row(static_cast<const char*>(a.logits) + b * a.ld * (kDtype == NB_F32 ? 4 : 2)),
+          v0(lo + 4 * (int)threadIdx.x), hi(hi_) {
+        load(v0);
+    }
+    __device__ __forceinline__ void load(int first) {
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-            const int v = v0 + j * 4 * kThreads;
+            const int v = first + j * 4 * kThreads;
             if (v + 3 < hi) {
-                if constexpr (kDtype == NB_F32) {
-                    const f4_any w = *reinterpret_cast<const f4_any*>(row + (int64_t)v * 4);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[j][e] = w[e];
-                } else {
-                    const u2_any w = *reinterpret_cast<const u2_any*>(row + (int64_t)v * 2);
-                    x[j][0] = __uint_as_float(w[0] << 16), x[j][1] = __uint_as_float(w[0] & 0xffff0000u);
-                    x[j][2] = __uint_as_float(w[1] << 16), x[j][3] = __uint_as_float(w[1] & 0xffff0000u);
-                }
+                x[j] = *reinterpret_cast<const Four*>(row + (int64_t)v * (kDtype == NB_F32 ? 4 : 2));
             } else {
+                float e4[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    x[j][e] = -INFINITY;
+                    e4[e] = -INFINITY;
                     if (v + e < hi) {
-                        x[j][e] = kDtype == NB_F32 ? reinterpret_cast<const float*>(row)[v + e]
-                                                   : bf16_to_f32(reinterpret_cast<const bf16_bits*>(row)[v + e]);
+                        e4[e] = kDtype == NB_F32 ? reinterpret_cast<const float*>(row)[v + e]
+                                                 : bf16_to_f32(reinterpret_cast<const bf16_bits*>(row)[v + e]);
                     }
+                }
+                if constexpr (kDtype == NB_F32) {
+                    x[j] = Four{e4[0], e4[1], e4[2], e4[3]};
+                } else {
+                    x[j] = Four{__float_as_uint(e4[0]) >> 16 | __float_as_uint(e4[1]),
+                                __float_as_uint(e4[2]) >> 16 | __float_as_uint(e4[3])};
                 }
             }
         }
+    }
+    // f(token, key), once
+    template <typename F>
+    __device__ __forceinline__ void each(F f) {
+        for (; v0 < hi; v0 += kStep) {
+            Four now[kBatch];
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
+            for (int j = 0; j < kBatch; ++j) now[j] = x[j];
+            if (v0 + kStep < hi) load(v0 + kStep);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) f(v0 + j * 4 * kThreads + e, key_of(x[j][e]));
+            for (int j = 0; j < kBatch; ++j) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float y;
+                    if constexpr (kDtype == NB_F32) y = now[j][e];
+                    else y = __uint_as_float(e & 1 ? now[j][e / 2] & 0xffff0000u : now[j][e / 2] << 16);
+                    f(v0 + j * 4 * kThreads + e, key_of(y));
+                }
+            }
         }
     }
+};
+template <int kDtype, int kThreads, typename F>
+__device__ __forceinline__ void for_tokens(const SampleArgs& a, int64_t b, int lo, int hi, F f) {
+    Tokens<kDtype, kThreads>(a, b, lo, hi).each(f);
 }
 
 // The bin of a weight by its log2.
 __device__ __forceinline__ int bin_of(double z) { return z > -kBins / 8 ? (int)(z * -8.0) : kBins; }
 
-constexpr int kFractions = 32;   // entries of 2^(i / 32)
+constexpr int kFractions = 128;   // entries of 2^(i / 128)
 
 struct Weights {
     double most, turn;   // the row's maximum, log2(e) / T
@@ -145,7 +172,7 @@ struct Weights {
         return x == most ? 0.0 : fmax((x - most) * turn, -4000.0);   // (of infinities: 0 or less)
     }
     // 2^(n + f): the table's entry by f's upper bits, a polynomial of the rest
-    // (|r| <= 1/64: its next term is 2e-15)
+    // (|r| <= 1/256: its next term is 2e-12)
     __device__ __forceinline__ uint64_t of(uint32_t key) const {
         return key ? of_log2(log2_of(key)) : 0;
     }
@@ -154,13 +181,11 @@ struct Weights {
         const double y = z * kFractions + kMagic;
         const int n = __double2loint(y);
         const double r = z - (y - kMagic) * (1.0 / kFractions);
-        double p = 0.0013333558146428443;
-        p = fma(p, r, 0.009618129107628477);
-        p = fma(p, r, 0.05550410866482158);
+        double p = 0.05550410866482158;
         p = fma(p, r, 0.2402265069591007);
         p = fma(p, r, 0.6931471805599453);
         p = fma(p, r, 1.0);
-        p = ldexp(p * table[n & (kFractions - 1)], (n >> 5) + shift);
+        p = ldexp(p * table[n & (kFractions - 1)], (n >> 7) + shift);
         return (uint64_t)__double_as_longlong(p + 4503599627370496.0) - 0x4330000000000000ull;
     }
 };
@@ -249,41 +274,57 @@ __global__ __launch_bounds__(kSliceThreads) void sample_max_kernel(SampleArgs a)
     a.first[b * a.slices + blockIdx.x] = first;
 }
 
+// Weights up to 2^-11 are most of a row's: in bins of a slice of up to 2^14 tokens
+// their sum is at most 2^48, and the count lies above it in the same word (one
+// atomic for both).  Four copies of the bins, a lane's by its number: lanes of a wave
+// hit the same word less often.
+constexpr int kPackedFrom = 88, kCountAt = 49, kCopies = 4;
+
 template <int kDtype, bool kRules>
 __global__ __launch_bounds__(kSliceThreads) void sample_bins_kernel(SampleArgs a) {
     __shared__ double table[kFractions];
-    __shared__ unsigned long long sums[kBins + 1];
+    __shared__ unsigned long long sums[(kBins + 1) * kCopies];
     __shared__ uint32_t counts[kBins + 1];
     const int64_t b = blockIdx.y, slice = b * a.slices + blockIdx.x;
     const int lo = blockIdx.x * a.length, hi = min(lo + a.length, a.V), tid = threadIdx.x;
+    Tokens<kDtype, kSliceThreads> tokens(a, b, lo, hi);   // (its first loads are under way meanwhile)
     make_table(table);
     const Rules r(a, b, table);
     if (r.greedy || r.first == 0) return;   // (nothing reads the row's bins)
     if (kRules) {
-        for (int i = tid; i <= kBins; i += kSliceThreads) sums[i] = 0, counts[i] = 0;
+        for (int i = tid; i < (kBins + 1) * kCopies; i += kSliceThreads) sums[i] = 0;
+        for (int i = tid; i <= kBins; i += kSliceThreads) counts[i] = 0;
     }
     __syncthreads();
+    const int packed_from = a.length <= 1 << 14 ? kPackedFrom : kBins;
     uint64_t sum = 0;       // without bins of all, else of the last bin
     uint32_t count = 0;
-    for_tokens<kDtype, kSliceThreads>(a, b, lo, hi, [&](int, uint32_t key) {
+    tokens.each([&](int, uint32_t key) {
         if (!key) return;
         const double z = r.w.log2_of(key);
-        const uint64_t w = r.w.of_log2(z);
+        uint64_t w = r.w.of_log2(z);
         const int bin = kRules ? bin_of(z) : kBins;
         if (bin < kBins) {
-            atomicAdd(&sums[bin], (unsigned long long)w);
-            atomicAdd(&counts[bin], 1u);
+            if (bin >= packed_from) w += 1ull << kCountAt;
+            else atomicAdd(&counts[bin], 1u);
+            atomicAdd(&sums[bin * kCopies + (tid & (kCopies - 1))], (unsigned long long)w);
         } else {
             sum += w, ++count;
         }
     });
     if (kRules) {
         sum = wave_sum(sum), count = (uint32_t)wave_sum(count);
-        if ((tid & 63) == 0) atomicAdd(&sums[kBins], (unsigned long long)sum), atomicAdd(&counts[kBins], count);
+        if ((tid & 63) == 0) {
+            atomicAdd(&sums[kBins * kCopies], (unsigned long long)sum);
+            atomicAdd(&counts[kBins], count);
+        }
         __syncthreads();
         for (int i = tid; i <= kBins; i += kSliceThreads) {
-            a.sums[slice * (kBins + 1) + i] = sums[i];
-            a.counts[slice * (kBins + 1) + i] = counts[i];
+            uint64_t all = 0;
+            for (int c = 0; c < kCopies; ++c) all += sums[i * kCopies + c];
+            const bool packed = i >= packed_from && i < kBins;
+            a.sums[slice * (kBins + 1) + i] = packed ? all & ((1ull << kCountAt) - 1) : all;
+            a.counts[slice * (kBins + 1) + i] = packed ? (uint32_t)(all >> kCountAt) : counts[i];
         }
     } else {
         sum = wave_sum(sum);
@@ -317,34 +358,41 @@ __device__ __forceinline__ uint64_t share_of(float p, uint64_t total) {
 struct CutShared {
     uint64_t sum[kBins + 2], above[kBins + 2];   // of a bin; of those before it
     uint32_t count[kBins + 2], before[kBins + 2];
+    uint64_t part[(kBins + 64) / 64 + 1];
+    uint32_t count_part[(kBins + 64) / 64 + 1];
     int found[4];
 };
-// By all threads of a workgroup of over kBins + 1.
-__device__ Cuts find_cuts(const SampleArgs& a, int64_t b, const Rules& r, CutShared& s) {
-    const int tid = threadIdx.x;
-    constexpr int kAll = kBins + 1, kNone = kBins + 1;
-    if (tid < kAll) {
-        uint64_t sum = 0;
-        uint32_t count = 0;
-#pragma unroll 8
+// A row's bin of each thread (of a workgroup of over kBins + 1).
+struct Bin {
+    uint64_t sum;
+    uint32_t count;
+    __device__ __forceinline__ Bin(const SampleArgs& a, int64_t b) : sum(0), count(0) {
+        constexpr int kAll = kBins + 1;
+        if (threadIdx.x >= kAll) return;
+#pragma unroll 16
         for (int i = 0; i < a.slices; ++i) {
-            sum += a.sums[(b * a.slices + i) * kAll + tid];
-            count += a.counts[(b * a.slices + i) * kAll + tid];
+            sum += a.sums[(b * a.slices + i) * kAll + threadIdx.x];
+            count += a.counts[(b * a.slices + i) * kAll + threadIdx.x];
         }
-        s.sum[tid] = sum, s.count[tid] = count;
+    }
+};
+__device__ Cuts find_cuts(const Rules& r, const Bin& mine, CutShared& s) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    constexpr int kAll = kBins + 1, kNone = kBins + 1, kParts = (kAll + 63) / 64;
+    const uint64_t sum = mine.sum;
+    const uint32_t count = mine.count;
+    uint64_t above = 0;
+    uint32_t before = 0;
+    if (tid < kParts * 64) {
+        above = wave_scan(sum, lane), before = (uint32_t)wave_scan((uint64_t)count, lane);
+        if (lane == 63) s.part[wave] = above, s.count_part[wave] = before;
+        above -= sum, before -= count;
     }
     if (tid < 4) s.found[tid] = kNone;
     __syncthreads();
-    if (tid < 64) {   // a wave: five bins a lane
-        constexpr int kEach = (kAll + 63) / 64;
-        uint64_t sum = 0, count = 0;
-        for (int i = tid * kEach; i < min((tid + 1) * kEach, kAll); ++i) sum += s.sum[i], count += s.count[i];
-        uint64_t above = wave_scan(sum, tid) - sum, before = wave_scan(count, tid) - count;
-        for (int i = tid * kEach; i < min((tid + 1) * kEach, kAll); ++i) {
-            s.above[i] = above, s.before[i] = (uint32_t)before;
-            above += s.sum[i], before += s.count[i];
-        }
-        if (tid == 63) s.above[kNone] = above, s.sum[kNone] = 0, s.before[kNone] = (uint32_t)before;
+    if (tid <= kAll) {   // (and one past the last: all of them)
+        for (int i = 0; i < wave; ++i) above += s.part[i], before += s.count_part[i];
+        s.sum[tid] = sum, s.above[tid] = above, s.count[tid] = count, s.before[tid] = before;
     }
     __syncthreads();
     if (r.k && tid < kAll && s.before[tid] < r.k && s.before[tid] + (uint64_t)s.count[tid] >= (uint64_t)r.k) {
@@ -376,24 +424,54 @@ __global__ __launch_bounds__(kSliceThreads) void sample_list_kernel(SampleArgs a
     __shared__ CutShared shared;
     __shared__ uint32_t count;
     const int64_t b = blockIdx.y, slice = b * a.slices + blockIdx.x;
-    const int lo = blockIdx.x * a.length, hi = min(lo + a.length, a.V);
-    const Rules r(a, b, nullptr);   // (no weights here, only their bins)
+    const int lo = blockIdx.x * a.length, hi = min(lo + a.length, a.V), tid = threadIdx.x, lane = tid & 63;
+    const Bin bin(a, b);
+    // (of the last wave: the slice's own bins)
+    uint64_t own[(kBins + 64) / 64] = {};
+    if (tid >= kSliceThreads - 64) {
+#pragma unroll
+        for (int i = 0; i * 64 <= kBins; ++i) {
+            own[i] = i * 64 + lane <= kBins ? a.sums[slice * (kBins + 1) + i * 64 + lane] : 0;
+        }
+    }
+    Tokens<kDtype, kSliceThreads> tokens(a, b, lo, hi);   // (its first loads are under way meanwhile)
+    const Rules r(a, b, nullptr);                         // (no weights here, only their bins)
     if (r.greedy || r.first == 0) return;
-    if (threadIdx.x == 0) count = 0;
-    const Cuts c = find_cuts(a, b, r, shared);
-    for_tokens<kDtype, kSliceThreads>(a, b, lo, hi, [&](int v, uint32_t key) {
-        if (!key || !c.listed(bin_of(r.w.log2_of(key)))) return;
-        const uint32_t at = atomicAdd(&count, 1u);
-        if (at < kListed) a.list[slice * kListed + at] = place_of(key, v);
-    });
+    if (tid == 0) count = 0;
+    const Cuts c = find_cuts(r, bin, shared);
+    if (tid == 0 && blockIdx.x == 0) a.cuts[b] = c;
+    if (tid >= kSliceThreads - 64) {
+        uint64_t sum = 0;
+#pragma unroll
+        for (int i = 0; i * 64 <= kBins; ++i) sum += i * 64 + lane < c.sure() ? own[i] : 0;
+        sum = wave_sum(sum);
+        if (lane == 0) a.whole[slice] = sum;
+    }
+    // Logits between those of the first and the last listed bin, an eighth of an
+    // octave and the roundings to either side: few, and only their bins are worked out.
+    int to = -1;
+    if (c.k <= kBins) to = c.k;
+    if (c.p_low <= kBins) to = max(to, c.p_high);
+    if (c.m_low <= kBins) to = max(to, c.m_high);
+    if (to >= 0) {
+        const double octave = 1.0 / r.w.turn, slack = 1e-6 * fabs(r.w.most);
+        const float high = (float)(r.w.most - (c.sure() - 1) * 0.125 * octave + slack);
+        const float low = to == kBins ? -INFINITY : (float)(r.w.most - (to + 2) * 0.125 * octave - slack);
+        tokens.each([&](int v, uint32_t key) {
+            const float x = logit_of(key);   // (a NaN where there is none)
+            if (x < low || x > high || !key || !c.listed(bin_of(r.w.log2_of(key)))) return;
+            const uint32_t at = atomicAdd(&count, 1u);
+            if (at < kListed) a.list[slice * kListed + at] = place_of(key, v);
+        });
+    }
     __syncthreads();
-    if (threadIdx.x == 0) a.listed[slice] = count;
+    if (tid == 0) a.listed[slice] = count;
 }
 
 // ---------------------------------------------------------------------------
 // rows
 // ---------------------------------------------------------------------------
-constexpr int kThreads = 1024, kWaves = kThreads / 64, kDigits = 2048;
+constexpr int kThreads = 1024, kWaves = kThreads / 64, kDigits = 2048, kRanked = 256;
 
 struct Shared {
     double table[kFractions];
@@ -401,7 +479,6 @@ struct Shared {
         uint64_t digits[kDigits];        // radix selection
         uint64_t list[kMostListed];      // the listed tokens
     };
-    CutShared cuts;
     uint64_t part[kWaves], ties[kWaves];
     uint64_t found[2];
 };
@@ -423,6 +500,7 @@ __device__ uint64_t block_sum(Shared& s, uint64_t v) {   // in all threads
     if ((threadIdx.x & 63) == 0) s.part[threadIdx.x >> 6] = v;
     __syncthreads();
     v = 0;
+#pragma unroll
     for (int i = 0; i < kWaves; ++i) v += s.part[i];
     return v;
 }
@@ -550,22 +628,38 @@ __device__ uint64_t last_of_row(const SampleArgs& a, int64_t b, const Rules& r, 
     return v == 0xffffffffu ? (uint64_t)edge << 32 : place_of(edge, (int)v);
 }
 
-// The same by the listed tokens; their kept weights are added to s.digits' place
-// of their slices' sums, `slice_sums`.
+// The same by the listed tokens; their kept weights are added to their slices'
+// sums.
 __device__ uint64_t last_of_list(const SampleArgs& a, const Rules& r, const Cuts& c, Shared& s, int n,
                                  unsigned long long* slice_sums) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int size = 64;
-    while (size < n) size *= 2;
-    for (int i = n + tid; i < size; i += kThreads) s.list[i] = 0;
-    // sorted into the order, largest place first
-    for (int k = 2; k <= size; k *= 2) {
-        for (int j = k / 2; j > 0; j /= 2) {
-            __syncthreads();
-            for (int i = tid; i < size / 2; i += kThreads) {
-                const int x = (i & ~(j - 1)) << 1 | (i & (j - 1)), y = x + j;   // (j: a power of two)
-                const uint64_t p = s.list[x], q = s.list[y];
-                if ((p < q) == ((x & k) == 0)) s.list[x] = q, s.list[y] = p;
+    // sorted into the order, largest place first: up to kRanked by counting the
+    // larger ones, more by merging runs
+    if (n <= kRanked) {
+        constexpr int kParts = kThreads / kRanked;   // threads of a token, a share of the others each
+        const int i = tid / kParts;
+        const uint64_t place = i < n ? s.list[i] : 0;
+        int rank = 0;
+        if (i < n) {
+#pragma unroll 4
+            for (int j = tid % kParts; j < n; j += kParts) rank += s.list[j] > place;
+        }
+#pragma unroll
+        for (int d = 1; d < kParts; d *= 2) rank += __shfl_xor(rank, d);
+        __syncthreads();
+        if (i < n && tid % kParts == 0) s.list[rank] = place;
+    } else {
+        int size = kRanked;
+        while (size < n) size *= 2;
+        for (int i = n + tid; i < size; i += kThreads) s.list[i] = 0;
+        for (int k = 2; k <= size; k *= 2) {
+            for (int j = k / 2; j > 0; j /= 2) {
+                __syncthreads();
+                for (int i = tid; i < size / 2; i += kThreads) {
+                    const int x = (i & ~(j - 1)) << 1 | (i & (j - 1)), y = x + j;   // (j: a power of two)
+                    const uint64_t p = s.list[x], q = s.list[y];
+                    if ((p < q) == ((x & k) == 0)) s.list[x] = q, s.list[y] = p;
+                }
             }
         }
     }
@@ -636,6 +730,16 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
     __shared__ int list_at[kMostSlices + 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t b = blockIdx.x, slice0 = b * a.slices;
+    // Asked for at once: u, the cuts, and of two slices a lane the listed tokens and
+    // the sums of whole bins.  (Of a greedy row they are not there, and not used.)
+    const float u = as_constant(a.u)[b];
+    const int i0 = 2 * lane, i1 = 2 * lane + 1;
+    const bool has0 = i0 < a.slices, has1 = i1 < a.slices, rules = a.rules();
+    const Cuts c = rules ? a.cuts[b] : Cuts{};
+    const uint64_t* whole = rules ? a.whole : a.sums;
+    const uint64_t w0 = has0 ? whole[slice0 + i0] : 0, w1 = has1 ? whole[slice0 + i1] : 0;
+    const uint32_t l0 = rules && has0 ? a.listed[slice0 + i0] : 0, l1 = rules && has1 ? a.listed[slice0 + i1] : 0;
+    if (wave == 0) slice_sums[i0] = w0, slice_sums[i1] = w1;
     make_table(s.table);
     const Rules r(a, b, s.table);
     if (r.first == 0 || r.greedy) {
@@ -645,42 +749,26 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
         }
         return;
     }
-    __syncthreads();
     Kept kept{0, r.least};
     bool known = true;   // slice_sums are those of kept weights
-    if (!a.rules()) {
-        if (tid < a.slices) slice_sums[tid] = a.sums[slice0 + tid];
-    } else {
-        const Cuts c = find_cuts(a, b, r, s.cuts);
-        // listed tokens: two slices a lane, their places one after the other
-        const uint32_t l0 = 2 * lane < a.slices ? a.listed[slice0 + 2 * lane] : 0;
-        const uint32_t l1 = 2 * lane + 1 < a.slices ? a.listed[slice0 + 2 * lane + 1] : 0;
+    if (rules) {
+        // the listed tokens, one slice's after the other's
         const uint64_t upto = wave_scan((uint64_t)l0 + l1, lane);
         const uint64_t listed = __shfl((unsigned long long)upto, 63);
         known = __ballot(l0 > kListed || l1 > kListed) == 0 && listed <= kMostListed;
-        const int n = known ? (int)listed : 0;
+        if (known && wave == 0) {
+            list_at[i0] = (int)(upto - l0 - l1);
+            list_at[i1] = (int)(upto - l1);
+            if (lane == 63) list_at[kMostSlices] = (int)listed;
+        }
+        __syncthreads();
         if (known) {
-            if (wave == 0) {
-                list_at[2 * lane] = (int)(upto - l0 - l1);
-                list_at[2 * lane + 1] = (int)(upto - l1);
-                if (lane == 63) list_at[kMostSlices] = n;
-            }
-            // sums of the bins that are kept whole, a wave a slice
-            for (int i = wave; i < a.slices; i += kWaves) {
-                uint64_t sum = 0;
-                for (int bin = lane; bin < c.sure() && bin <= kBins; bin += 64) {
-                    sum += a.sums[(slice0 + i) * (kBins + 1) + bin];
-                }
-                sum = wave_sum(sum);
-                if (lane == 0) slice_sums[i] = sum;
-            }
-            __syncthreads();
             for (int i = wave; i < a.slices; i += kWaves) {
                 const int at = list_at[i], count = list_at[i + 1] - at;
                 for (int e = lane; e < count; e += 64) s.list[at + e] = a.list[(slice0 + i) * kListed + e];
             }
             __syncthreads();
-            kept.last = last_of_list(a, r, c, s, n, slice_sums);
+            kept.last = last_of_list(a, r, c, s, (int)listed, slice_sums);
         } else {
             kept.last = last_of_row<kDtype>(a, b, r, s);
         }
@@ -697,11 +785,9 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
         __syncthreads();
     }
     // the slice that u falls in: two slices a lane, every wave by itself
-    const uint64_t s0 = 2 * lane < a.slices ? slice_sums[2 * lane] : 0;
-    const uint64_t s1 = 2 * lane + 1 < a.slices ? slice_sums[2 * lane + 1] : 0;
+    const uint64_t s0 = slice_sums[2 * lane], s1 = slice_sums[2 * lane + 1];
     const uint64_t sums = wave_scan(s0 + s1, lane), total = __shfl((unsigned long long)sums, 63);
     // u of it, rounded down: u in 64 bits of fraction, exact
-    const float u = as_constant(a.u)[b];
     const uint64_t fraction = u >= 1.f ? ~0ull : u > 0.f ? (uint64_t)((double)u * 18446744073709551616.0) : 0;
     uint64_t rest = __umul64hi(fraction, total);
     const int pair = __popcll(__ballot(sums <= rest));   // (under 64: rest is under the total)
@@ -710,9 +796,10 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
     rest -= before;
     int part = 2 * pair;
     if (rest >= first) rest -= first, ++part;
-    // the slice is split over the waves, the part with the token split again
+    // the slice is split over the waves, a large one's part with the token again
     int lo = part * a.length, hi = min(lo + a.length, a.V);
-    while (hi - lo > 64) {
+    constexpr int kAtOnce = 16;   // groups of 64 tokens of a wave
+    while (hi - lo > kThreads * kAtOnce) {
         const int each = ((hi - lo + kWaves - 1) / kWaves + 63) / 64 * 64;
         const int begin = min(lo + wave * each, hi), end = min(begin + each, hi);
         uint64_t sum = 0;
@@ -726,27 +813,55 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
         lo = min(lo + part * each, hi);
         hi = min(lo + each, hi);
     }
-    if (wave) return;
-    const int v = lo + lane;
-    const uint32_t key = v < hi ? key_at<kDtype>(a, b, v) : 0;
-    const uint64_t mine = kept.weight(r.w, key, v), upto = wave_scan(mine, lane);
-    if (upto > rest && upto - mine <= rest) {   // one lane
-        a.tokens[b] = v;
-        if (a.logprobs) {
-            a.logprobs[b] = (float)(r.w.log2_of(key) * 0.6931471805599453 -
-                                    log((double)total / (double)(1ull << a.shift)));
+    // then its weights are in registers, 64 neighbours in those of a number
+    const int groups = (hi - lo + kThreads - 1) / kThreads;   // of a wave
+    const int begin = lo + wave * groups * 64;
+    uint64_t weights[kAtOnce], sum = 0;
+    {
+        uint32_t keys[kAtOnce];
+#pragma unroll
+        for (int g = 0; g < kAtOnce; ++g) {
+            const int v = begin + g * 64 + lane;
+            keys[g] = g < groups && v < hi ? key_at<kDtype>(a, b, v) : 0;
         }
+#pragma unroll
+        for (int g = 0; g < kAtOnce; ++g) {
+            weights[g] = g < groups ? kept.weight(r.w, keys[g], begin + g * 64 + lane) : 0;
+            sum += weights[g];
+        }
+    }
+    sum = wave_sum(sum);
+    __syncthreads();
+    if (lane == 0) s.part[wave] = sum;
+    __syncthreads();
+    for (part = 0; part < kWaves - 1 && rest >= s.part[part]; ++part) rest -= s.part[part];
+    if (wave != part) return;
+#pragma unroll
+    for (int g = 0; g < kAtOnce; ++g) {
+        const uint64_t upto = wave_scan(weights[g], lane), all = __shfl((unsigned long long)upto, 63);
+        if (rest < all) {
+            if (upto > rest && upto - weights[g] <= rest) {   // one lane
+                const int v = begin + g * 64 + lane;
+                a.tokens[b] = v;
+                if (a.logprobs) {
+                    a.logprobs[b] = (float)(r.w.log2_of(key_at<kDtype>(a, b, v)) * 0.6931471805599453 -
+                                            log((double)total / (double)(1ull << a.shift)));
+                }
+            }
+            return;
+        }
+        rest -= all;
     }
 }
 
-// Slices of a row.  About 1024 workgroups, each of at least 2048 tokens (one
-// batch of loads is 8192).
+// Slices of a row: about 1024 workgroups, each of 2048 to 16384 tokens (more where
+// a row would have over kMostSlices).
 struct Slices {
     int count, length;
 };
 Slices slices_of(int rows, int V) {
     const int64_t each = ((int64_t)rows * V + 1023) / 1024;
-    int64_t length = std::max<int64_t>((each + 2047) / 2048 * 2048, 2048);
+    int64_t length = std::min<int64_t>(std::max<int64_t>((each + 2047) / 2048 * 2048, 2048), 1 << 14);
     while (((int64_t)V + length - 1) / length > kMostSlices) length *= 2;
     return {(int)(((int64_t)V + length - 1) / length), (int)length};
 }
@@ -761,7 +876,7 @@ int shift_of(int V) {   // a row's sum stays under 2^63
 
 int64_t sample_bytes(int rows, int V) {
     const int64_t slices = (int64_t)rows * slices_of(rows, V).count;
-    return slices * (8 + (kBins + 1) * 8 + kListed * 8 + (kBins + 1) * 4 + 4);
+    return rows * (int64_t)sizeof(Cuts) + slices * (8 + 8 + (kBins + 1) * 8 + kListed * 8 + (kBins + 1) * 4 + 4);
 }
 
 int launch_sample(const void* logits, int dtype, int64_t ld, int rows, int V, const float* u,
@@ -772,8 +887,10 @@ int launch_sample(const void* logits, int dtype, int64_t ld, int rows, int V, co
     const int64_t slices = (int64_t)rows * cut.count;
     SampleArgs a{logits, ld, V, shift_of(V), cut.count, cut.length, u, temperature, top_k, top_p, min_p,
                  tokens, logprobs};
-    a.first = static_cast<uint64_t*>(workspace);
-    a.sums = a.first + slices;
+    a.cuts = static_cast<Cuts*>(workspace);
+    a.first = reinterpret_cast<uint64_t*>(a.cuts + rows);
+    a.whole = a.first + slices;
+    a.sums = a.whole + slices;
     a.list = a.sums + slices * (kBins + 1);
     a.counts = reinterpret_cast<uint32_t*>(a.list + slices * kListed);
     a.listed = a.counts + slices * (kBins + 1);
@@ -781,12 +898,9 @@ int launch_sample(const void* logits, int dtype, int64_t ld, int rows, int V, co
     auto run = [&](auto type) {
         constexpr int kDtype = decltype(type)::value;
         hipLaunchKernelGGL(sample_max_kernel<kDtype>, grid, dim3(kSliceThreads), 0, stream, a);
-        if (top_k || top_p || min_p) {
-            hipLaunchKernelGGL((sample_bins_kernel<kDtype, true>), grid, dim3(kSliceThreads), 0, stream, a);
-            hipLaunchKernelGGL(sample_list_kernel<kDtype>, grid, dim3(kSliceThreads), 0, stream, a);
-        } else {
-            hipLaunchKernelGGL((sample_bins_kernel<kDtype, false>), grid, dim3(kSliceThreads), 0, stream, a);
-        }
+        auto* bins = a.rules() ? sample_bins_kernel<kDtype, true> : sample_bins_kernel<kDtype, false>;
+        hipLaunchKernelGGL(bins, grid, dim3(kSliceThreads), 0, stream, a);
+        if (a.rules()) hipLaunchKernelGGL(sample_list_kernel<kDtype>, grid, dim3(kSliceThreads), 0, stream, a);
         hipLaunchKernelGGL(sample_finish_kernel<kDtype>, dim3(rows), dim3(kThreads), 0, stream, a);
     };
     if (dtype == NB_F32) run(std::integral_constant<int, NB_F32>{});
