@@ -17,9 +17,10 @@
 //   2. sample_bins_kernel    each slice's weights, summed and counted in bins of an
 //                            eighth of an octave of w (257: the last holds all
 //                            under 2^-32); without rules one sum
-//   3. sample_list_kernel    (with rules) the row's bins say where the rules cut; each
-//                            slice's tokens of the bins that they cut through are listed
-//   4. sample_finish_kernel  one workgroup a row: the listed tokens, sorted, give
+//   3. sample_cuts_kernel    (with rules) a row's bins say where the rules cut
+//   4. sample_list_kernel    (with rules) each slice's tokens of the bins that they cut
+//                            through are listed
+//   5. sample_finish_kernel  one workgroup a row: the listed tokens, sorted, give
 //                            the cuts; bins and list each slice's sum of kept
 //                            weights, u the slice, the slice read again the token
 // A row with over kMostListed listed tokens (equal logits, mostly) is worked out by
@@ -190,26 +191,35 @@ struct Weights {
     }
 };
 
+// Over the lanes of a wave by DPP moves (a 64-bit shuffle is two LDS round trips): rows
+// of 16 lanes by shifts, then a row's last lane to the next, and the second's to the
+// other half.  All lanes must be active.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ uint64_t dpp64(uint64_t v) {   // 0 where no lane is read
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, kCtrl, kRows, 0xf, true);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), kCtrl, kRows, 0xf, true);
+    return (uint64_t)(uint32_t)hi << 32 | (uint32_t)lo;
+}
+template <typename Join>
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v, Join join) {   // of lanes 0 .. this one
+    v = join(v, dpp64<0x111, 0xf>(v));   // row_shr 1, 2, 4, 8
+    v = join(v, dpp64<0x112, 0xf>(v));
+    v = join(v, dpp64<0x114, 0xf>(v));
+    v = join(v, dpp64<0x118, 0xf>(v));
+    v = join(v, dpp64<0x142, 0xa>(v));   // row_bcast 15 into rows 1 and 3
+    return join(v, dpp64<0x143, 0xc>(v));   // row_bcast 31 into rows 2 and 3
+}
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+    const uint32_t hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
+    return (uint64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
+    return wave_scan(v, [](uint64_t x, uint64_t y) { return x + y; });
+}
+__device__ __forceinline__ uint64_t wave_sum(uint64_t v) { return lane_of(wave_scan(v), 63); }
 __device__ __forceinline__ uint64_t wave_max(uint64_t v) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = __shfl_xor((unsigned long long)v, d);
-        v = o > v ? o : v;
-    }
-    return v;
-}
-__device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor((unsigned long long)v, d);
-    return v;
-}
-__device__ __forceinline__ uint64_t wave_scan(uint64_t v, int lane) {   // sum of lanes 0 .. lane
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = __shfl_up((unsigned long long)v, d);
-        if (lane >= d) v += o;
-    }
-    return v;
+    return lane_of(wave_scan(v, [](uint64_t x, uint64_t y) { return x > y ? x : y; }), 63);
 }
 __device__ __forceinline__ uint64_t lesser(uint64_t x, uint64_t y) { return x < y ? x : y; }
 
@@ -343,11 +353,13 @@ struct Cuts {
                          // is not known yet)
     int m_low, m_high;   // those around min_p
     uint64_t above_k, sum_k, above_p;   // tokens and weights over bin k, weights over p_low
+    float low, high;     // the logits of all listed tokens lie between
+    double most, turn;   // of Weights
     __device__ __forceinline__ bool listed(int bin) const {
         return bin == k || (bin >= p_low && bin <= p_high) || (bin >= m_low && bin <= m_high);
     }
     // all tokens of the bins before it are kept, of those after it only listed ones
-    __device__ __forceinline__ int sure() const { return min(k, min(p_low, m_low)); }
+    __host__ __device__ __forceinline__ int sure() const { return std::min(k, std::min(p_low, m_low)); }
 };
 // The least sum of a beginning that makes up p of `total`: at least one unit.
 __device__ __forceinline__ uint64_t share_of(float p, uint64_t total) {
@@ -362,29 +374,14 @@ struct CutShared {
     uint32_t count_part[(kBins + 64) / 64 + 1];
     int found[4];
 };
-// A row's bin of each thread (of a workgroup of over kBins + 1).
-struct Bin {
-    uint64_t sum;
-    uint32_t count;
-    __device__ __forceinline__ Bin(const SampleArgs& a, int64_t b) : sum(0), count(0) {
-        constexpr int kAll = kBins + 1;
-        if (threadIdx.x >= kAll) return;
-#pragma unroll 16
-        for (int i = 0; i < a.slices; ++i) {
-            sum += a.sums[(b * a.slices + i) * kAll + threadIdx.x];
-            count += a.counts[(b * a.slices + i) * kAll + threadIdx.x];
-        }
-    }
-};
-__device__ Cuts find_cuts(const Rules& r, const Bin& mine, CutShared& s) {
+// By all threads of a workgroup of over kBins + 1, each with its bin of the row.
+__device__ Cuts find_cuts(const Rules& r, uint64_t sum, uint32_t count, CutShared& s) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     constexpr int kAll = kBins + 1, kNone = kBins + 1, kParts = (kAll + 63) / 64;
-    const uint64_t sum = mine.sum;
-    const uint32_t count = mine.count;
     uint64_t above = 0;
     uint32_t before = 0;
     if (tid < kParts * 64) {
-        above = wave_scan(sum, lane), before = (uint32_t)wave_scan((uint64_t)count, lane);
+        above = wave_scan(sum), before = (uint32_t)wave_scan((uint64_t)count);
         if (lane == 63) s.part[wave] = above, s.count_part[wave] = before;
         above -= sum, before -= count;
     }
@@ -416,50 +413,69 @@ __device__ Cuts find_cuts(const Rules& r, const Bin& mine, CutShared& s) {
         c.m_low = bin_of(r.least_high);
         c.m_high = bin_of(r.least_low);
     }
-    return c;
-}
-
-template <int kDtype>
-__global__ __launch_bounds__(kSliceThreads) void sample_list_kernel(SampleArgs a) {
-    __shared__ CutShared shared;
-    __shared__ uint32_t count;
-    const int64_t b = blockIdx.y, slice = b * a.slices + blockIdx.x;
-    const int lo = blockIdx.x * a.length, hi = min(lo + a.length, a.V), tid = threadIdx.x, lane = tid & 63;
-    const Bin bin(a, b);
-    // (of the last wave: the slice's own bins)
-    uint64_t own[(kBins + 64) / 64] = {};
-    if (tid >= kSliceThreads - 64) {
-#pragma unroll
-        for (int i = 0; i * 64 <= kBins; ++i) {
-            own[i] = i * 64 + lane <= kBins ? a.sums[slice * (kBins + 1) + i * 64 + lane] : 0;
-        }
-    }
-    Tokens<kDtype, kSliceThreads> tokens(a, b, lo, hi);   // (its first loads are under way meanwhile)
-    const Rules r(a, b, nullptr);                         // (no weights here, only their bins)
-    if (r.greedy || r.first == 0) return;
-    if (tid == 0) count = 0;
-    const Cuts c = find_cuts(r, bin, shared);
-    if (tid == 0 && blockIdx.x == 0) a.cuts[b] = c;
-    if (tid >= kSliceThreads - 64) {
-        uint64_t sum = 0;
-#pragma unroll
-        for (int i = 0; i * 64 <= kBins; ++i) sum += i * 64 + lane < c.sure() ? own[i] : 0;
-        sum = wave_sum(sum);
-        if (lane == 0) a.whole[slice] = sum;
-    }
-    // Logits between those of the first and the last listed bin, an eighth of an
-    // octave and the roundings to either side: few, and only their bins are worked out.
+    // an eighth of an octave and the roundings to either side of the first and the
+    // last listed bin (none: no logit is infinite both ways)
     int to = -1;
     if (c.k <= kBins) to = c.k;
     if (c.p_low <= kBins) to = max(to, c.p_high);
     if (c.m_low <= kBins) to = max(to, c.m_high);
-    if (to >= 0) {
-        const double octave = 1.0 / r.w.turn, slack = 1e-6 * fabs(r.w.most);
-        const float high = (float)(r.w.most - (c.sure() - 1) * 0.125 * octave + slack);
-        const float low = to == kBins ? -INFINITY : (float)(r.w.most - (to + 2) * 0.125 * octave - slack);
+    const double octave = 1.0 / r.w.turn, slack = 1e-6 * fabs(r.w.most);
+    c.high = to < 0 ? -INFINITY : (float)(r.w.most - (c.sure() - 1) * 0.125 * octave + slack);
+    c.low = to < 0 ? INFINITY : to == kBins ? -INFINITY : (float)(r.w.most - (to + 2) * 0.125 * octave - slack);
+    c.most = r.w.most, c.turn = r.w.turn;
+    return c;
+}
+
+constexpr int kCutThreads = (kBins + 64) / 64 * 64;
+
+__global__ __launch_bounds__(kCutThreads) void sample_cuts_kernel(SampleArgs a) {
+    __shared__ CutShared shared;
+    constexpr int kAll = kBins + 1;
+    const int64_t b = blockIdx.x, slice0 = b * a.slices;
+    const int tid = threadIdx.x, lane = tid & 63;
+    uint64_t sum = 0;
+    uint32_t count = 0;
+    if (tid < kAll) {
+#pragma unroll 16
+        for (int i = 0; i < a.slices; ++i) {
+            sum += a.sums[(slice0 + i) * kAll + tid];
+            count += a.counts[(slice0 + i) * kAll + tid];
+        }
+    }
+    const Rules r(a, b, nullptr);   // (no weights here, only their bins)
+    if (r.greedy || r.first == 0) {
+        for (int i = tid; i < a.slices; i += kCutThreads) a.listed[slice0 + i] = 0;
+        if (tid == 0) a.cuts[b].low = INFINITY, a.cuts[b].high = -INFINITY;
+        return;
+    }
+    const Cuts c = find_cuts(r, sum, count, shared);
+    if (tid == 0) a.cuts[b] = c;
+    // sums of the bins that are kept whole, a wave a slice
+    for (int i = tid >> 6; i < a.slices; i += kCutThreads / 64) {
+        uint64_t whole = 0;
+#pragma unroll
+        for (int bin = 0; bin < kAll; bin += 64) {
+            if (bin + lane < min(c.sure(), kAll)) whole += a.sums[(slice0 + i) * kAll + bin + lane];
+        }
+        whole = wave_sum(whole);
+        if (lane == 0) a.whole[slice0 + i] = whole;
+    }
+}
+
+template <int kDtype>
+__global__ __launch_bounds__(kSliceThreads) void sample_list_kernel(SampleArgs a) {
+    __shared__ uint32_t count;
+    const int64_t b = blockIdx.y, slice = b * a.slices + blockIdx.x;
+    const int lo = blockIdx.x * a.length, hi = min(lo + a.length, a.V), tid = threadIdx.x;
+    Tokens<kDtype, kSliceThreads> tokens(a, b, lo, hi);   // (its first loads are under way meanwhile)
+    const Cuts c = a.cuts[b];
+    if (tid == 0) count = 0;
+    __syncthreads();
+    const Weights w{c.most, c.turn, nullptr, 0};
+    if (!(c.low > c.high)) {
         tokens.each([&](int v, uint32_t key) {
             const float x = logit_of(key);   // (a NaN where there is none)
-            if (x < low || x > high || !key || !c.listed(bin_of(r.w.log2_of(key)))) return;
+            if (x < c.low || x > c.high || !key || !c.listed(bin_of(w.log2_of(key)))) return;
             const uint32_t at = atomicAdd(&count, 1u);
             if (at < kListed) a.list[slice * kListed + at] = place_of(key, v);
         });
@@ -518,7 +534,7 @@ __device__ Crossing cross(Shared& s, uint64_t bound) {
     uint64_t mine = 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) mine += s.digits[kDigits - 1 - (tid * kEach + i)];
-    const uint64_t upto = wave_scan(mine, lane);
+    const uint64_t upto = wave_scan(mine);
     __syncthreads();
     if (lane == 63) s.part[tid >> 6] = upto;
     if (tid == 0) s.found[0] = 0, s.found[1] = 0;
@@ -628,8 +644,40 @@ __device__ uint64_t last_of_row(const SampleArgs& a, int64_t b, const Rules& r, 
     return v == 0xffffffffu ? (uint64_t)edge << 32 : place_of(edge, (int)v);
 }
 
-// The same by the listed tokens; their kept weights are added to their slices'
-// sums.
+// The same by up to 64 listed tokens, by one wave; their kept weights are added to their
+// slices' sums.
+__device__ uint64_t last_of_few(const SampleArgs& a, const Rules& r, const Cuts& c, uint64_t* list, int n,
+                                unsigned long long* slice_sums) {
+    const int lane = threadIdx.x & 63;
+    uint64_t place = lane < n ? list[lane] : 0;
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) rank += list[j] > place;
+    // (into the order; the wave's LDS operations are in order)
+    if (lane < n) list[rank] = place;
+    place = lane < n ? list[lane] : 0;
+    const uint32_t key = key_of_place(place);
+    const double z = key ? r.w.log2_of(key) : 0.0;
+    const uint64_t weight = key ? r.w.of_log2(z) : 0;
+    const int bin = key ? bin_of(z) : kBins + 2;
+    const uint64_t number = c.above_k + lane - __popcll(__ballot(bin < c.k));   // (of bin k's)
+    const bool in_k = bin < c.k || (bin == c.k && number < (uint64_t)r.k);
+    bool kept = place && in_k;
+    if (r.p < 1.f) {
+        const uint64_t bound = share_of(r.p, c.sum_k + wave_sum(bin == c.k && in_k ? weight : 0));
+        const bool inside = bin >= c.p_low && bin <= c.p_high;
+        const uint64_t upto = wave_scan(inside ? weight : 0);
+        kept = kept && (bin < c.p_low || (inside && c.above_p + upto - weight < bound));
+    }
+    if (kept && weight >= r.least) {
+        atomicAdd(&slice_sums[token_of_place(place) / a.length], (unsigned long long)weight);
+    }
+    if (c.k > kBins && !(r.p < 1.f)) return 0;   // (min_p alone)
+    const uint64_t all = __ballot(kept);
+    return all ? lane_of(place, 63 - __clzll((long long)all)) : 0;
+}
+
+// The same by the listed tokens of a workgroup.
 __device__ uint64_t last_of_list(const SampleArgs& a, const Rules& r, const Cuts& c, Shared& s, int n,
                                  unsigned long long* slice_sums) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -692,7 +740,7 @@ __device__ uint64_t last_of_list(const SampleArgs& a, const Rules& r, const Cuts
     kept_k = block_sum(s, kept_k);
     const uint64_t bound = r.p < 1.f ? share_of(r.p, c.sum_k + kept_k) : 0;
     // weights of the order before a token, over p_low's bin
-    uint64_t upto = wave_scan(in_p, lane);
+    uint64_t upto = wave_scan(in_p);
     __syncthreads();
     if (lane == 63) s.part[wave] = upto;
     __syncthreads();
@@ -753,8 +801,8 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
     bool known = true;   // slice_sums are those of kept weights
     if (rules) {
         // the listed tokens, one slice's after the other's
-        const uint64_t upto = wave_scan((uint64_t)l0 + l1, lane);
-        const uint64_t listed = __shfl((unsigned long long)upto, 63);
+        const uint64_t upto = wave_scan((uint64_t)l0 + l1);
+        const uint64_t listed = lane_of(upto, 63);
         known = __ballot(l0 > kListed || l1 > kListed) == 0 && listed <= kMostListed;
         if (known && wave == 0) {
             list_at[i0] = (int)(upto - l0 - l1);
@@ -768,7 +816,16 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
                 for (int e = lane; e < count; e += 64) s.list[at + e] = a.list[(slice0 + i) * kListed + e];
             }
             __syncthreads();
-            kept.last = last_of_list(a, r, c, s, (int)listed, slice_sums);
+            if (listed <= 64) {
+                if (wave == 0) {
+                    const uint64_t last = last_of_few(a, r, c, s.list, (int)listed, slice_sums);
+                    if (lane == 0) s.found[0] = last;
+                }
+                __syncthreads();
+                kept.last = s.found[0];
+            } else {
+                kept.last = last_of_list(a, r, c, s, (int)listed, slice_sums);
+            }
         } else {
             kept.last = last_of_row<kDtype>(a, b, r, s);
         }
@@ -786,13 +843,12 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
     }
     // the slice that u falls in: two slices a lane, every wave by itself
     const uint64_t s0 = slice_sums[2 * lane], s1 = slice_sums[2 * lane + 1];
-    const uint64_t sums = wave_scan(s0 + s1, lane), total = __shfl((unsigned long long)sums, 63);
+    const uint64_t sums = wave_scan(s0 + s1), total = lane_of(sums, 63);
     // u of it, rounded down: u in 64 bits of fraction, exact
     const uint64_t fraction = u >= 1.f ? ~0ull : u > 0.f ? (uint64_t)((double)u * 18446744073709551616.0) : 0;
     uint64_t rest = __umul64hi(fraction, total);
     const int pair = __popcll(__ballot(sums <= rest));   // (under 64: rest is under the total)
-    const uint64_t before = __shfl((unsigned long long)(sums - s0 - s1), pair);
-    const uint64_t first = __shfl((unsigned long long)s0, pair);
+    const uint64_t before = lane_of(sums - s0 - s1, pair), first = lane_of(s0, pair);
     rest -= before;
     int part = 2 * pair;
     if (rest >= first) rest -= first, ++part;
@@ -838,7 +894,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
     if (wave != part) return;
 #pragma unroll
     for (int g = 0; g < kAtOnce; ++g) {
-        const uint64_t upto = wave_scan(weights[g], lane), all = __shfl((unsigned long long)upto, 63);
+        const uint64_t upto = wave_scan(weights[g]), all = lane_of(upto, 63);
         if (rest < all) {
             if (upto > rest && upto - weights[g] <= rest) {   // one lane
                 const int v = begin + g * 64 + lane;
@@ -854,14 +910,14 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
     }
 }
 
-// Slices of a row: about 1024 workgroups, each of 2048 to 16384 tokens (more where
-// a row would have over kMostSlices).
+// Slices of a row: up to 16 of at least 4096 tokens (a batch of loads is 8192, and a
+// thread of the cuts reads a bin of 16 slices at once), of at most 16384 while that
+// makes no more than kMostSlices.
 struct Slices {
     int count, length;
 };
-Slices slices_of(int rows, int V) {
-    const int64_t each = ((int64_t)rows * V + 1023) / 1024;
-    int64_t length = std::min<int64_t>(std::max<int64_t>((each + 2047) / 2048 * 2048, 2048), 1 << 14);
+Slices slices_of(int V) {
+    int64_t length = std::min<int64_t>(std::max<int64_t>(((V + 15) / 16 + 2047) / 2048 * 2048, 4096), 1 << 14);
     while (((int64_t)V + length - 1) / length > kMostSlices) length *= 2;
     return {(int)(((int64_t)V + length - 1) / length), (int)length};
 }
@@ -875,7 +931,7 @@ int shift_of(int V) {   // a row's sum stays under 2^63
 }  // namespace
 
 int64_t sample_bytes(int rows, int V) {
-    const int64_t slices = (int64_t)rows * slices_of(rows, V).count;
+    const int64_t slices = (int64_t)rows * slices_of(V).count;
     return rows * (int64_t)sizeof(Cuts) + slices * (8 + 8 + (kBins + 1) * 8 + kListed * 8 + (kBins + 1) * 4 + 4);
 }
 
@@ -883,7 +939,7 @@ int launch_sample(const void* logits, int dtype, int64_t ld, int rows, int V, co
                   const float* temperature, const int32_t* top_k, const float* top_p,
                   const float* min_p, int32_t* tokens, float* logprobs, void* workspace,
                   hipStream_t stream) {
-    const Slices cut = slices_of(rows, V);
+    const Slices cut = slices_of(V);
     const int64_t slices = (int64_t)rows * cut.count;
     SampleArgs a{logits, ld, V, shift_of(V), cut.count, cut.length, u, temperature, top_k, top_p, min_p,
                  tokens, logprobs};
@@ -900,7 +956,10 @@ int launch_sample(const void* logits, int dtype, int64_t ld, int rows, int V, co
         hipLaunchKernelGGL(sample_max_kernel<kDtype>, grid, dim3(kSliceThreads), 0, stream, a);
         auto* bins = a.rules() ? sample_bins_kernel<kDtype, true> : sample_bins_kernel<kDtype, false>;
         hipLaunchKernelGGL(bins, grid, dim3(kSliceThreads), 0, stream, a);
-        if (a.rules()) hipLaunchKernelGGL(sample_list_kernel<kDtype>, grid, dim3(kSliceThreads), 0, stream, a);
+        if (a.rules()) {
+            hipLaunchKernelGGL(sample_cuts_kernel, dim3(rows), dim3(kCutThreads), 0, stream, a);
+            hipLaunchKernelGGL(sample_list_kernel<kDtype>, grid, dim3(kSliceThreads), 0, stream, a);
+        }
         hipLaunchKernelGGL(sample_finish_kernel<kDtype>, dim3(rows), dim3(kThreads), 0, stream, a);
     };
     if (dtype == NB_F32) run(std::integral_constant<int, NB_F32>{});
