@@ -781,6 +781,12 @@ int nb_rmsnorm8(const void* x, int dtype, int64_t ld_x, const void* residual, in
                 void* sum, int64_t ld_sum, const float* weight, float eps, int rows, int width,
                 int8_t* codes, float* scale, void* stream);
 /*
+ * The values code * scale of rows in 8 bits, in out (NB_F32, or rounded to
+ * NB_BF16; stride ld_out).
+ */
+int nb_rows8_values(const int8_t* codes, const float* scale, int rows, int width, void* out,
+                    int out_dtype, int64_t ld_out, void* stream);
+/*
  * A 3-bit / 8-entry / block-128 layer (packed as above, K % 128 == 0, K <=
  * 2^17, N <= 2^24) for nb_linear8, once at load: for output n, a = the largest magnitude
  * among its blocks' entries, scale[n] = a / 127 (fp32 [N]), each entry's code

@@ -119,6 +119,7 @@ SIGNATURES = {
     "nb_sample": (_I, [_P, _I, _L, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _L, _P]),
     "nb_quantize8": (_I, [_P, _I, _L, _I, _I, _P, _P, _P]),
     "nb_rmsnorm8": (_I, [_P, _I, _L, _P, _L, _P, _L, _P, ctypes.c_float, _I, _I, _P, _P, _P]),
+    "nb_rows8_values": (_I, [_P, _P, _I, _I, _P, _I, _L, _P]),
     "nb_linear8_tiles_bytes": (_L, [_I, _I]),
     "nb_linear8_layout": (_I, [_P, _P, _I, _I, _P, _P, _P]),
     "nb_linear8": (_I, [_P, _L, _P, _P, _P, _P, _I, _P, _L, _P, _I, _L, _I, _I, _I, _P]),

@@ -1484,7 +1484,7 @@ int nb_sample(const void* logits, int dtype, int64_t ld, int rows, int V, const 
 // ---------------------------------------------------------------------------
 namespace {
 int check_rows8(const char* fn, const void* x, int dtype, int64_t ld, int rows, int width,
-                const void* codes, const void* scale) {
+                const void* codes, const void* scale) {   // x: the rows in fp32 or bf16
     if (rows < 0 || width < 1) return fail(NB_EINVAL, "%s: rows=%d width=%d", fn, rows, width);
     if (width > 1 << 24) return fail(NB_EUNSUPPORTED, "%s: width=%d (<= 2^24)", fn, width);
     if (rows >= 1 << 22) return fail(NB_EUNSUPPORTED, "%s: rows=%d (< 2^22)", fn, rows);
@@ -1547,6 +1547,17 @@ int nb_rmsnorm8(const void* x, int dtype, int64_t ld_x, const void* residual, in
     if (st) return st;
     return launch_rmsnorm8(x, dtype, ld_x, residual, ld_residual, sum, ld_sum, weight, eps, rows,
                            width, codes, scale, static_cast<hipStream_t>(stream));
+}
+
+int nb_rows8_values(const int8_t* codes, const float* scale, int rows, int width, void* out,
+                    int out_dtype, int64_t ld_out, void* stream) {
+    const char* fn = "nb_rows8_values";
+    int st = check_rows8(fn, out, out_dtype, ld_out, rows, width, codes, scale);
+    if (st || rows == 0) return st;
+    st = ensure_device();
+    if (st) return st;
+    return launch_rows8_values(codes, scale, rows, width, out, out_dtype, ld_out,
+                               static_cast<hipStream_t>(stream));
 }
 
 int64_t nb_linear8_tiles_bytes(int N, int K) {

@@ -264,6 +264,8 @@ int launch_quantize8(const void* x, int dtype, int64_t ld_x, int rows, int width
 int launch_rmsnorm8(const void* x, int dtype, int64_t ld_x, const void* residual,
                     int64_t ld_residual, void* sum, int64_t ld_sum, const float* weight, float eps,
                     int rows, int width, int8_t* codes, float* scale, hipStream_t stream);
+int launch_rows8_values(const int8_t* codes, const float* scale, int rows, int width, void* out,
+                        int dtype, int64_t ld, hipStream_t stream);
 // nb_linear8.hip
 int64_t linear8_tiles_bytes(int N, int K);
 int launch_linear8_layout(const uint8_t* packed, const float* codebook, int N, int K,

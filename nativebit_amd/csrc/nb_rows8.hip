@@ -1,4 +1,5 @@
-// Rows in 8 bits with one scale each (gfx950): nb_quantize8, nb_rmsnorm8.
+// Rows in 8 bits with one scale each (gfx950): nb_quantize8, nb_rmsnorm8, and the
+// values they stand for: nb_rows8_values.
 //
 // For a row v of `width` values, a = max |v|:
 //     code  = rint(v * (127 / a)),  scale = a / 127            (0 where a = 0)
@@ -218,7 +219,60 @@ void launch(const RowsArgs& a, int rows, hipStream_t stream) {
     return run(integral_constant<int, 512>{}, integral_constant<int, 4>{});
 }
 
+// The values of a row's codes, four a thread at once.
+template <int kDtype, int kThreads>
+__global__ __launch_bounds__(kThreads) void rows8_values_kernel(const int8_t* codes, const float* scale,
+                                                                int width, void* out, int64_t ld) {
+    constexpr int kGroups = 4;
+    const int64_t b = blockIdx.y;
+    const int first = blockIdx.x * kThreads * 4 * kGroups + 4 * (int)threadIdx.x;
+    const int8_t* row = codes + b * width;
+    char* to = static_cast<char*>(out) + b * ld * (kDtype == NB_F32 ? 4 : 2);
+    const float s = as_constant(scale)[b];
+    uint32_t c[kGroups];
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+        const int i = first + g * 4 * kThreads;
+        c[g] = 0;
+        if (i + 3 < width) {
+            c[g] = *reinterpret_cast<const u1_any*>(row + i);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (i + e < width) c[g] |= (uint32_t)(uint8_t)row[i + e] << (8 * e);
+            }
+        }
+    }
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+        const int i = first + g * 4 * kThreads;
+        if (i >= width) break;
+        f4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[e] = (float)(int8_t)(c[g] >> (8 * e)) * s;
+            if constexpr (kDtype == NB_BF16) v[e] = round_bf16(v[e]);
+        }
+        store4<kDtype>(to, i, width, v);
+    }
+}
+
 }  // namespace
+
+int launch_rows8_values(const int8_t* codes, const float* scale, int rows, int width, void* out,
+                        int dtype, int64_t ld, hipStream_t stream) {
+    const bool narrow = width <= 1024;
+    const int threads = narrow ? 64 : 256, columns = (width + threads * 16 - 1) / (threads * 16);
+    auto* kernel = dtype == NB_F32
+                       ? (narrow ? rows8_values_kernel<NB_F32, 64> : rows8_values_kernel<NB_F32, 256>)
+                       : (narrow ? rows8_values_kernel<NB_BF16, 64> : rows8_values_kernel<NB_BF16, 256>);
+    for (int row = 0; row < rows; row += 65535) {   // (a grid's second dimension)
+        const int n = std::min(rows - row, 65535);
+        hipLaunchKernelGGL(kernel, dim3(columns, n), dim3(threads), 0, stream, codes + (int64_t)row * width,
+                           scale + row, width, static_cast<char*>(out) + row * ld * (dtype == NB_F32 ? 4 : 2), ld);
+    }
+    return check_launch("nb_rows8_values");
+}
 
 int launch_quantize8(const void* x, int dtype, int64_t ld_x, int rows, int width, int8_t* codes,
                      float* scale, hipStream_t stream) {

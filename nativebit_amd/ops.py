@@ -1003,9 +1003,30 @@ class Rows8(NamedTuple):
     codes: torch.Tensor
     scale: torch.Tensor
 
-    def values(self) -> torch.Tensor:
-        """The float32 values that they stand for."""
-        return self.codes * self.scale[:, None]
+    def values(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values that they stand for, float32 or rounded to bfloat16
+        (nb_rows8_values)."""
+        codes, scale = self
+        _require_cuda("codes", codes)
+        dev = codes.get_device()
+        if not _here(dev):
+            with torch.cuda.device(dev):
+                return self.values(dtype)
+        if dtype not in _DT:
+            raise TypeError(f"dtype {dtype} not supported (float32 or bfloat16)")
+        if codes.dim() != 2 or not _is(codes, torch.int8, codes.shape, dev) or \
+                not _is(scale, torch.float32, codes.shape[:1], dev):
+            _require("codes", codes, torch.int8, (None, None), dev)
+            _require("scale", scale, torch.float32, codes.shape[:1], dev)
+        rows, width = codes.shape
+        out = torch.empty((rows, width), dtype=dtype, device=codes.device)
+        if rows and width:
+            status = _lib.load().nb_rows8_values(
+                codes.data_ptr(), scale.data_ptr(), rows, width, out.data_ptr(), _DT[dtype], width,
+                torch._C._cuda_getCurrentRawStream(dev))
+            if status:
+                _lib.check(status)
+        return out
 
 
 class Weights8(NamedTuple):

@@ -48,8 +48,9 @@ def test_quantize8(dev, n, width, dtype):
         got = ops.quantize8(xd)
         check(got, q, scale)
         assert np.array_equal(got.scale.cpu().numpy(), scale)   # (a / 127 rounds once)
-        assert torch.equal(got.values().cpu(), torch.from_numpy(q.astype(np.float32)) *
-                           torch.from_numpy(scale)[:, None])
+        values = torch.from_numpy(q.astype(np.float32)) * torch.from_numpy(scale)[:, None]
+        assert torch.equal(got.values().cpu(), values)
+        assert torch.equal(got.values(torch.bfloat16).cpu(), values.to(torch.bfloat16))
 
 
 @pytest.mark.parametrize("dtype", DT)

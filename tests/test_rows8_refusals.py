@@ -43,6 +43,18 @@ def test_nothing_to_do():
     assert call("nb_sample", SAMPLE, dict(rows=0)) == 0
 
 
+VALUES = dict(codes=P, scale=P, rows=4, width=300, out=P, dtype=F32, ld=300, stream=None)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(rows=-1), EINVAL), (dict(width=0), EINVAL), (dict(out=None), EINVAL), (dict(codes=None), EINVAL),
+    (dict(scale=None), EINVAL), (dict(ld=299), EINVAL), (dict(dtype=2), EINVAL), (dict(out=P + 2), EALIGN),
+    (dict(scale=P + 1), EALIGN), (dict(rows=1 << 22), EUNSUP),
+])
+def test_values_refuse(kw, status):
+    assert call("nb_rows8_values", VALUES, kw) == status and _lib.last_error()
+
+
 NORM = dict(x=P, dtype=F32, ld_x=300, residual=P + (1 << 20), ld_residual=300, sum=P + (2 << 20),
             ld_sum=300, weight=P, eps=1e-6, rows=4, width=300, codes=P, scale=P, stream=None)
 
@@ -130,7 +142,8 @@ def test_sample_refuses(kw, status):
 def test_wrappers_refuse_host_tensors():
     x = torch.zeros(2, 128)
     w = ops.Weights8(torch.zeros(896, dtype=torch.uint8), torch.zeros(16), 16, 128)
-    for f in (lambda: ops.quantize8(x), lambda: ops.rmsnorm8(x, torch.ones(128)),
+    for f in (lambda: ops.quantize8(x), lambda: ops.Rows8(x.to(torch.int8), torch.ones(2)).values(),
+              lambda: ops.rmsnorm8(x, torch.ones(128)),
               lambda: ops.linear8(ops.Rows8(x.to(torch.int8), torch.ones(2)), w),
               lambda: ops.linear8_layout(torch.zeros(768, dtype=torch.uint8), torch.zeros(16, 8), 16, 128),
               lambda: ops.sample(x, torch.zeros(2))):
