@@ -15,8 +15,8 @@
 // A row is cut into slices, one workgroup each:
 //   1. sample_max_kernel     each slice's first token of the order
 //   2. sample_bins_kernel    each slice's weights, summed and counted in bins of an
-//                            eighth of an octave of w (257: the last holds all
-//                            under 2^-32); without rules one sum
+//                            eighth of an octave of w, down to 2^-46 where it rounds
+//                            to 0; without rules one sum
 //   3. sample_cuts_kernel    (with rules) a row's bins say where the rules cut
 //   4. sample_list_kernel    (with rules) each slice's tokens of the bins that they cut
 //                            through are listed
@@ -39,7 +39,7 @@ namespace {
 typedef __attribute__((ext_vector_type(4), aligned(4))) float f4_any;
 typedef __attribute__((ext_vector_type(2), aligned(2))) uint32_t u2_any;
 
-constexpr int kBins = 256;          // of an eighth of an octave; one more below them
+constexpr int kBins = 368;          // of an eighth of an octave: 46 octaves; one more below
 constexpr int kListed = 2048;       // listed tokens of a slice
 constexpr int kMostListed = 4096;   // and of a row (a power of two)
 constexpr int kSliceThreads = 512;
@@ -397,7 +397,7 @@ __device__ Cuts find_cuts(const Rules& r, uint64_t sum, uint32_t count, CutShare
     }
     __syncthreads();
     Cuts c;
-    c.k = s.found[0];
+    c.k = s.found[0] == kBins ? kNone : s.found[0];   // (a cut among weights of 0 changes nothing)
     c.above_k = s.before[c.k], c.sum_k = s.above[c.k];
     if (r.p < 1.f && tid < kAll) {
         const uint64_t low = share_of(r.p, max(s.above[c.k], (uint64_t)1));
