@@ -8,7 +8,7 @@ libnativebit_amd.so behind a C ABI (include/nativebit_amd.h).
     layer = PackedLinear.from_packed(indices_np, codebook_np, (out, in), "cuda")
     y = layer(x)            # x (..., in) float32/bfloat16 on the GPU -> float32
 """
-from .linear import BS, NE, PackedLinear  # noqa: F401
+from .linear import BS, NE, PackedLinear, PackedLinear8  # noqa: F401
 from ._lib import NativeBitError  # noqa: F401
 
-__all__ = ["PackedLinear", "NativeBitError", "BS", "NE"]
+__all__ = ["PackedLinear", "PackedLinear8", "NativeBitError", "BS", "NE"]

@@ -193,12 +193,14 @@ struct Finished {
                                      (a.N - n) * kCount / 4, v);
         }
     }
-    // xs: the row's scale; kResidual: v holds the residual
+    // xs: the row's scale; kResidual: v holds the residual.  Which products and sums
+    // are one step is written out: a row's outputs are the same in every form.
     template <bool kResidual>
     __device__ __forceinline__ void finish(const Column& c, float xs, i4 sum) {
+#pragma clang fp contract(off)
         float y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = (float)sum[e] * (xs * c.scale[e]) + c.bias[e];
+        for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf((float)sum[e], xs * c.scale[e], c.bias[e]);
 #pragma unroll
         for (int e = 0; e < kCount; ++e) {
             float out = y[e];

@@ -31,7 +31,7 @@ import time
 import torch
 
 from . import _lib, ops
-from .model import PackedGPT, precompute_rope
+from .model import PackedGPT, _packed_blocks, precompute_rope
 
 
 def _ptr(t):
@@ -74,6 +74,7 @@ class _DecoderBase:
         dev = model.embedding.weight.device
         if dev.type != "cuda":
             raise ValueError(f"{type(self).__name__} runs on a ROCm GPU")
+        _packed_blocks(model)
         self.model, self.cfg, self.dev = model, cfg, dev
         C, F, H = cfg.n_embd, cfg.ffn_hidden, cfg.n_head
         D = C // H

@@ -141,3 +141,69 @@ class PackedLinear(torch.nn.Module):
     def extra_repr(self) -> str:
         return (f"in_features={self.in_features}, out_features={self.out_features}, "
                 f"bits={self.bits}, n_entries={self.n_entries}, block_size={self.block_size}")
+
+
+def check_rows8(layer) -> None:
+    """Raises for a layer that PackedLinear8 does not take."""
+    if not isinstance(layer, PackedLinear) or not layer._standard():
+        raise ValueError("rows in 8 bits are for PackedLinear layers of 3 bits, 8 entries and blocks "
+                         f"of 128 along whole rows, got {layer}")
+
+
+class PackedLinear8(torch.nn.Module):
+    """y = x @ W.T with x in 8 bits (one scale a row) and the packed layer's
+    codebooks in 8 bits (one scale an output): whole-number products and sums,
+    then bias, activation and residual in fp32 (ops.linear8).  ``x`` is an
+    ops.Rows8, whose rows' outputs come as (rows, outputs), or float32 /
+    bfloat16 with any leading dimensions, quantized row by row.
+
+    No counterpart in the reference: its layers multiply fp32 or bf16
+    activations with the fp32 or bf16 entries (triton_kernel.py:240-275)."""
+
+    def __init__(self, weights: ops.Weights8, bias: torch.Tensor | None = None):
+        super().__init__()
+        self.register_buffer("tiles", weights.tiles)
+        self.register_buffer("scale", weights.scale)
+        self.register_buffer("bias", bias)
+        self.out_features, self.in_features = int(weights.N), int(weights.K)
+
+    @staticmethod
+    def from_packed_linear(layer: PackedLinear, bias: torch.Tensor | None = None) -> "PackedLinear8":
+        """The layer with its codebooks in 8 bits (3 bits, 8 entries, blocks of 128
+        along whole rows)."""
+        check_rows8(layer)
+        N, K = layer.out_features, layer.in_features
+        return PackedLinear8(ops.linear8_layout(layer.packed_indices, layer.codebook, N, K), bias)
+
+    @staticmethod
+    def from_pairs(gate: PackedLinear, up: PackedLinear) -> "PackedLinear8":
+        """One layer whose outputs 2 i and 2 i + 1 are gate's and up's output i, as
+        the activation "swiglu" takes them."""
+        for layer in (gate, up):
+            check_rows8(layer)
+        N, K = gate.out_features, gate.in_features
+        if (up.out_features, up.in_features) != (N, K):
+            raise ValueError(f"gate {N}x{K}, up {up.out_features}x{up.in_features}")
+        blocks = K // BS
+        packed = torch.stack([layer.packed_indices[:N * blocks * 48].view(N, blocks * 48)
+                              for layer in (gate, up)], dim=1)
+        codebook = torch.stack([layer.codebook.view(N, blocks * NE) for layer in (gate, up)], dim=1)
+        return PackedLinear8(ops.linear8_layout(packed.view(-1), codebook.view(-1, NE), 2 * N, K))
+
+    def forward(self, x, *, activation: str | None = None, residual: torch.Tensor | None = None,
+                out_dtype: torch.dtype | None = None) -> torch.Tensor:
+        shape = None
+        if not isinstance(x, ops.Rows8):
+            if x.dim() == 0 or x.shape[-1] != self.in_features:
+                raise ValueError(f"x last dim must be {self.in_features}, got {tuple(x.shape)}")
+            shape = x.shape[:-1]
+            x = ops.quantize8(x.reshape(-1, self.in_features))
+        weights = ops.Weights8(self.tiles, self.scale, self.out_features, self.in_features)
+        if residual is not None and shape is not None:
+            residual = residual.reshape(-1, residual.shape[-1])
+        y = ops.linear8(x, weights, bias=self.bias, activation=activation, residual=residual,
+                        out_dtype=out_dtype)
+        return y if shape is None else y.view(*shape, y.shape[1])
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}"

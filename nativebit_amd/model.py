@@ -19,7 +19,8 @@ PackedLinear (fused dequant-GEMV for up to 16 rows, the packed MFMA kernels or
 a device gather + dense GEMM beyond), the norms nb_rmsnorm_rows (the residual
 add fused into the second norm of a block), RoPE and the cache appends
 nb_rope_kv_batch, attention nb_attention_batch, the SwiGLU product
-nb_silu_mul_rows.  Activations stay fp32 (the reference's module numerics);
+nb_silu_mul_rows.  Activations stay fp32 (the reference's module numerics;
+``quantize_activations`` takes them through the layers in 8 bits);
 ``nativebit_amd.decode.DecodeEngine`` runs the same model with bf16 GEMV
 inputs, one HIP graph per token, for speed.
 
@@ -42,8 +43,8 @@ import numpy as np
 import torch
 import torch.nn as nn
 
-from . import _lib, formats, synth
-from .linear import PackedLinear
+from . import _lib, formats, ops, synth
+from .linear import PackedLinear, PackedLinear8, check_rows8
 from .ops import _stream
 from .paged import PagedCache, PagedLayer
 
@@ -197,15 +198,23 @@ class CausalAttention(nn.Module):
 
     def forward(self, x, kv_cache=None, pos_offset=0):
         B, T, C = x.shape
-        H, D = self.n_head, self.head_dim
-        dev = x.device
         qkv = _f32(self.qkv(x))
         if qkv.shape != (B, T, 3 * C):
             qkv = qkv.reshape(B, T, 3 * C)
+        att, cache = self.attend(qkv, kv_cache, pos_offset)
+        return self.out_proj(att), cache
+
+    def attend(self, qkv, kv_cache=None, pos_offset=0):
+        """Attention of the rows q | k | v (B, T, 3 n_embd) float32, without the
+        projections: (B, T, n_embd) float32 and the cache."""
+        B, T, C = qkv.shape
+        C //= 3
+        H, D = self.n_head, self.head_dim
+        dev = qkv.device
         cos, sin = _f32(self.cos.to(dev)), _f32(self.sin.to(dev))
         if isinstance(kv_cache, PagedLayer):
             att = kv_cache.attend(qkv.view(B * T, 3 * C), cos, sin, H)
-            return self.out_proj(att.view(B, T, C)), kv_cache
+            return att.view(B, T, C), kv_cache
         if kv_cache is not None:
             k_buf, v_buf, pos0 = kv_cache
             pos0 = int(pos0)
@@ -233,14 +242,13 @@ class CausalAttention(nn.Module):
                                         _p(q), B, H, D, ctx, s))
         _lib.check(lib.nb_attention_batch(_p(q), _p(kt), _p(vt), pos0, T, _p(att), _lib.NB_F32, B,
                                           H, D, ctx, s))
-        out = self.out_proj(att)
         if kv_cache is None:
-            return out, None
+            return att, None
         if k_copy:
             k_buf[:, :, pos0:pos0 + T] = kt[..., pos0:pos0 + T].transpose(-1, -2)
         if v_copy:
             v_buf[:, :, pos0:pos0 + T] = vt[:, :, pos0:pos0 + T]
-        return out, (k_buf, v_buf, pos0 + T)
+        return att, (k_buf, v_buf, pos0 + T)
 
 
 class SwiGLU(nn.Module):
@@ -293,6 +301,33 @@ class TransformerBlock(nn.Module):
         res = res.reshape(x.shape).to(x1_dtype)
         f = self.ffn(h.reshape(x.shape).to(x1_dtype))
         return res + f, new_cache
+
+
+class TransformerBlock8(nn.Module):
+    """A TransformerBlock with its activations in 8 bits (one scale a row) and
+    its layers' codebooks in 8 bits (one scale an output): the norms' outputs leave
+    them in 8 bits (nb_rmsnorm8), the attention's and the gated products are
+    quantized (nb_quantize8); the projections add to the stream in their
+    epilogue, gate and up are one layer with the gated product in its
+    (nb_linear8).  The stream, attention and its cache are what they were."""
+
+    def __init__(self, block: TransformerBlock):
+        super().__init__()
+        self.ln1, self.ln2, self.attn = block.ln1, block.ln2, block.attn
+        self.attn.qkv = PackedLinear8.from_packed_linear(block.attn.qkv)
+        self.attn.out_proj = PackedLinear8.from_packed_linear(block.attn.out_proj)
+        self.gate_up = PackedLinear8.from_pairs(block.ffn.gate, block.ffn.up)
+        self.down = PackedLinear8.from_packed_linear(block.ffn.down)
+
+    def forward(self, x, kv_cache=None, pos_offset=0):
+        B, T, C = x.shape
+        rows = _f32(x).reshape(-1, C)
+        h = ops.rmsnorm8(rows, _f32(self.ln1.weight.detach()), float(self.ln1.eps))
+        att, new_cache = self.attn.attend(self.attn.qkv(h).view(B, T, -1), kv_cache, pos_offset)
+        rows = self.attn.out_proj(ops.quantize8(att.view(-1, C)), residual=rows)
+        h = ops.rmsnorm8(rows, _f32(self.ln2.weight.detach()), float(self.ln2.eps))
+        gated = self.gate_up(h, activation="swiglu")
+        return self.down(ops.quantize8(gated), residual=rows).view(B, T, C), new_cache
 
 
 class PackedGPT(nn.Module):
@@ -368,6 +403,20 @@ class PackedGPT(nn.Module):
         if isinstance(kv_caches, PagedCache):
             return logits, kv_caches
         return (logits, caches) if kv_caches is not None else logits
+
+
+def quantize_activations(model: PackedGPT) -> PackedGPT:
+    """The model with every block in 8 bits (TransformerBlock8), changed in place and
+    returned.  Its layers are PackedLinear of 3 bits, 8 entries and blocks of
+    128; the packed streams are replaced by the layout that the products
+    read, so DecodeEngine and to_nbpack_params take a model before it."""
+    for block in model.blocks:      # (all before the first is changed)
+        if not isinstance(block, TransformerBlock8):
+            for layer in (block.attn.qkv, block.attn.out_proj, block.ffn.gate, block.ffn.up, block.ffn.down):
+                check_rows8(layer)
+    model.blocks = nn.ModuleList([block if isinstance(block, TransformerBlock8) else
+                                  TransformerBlock8(block) for block in model.blocks])
+    return model
 
 
 def init_kv_cache(model: PackedGPT, batch_size=1, device="cuda", dtype=torch.float32):
@@ -510,10 +559,18 @@ def random_packed_model(cfg, seed: int = 0, device="cuda",
     return model
 
 
+def _packed_blocks(model: PackedGPT) -> None:
+    """Raises where the packed streams are gone."""
+    if any(isinstance(block, TransformerBlock8) for block in model.blocks):
+        raise ValueError("the model's blocks are in 8 bits (quantize_activations): their packed "
+                         "streams are gone")
+
+
 def to_nbpack_params(model: PackedGPT) -> dict:
     """The model as .nbpack.npz contents (key -> array), in the layout
     load_packed_model reads; used to round-trip a model through a file."""
     out = {}
+    _packed_blocks(model)
     for i, blk in enumerate(model.blocks):
         lin = [blk.attn.qkv, blk.attn.out_proj, blk.ffn.gate, blk.ffn.up, blk.ffn.down]
         names = ["CausalSelfAttention_0.NativeBitDense_0", "CausalSelfAttention_0.NativeBitDense_1",

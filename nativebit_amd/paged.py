@@ -186,25 +186,31 @@ class PagedCache:
         return keys.transpose(0, 1), values.transpose(0, 1)
 
 
-def _per_request(x, n, device):
-    """A number for all requests, or one for each, as a float32 tensor."""
+def _per_request(x, n, device, dtype=torch.float32):
+    """A number for all requests, or one for each, as a tensor."""
     if x is None:
         return None
-    t = torch.as_tensor(x, dtype=torch.float32)
+    t = torch.as_tensor(x, dtype=dtype)
     return (t.expand(n) if t.dim() == 0 else t).contiguous().to(device)
 
 
 @torch.no_grad()
 def generate(model, prompts, n_generate: int, *, repetition=None, frequency=None, presence=None,
-             bias=None, mask=None, cache: PagedCache | None = None):
-    """Greedy continuations of several prompts at once, ``n_generate`` tokens
-    each: the prompts as one ragged pass, then one token of every request a
-    step, chosen by ops.logits_rules.  ``repetition``, ``frequency`` and
+             bias=None, mask=None, cache: PagedCache | None = None, temperature=None, top_k=None,
+             top_p=None, min_p=None, u=None, generator: torch.Generator | None = None):
+    """Continuations of several prompts at once, ``n_generate`` tokens each:
+    the prompts as one ragged pass, then one token of every request a step,
+    chosen by ops.logits_rules.  ``repetition``, ``frequency`` and
     ``presence``: a number or one for each request; ``bias``: a dict token ->
     bias for each request; ``mask``: int32 (requests, vocabulary / 32) bit
     masks of the allowed tokens.  A request whose mask and biases leave no
     token gets -1 (fed as token 0).  ``cache``: an empty cache to use, with room
-    for all requests to their ends; they stay in it."""
+    for all requests to their ends; they stay in it.
+
+    With a ``temperature`` the tokens are drawn instead of the largest taken
+    (ops.sample, after those rules); it, ``top_k``, ``top_p`` and ``min_p`` are a
+    number or one for each request.  The numbers drawn by are ``u`` (requests,
+    n_generate) in [0, 1), or torch's, of ``generator``."""
     prompts = [[int(t) for t in p] for p in prompts]
     n = len(prompts)
     if not n or not all(prompts) or n_generate < 0:
@@ -217,6 +223,21 @@ def generate(model, prompts, n_generate: int, *, repetition=None, frequency=None
     room = model.context_len if cache is None else cache.max_len
     if max(lengths) + n_generate - 1 > room:     # (the last token is not fed)
         raise ValueError(f"{max(lengths)} prompt tokens and {n_generate} more exceed {room}")
+    if temperature is None and not (top_k is None and top_p is None and min_p is None and
+                                    u is None and generator is None):
+        raise ValueError("top_k, top_p, min_p, u and generator draw tokens: they need a temperature")
+    if u is not None and generator is not None:
+        raise ValueError("tokens are drawn by u or by a generator's numbers")
+    if u is not None:
+        u = torch.as_tensor(u, dtype=torch.float32)
+        if u.shape != (n, n_generate):
+            raise ValueError(f"u must be ({n}, {n_generate}), got {tuple(u.shape)}")
+    draws = {"temperature": _per_request(temperature, n, dev),
+             "top_k": _per_request(top_k, n, dev, torch.int32),
+             "top_p": _per_request(top_p, n, dev), "min_p": _per_request(min_p, n, dev)}
+    for name, t in draws.items():
+        if t is not None and t.shape != (n,):
+            raise ValueError(f"{name} must be a number or {n} of them, got {tuple(t.shape)}")
     if bias is not None and len(bias) != n:
         raise ValueError(f"{len(bias)} bias dicts for {n} prompts")
     if cache is not None and bool(cache.lens.any()):
@@ -245,6 +266,9 @@ def generate(model, prompts, n_generate: int, *, repetition=None, frequency=None
                                          dtype=torch.int32, device=dev).view(n, most)
         rules["bias"] = torch.tensor([list(b.values()) + [0.0] * (most - len(b)) for b in bias],
                                      dtype=torch.float32, device=dev).view(n, most)
+    if temperature is not None:
+        u = torch.rand(n_generate, n, generator=generator, device=dev) if u is None else \
+            u.to(dev).t().contiguous()
     idx = torch.tensor([sum(prompts, [])], device=dev)
     rows = torch.tensor(lengths, device=dev).cumsum(0) - 1     # of the requests' last tokens
     cache.step(lengths)
@@ -252,7 +276,11 @@ def generate(model, prompts, n_generate: int, *, repetition=None, frequency=None
     for i in range(n_generate):
         hidden, _ = model.hidden(idx, cache)
         logits = model.head(hidden[0, rows])
-        _, tokens = ops.logits_rules(logits.contiguous(), out=logits, choose=True, **rules)
+        if temperature is None:
+            _, tokens = ops.logits_rules(logits.contiguous(), out=logits, choose=True, **rules)
+        else:
+            logits = ops.logits_rules(logits.contiguous(), out=logits, **rules)
+            tokens = ops.sample(logits, u[i], **draws)
         out.append(tokens)
         if i + 1 == n_generate:
             break
