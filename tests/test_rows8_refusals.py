@@ -17,9 +17,8 @@ def call(fn, base, kw):
     return getattr(_lib.load(), fn)(*{**base, **kw}.values())
 
 
-def here(status):
-    """The status of arguments that are fine: the launch needs a GPU."""
-    return status == _lib.NB_ENODEV if not gpu_available() else True
+# Arguments that are taken end at the missing device; with one they would be launched.
+no_gpu = pytest.mark.skipif(gpu_available(), reason="made-up addresses would reach a kernel")
 
 
 QUANTIZE = dict(x=P, dtype=F32, ld=300, rows=4, width=300, codes=P, scale=P, stream=None)
@@ -71,9 +70,10 @@ def test_norm_refuses(kw, status):
     assert call("nb_rmsnorm8", NORM, kw) == status and _lib.last_error()
 
 
+@no_gpu
 def test_norm_in_place_is_taken():
     for kw in (dict(sum=P), dict(sum=P + (1 << 20)), dict(sum=None), dict(residual=None, sum=None)):
-        assert here(call("nb_rmsnorm8", NORM, kw))
+        assert call("nb_rmsnorm8", NORM, kw) == _lib.NB_ENODEV
 
 
 LAYOUT = dict(packed=P, codebook=P, N=40, K=256, tiles=P, scale=P, stream=None)
@@ -117,10 +117,11 @@ def test_linear_refuses(kw, status):
     assert call("nb_linear8", LINEAR, kw) == status and _lib.last_error()
 
 
+@no_gpu
 def test_linear_takes():
     for kw in (dict(y=P + (1 << 20)), dict(bias=None, residual=None), dict(activation=3, ld_y=20),
                dict(activation=3, N=40, ld_y=20, ld_residual=20)):
-        assert here(call("nb_linear8", LINEAR, kw))
+        assert call("nb_linear8", LINEAR, kw) == _lib.NB_ENODEV
 
 
 SAMPLE = dict(logits=P, dtype=F32, ld=100, rows=3, V=100, u=P, temperature=P, top_k=P, top_p=P, min_p=P,
