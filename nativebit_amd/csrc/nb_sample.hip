@@ -13,16 +13,21 @@
 // them is a 64-bit integer, the same in any order.
 //
 // A row is cut into slices, one workgroup each:
-//   1. sample_max_kernel     each slice's first token of the order
+//   1. sample_max_kernel     each slice's first token of the order, and (with rules)
+//                            the largest logit of every group of 32 tokens
 //   2. sample_bins_kernel    each slice's weights, summed and counted in bins of an
 //                            eighth of an octave of w, down to 2^-46 where it rounds
 //                            to 0; without rules one sum
 //   3. sample_cuts_kernel    (with rules) a row's bins say where the rules cut
 //   4. sample_list_kernel    (with rules) each slice's tokens of the bins that they cut
-//                            through are listed
+//                            through are listed, of the groups that reach them
 //   5. sample_finish_kernel  one workgroup a row: the listed tokens, sorted, give
 //                            the cuts; bins and list each slice's sum of kept
 //                            weights, u the slice, the slice read again the token
+// A row whose top_k is small (few_kept) skips 2 to 4: the k-th largest of its groups'
+// largest logits is a logit that k tokens reach, so what it keeps is among the
+// tokens that reach it, and those are in the groups that do; k of them, but for
+// ties.  The last kernel lists them, and that is all it reads again of the row.
 // A row with over kMostListed listed tokens (equal logits, mostly) is worked out by
 // its last workgroup alone: radix selection over the row.
 #include <math.h>
@@ -44,6 +49,8 @@ constexpr int kListed = 2048;       // listed tokens of a slice
 constexpr int kMostListed = 4096;   // and of a row (a power of two)
 constexpr int kSliceThreads = 512;
 constexpr int kMostSlices = 128;
+constexpr int kFewKept = 2048;
+constexpr int kGroup = 32;          // 128 bytes of fp32 logits
 
 struct SampleArgs {
     const void* logits;
@@ -57,6 +64,7 @@ struct SampleArgs {
     float* logprobs;
     // workspace, for each row and slice
     uint64_t* first;       // the slice's first token of the order (place_of)
+    uint32_t* groups;      // of a row, with rules: the largest key of every kGroup tokens
     uint64_t* sums;        // [kBins + 1] with rules, else one
     uint32_t* counts;      // [kBins + 1]
     uint32_t* listed;      // how many are listed (more than kListed: not all are)
@@ -64,6 +72,14 @@ struct SampleArgs {
     uint64_t* whole;       // the sum of the bins that are kept whole
     struct Cuts* cuts;     // of a row
     __host__ __device__ __forceinline__ bool rules() const { return top_k || top_p || min_p; }
+    __host__ __device__ __forceinline__ int groups_of_row() const { return (V + kGroup - 1) / kGroup; }
+    // A row whose kept tokens are in few groups: its bins are not needed.  48 rows of
+    // 50257 (1571 groups) with k = 50, 500, 1024, 1177, 1300, 1500: 23, 31, 38, 41, 45 and
+    // 84 us so, 38, 46, 49, 48, 49 and 49 us by bins; 160 rows of 131077 with 2048: 77, 122.
+    __device__ __forceinline__ bool few_kept(int64_t b) const {
+        const int64_t k = top_k ? as_constant(top_k)[b] : 0;
+        return k > 0 && k <= kFewKept && k <= groups_of_row() * 3ll / 4;
+    }
 };
 
 // Larger for larger logits; 0 for -inf and NaN.
@@ -132,25 +148,35 @@ struct Tokens {
             }
         }
     }
-    // f(token, key), once
+    // f(token, keys of four from it on), once; lanes of a wave stay together
     template <typename F>
-    __device__ __forceinline__ void each(F f) {
-        for (; v0 < hi; v0 += kStep) {
+    __device__ __forceinline__ void each_four(F f) {
+        for (; (v0 & ~255) < hi; v0 += kStep) {
             Four now[kBatch];
 #pragma unroll
             for (int j = 0; j < kBatch; ++j) now[j] = x[j];
-            if (v0 + kStep < hi) load(v0 + kStep);
+            if (((v0 + kStep) & ~255) < hi) load(v0 + kStep);
 #pragma unroll
             for (int j = 0; j < kBatch; ++j) {
+                uint32_t keys[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float y;
                     if constexpr (kDtype == NB_F32) y = now[j][e];
                     else y = __uint_as_float(e & 1 ? now[j][e / 2] & 0xffff0000u : now[j][e / 2] << 16);
-                    f(v0 + j * 4 * kThreads + e, key_of(y));
+                    keys[e] = key_of(y);
                 }
+                f(v0 + j * 4 * kThreads, keys);
             }
         }
+    }
+    // f(token, key), once (0 past the last)
+    template <typename F>
+    __device__ __forceinline__ void each(F f) {
+        each_four([&](int v, const uint32_t* keys) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f(v + e, keys[e]);
+        });
     }
 };
 template <int kDtype, int kThreads, typename F>
@@ -199,6 +225,10 @@ __device__ __forceinline__ uint64_t dpp64(uint64_t v) {   // 0 where no lane is 
     const int lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, kCtrl, kRows, 0xf, true);
     const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), kCtrl, kRows, 0xf, true);
     return (uint64_t)(uint32_t)hi << 32 | (uint32_t)lo;
+}
+template <int kCtrl>
+__device__ __forceinline__ uint32_t dpp32(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, 0xf, 0xf, true);
 }
 template <typename Join>
 __device__ __forceinline__ uint64_t wave_scan(uint64_t v, Join join) {   // of lanes 0 .. this one
@@ -266,15 +296,26 @@ __device__ __forceinline__ void make_table(double* table) {
 // ---------------------------------------------------------------------------
 // slices
 // ---------------------------------------------------------------------------
-template <int kDtype>
+template <int kDtype, bool kRules>
 __global__ __launch_bounds__(kSliceThreads) void sample_max_kernel(SampleArgs a) {
     __shared__ uint64_t part[kSliceThreads / 64];
     const int64_t b = blockIdx.y;
     const int lo = blockIdx.x * a.length, hi = min(lo + a.length, a.V), tid = threadIdx.x;
     uint64_t first = 0;
-    for_tokens<kDtype, kSliceThreads>(a, b, lo, hi, [&](int v, uint32_t key) {
-        const uint64_t place = place_of(key, v);
-        first = place > first ? place : first;
+    Tokens<kDtype, kSliceThreads>(a, b, lo, hi).each_four([&](int v, const uint32_t* keys) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint64_t place = place_of(keys[e], v + e);
+            first = place > first ? place : first;
+        }
+        if constexpr (kRules) {   // (8 lanes have a group, half a DPP row)
+            static_assert(kGroup == 32, "lanes of a group");
+            uint32_t most = max(max(keys[0], keys[1]), max(keys[2], keys[3]));
+            most = max(most, dpp32<0x111>(most));
+            most = max(most, dpp32<0x112>(most));
+            most = max(most, dpp32<0x114>(most));
+            if ((tid & 7) == 7 && v / kGroup * kGroup < hi) a.groups[b * a.groups_of_row() + v / kGroup] = most;
+        }
     });
     first = wave_max(first);
     if ((tid & 63) == 0) part[tid >> 6] = first;
@@ -297,6 +338,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_bins_kernel(SampleArgs a
     __shared__ uint32_t counts[kBins + 1];
     const int64_t b = blockIdx.y, slice = b * a.slices + blockIdx.x;
     const int lo = blockIdx.x * a.length, hi = min(lo + a.length, a.V), tid = threadIdx.x;
+    if (kRules && a.few_kept(b)) return;
     Tokens<kDtype, kSliceThreads> tokens(a, b, lo, hi);   // (its first loads are under way meanwhile)
     make_table(table);
     const Rules r(a, b, table);
@@ -355,6 +397,10 @@ struct Cuts {
     uint64_t above_k, sum_k, above_p;   // tokens and weights over bin k, weights over p_low
     float low, high;     // the logits of all listed tokens lie between
     double most, turn;   // of Weights
+    // The bin of a listed token by its log2; where all of a row's first tokens are listed
+    // (few_kept) they are one bin.
+    bool one;
+    __device__ __forceinline__ int bin(double z) const { return one ? 0 : bin_of(z); }
     __device__ __forceinline__ bool listed(int bin) const {
         return bin == k || (bin >= p_low && bin <= p_high) || (bin >= m_low && bin <= m_high);
     }
@@ -423,6 +469,7 @@ __device__ Cuts find_cuts(const Rules& r, uint64_t sum, uint32_t count, CutShare
     c.high = to < 0 ? -INFINITY : (float)(r.w.most - (c.sure() - 1) * 0.125 * octave + slack);
     c.low = to < 0 ? INFINITY : to == kBins ? -INFINITY : (float)(r.w.most - (to + 2) * 0.125 * octave - slack);
     c.most = r.w.most, c.turn = r.w.turn;
+    c.one = false;
     return c;
 }
 
@@ -433,6 +480,7 @@ __global__ __launch_bounds__(kCutThreads) void sample_cuts_kernel(SampleArgs a) 
     constexpr int kAll = kBins + 1;
     const int64_t b = blockIdx.x, slice0 = b * a.slices;
     const int tid = threadIdx.x, lane = tid & 63;
+    if (a.few_kept(b)) return;
     uint64_t sum = 0;
     uint32_t count = 0;
     if (tid < kAll) {
@@ -467,18 +515,37 @@ __global__ __launch_bounds__(kSliceThreads) void sample_list_kernel(SampleArgs a
     __shared__ uint32_t count;
     const int64_t b = blockIdx.y, slice = b * a.slices + blockIdx.x;
     const int lo = blockIdx.x * a.length, hi = min(lo + a.length, a.V), tid = threadIdx.x;
-    Tokens<kDtype, kSliceThreads> tokens(a, b, lo, hi);   // (its first loads are under way meanwhile)
+    const int lane = tid & 63, end = (hi + kGroup - 1) / kGroup;
+    if (a.few_kept(b)) return;
     const Cuts c = a.cuts[b];
     if (tid == 0) count = 0;
     __syncthreads();
     const Weights w{c.most, c.turn, nullptr, 0};
     if (!(c.low > c.high)) {
-        tokens.each([&](int v, uint32_t key) {
-            const float x = logit_of(key);   // (a NaN where there is none)
-            if (x < c.low || x > c.high || !key || !c.listed(bin_of(w.log2_of(key)))) return;
-            const uint32_t at = atomicAdd(&count, 1u);
-            if (at < kListed) a.list[slice * kListed + at] = place_of(key, v);
-        });
+        // a wave looks at 32 groups' largest keys, and into those that reach low, two at once
+        constexpr int kGroups = 32, kAtOnce = 4;
+        for (int g0 = lo / kGroup + tid / 64 * kGroups; g0 < end; g0 += kSliceThreads / 64 * kGroups) {
+            const uint32_t most = lane < kGroups && g0 + lane < end ? a.groups[b * a.groups_of_row() + g0 + lane] : 0;
+            uint64_t some = __ballot(most && !(logit_of(most) < c.low));
+            while (some) {
+                int at[kAtOnce];
+                uint32_t keys[kAtOnce];
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    const uint64_t rest = some & (some - 1), mine = lane < kGroup ? some : rest;
+                    at[i] = mine ? (g0 + __ffsll((unsigned long long)mine) - 1) * kGroup + lane % kGroup : hi;
+                    keys[i] = at[i] < hi ? key_at<kDtype>(a, b, at[i]) : 0;
+                    some = rest & (rest - 1);
+                }
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    const float x = logit_of(keys[i]);   // (a NaN where there is none)
+                    if (x < c.low || x > c.high || !keys[i] || !c.listed(bin_of(w.log2_of(keys[i])))) continue;
+                    const uint32_t n = atomicAdd(&count, 1u);
+                    if (n < kListed) a.list[slice * kListed + n] = place_of(keys[i], at[i]);
+                }
+            }
+        }
     }
     __syncthreads();
     if (tid == 0) a.listed[slice] = count;
@@ -487,16 +554,25 @@ __global__ __launch_bounds__(kSliceThreads) void sample_list_kernel(SampleArgs a
 // ---------------------------------------------------------------------------
 // rows
 // ---------------------------------------------------------------------------
-constexpr int kThreads = 1024, kWaves = kThreads / 64, kDigits = 2048, kRanked = 256;
+constexpr int kThreads = 1024, kWaves = kThreads / 64, kDigits = 2048;
+constexpr int kMostGroups = 4096;   // of a row whose kept tokens are in few groups
 
 struct Shared {
     double table[kFractions];
+    uint64_t list[kMostListed];              // the listed tokens
     union {
-        uint64_t digits[kDigits];        // radix selection
-        uint64_t list[kMostListed];      // the listed tokens
+        struct {
+            uint64_t digits[kDigits];        // radix selection
+            uint32_t groups[kMostGroups];    // list_first's
+        };
+        struct {
+            uint64_t sorted[kMostListed];    // sort_list's
+        };
     };
+    uint32_t bucket[kDigits];
     uint64_t part[kWaves], ties[kWaves];
     uint64_t found[2];
+    uint32_t some_groups, some, key_low, key_high;
 };
 
 // What is kept: tokens up to `last` in the order, of weights of `least` or more.
@@ -582,6 +658,87 @@ __device__ uint64_t select(const SampleArgs& a, int64_t b, Shared& s, uint32_t l
     return above;
 }
 
+// A key that k or more of those that each(f) gives reach, and but for its lower ten bits
+// no larger one that so many do; 1 where they are fewer.
+template <typename Each>
+__device__ uint32_t edge_of(Shared& s, uint64_t k, Each each) {
+    uint64_t above = 0;
+    uint32_t prefix = 0, mask = 0;
+    for (int shift = 21; shift >= 10; shift -= 11) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < kDigits; i += kThreads) s.digits[i] = 0;
+        __syncthreads();
+        each([&](uint32_t key) {
+            if (key && (key & mask) == prefix) {
+                atomicAdd((unsigned long long*)&s.digits[key >> shift & (kDigits - 1)], 1ull);
+            }
+        });
+        __syncthreads();
+        const Crossing c = cross(s, k - above);   // (none: digit 0)
+        above += c.above;
+        prefix |= (uint32_t)c.bin << shift;
+        mask |= (uint32_t)(kDigits - 1) << shift;
+    }
+    return max(prefix, 1u);
+}
+
+// Lists a row's first tokens, k or more of them (all, if they are fewer): a key that the
+// largest of k groups reach is one that k tokens do, and all that reach it are in
+// those groups.  Returns how many; -1: they are too many to list.
+constexpr int kHeld = 4;   // groups of a thread in registers
+template <int kDtype>
+__device__ int list_first(const SampleArgs& a, int64_t b, uint64_t k, const uint32_t* held, Shared& s) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, groups = a.groups_of_row();
+    const uint32_t* most = a.groups + b * groups;
+    constexpr int kAtOnce = 8;   // pairs of groups of a wave
+    auto each_group = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) f(i * kThreads + tid, held[i]);
+        for (int g = kHeld * kThreads + tid; g < groups; g += kThreads) f(g, most[g]);
+    };
+    uint32_t edge = edge_of(s, k, [&](auto f) { each_group([&](int, uint32_t key) { f(key); }); });
+    if (tid == 0) s.some_groups = 0;
+    __syncthreads();
+    each_group([&](int g, uint32_t key) {
+        if (key < edge) return;
+        const uint32_t at = atomicAdd(&s.some_groups, 1u);
+        if (at < kMostGroups) s.groups[at] = (uint32_t)g;
+    });
+    __syncthreads();
+    const int some = (int)s.some_groups;
+    if (some > kMostGroups) return -1;
+    auto each_token = [&](auto f) {
+        const int half = lane / kGroup;   // (two groups a load)
+        for (int i0 = 2 * wave + half; i0 - half < some; i0 += 2 * kWaves * kAtOnce) {
+            int v[kAtOnce];
+            uint32_t keys[kAtOnce];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+                const int at = i0 + i * 2 * kWaves;
+                v[i] = at < some ? (int)s.groups[at] * kGroup + lane % kGroup : a.V;
+                keys[i] = v[i] < a.V ? key_at<kDtype>(a, b, v[i]) : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) f(v[i], keys[i]);
+        }
+    };
+    for (int turn = 0;; ++turn) {
+        if (tid == 0) s.some = 0;
+        __syncthreads();
+        each_token([&](int v, uint32_t key) {
+            if (key < edge) return;
+            const uint32_t at = atomicAdd(&s.some, 1u);
+            if (at < kMostListed) s.list[at] = place_of(key, v);
+        });
+        __syncthreads();
+        const int n = (int)s.some;
+        if (n <= kMostListed) return n;
+        if (turn) return -1;
+        // groups with many such tokens (neighbours that are alike): the edge of tokens
+        edge = edge_of(s, k, [&](auto f) { each_token([&](int, uint32_t key) { f(key); }); });
+    }
+}
+
 // The last kept token of the row (its place), of what top_k and top_p keep, by
 // selection over the whole row: any number of tokens in a bin.
 template <int kDtype>
@@ -644,10 +801,60 @@ __device__ uint64_t last_of_row(const SampleArgs& a, int64_t b, const Rules& r, 
     return v == 0xffffffffu ? (uint64_t)edge << 32 : place_of(edge, (int)v);
 }
 
+// Sorts n listed tokens into the order: into buckets of neighbouring keys, and by
+// counting in a bucket.
+__device__ void sort_list(Shared& s, int n) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    static_assert(kDigits == 2 * kThreads, "two buckets a thread");
+    s.bucket[2 * tid] = s.bucket[2 * tid + 1] = 0;
+    if (tid == 0) s.key_low = ~0u, s.key_high = 0;
+    __syncthreads();
+    uint32_t low = ~0u, high = 0;
+    for (int i = tid; i < n; i += kThreads) {
+        const uint32_t key = key_of_place(s.list[i]);
+        low = min(low, key), high = max(high, key);
+    }
+    low = ~(uint32_t)wave_max(~low), high = (uint32_t)wave_max(high);
+    if (lane == 0) atomicMin(&s.key_low, low), atomicMax(&s.key_high, high);
+    __syncthreads();
+    high = s.key_high;
+    const int shift = max(32 - __clz((int)(high - s.key_low)) - 11, 0);
+    auto bucket_of = [&](uint64_t place) { return (high - key_of_place(place)) >> shift; };
+    for (int i = tid; i < n; i += kThreads) atomicAdd(&s.bucket[bucket_of(s.list[i])], 1u);
+    __syncthreads();
+    const uint32_t first = s.bucket[2 * tid], both = first + s.bucket[2 * tid + 1];
+    uint32_t upto = (uint32_t)wave_scan((uint64_t)both);
+    if (lane == 63) s.part[wave] = upto;
+    __syncthreads();
+    for (int i = 0; i < wave; ++i) upto += (uint32_t)s.part[i];
+    s.bucket[2 * tid] = upto - both, s.bucket[2 * tid + 1] = upto - both + first;
+    __syncthreads();
+    for (int i = tid; i < n; i += kThreads) {
+        const uint64_t place = s.list[i];
+        s.sorted[atomicAdd(&s.bucket[bucket_of(place)], 1u)] = place;   // (in the end a bucket's end)
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += kThreads) {
+        const uint64_t place = s.sorted[i];
+        const int bucket = (int)bucket_of(place), end = (int)s.bucket[bucket];
+        const int begin = bucket ? (int)s.bucket[bucket - 1] : 0;
+        int rank = begin;
+        for (int j = begin; j < end; ++j) rank += s.sorted[j] > place;
+        s.list[rank] = place;
+    }
+    __syncthreads();
+}
+
+// Listed tokens of a thread, and their weights: 0 if they are not kept.
+constexpr int kEach = kMostListed / kThreads;
+struct Own {
+    uint64_t place[kEach], weight[kEach];
+};
+
 // The same by up to 64 listed tokens, by one wave; their kept weights are added to their
 // slices' sums.
 __device__ uint64_t last_of_few(const SampleArgs& a, const Rules& r, const Cuts& c, uint64_t* list, int n,
-                                unsigned long long* slice_sums) {
+                                unsigned long long* slice_sums, Own& own) {
     const int lane = threadIdx.x & 63;
     uint64_t place = lane < n ? list[lane] : 0;
     int rank = 0;
@@ -659,7 +866,7 @@ __device__ uint64_t last_of_few(const SampleArgs& a, const Rules& r, const Cuts&
     const uint32_t key = key_of_place(place);
     const double z = key ? r.w.log2_of(key) : 0.0;
     const uint64_t weight = key ? r.w.of_log2(z) : 0;
-    const int bin = key ? bin_of(z) : kBins + 2;
+    const int bin = key ? c.bin(z) : kBins + 2;
     const uint64_t number = c.above_k + lane - __popcll(__ballot(bin < c.k));   // (of bin k's)
     const bool in_k = bin < c.k || (bin == c.k && number < (uint64_t)r.k);
     bool kept = place && in_k;
@@ -671,6 +878,7 @@ __device__ uint64_t last_of_few(const SampleArgs& a, const Rules& r, const Cuts&
     }
     if (kept && weight >= r.least) {
         atomicAdd(&slice_sums[token_of_place(place) / a.length], (unsigned long long)weight);
+        own.place[0] = place, own.weight[0] = weight;
     }
     if (c.k > kBins && !(r.p < 1.f)) return 0;   // (min_p alone)
     const uint64_t all = __ballot(kept);
@@ -681,39 +889,8 @@ __device__ uint64_t last_of_few(const SampleArgs& a, const Rules& r, const Cuts&
 __device__ uint64_t last_of_list(const SampleArgs& a, const Rules& r, const Cuts& c, Shared& s, int n,
                                  unsigned long long* slice_sums) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    // sorted into the order, largest place first: up to kRanked by counting the
-    // larger ones, more by merging runs
-    if (n <= kRanked) {
-        constexpr int kParts = kThreads / kRanked;   // threads of a token, a share of the others each
-        const int i = tid / kParts;
-        const uint64_t place = i < n ? s.list[i] : 0;
-        int rank = 0;
-        if (i < n) {
-#pragma unroll 4
-            for (int j = tid % kParts; j < n; j += kParts) rank += s.list[j] > place;
-        }
-#pragma unroll
-        for (int d = 1; d < kParts; d *= 2) rank += __shfl_xor(rank, d);
-        __syncthreads();
-        if (i < n && tid % kParts == 0) s.list[rank] = place;
-    } else {
-        int size = kRanked;
-        while (size < n) size *= 2;
-        for (int i = n + tid; i < size; i += kThreads) s.list[i] = 0;
-        for (int k = 2; k <= size; k *= 2) {
-            for (int j = k / 2; j > 0; j /= 2) {
-                __syncthreads();
-                for (int i = tid; i < size / 2; i += kThreads) {
-                    const int x = (i & ~(j - 1)) << 1 | (i & (j - 1)), y = x + j;   // (j: a power of two)
-                    const uint64_t p = s.list[x], q = s.list[y];
-                    if ((p < q) == ((x & k) == 0)) s.list[x] = q, s.list[y] = p;
-                }
-            }
-        }
-    }
-    __syncthreads();
+    sort_list(s, n);
     // thread t has the tokens 4 t .. 4 t + 3
-    constexpr int kEach = kMostListed / kThreads;
     uint64_t place[kEach], weight[kEach];
     int bin[kEach];
     uint64_t first_k = 0, in_p = 0;
@@ -771,6 +948,45 @@ __device__ uint64_t last_of_list(const SampleArgs& a, const Rules& r, const Cuts
     return s.list[last - 1];
 }
 
+__device__ __forceinline__ float logprob_of(const Rules& r, uint32_t key, uint64_t total) {
+    return (float)(r.w.log2_of(key) * 0.6931471805599453 - log((double)total / (double)(1ull << r.w.shift)));
+}
+
+// The kept ones of the n first tokens of a row (few_kept), of a thread kMine; their weights
+// are added to their slices' sums.
+template <int kMine>
+__device__ void keep_first(const SampleArgs& a, const Rules& r, Shared& s, int n, unsigned long long* slice_sums,
+                           Own& own) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint64_t weight[kMine], sum = 0;
+#pragma unroll
+    for (int e = 0; e < kMine; ++e) {
+        const int i = tid * kMine + e;
+        own.place[e] = i < n && i < r.k ? s.list[i] : 0;
+        weight[e] = own.place[e] ? r.w.of(key_of_place(own.place[e])) : 0;
+        sum += weight[e];
+    }
+    uint64_t upto = wave_scan(sum), total = 0;
+    if (lane == 63) s.part[wave] = upto;
+    __syncthreads();
+    uint64_t before = upto - sum;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        const uint64_t part = s.part[i];
+        total += part;
+        if (i < wave) before += part;
+    }
+    const uint64_t bound = r.p < 1.f ? share_of(r.p, total) : ~0ull;
+#pragma unroll
+    for (int e = 0; e < kMine; ++e) {
+        own.weight[e] = before < bound && weight[e] >= r.least ? weight[e] : 0;
+        before += weight[e];
+        if (own.weight[e]) {
+            atomicAdd(&slice_sums[token_of_place(own.place[e]) / a.length], (unsigned long long)own.weight[e]);
+        }
+    }
+}
+
 template <int kDtype>
 __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
     __shared__ Shared s;
@@ -783,11 +999,18 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
     const float u = as_constant(a.u)[b];
     const int i0 = 2 * lane, i1 = 2 * lane + 1;
     const bool has0 = i0 < a.slices, has1 = i1 < a.slices, rules = a.rules();
-    const Cuts c = rules ? a.cuts[b] : Cuts{};
+    const bool few = a.few_kept(b);   // (then there are no bins and no list)
+    Cuts c = rules && !few ? a.cuts[b] : Cuts{};
     const uint64_t* whole = rules ? a.whole : a.sums;
-    const uint64_t w0 = has0 ? whole[slice0 + i0] : 0, w1 = has1 ? whole[slice0 + i1] : 0;
-    const uint32_t l0 = rules && has0 ? a.listed[slice0 + i0] : 0, l1 = rules && has1 ? a.listed[slice0 + i1] : 0;
+    const uint64_t w0 = has0 && !few ? whole[slice0 + i0] : 0, w1 = has1 && !few ? whole[slice0 + i1] : 0;
+    const uint32_t l0 = rules && has0 && !few ? a.listed[slice0 + i0] : 0;
+    const uint32_t l1 = rules && has1 && !few ? a.listed[slice0 + i1] : 0;
     if (wave == 0) slice_sums[i0] = w0, slice_sums[i1] = w1;
+    uint32_t held[kHeld] = {};
+    for (int i = 0; i < kHeld && few; ++i) {
+        const int g = i * kThreads + tid, groups = a.groups_of_row();
+        held[i] = g < groups ? a.groups[b * groups + g] : 0;
+    }
     make_table(s.table);
     const Rules r(a, b, s.table);
     if (r.first == 0 || r.greedy) {
@@ -799,35 +1022,46 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
     }
     Kept kept{0, r.least};
     bool known = true;   // slice_sums are those of kept weights
+    Own own{};
     if (rules) {
-        // the listed tokens, one slice's after the other's
-        const uint64_t upto = wave_scan((uint64_t)l0 + l1);
-        const uint64_t listed = lane_of(upto, 63);
-        known = __ballot(l0 > kListed || l1 > kListed) == 0 && listed <= kMostListed;
-        if (known && wave == 0) {
-            list_at[i0] = (int)(upto - l0 - l1);
-            list_at[i1] = (int)(upto - l1);
-            if (lane == 63) list_at[kMostSlices] = (int)listed;
-        }
-        __syncthreads();
-        if (known) {
-            for (int i = wave; i < a.slices; i += kWaves) {
+        int listed;
+        if (few) {
+            listed = list_first<kDtype>(a, b, (uint64_t)r.k, held, s);
+            known = listed >= 0;
+            c.one = true;
+            c.m_low = c.m_high = kBins + 1;
+        } else {
+            // the listed tokens, one slice's after the other's
+            const uint64_t upto = wave_scan((uint64_t)l0 + l1), all = lane_of(upto, 63);
+            known = __ballot(l0 > kListed || l1 > kListed) == 0 && all <= kMostListed;
+            listed = (int)all;
+            if (known && wave == 0) {
+                list_at[i0] = (int)(upto - l0 - l1);
+                list_at[i1] = (int)(upto - l1);
+                if (lane == 63) list_at[kMostSlices] = listed;
+            }
+            __syncthreads();
+            for (int i = wave; known && i < a.slices; i += kWaves) {
                 const int at = list_at[i], count = list_at[i + 1] - at;
                 for (int e = lane; e < count; e += 64) s.list[at + e] = a.list[(slice0 + i) * kListed + e];
             }
             __syncthreads();
-            if (listed <= 64) {
-                if (wave == 0) {
-                    const uint64_t last = last_of_few(a, r, c, s.list, (int)listed, slice_sums);
-                    if (lane == 0) s.found[0] = last;
-                }
-                __syncthreads();
-                kept.last = s.found[0];
-            } else {
-                kept.last = last_of_list(a, r, c, s, (int)listed, slice_sums);
-            }
-        } else {
+        }
+        if (!known) {
             kept.last = last_of_row<kDtype>(a, b, r, s);
+        } else if (listed <= 64) {
+            if (wave == 0) {
+                const uint64_t last = last_of_few(a, r, c, s.list, listed, slice_sums, own);
+                if (lane == 0) s.found[0] = last;
+            }
+            __syncthreads();
+            kept.last = s.found[0];
+        } else if (few) {
+            sort_list(s, listed);
+            if (r.k <= kThreads) keep_first<1>(a, r, s, listed, slice_sums, own);
+            else keep_first<kFewKept / kThreads>(a, r, s, listed, slice_sums, own);
+        } else {
+            kept.last = last_of_list(a, r, c, s, listed, slice_sums);
         }
     }
     __syncthreads();
@@ -852,6 +1086,30 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
     rest -= before;
     int part = 2 * pair;
     if (rest >= first) rest -= first, ++part;
+    if (c.one && known) {
+        // all kept tokens are at hand: those of the slice, with the weights before them
+        if (tid == 0) s.some = 0;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            if (!own.weight[e] || token_of_place(own.place[e]) / a.length != part) continue;
+            const uint32_t at = atomicAdd(&s.some, 1u);
+            s.list[2 * at] = ~own.place[e] & 0xffffffffu, s.list[2 * at + 1] = own.weight[e];
+        }
+        __syncthreads();
+        const int n = (int)s.some;
+        for (int i = tid; i < n; i += kThreads) {
+            const uint64_t v = s.list[2 * i], weight = s.list[2 * i + 1];
+            uint64_t upto = 0;
+#pragma unroll 8
+            for (int j = 0; j < n; ++j) upto += s.list[2 * j] < v ? s.list[2 * j + 1] : 0;
+            if (upto <= rest && rest - upto < weight) {   // one token
+                a.tokens[b] = (int)v;
+                if (a.logprobs) a.logprobs[b] = logprob_of(r, key_at<kDtype>(a, b, (int)v), total);
+            }
+        }
+        return;
+    }
     // the slice is split over the waves, a large one's part with the token again
     int lo = part * a.length, hi = min(lo + a.length, a.V);
     constexpr int kAtOnce = 16;   // groups of 64 tokens of a wave
@@ -899,10 +1157,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
             if (upto > rest && upto - weights[g] <= rest) {   // one lane
                 const int v = begin + g * 64 + lane;
                 a.tokens[b] = v;
-                if (a.logprobs) {
-                    a.logprobs[b] = (float)(r.w.log2_of(key_at<kDtype>(a, b, v)) * 0.6931471805599453 -
-                                            log((double)total / (double)(1ull << a.shift)));
-                }
+                if (a.logprobs) a.logprobs[b] = logprob_of(r, key_at<kDtype>(a, b, v), total);
             }
             return;
         }
@@ -932,7 +1187,8 @@ int shift_of(int V) {   // a row's sum stays under 2^63
 
 int64_t sample_bytes(int rows, int V) {
     const int64_t slices = (int64_t)rows * slices_of(V).count;
-    return rows * (int64_t)sizeof(Cuts) + slices * (8 + 8 + (kBins + 1) * 8 + kListed * 8 + (kBins + 1) * 4 + 4);
+    return rows * ((int64_t)sizeof(Cuts) + ((int64_t)V + 63) / 64 * 4) +
+           slices * (8 + 8 + (kBins + 1) * 8 + kListed * 8 + (kBins + 1) * 4 + 4);
 }
 
 int launch_sample(const void* logits, int dtype, int64_t ld, int rows, int V, const float* u,
@@ -950,10 +1206,12 @@ int launch_sample(const void* logits, int dtype, int64_t ld, int rows, int V, co
     a.list = a.sums + slices * (kBins + 1);
     a.counts = reinterpret_cast<uint32_t*>(a.list + slices * kListed);
     a.listed = a.counts + slices * (kBins + 1);
+    a.groups = a.listed + slices;
     const dim3 grid(cut.count, rows);
     auto run = [&](auto type) {
         constexpr int kDtype = decltype(type)::value;
-        hipLaunchKernelGGL(sample_max_kernel<kDtype>, grid, dim3(kSliceThreads), 0, stream, a);
+        auto* most = a.rules() ? sample_max_kernel<kDtype, true> : sample_max_kernel<kDtype, false>;
+        hipLaunchKernelGGL(most, grid, dim3(kSliceThreads), 0, stream, a);
         auto* bins = a.rules() ? sample_bins_kernel<kDtype, true> : sample_bins_kernel<kDtype, false>;
         hipLaunchKernelGGL(bins, grid, dim3(kSliceThreads), 0, stream, a);
         if (a.rules()) {

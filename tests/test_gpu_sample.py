@@ -149,3 +149,47 @@ def test_large_vocabulary(dev):
 def test_no_rows(dev):
     tokens, logp = ops.sample(torch.empty(0, 10, device=dev), torch.empty(0, device=dev), logprobs=True)
     assert tokens.shape == (0,) and logp.shape == (0,)
+
+
+KS = [1, 2, 63, 64, 65, 200, 469, 470, 1000, 1024, 1500, 3000]
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("order", ["rising", "falling", "blocks", "any"])
+def test_few_or_many_kept(dev, dtype, order):
+    """Tokens that top_k keeps next to each other, more of them among 64
+    neighbours than can be listed, many that are equal."""
+    B, V = len(KS), 20011
+    x = torch.randn(B, V, generator=torch.Generator().manual_seed(11)) * 2
+    if order == "rising":
+        x = x.sort(1).values
+    elif order == "falling":
+        x = x.sort(1, descending=True).values
+    elif order == "blocks":
+        x = x[:, :V // 64 + 1].repeat_interleave(64, 1)[:, :V].contiguous()
+    x = x.to(DT[dtype])
+    u = numbers(B, 1)
+    check(dev, x, u, top_k=KS)
+    check(dev, x, u, pad=5, top_k=KS[::-1], top_p=numbers(B, 2, 0.2, 1), temperature=numbers(B, 3, 0.3, 30))
+    check(dev, x, u, top_k=[2000] * B, top_p=numbers(B, 4, 0.2, 1), min_p=numbers(B, 5, 0, 0.01))
+    x[:, 100:19000] = -math.inf
+    check(dev, x, u, top_k=KS)
+    x[:, 5:] = -math.inf
+    check(dev, x, u, top_k=KS, temperature=numbers(B, 6, 0.3, 30))
+
+
+def test_more_equal_groups_than_are_looked_into(dev):
+    V = 300001
+    x = torch.zeros(3, V)
+    x[1, ::3] = 1.0
+    x[2, 299_000] = 2.0
+    check(dev, x, [0.1, 0.5, 0.99], top_k=[500, 1000, 1024])
+    check(dev, x, [0.1, 0.5, 0.99], top_k=[500, 1000, 1024], top_p=[0.7] * 3)
+
+
+def test_most_of_a_large_vocabulary_kept(dev):
+    """top_k around the largest that is looked up in groups."""
+    ks = [1023, 1024, 1025, 2047, 2048, 2049]
+    x = torch.randn(6, 100003, generator=torch.Generator().manual_seed(12)) * 3
+    check(dev, x, numbers(6, 1), top_k=ks, temperature=[5.0] * 6)
+    check(dev, x, numbers(6, 2), top_k=ks, top_p=[0.97] * 6, min_p=[1e-3] * 6)
