@@ -18,16 +18,15 @@
 //   2. sample_bins_kernel    each slice's weights, summed and counted in bins of an
 //                            eighth of an octave of w, down to 2^-46 where it rounds
 //                            to 0; without rules one sum
-//   3. sample_cuts_kernel    (with rules) a row's bins say where the rules cut
-//   4. sample_list_kernel    (with rules) each slice's tokens of the bins that they cut
-//                            through are listed, of the groups that reach them
-//   5. sample_finish_kernel  one workgroup a row: the listed tokens, sorted, give
-//                            the cuts; bins and list each slice's sum of kept
-//                            weights, u the slice, the slice read again the token
-// A row whose top_k is small (few_kept) skips 2 to 4: the k-th largest of its groups'
+//   3. sample_finish_kernel  one workgroup a row: the bins say where the rules cut; the
+//                            tokens of the bins that they cut through are listed, from
+//                            the groups that reach them, and sorted, and give the
+//                            cuts; bins and list each slice's sum of kept weights, u
+//                            the slice, the slice read again the token
+// A row whose top_k is small (few_kept) has no bins: the k-th largest of its groups'
 // largest logits is a logit that k tokens reach, so what it keeps is among the
 // tokens that reach it, and those are in the groups that do; k of them, but for
-// ties.  The last kernel lists them, and that is all it reads again of the row.
+// ties.  They are listed, and that is all that is read again of the row.
 // A row with over kMostListed listed tokens (equal logits, mostly) is worked out by
 // its last workgroup alone: radix selection over the row.
 #include <math.h>
@@ -45,8 +44,7 @@ typedef __attribute__((ext_vector_type(4), aligned(4))) float f4_any;
 typedef __attribute__((ext_vector_type(2), aligned(2))) uint32_t u2_any;
 
 constexpr int kBins = 368;          // of an eighth of an octave: 46 octaves; one more below
-constexpr int kListed = 2048;       // listed tokens of a slice
-constexpr int kMostListed = 4096;   // and of a row (a power of two)
+constexpr int kMostListed = 4096;   // listed tokens of a row
 constexpr int kSliceThreads = 512;
 constexpr int kMostSlices = 128;
 constexpr int kFewKept = 2048;
@@ -67,10 +65,6 @@ struct SampleArgs {
     uint32_t* groups;      // of a row, with rules: the largest key of every kGroup tokens
     uint64_t* sums;        // [kBins + 1] with rules, else one
     uint32_t* counts;      // [kBins + 1]
-    uint32_t* listed;      // how many are listed (more than kListed: not all are)
-    uint64_t* list;        // [kListed] places
-    uint64_t* whole;       // the sum of the bins that are kept whole
-    struct Cuts* cuts;     // of a row
     __host__ __device__ __forceinline__ bool rules() const { return top_k || top_p || min_p; }
     __host__ __device__ __forceinline__ int groups_of_row() const { return (V + kGroup - 1) / kGroup; }
     // A row whose kept tokens are in few groups: its bins are not needed.  48 rows of
@@ -179,10 +173,6 @@ struct Tokens {
         });
     }
 };
-template <int kDtype, int kThreads, typename F>
-__device__ __forceinline__ void for_tokens(const SampleArgs& a, int64_t b, int lo, int hi, F f) {
-    Tokens<kDtype, kThreads>(a, b, lo, hi).each(f);
-}
 
 // The bin of a weight by its log2.
 __device__ __forceinline__ int bin_of(double z) { return z > -kBins / 8 ? (int)(z * -8.0) : kBins; }
@@ -396,7 +386,6 @@ struct Cuts {
     int m_low, m_high;   // those around min_p
     uint64_t above_k, sum_k, above_p;   // tokens and weights over bin k, weights over p_low
     float low, high;     // the logits of all listed tokens lie between
-    double most, turn;   // of Weights
     // The bin of a listed token by its log2; where all of a row's first tokens are listed
     // (few_kept) they are one bin.
     bool one;
@@ -416,9 +405,9 @@ __device__ __forceinline__ uint64_t share_of(float p, uint64_t total) {
 struct CutShared {
     uint64_t sum[kBins + 2], above[kBins + 2];   // of a bin; of those before it
     uint32_t count[kBins + 2], before[kBins + 2];
-    uint64_t part[(kBins + 64) / 64 + 1];
-    uint32_t count_part[(kBins + 64) / 64 + 1];
-    int found[4];
+    uint64_t part[(kBins + 64) / 64];
+    uint32_t count_part[(kBins + 64) / 64];
+    int found[3];
 };
 // By all threads of a workgroup of over kBins + 1, each with its bin of the row.
 __device__ Cuts find_cuts(const Rules& r, uint64_t sum, uint32_t count, CutShared& s) {
@@ -431,8 +420,9 @@ __device__ Cuts find_cuts(const Rules& r, uint64_t sum, uint32_t count, CutShare
         if (lane == 63) s.part[wave] = above, s.count_part[wave] = before;
         above -= sum, before -= count;
     }
-    if (tid < 4) s.found[tid] = kNone;
+    if (tid < 3) s.found[tid] = kNone;
     __syncthreads();
+    static_assert(kAll < kParts * 64, "one past the last");
     if (tid <= kAll) {   // (and one past the last: all of them)
         for (int i = 0; i < wave; ++i) above += s.part[i], before += s.count_part[i];
         s.sum[tid] = sum, s.above[tid] = above, s.count[tid] = count, s.before[tid] = before;
@@ -443,8 +433,10 @@ __device__ Cuts find_cuts(const Rules& r, uint64_t sum, uint32_t count, CutShare
     }
     __syncthreads();
     Cuts c;
-    c.k = s.found[0] == kBins ? kNone : s.found[0];   // (a cut among weights of 0 changes nothing)
-    c.above_k = s.before[c.k], c.sum_k = s.above[c.k];
+    // (what all threads have alike is kept once for a wave)
+    c.k = __builtin_amdgcn_readfirstlane(s.found[0]);
+    if (c.k == kBins) c.k = kNone;   // (a cut among weights of 0 changes nothing)
+    c.above_k = lane_of(s.before[c.k], 0), c.sum_k = lane_of(s.above[c.k], 0);
     if (r.p < 1.f && tid < kAll) {
         const uint64_t low = share_of(r.p, max(s.above[c.k], (uint64_t)1));
         const uint64_t high = share_of(r.p, s.above[c.k] + s.sum[c.k]);
@@ -452,8 +444,8 @@ __device__ Cuts find_cuts(const Rules& r, uint64_t sum, uint32_t count, CutShare
         if (s.above[tid] < high && s.above[tid] + s.sum[tid] >= high) s.found[2] = tid;
     }
     __syncthreads();
-    c.p_low = s.found[1], c.p_high = s.found[2];
-    c.above_p = s.above[c.p_low];
+    c.p_low = __builtin_amdgcn_readfirstlane(s.found[1]), c.p_high = __builtin_amdgcn_readfirstlane(s.found[2]);
+    c.above_p = lane_of(s.above[c.p_low], 0);
     c.m_low = c.m_high = kNone;
     if (r.least) {
         c.m_low = bin_of(r.least_high);
@@ -468,102 +460,26 @@ __device__ Cuts find_cuts(const Rules& r, uint64_t sum, uint32_t count, CutShare
     const double octave = 1.0 / r.w.turn, slack = 1e-6 * fabs(r.w.most);
     c.high = to < 0 ? -INFINITY : (float)(r.w.most - (c.sure() - 1) * 0.125 * octave + slack);
     c.low = to < 0 ? INFINITY : to == kBins ? -INFINITY : (float)(r.w.most - (to + 2) * 0.125 * octave - slack);
-    c.most = r.w.most, c.turn = r.w.turn;
     c.one = false;
     return c;
-}
-
-constexpr int kCutThreads = (kBins + 64) / 64 * 64;
-
-__global__ __launch_bounds__(kCutThreads) void sample_cuts_kernel(SampleArgs a) {
-    __shared__ CutShared shared;
-    constexpr int kAll = kBins + 1;
-    const int64_t b = blockIdx.x, slice0 = b * a.slices;
-    const int tid = threadIdx.x, lane = tid & 63;
-    if (a.few_kept(b)) return;
-    uint64_t sum = 0;
-    uint32_t count = 0;
-    if (tid < kAll) {
-#pragma unroll 16
-        for (int i = 0; i < a.slices; ++i) {
-            sum += a.sums[(slice0 + i) * kAll + tid];
-            count += a.counts[(slice0 + i) * kAll + tid];
-        }
-    }
-    const Rules r(a, b, nullptr);   // (no weights here, only their bins)
-    if (r.greedy || r.first == 0) {
-        for (int i = tid; i < a.slices; i += kCutThreads) a.listed[slice0 + i] = 0;
-        if (tid == 0) a.cuts[b].low = INFINITY, a.cuts[b].high = -INFINITY;
-        return;
-    }
-    const Cuts c = find_cuts(r, sum, count, shared);
-    if (tid == 0) a.cuts[b] = c;
-    // sums of the bins that are kept whole, a wave a slice
-    for (int i = tid >> 6; i < a.slices; i += kCutThreads / 64) {
-        uint64_t whole = 0;
-#pragma unroll
-        for (int bin = 0; bin < kAll; bin += 64) {
-            if (bin + lane < min(c.sure(), kAll)) whole += a.sums[(slice0 + i) * kAll + bin + lane];
-        }
-        whole = wave_sum(whole);
-        if (lane == 0) a.whole[slice0 + i] = whole;
-    }
-}
-
-template <int kDtype>
-__global__ __launch_bounds__(kSliceThreads) void sample_list_kernel(SampleArgs a) {
-    __shared__ uint32_t count;
-    const int64_t b = blockIdx.y, slice = b * a.slices + blockIdx.x;
-    const int lo = blockIdx.x * a.length, hi = min(lo + a.length, a.V), tid = threadIdx.x;
-    const int lane = tid & 63, end = (hi + kGroup - 1) / kGroup;
-    if (a.few_kept(b)) return;
-    const Cuts c = a.cuts[b];
-    if (tid == 0) count = 0;
-    __syncthreads();
-    const Weights w{c.most, c.turn, nullptr, 0};
-    if (!(c.low > c.high)) {
-        // a wave looks at 32 groups' largest keys, and into those that reach low, two at once
-        constexpr int kGroups = 32, kAtOnce = 4;
-        for (int g0 = lo / kGroup + tid / 64 * kGroups; g0 < end; g0 += kSliceThreads / 64 * kGroups) {
-            const uint32_t most = lane < kGroups && g0 + lane < end ? a.groups[b * a.groups_of_row() + g0 + lane] : 0;
-            uint64_t some = __ballot(most && !(logit_of(most) < c.low));
-            while (some) {
-                int at[kAtOnce];
-                uint32_t keys[kAtOnce];
-#pragma unroll
-                for (int i = 0; i < kAtOnce; ++i) {
-                    const uint64_t rest = some & (some - 1), mine = lane < kGroup ? some : rest;
-                    at[i] = mine ? (g0 + __ffsll((unsigned long long)mine) - 1) * kGroup + lane % kGroup : hi;
-                    keys[i] = at[i] < hi ? key_at<kDtype>(a, b, at[i]) : 0;
-                    some = rest & (rest - 1);
-                }
-#pragma unroll
-                for (int i = 0; i < kAtOnce; ++i) {
-                    const float x = logit_of(keys[i]);   // (a NaN where there is none)
-                    if (x < c.low || x > c.high || !keys[i] || !c.listed(bin_of(w.log2_of(keys[i])))) continue;
-                    const uint32_t n = atomicAdd(&count, 1u);
-                    if (n < kListed) a.list[slice * kListed + n] = place_of(keys[i], at[i]);
-                }
-            }
-        }
-    }
-    __syncthreads();
-    if (tid == 0) a.listed[slice] = count;
 }
 
 // ---------------------------------------------------------------------------
 // rows
 // ---------------------------------------------------------------------------
 constexpr int kThreads = 1024, kWaves = kThreads / 64, kDigits = 2048;
-constexpr int kMostGroups = 4096;   // of a row whose kept tokens are in few groups
+constexpr int kHeld = 4, kMostGroups = kHeld * kThreads;   // groups of a row at once, kHeld a thread
 
 struct Shared {
     double table[kFractions];
     uint64_t list[kMostListed];              // the listed tokens
     union {
         struct {
-            uint64_t digits[kDigits];        // radix selection
-            uint32_t groups[kMostGroups];    // list_first's
+            union {
+                uint64_t digits[kDigits];    // radix selection
+                CutShared cuts;
+            };
+            uint32_t groups[kMostGroups];    // those that are looked into
         };
         struct {
             uint64_t sorted[kMostListed];    // sort_list's
@@ -630,6 +546,13 @@ __device__ Crossing cross(Shared& s, uint64_t bound) {
     return Crossing{(int)s.found[0], s.found[1]};
 }
 
+// f(key) for a row's tokens.
+template <int kDtype, typename F>
+__device__ __forceinline__ void for_row(const SampleArgs& a, int64_t b, F f) {
+#pragma unroll 4
+    for (int v = threadIdx.x; v < a.V; v += kThreads) f(key_at<kDtype>(a, b, v));
+}
+
 // The key at which the order's sum of `value(key)` over keys >= least first
 // reaches `bound` (> 0, at most the sum of all), and the sum above that key.
 template <int kDtype, typename Value>
@@ -642,7 +565,7 @@ __device__ uint64_t select(const SampleArgs& a, int64_t b, Shared& s, uint32_t l
         __syncthreads();
         for (int i = threadIdx.x; i < kDigits; i += kThreads) s.digits[i] = 0;
         __syncthreads();
-        for_tokens<kDtype, kThreads>(a, b, 0, a.V, [&](int, uint32_t key) {
+        for_row<kDtype>(a, b, [&](uint32_t key) {
             if (key && key >= least && (key & mask) == prefix) {
                 atomicAdd((unsigned long long*)&s.digits[key >> low & ((1u << bits) - 1)],
                           (unsigned long long)value(key));
@@ -682,61 +605,144 @@ __device__ uint32_t edge_of(Shared& s, uint64_t k, Each each) {
     return max(prefix, 1u);
 }
 
-// Lists a row's first tokens, k or more of them (all, if they are fewer): a key that the
-// largest of k groups reach is one that k tokens do, and all that reach it are in
-// those groups.  Returns how many; -1: they are too many to list.
-constexpr int kHeld = 4;   // groups of a thread in registers
-template <int kDtype>
-__device__ int list_first(const SampleArgs& a, int64_t b, uint64_t k, const uint32_t* held, Shared& s) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, groups = a.groups_of_row();
-    const uint32_t* most = a.groups + b * groups;
-    constexpr int kAtOnce = 8;   // pairs of groups of a wave
-    auto each_group = [&](auto f) {
+// A row's largest keys of groups, the first kMostGroups in registers.
+struct Groups {
+    const uint32_t* most;
+    int count;
+    uint32_t held[kHeld];
+    __device__ __forceinline__ Groups(const SampleArgs& a, int64_t b)
+        : most(a.groups + b * a.groups_of_row()), count(a.rules() ? a.groups_of_row() : 0) {
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) f(i * kThreads + tid, held[i]);
-        for (int g = kHeld * kThreads + tid; g < groups; g += kThreads) f(g, most[g]);
-    };
-    uint32_t edge = edge_of(s, k, [&](auto f) { each_group([&](int, uint32_t key) { f(key); }); });
-    if (tid == 0) s.some_groups = 0;
-    __syncthreads();
-    each_group([&](int g, uint32_t key) {
-        if (key < edge) return;
-        const uint32_t at = atomicAdd(&s.some_groups, 1u);
-        if (at < kMostGroups) s.groups[at] = (uint32_t)g;
-    });
-    __syncthreads();
-    const int some = (int)s.some_groups;
-    if (some > kMostGroups) return -1;
-    auto each_token = [&](auto f) {
-        const int half = lane / kGroup;   // (two groups a load)
-        for (int i0 = 2 * wave + half; i0 - half < some; i0 += 2 * kWaves * kAtOnce) {
+        for (int i = 0; i < kHeld; ++i) held[i] = at(i * kThreads + threadIdx.x);
+    }
+    __device__ __forceinline__ uint32_t at(int g) const { return g < count ? most[g] : 0; }
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) f(held[i]);
+        for (int g = kMostGroups + threadIdx.x; g < count; g += kThreads) f(most[g]);
+    }
+};
+
+// f(token, key) for the tokens of the groups whose largest key is `least` (not 0) or more,
+// by all threads; waits before it and after.
+template <int kDtype, typename F>
+__device__ __forceinline__ void for_groups(const SampleArgs& a, int64_t b, const Groups& groups, uint32_t least,
+                                           Shared& s, F f) {
+    const int tid = threadIdx.x;
+    constexpr int kLanes = kGroup / 4, kStep = kThreads / kLanes, kAtOnce = 4;   // four tokens a lane
+    const int64_t size = kDtype == NB_F32 ? 4 : 2;
+    const char* row = static_cast<const char*>(a.logits) + b * a.ld * size;
+    for (int g0 = 0; g0 < groups.count; g0 += kMostGroups) {
+        __syncthreads();
+        if (tid == 0) s.some_groups = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int g = g0 + i * kThreads + tid;
+            const uint32_t most = g0 ? groups.at(g) : groups.held[i];
+            if (most >= least) s.groups[atomicAdd(&s.some_groups, 1u)] = (uint32_t)g;
+        }
+        __syncthreads();
+        const int some = (int)s.some_groups;
+        for (int i0 = tid / kLanes; i0 < some; i0 += kStep * kAtOnce) {
             int v[kAtOnce];
-            uint32_t keys[kAtOnce];
+            uint32_t x[kAtOnce][kDtype == NB_F32 ? 4 : 2];
 #pragma unroll
             for (int i = 0; i < kAtOnce; ++i) {
-                const int at = i0 + i * 2 * kWaves;
-                v[i] = at < some ? (int)s.groups[at] * kGroup + lane % kGroup : a.V;
-                keys[i] = v[i] < a.V ? key_at<kDtype>(a, b, v[i]) : 0;
+                const int at = i0 + i * kStep;
+                v[i] = at < some ? (int)s.groups[at] * kGroup + tid % kLanes * 4 : a.V;
+                if (v[i] + 3 < a.V) {
+                    if constexpr (kDtype == NB_F32) {
+                        const f4_any four = *reinterpret_cast<const f4_any*>(row + v[i] * size);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[i][e] = __float_as_uint(four[e]);
+                    } else {
+                        const u2_any four = *reinterpret_cast<const u2_any*>(row + v[i] * size);
+                        x[i][0] = four[0], x[i][1] = four[1];
+                    }
+                } else {   // the row's end
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const bool there = v[i] + e < a.V;
+                        if constexpr (kDtype == NB_F32) {
+                            x[i][e] = there ? reinterpret_cast<const uint32_t*>(row)[v[i] + e] : 0xff800000u;
+                        } else {
+                            const uint32_t y = there ? reinterpret_cast<const bf16_bits*>(row)[v[i] + e] : 0xff80u;
+                            x[i][e / 2] = e & 1 ? x[i][e / 2] | y << 16 : y;
+                        }
+                    }
+                }
             }
 #pragma unroll
-            for (int i = 0; i < kAtOnce; ++i) f(v[i], keys[i]);
+            for (int i = 0; i < kAtOnce; ++i) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t y;
+                    if constexpr (kDtype == NB_F32) y = x[i][e];
+                    else y = e & 1 ? x[i][e / 2] & 0xffff0000u : x[i][e / 2] << 16;
+                    f(v[i] + e, key_of(__uint_as_float(y)));
+                }
+            }
         }
-    };
-    for (int turn = 0;; ++turn) {
-        if (tid == 0) s.some = 0;
-        __syncthreads();
-        each_token([&](int v, uint32_t key) {
-            if (key < edge) return;
-            const uint32_t at = atomicAdd(&s.some, 1u);
-            if (at < kMostListed) s.list[at] = place_of(key, v);
-        });
-        __syncthreads();
-        const int n = (int)s.some;
-        if (n <= kMostListed) return n;
-        if (turn) return -1;
-        // groups with many such tokens (neighbours that are alike): the edge of tokens
-        edge = edge_of(s, k, [&](auto f) { each_token([&](int, uint32_t key) { f(key); }); });
     }
+    __syncthreads();
+}
+
+// Lists the tokens of groups from `least` on that take(key) names; how many they are,
+// more than kMostListed: not all are listed.
+template <int kDtype, typename Take>
+__device__ __forceinline__ int list_tokens(const SampleArgs& a, int64_t b, const Groups& groups, uint32_t least,
+                                           Shared& s, Take take) {
+    if (threadIdx.x == 0) s.some = 0;
+    for_groups<kDtype>(a, b, groups, least, s, [&](int v, uint32_t key) {
+        if (!key || !take(key)) return;
+        const uint32_t at = atomicAdd(&s.some, 1u);
+        if (at < kMostListed) s.list[at] = place_of(key, v);
+    });
+    return (int)s.some;
+}
+
+// Lists a row's first tokens, k or more of them (all, if they are fewer): a key that the
+// largest of k groups reach is one that k tokens do, and all that reach it are in
+// those groups.
+template <int kDtype>
+__device__ int list_first(const SampleArgs& a, int64_t b, uint64_t k, const Groups& groups, Shared& s) {
+    uint32_t edge = edge_of(s, k, [&](auto f) { groups.each(f); });
+    for (int turn = 0;; ++turn) {
+        const int n = list_tokens<kDtype>(a, b, groups, edge, s, [&](uint32_t key) { return key >= edge; });
+        if (n <= kMostListed || turn) return n;
+        // groups with many such tokens (neighbours that are alike): the edge of tokens
+        edge = edge_of(s, k, [&](auto f) {
+            for_groups<kDtype>(a, b, groups, edge, s, [&](int, uint32_t key) { f(key); });
+        });
+    }
+}
+
+// A row's cuts from its bins, the sums of those that are kept whole into slice_sums.
+__device__ Cuts cuts_of_row(const SampleArgs& a, int64_t b, const Rules& r, Shared& s,
+                            unsigned long long* slice_sums) {
+    constexpr int kAll = kBins + 1;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const uint64_t* sums = a.sums + b * a.slices * kAll;
+    const uint32_t* counts = a.counts + b * a.slices * kAll;
+    uint64_t sum = 0;
+    uint32_t count = 0;
+    if (tid < kAll) {
+#pragma unroll 16
+        for (int i = 0; i < a.slices; ++i) sum += sums[i * kAll + tid], count += counts[i * kAll + tid];
+    }
+    const Cuts c = find_cuts(r, sum, count, s.cuts);
+    for (int i = tid >> 6; i < a.slices; i += kWaves) {   // a wave a slice
+        uint64_t whole = 0;
+#pragma unroll
+        for (int bin = 0; bin < kAll; bin += 64) {
+            if (bin + lane < min(c.sure(), kAll)) whole += sums[i * kAll + bin + lane];
+        }
+        whole = wave_sum(whole);
+        if (lane == 0) slice_sums[i] = whole;
+    }
+    return c;
 }
 
 // The last kept token of the row (its place), of what top_k and top_p keep, by
@@ -748,7 +754,7 @@ __device__ uint64_t last_of_row(const SampleArgs& a, int64_t b, const Rules& r, 
     uint64_t edge_ties = ~0ull;
     if (r.k) {
         uint64_t some = 0;
-        for_tokens<kDtype, kThreads>(a, b, 0, a.V, [&](int, uint32_t key) { some += key != 0; });
+        for_row<kDtype>(a, b, [&](uint32_t key) { some += key != 0; });
         if ((uint64_t)r.k < block_sum(s, some)) {
             edge_ties = (uint64_t)r.k -
                         select<kDtype>(a, b, s, 1, (uint64_t)r.k, [](uint32_t) { return 1ull; }, edge);
@@ -757,7 +763,7 @@ __device__ uint64_t last_of_row(const SampleArgs& a, int64_t b, const Rules& r, 
     uint64_t ties = 0;
     if (r.p < 1.f) {
         uint64_t total = 0;
-        for_tokens<kDtype, kThreads>(a, b, 0, a.V, [&](int, uint32_t key) {
+        for_row<kDtype>(a, b, [&](uint32_t key) {
             if (key > edge) total += r.w.of(key);
             ties += key == edge;
         });
@@ -991,26 +997,12 @@ template <int kDtype>
 __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
     __shared__ Shared s;
     __shared__ unsigned long long slice_sums[kMostSlices];
-    __shared__ int list_at[kMostSlices + 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t b = blockIdx.x, slice0 = b * a.slices;
-    // Asked for at once: u, the cuts, and of two slices a lane the listed tokens and
-    // the sums of whole bins.  (Of a greedy row they are not there, and not used.)
     const float u = as_constant(a.u)[b];
-    const int i0 = 2 * lane, i1 = 2 * lane + 1;
-    const bool has0 = i0 < a.slices, has1 = i1 < a.slices, rules = a.rules();
-    const bool few = a.few_kept(b);   // (then there are no bins and no list)
-    Cuts c = rules && !few ? a.cuts[b] : Cuts{};
-    const uint64_t* whole = rules ? a.whole : a.sums;
-    const uint64_t w0 = has0 && !few ? whole[slice0 + i0] : 0, w1 = has1 && !few ? whole[slice0 + i1] : 0;
-    const uint32_t l0 = rules && has0 && !few ? a.listed[slice0 + i0] : 0;
-    const uint32_t l1 = rules && has1 && !few ? a.listed[slice0 + i1] : 0;
-    if (wave == 0) slice_sums[i0] = w0, slice_sums[i1] = w1;
-    uint32_t held[kHeld] = {};
-    for (int i = 0; i < kHeld && few; ++i) {
-        const int g = i * kThreads + tid, groups = a.groups_of_row();
-        held[i] = g < groups ? a.groups[b * groups + g] : 0;
-    }
+    const bool rules = a.rules(), few = a.few_kept(b);
+    const Groups most(a, b);   // (asked for ahead of the rules)
+    if (tid < kMostSlices) slice_sums[tid] = !rules && tid < a.slices ? a.sums[slice0 + tid] : 0;
     make_table(s.table);
     const Rules r(a, b, s.table);
     if (r.first == 0 || r.greedy) {
@@ -1022,31 +1014,26 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
     }
     Kept kept{0, r.least};
     bool known = true;   // slice_sums are those of kept weights
+    Cuts c{};
     Own own{};
     if (rules) {
-        int listed;
+        __syncthreads();
+        int listed = 0;
         if (few) {
-            listed = list_first<kDtype>(a, b, (uint64_t)r.k, held, s);
-            known = listed >= 0;
+            listed = list_first<kDtype>(a, b, (uint64_t)r.k, most, s);
             c.one = true;
-            c.m_low = c.m_high = kBins + 1;
         } else {
-            // the listed tokens, one slice's after the other's
-            const uint64_t upto = wave_scan((uint64_t)l0 + l1), all = lane_of(upto, 63);
-            known = __ballot(l0 > kListed || l1 > kListed) == 0 && all <= kMostListed;
-            listed = (int)all;
-            if (known && wave == 0) {
-                list_at[i0] = (int)(upto - l0 - l1);
-                list_at[i1] = (int)(upto - l1);
-                if (lane == 63) list_at[kMostSlices] = listed;
+            c = cuts_of_row(a, b, r, s, slice_sums);
+            if (!(c.low > c.high)) {
+                listed = list_tokens<kDtype>(a, b, most, max(key_of(c.low), 1u), s, [&](uint32_t key) {
+                    const float x = logit_of(key);
+                    return !(x < c.low || x > c.high) && c.listed(bin_of(r.w.log2_of(key)));   // (T = inf: no high)
+                });
+            } else {
+                __syncthreads();
             }
-            __syncthreads();
-            for (int i = wave; known && i < a.slices; i += kWaves) {
-                const int at = list_at[i], count = list_at[i + 1] - at;
-                for (int e = lane; e < count; e += 64) s.list[at + e] = a.list[(slice0 + i) * kListed + e];
-            }
-            __syncthreads();
         }
+        known = listed <= kMostListed;
         if (!known) {
             kept.last = last_of_row<kDtype>(a, b, r, s);
         } else if (listed <= 64) {
@@ -1187,8 +1174,7 @@ int shift_of(int V) {   // a row's sum stays under 2^63
 
 int64_t sample_bytes(int rows, int V) {
     const int64_t slices = (int64_t)rows * slices_of(V).count;
-    return rows * ((int64_t)sizeof(Cuts) + ((int64_t)V + 63) / 64 * 4) +
-           slices * (8 + 8 + (kBins + 1) * 8 + kListed * 8 + (kBins + 1) * 4 + 4);
+    return rows * (((int64_t)V + kGroup - 1) / kGroup) * 4 + slices * (8 + (kBins + 1) * (8 + 4));
 }
 
 int launch_sample(const void* logits, int dtype, int64_t ld, int rows, int V, const float* u,
@@ -1199,14 +1185,10 @@ int launch_sample(const void* logits, int dtype, int64_t ld, int rows, int V, co
     const int64_t slices = (int64_t)rows * cut.count;
     SampleArgs a{logits, ld, V, shift_of(V), cut.count, cut.length, u, temperature, top_k, top_p, min_p,
                  tokens, logprobs};
-    a.cuts = static_cast<Cuts*>(workspace);
-    a.first = reinterpret_cast<uint64_t*>(a.cuts + rows);
-    a.whole = a.first + slices;
-    a.sums = a.whole + slices;
-    a.list = a.sums + slices * (kBins + 1);
-    a.counts = reinterpret_cast<uint32_t*>(a.list + slices * kListed);
-    a.listed = a.counts + slices * (kBins + 1);
-    a.groups = a.listed + slices;
+    a.first = static_cast<uint64_t*>(workspace);
+    a.sums = a.first + slices;
+    a.counts = reinterpret_cast<uint32_t*>(a.sums + slices * (kBins + 1));
+    a.groups = a.counts + slices * (kBins + 1);
     const dim3 grid(cut.count, rows);
     auto run = [&](auto type) {
         constexpr int kDtype = decltype(type)::value;
@@ -1214,10 +1196,6 @@ int launch_sample(const void* logits, int dtype, int64_t ld, int rows, int V, co
         hipLaunchKernelGGL(most, grid, dim3(kSliceThreads), 0, stream, a);
         auto* bins = a.rules() ? sample_bins_kernel<kDtype, true> : sample_bins_kernel<kDtype, false>;
         hipLaunchKernelGGL(bins, grid, dim3(kSliceThreads), 0, stream, a);
-        if (a.rules()) {
-            hipLaunchKernelGGL(sample_cuts_kernel, dim3(rows), dim3(kCutThreads), 0, stream, a);
-            hipLaunchKernelGGL(sample_list_kernel<kDtype>, grid, dim3(kSliceThreads), 0, stream, a);
-        }
         hipLaunchKernelGGL(sample_finish_kernel<kDtype>, dim3(rows), dim3(kThreads), 0, stream, a);
     };
     if (dtype == NB_F32) run(std::integral_constant<int, NB_F32>{});
