@@ -178,6 +178,28 @@ __device__ __forceinline__ Column column(const Args& a, int n) {
     return c;
 }
 
+// v Phi(v).  Phi(-a) = exp(-a^2 / 2) t P(t) for a >= 0 with t = 1 / (1 + 0.21 a): what is
+// left beside the exponential is smooth in t from 1/2 at 0 to its end, and a
+// polynomial of degree 8 (least largest relative error, fitted in 64 bits for
+// t of a up to 15, where the exponential is below fp32) is within 2.3e-8 of it.
+// Nothing cancels: a product on the left, at most half of v taken off on the right.
+// 18 instructions, no branch: 500 rows of 5003 x 1280 with erfcf 16.1 us, without
+// an activation 11.1, with this 13.1 (launches of a graph).
+__device__ __forceinline__ float gelu(float v) {
+    const float a = __builtin_fabsf(v), t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.21f, a, 1.f));
+    float p = -0.07094477862119675f;
+    p = __builtin_fmaf(p, t, 0.2800799608230591f);
+    p = __builtin_fmaf(p, t, -0.3228669762611389f);
+    p = __builtin_fmaf(p, t, 0.34074342250823975f);
+    p = __builtin_fmaf(p, t, -0.08775527775287628f);
+    p = __builtin_fmaf(p, t, 0.12213890254497528f);
+    p = __builtin_fmaf(p, t, 0.06992674618959427f);
+    p = __builtin_fmaf(p, t, 0.08495952934026718f);
+    p = __builtin_fmaf(p, t, 0.0837184712290764f);
+    const float tail = __builtin_amdgcn_exp2f(a * a * -0.72134752f) * (t * p);
+    return v < 0.f ? v * tail : __builtin_fmaf(-v, tail, v);
+}
+
 // The outputs of four sums: row m, layer outputs n .. n + 3.  Loads, arithmetic and
 // stores are apart, so that a loop can put several in flight (stores count among
 // the loads that a wait is for).
@@ -206,8 +228,7 @@ struct Finished {
             float out = y[e];
             if constexpr (kAct == NB_ACT_SWIGLU) out = silu(y[2 * e]) * y[2 * e + 1];
             else if constexpr (kAct == NB_ACT_SILU) out = silu(y[e]);
-            // v Phi(v) by erfc: no cancellation for negative v
-            else if constexpr (kAct == NB_ACT_GELU) out = 0.5f * y[e] * erfcf(-0.70710678f * y[e]);
+            else if constexpr (kAct == NB_ACT_GELU) out = gelu(y[e]);
             v[e] = kResidual ? out + v[e] : out;
         }
     }

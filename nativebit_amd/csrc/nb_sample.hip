@@ -35,8 +35,8 @@
 // by how many tokens are listed (4, 6, and 11 to 20).
 // Other ways measured: cuts and list as launches of their own, a slice each, 34 and
 // 59 us where it is now 29 and 48 (48 rows of 50257, 160 of 131077); a list that scans the
-// slice again instead of its groups 21 us at 160 rows, now 2 to 5; lists sorted by merging
-// 256 to 4096 neighbours 40 us of one row, through buckets 2.
+// slice again instead of its groups 21 us at 160 rows, now 2 to 5; 1000 tokens sorted by
+// merging 40 us, through buckets 2.
 // A row with over kMostListed listed tokens (equal logits, mostly) is worked out by
 // its last workgroup alone: radix selection over the row.
 #include <math.h>
