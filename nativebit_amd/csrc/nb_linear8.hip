@@ -2,7 +2,7 @@
 // nb_linear8_layout and nb_linear8.  Formulas and layout: nb_linear8.h.
 //
 // Few rows: bound by latency (a launch, one trip to the weights, the sum over the
-// waves; 2560 x 2560 at one row 3.9 us, 13824 x 2560 5.1 for 15.5 MB).  Many rows: bound
+// waves; 2560 x 2560 at one row 3.6 us, 13824 x 2560 5.1 for 15.5 MB).  Many rows: bound
 // by the LDS reads of rows and units beside the products (about 1700 of the 2048
 // cycles that a 256 x 256 x 128 step's products take, in a step of 3000; without
 // barriers 2600, without operands made 2400, loads alone 100), and at the ends by
