@@ -21,6 +21,9 @@ def test_generate_refuses_draws():
     for bad in (u[:1], u[0], u[:, :2], u[..., None]):
         with pytest.raises(ValueError, match="u must"):
             paged.generate(model, [[1], [2, 3]], 3, temperature=1.0, u=bad)
+    for k in (2.5, [1, 2.0]):
+        with pytest.raises(ValueError, match="whole"):
+            paged.generate(model, [[1], [2, 3]], 3, temperature=1.0, top_k=k)
     for kw in (dict(temperature=[1.0]), dict(top_k=[1, 2, 3]), dict(top_p=[[0.5, 0.5]]), dict(min_p=[])):
         with pytest.raises(ValueError, match="must be a number"):
             paged.generate(model, [[1], [2, 3]], 3, **{"temperature": 1.0, **kw})

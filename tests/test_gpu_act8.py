@@ -272,3 +272,27 @@ def test_rows_do_not_depend_on_the_batch(dev, N, K, activation, dtype):
         for a, b in ((h, h1), (q, q1)):
             assert torch.equal(a.codes[rows], b.codes) and torch.equal(a.scale[rows], b.scale)
         assert torch.equal(y[rows], y1)
+
+
+def test_rows_far_apart(dev):
+    """Inputs, sums, residuals and outputs whose rows pass 32 bits."""
+    far, K, N = (1 << 30) + 16, 256, 48
+    g = torch.Generator().manual_seed(16)
+
+    def wide(t):
+        out = torch.empty(2 * far + t.shape[1], dtype=t.dtype, device=dev).as_strided(t.shape, (far, 1))
+        return out.copy_(t)
+    x, y = (torch.randn(3, K, generator=g).to(dev) for _ in range(2))
+    weight = torch.rand(K, generator=g).to(dev)
+    packed = ops.pack(torch.randint(0, 8, (N * K,), generator=g, dtype=torch.uint8).to(dev), 3)
+    w = ops.linear8_layout(packed, torch.randn(N * K // 128, 8, generator=g).to(dev), N, K)
+    h, s = ops.rmsnorm8(x, weight, residual=y)
+    a = wide(x)
+    h1, s1 = ops.rmsnorm8(a, weight, residual=y, out=a)
+    assert s1 is a and torch.equal(s, a) and torch.equal(h.codes, h1.codes) and torch.equal(h.scale, h1.scale)
+    q, q1 = ops.quantize8(s), ops.quantize8(a)
+    assert torch.equal(q.codes, q1.codes) and torch.equal(q.scale, q1.scale)
+    r = torch.randn(3, N, generator=g).to(dev)
+    out = wide(r)
+    assert ops.linear8(q, w, residual=out, out=out) is out
+    assert torch.equal(out, ops.linear8(q, w, residual=r))

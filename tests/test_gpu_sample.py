@@ -193,3 +193,45 @@ def test_most_of_a_large_vocabulary_kept(dev):
     x = torch.randn(6, 100003, generator=torch.Generator().manual_seed(12)) * 3
     check(dev, x, numbers(6, 1), top_k=ks, temperature=[5.0] * 6)
     check(dev, x, numbers(6, 2), top_k=ks, top_p=[0.97] * 6, min_p=[1e-3] * 6)
+
+
+def test_vocabularies_of_many_groups(dev):
+    """More groups of 32 tokens than are looked at together."""
+    B, V = 4, 300001
+    x = torch.randn(B, V, generator=torch.Generator().manual_seed(13)) * 3
+    check(dev, x, numbers(B, 1), top_k=[3, 100, 2048, 2049])
+    check(dev, x, numbers(B, 2), top_p=[0.3, 0.9, 0.99, 0.9999], temperature=[1.0, 1.0, 1.5, 3.0])
+    check(dev, x, numbers(B, 3), min_p=[0.5, 1e-2, 1e-4, 1e-6])
+
+
+@pytest.mark.parametrize("rules", [{}, {"top_k": 700}, {"top_k": 2900}, {"top_p": 0.97}, {"min_p": 1e-3},
+                                   {"top_k": 200, "top_p": 0.8, "min_p": 1e-3}])
+def test_largest_vocabulary(dev, rules):
+    """2^24 tokens, all but 3000 of them masked, against those 3000 by themselves (their
+    weights are whole numbers of 2^-38 and 2^-45: u is not near a border)."""
+    B, V, n = 3, 1 << 24, 3000
+    g = torch.Generator().manual_seed(14)
+    few = (torch.randn(B, n, generator=g) * 3).to(dev)
+    at = torch.randperm(V, generator=g)[:n].sort().values.to(dev)
+    x = torch.full((B, V), -math.inf, device=dev)
+    x[:, at] = few
+    args = {k: torch.full((B,), v, dtype=torch.int32 if k == "top_k" else torch.float32, device=dev)
+            for k, v in rules.items()}
+    for u in ([0.1, 0.5, 0.9], [0.3141, 0.001, 0.77]):
+        u = torch.tensor(u, device=dev)
+        want, lp = ops.sample(few, u, logprobs=True, **args)
+        got, lq = ops.sample(x, u, logprobs=True, **args)
+        assert torch.equal(at[want.long()].int(), got)
+        # (sums of up to 3000 weights that are half of 2^-38 off, of 1 or more; fp32's half step)
+        assert ((lp - lq).abs() <= 3000 * 2.0 ** -38 + 2.0 ** -24 * lp.abs() * 2).all()
+
+
+def test_rows_far_apart(dev):
+    """Rows whose elements' numbers and bytes pass 32 bits."""
+    far, V = (1 << 31) + 24, 700
+    x = torch.randn(3, V, generator=torch.Generator().manual_seed(15)).to(torch.bfloat16)
+    wide = torch.empty(2 * far + V, dtype=torch.bfloat16, device=dev).as_strided((3, V), (far, 1))
+    wide.copy_(x)
+    u = torch.tensor([0.2, 0.6, 0.95], device=dev)
+    for k in (None, torch.tensor([5, 40, 0], dtype=torch.int32, device=dev)):
+        assert torch.equal(ops.sample(wide, u, top_k=k), ops.sample(x.to(dev), u, top_k=k))
