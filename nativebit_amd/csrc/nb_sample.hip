@@ -28,13 +28,13 @@
 // tokens that reach it, and those are in the groups that do; k of them, but for
 // ties.  They are listed, and that is all that is read again of the row.
 // What it takes: 160 rows of 131077 fp32 logits with every rule and top_k of 1 to 1024
-// 48 us, 84 MB.  1 reads them at 3.6 TB/s in 23.5; 2 finds nothing to do in 4; 3 is
+// 47 us, 84 MB.  1 reads them at 3.6 TB/s in 23.5; 2 finds nothing to do in 4; 3 is
 // one memory round trip after the other (rules, groups, tokens, 2 us each) and some
-// twenty waits of a workgroup between, 22.  Without top_k 90 us: 2 takes 41, an exp in
-// 64 bits and an atomic in LDS for every token.  One row of 50257 with top_p 25 to 35 us
+// twenty waits of a workgroup between, 20.  Without top_k 90 us: 2 takes 41, an exp in
+// 64 bits and an atomic in LDS for every token.  One row of 50257 with top_p 25 to 36 us
 // by how many tokens are listed (4, 6, and 11 to 20).
 // Other ways measured: cuts and list as launches of their own, a slice each, 34 and
-// 59 us where it is now 29 and 48 (48 rows of 50257, 160 of 131077); a list that scans the
+// 59 us where one took 29 and 48 (48 rows of 50257, 160 of 131077); a list that scans the
 // slice again instead of its groups 21 us at 160 rows, now 2 to 5; 1000 tokens sorted by
 // merging 40 us, through buckets 2.
 // A row with over kMostListed listed tokens (equal logits, mostly) is worked out by
@@ -78,11 +78,12 @@ struct SampleArgs {
     __host__ __device__ __forceinline__ bool rules() const { return top_k || top_p || min_p; }
     __host__ __device__ __forceinline__ int groups_of_row() const { return (V + kGroup - 1) / kGroup; }
     // A row whose kept tokens are in few groups: its bins are not needed.  48 rows of
-    // 50257 (1571 groups) with k = 50, 500, 1024, 1177, 1300, 1500: 23, 31, 38, 41, 45 and
-    // 84 us so, 38, 46, 49, 48, 49 and 49 us by bins; 160 rows of 131077 with 2048: 77, 122.
+    // 50257 (1571 groups) with k = 50, 500, 1024, 1300 and 1500 and the other rules: 20, 26,
+    // 30, 36 and 43 us so, 38, 46, 49, 48 and 48 us by bins; 300 of 10007 (313 groups) 21 and
+    // 26 (without the other rules 26 and 24); 160 rows of 131077 with 2048: 57 and 111.
     __device__ __forceinline__ bool few_kept(int64_t b) const {
         const int64_t k = top_k ? as_constant(top_k)[b] : 0;
-        return k > 0 && k <= kFewKept && k <= groups_of_row() * 3ll / 4;
+        return k > 0 && k < V && k <= kFewKept && k <= groups_of_row();
     }
 };
 
@@ -226,9 +227,17 @@ __device__ __forceinline__ uint64_t dpp64(uint64_t v) {   // 0 where no lane is 
     const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), kCtrl, kRows, 0xf, true);
     return (uint64_t)(uint32_t)hi << 32 | (uint32_t)lo;
 }
-template <int kCtrl>
+template <int kCtrl, int kRows = 0xf>
 __device__ __forceinline__ uint32_t dpp32(uint32_t v) {
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, 0xf, 0xf, true);
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, kRows, 0xf, true);
+}
+__device__ __forceinline__ uint32_t wave_scan32(uint32_t v) {
+    v += dpp32<0x111>(v);
+    v += dpp32<0x112>(v);
+    v += dpp32<0x114>(v);
+    v += dpp32<0x118>(v);
+    v += dpp32<0x142, 0xa>(v);
+    return v + dpp32<0x143, 0xc>(v);
 }
 template <typename Join>
 __device__ __forceinline__ uint64_t wave_scan(uint64_t v, Join join) {   // of lanes 0 .. this one
@@ -591,28 +600,54 @@ __device__ uint64_t select(const SampleArgs& a, int64_t b, Shared& s, uint32_t l
     return above;
 }
 
-// A key that k or more of those that each(f) gives reach, and but for its lower ten bits
-// no larger one that so many do; 1 where they are fewer.
+// A key that k or more of those that each(f) gives reach, and few more than k do (but for
+// equal ones); 1 where they are fewer.  `high`: none is larger.  Counted in buckets of
+// neighbouring keys between the least and it (by the keys' upper bits 64 lanes would
+// meet in a handful of words: 5 us of a row), once, or again in the bucket of the k-th
+// where outliers leave many in it.
 template <typename Each>
-__device__ uint32_t edge_of(Shared& s, uint64_t k, Each each) {
-    uint64_t above = 0;
-    uint32_t prefix = 0, mask = 0;
-    for (int shift = 21; shift >= 10; shift -= 11) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < kDigits; i += kThreads) s.digits[i] = 0;
+__device__ __forceinline__ uint32_t edge_of(Shared& s, uint32_t k, uint32_t high, Each each) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint32_t least = ~0u;
+    each([&](uint32_t key) { least = min(least, key ? key : ~0u); });
+    least = ~(uint32_t)wave_max(~least);
+    __syncthreads();
+    if (tid == 0) s.key_low = ~0u;
+    __syncthreads();
+    if (lane == 0) atomicMin(&s.key_low, least);
+    __syncthreads();
+    uint32_t low = s.key_low;
+    if (low > high) return 1;   // (there are none)
+    for (;;) {
+        const int shift = max(32 - __clz((int)(high - low)) - 11, 0);
+        s.bucket[2 * tid] = s.bucket[2 * tid + 1] = 0;
+        if (tid == 0) s.found[1] = kDigits;
         __syncthreads();
         each([&](uint32_t key) {
-            if (key && (key & mask) == prefix) {
-                atomicAdd((unsigned long long*)&s.digits[key >> shift & (kDigits - 1)], 1ull);
-            }
+            if (key >= low && key <= high) atomicAdd(&s.bucket[(high - key) >> shift], 1u);
         });
         __syncthreads();
-        const Crossing c = cross(s, k - above);   // (none: digit 0)
-        above += c.above;
-        prefix |= (uint32_t)c.bin << shift;
-        mask |= (uint32_t)(kDigits - 1) << shift;
+        const uint32_t first = s.bucket[2 * tid], both = first + s.bucket[2 * tid + 1];
+        uint32_t before = wave_scan32(both);
+        if (lane == 63) s.part[wave] = before;
+        __syncthreads();
+        for (int i = 0; i < wave; ++i) before += (uint32_t)s.part[i];
+        before -= both;
+        if (before < k && before + both >= k) {   // one thread
+            const bool second = before + first < k;
+            s.found[1] = 2 * tid + second;
+            s.found[0] = before + (second ? first : 0);
+        }
+        __syncthreads();
+        const uint32_t bucket = (uint32_t)s.found[1], above = (uint32_t)s.found[0];
+        if (bucket == kDigits) return 1;
+        const uint32_t count = s.bucket[bucket];
+        high -= bucket << shift;
+        low = max(low, high - min(high, (1u << shift) - 1));
+        if (shift == 0 || above + count <= k + k / 8 + 32) return max(low, 1u);
+        k -= above;
+        __syncthreads();
     }
-    return max(prefix, 1u);
 }
 
 // A row's largest keys of groups, the first kMostGroups in registers.
@@ -634,30 +669,46 @@ struct Groups {
     }
 };
 
-// f(token, key) for the tokens of the groups whose largest key is `least` (not 0) or more,
-// by all threads; waits before it and after.
+// Where a lane's n entries go in an array that all waves fill: `filled` counts them.
+__device__ __forceinline__ uint32_t append(uint32_t* filled, uint32_t n) {
+    const uint32_t upto = wave_scan32(n), all = __builtin_amdgcn_readlane((int)upto, 63);
+    uint32_t at = 0;
+    if ((threadIdx.x & 63) == 63 && all) at = atomicAdd(filled, all);
+    return (uint32_t)__builtin_amdgcn_readlane((int)at, 63) + upto - n;
+}
+
+// f(tokens, keys of four from each on) for the tokens of the groups whose largest key is
+// `least` (not 0) or more, by all threads, lanes of a wave together; waits before it and
+// after.
+constexpr int kAtOnce = 4;   // groups of a lane
 template <int kDtype, typename F>
 __device__ __forceinline__ void for_groups(const SampleArgs& a, int64_t b, const Groups& groups, uint32_t least,
                                            Shared& s, F f) {
     const int tid = threadIdx.x;
-    constexpr int kLanes = kGroup / 4, kStep = kThreads / kLanes, kAtOnce = 4;   // four tokens a lane
+    constexpr int kLanes = kGroup / 4, kStep = kThreads / kLanes;   // four tokens a lane
     const int64_t size = kDtype == NB_F32 ? 4 : 2;
     const char* row = static_cast<const char*>(a.logits) + b * a.ld * size;
     for (int g0 = 0; g0 < groups.count; g0 += kMostGroups) {
         __syncthreads();
         if (tid == 0) s.some_groups = 0;
         __syncthreads();
+        bool reach[kHeld];
+        uint32_t count = 0;
 #pragma unroll
         for (int i = 0; i < kHeld; ++i) {
-            const int g = g0 + i * kThreads + tid;
-            const uint32_t most = g0 ? groups.at(g) : groups.held[i];
-            if (most >= least) s.groups[atomicAdd(&s.some_groups, 1u)] = (uint32_t)g;
+            reach[i] = (g0 ? groups.at(g0 + i * kThreads + tid) : groups.held[i]) >= least;
+            count += reach[i];
+        }
+        uint32_t at = append(&s.some_groups, count);
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            if (reach[i]) s.groups[at++] = (uint32_t)(g0 + i * kThreads + tid);
         }
         __syncthreads();
         const int some = (int)s.some_groups;
-        for (int i0 = tid / kLanes; i0 < some; i0 += kStep * kAtOnce) {
+        for (int i0 = tid / kLanes; i0 - i0 % (64 / kLanes) < some; i0 += kStep * kAtOnce) {
             int v[kAtOnce];
-            uint32_t x[kAtOnce][kDtype == NB_F32 ? 4 : 2];
+            uint32_t keys[kAtOnce][4], x[kAtOnce][kDtype == NB_F32 ? 4 : 2];
 #pragma unroll
             for (int i = 0; i < kAtOnce; ++i) {
                 const int at = i0 + i * kStep;
@@ -691,46 +742,67 @@ __device__ __forceinline__ void for_groups(const SampleArgs& a, int64_t b, const
                     uint32_t y;
                     if constexpr (kDtype == NB_F32) y = x[i][e];
                     else y = e & 1 ? x[i][e / 2] & 0xffff0000u : x[i][e / 2] << 16;
-                    f(v[i] + e, key_of(__uint_as_float(y)));
+                    keys[i][e] = key_of(__uint_as_float(y));
                 }
             }
+            f(v, keys);
         }
     }
     __syncthreads();
 }
 
 // Lists the tokens of groups from `least` on that take(key) names; how many they are,
-// more than kMostListed: not all are listed.
-template <int kDtype, typename Take>
+// more than kMostListed: not all are listed.  kDense: many are, so a wave finds its room
+// at once; else each token by itself (a row cut by top_p takes 1 us less of 29 so, rows
+// cut by top_k 1.5 to 2 more, of 28 and 47).
+template <int kDtype, bool kDense, typename Take>
 __device__ __forceinline__ int list_tokens(const SampleArgs& a, int64_t b, const Groups& groups, uint32_t least,
                                            Shared& s, Take take) {
     if (threadIdx.x == 0) s.some = 0;
-    for_groups<kDtype>(a, b, groups, least, s, [&](int v, uint32_t key) {
-        if (!key || !take(key)) return;
-        const uint32_t at = atomicAdd(&s.some, 1u);
-        if (at < kMostListed) s.list[at] = place_of(key, v);
+    for_groups<kDtype>(a, b, groups, least, s, [&](const int (&v)[kAtOnce], const uint32_t (&keys)[kAtOnce][4]) {
+        uint32_t taken = 0, at = 0;
+        if (kDense) {
+#pragma unroll
+            for (int i = 0; i < kAtOnce * 4; ++i) {
+                if (take(keys[i / 4][i % 4])) taken |= 1u << i;
+            }
+            if (!__ballot(taken)) return;
+            at = append(&s.some, __popc(taken));
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce * 4; ++i) {
+            const uint32_t key = keys[i / 4][i % 4];
+            if (kDense ? !(taken >> i & 1) : !key || !take(key)) continue;
+            if (!kDense) at = atomicAdd(&s.some, 1u);
+            if (at < kMostListed) s.list[at] = place_of(key, v[i / 4] + i % 4);
+            ++at;
+        }
     });
     return (int)s.some;
 }
 
 // Lists a row's first tokens, k or more of them (all, if they are fewer): a key that the
 // largest of k groups reach is one that k tokens do, and all that reach it are in
-// those groups.
+// those groups.  Returns how many they are, over kMostListed: not all are listed.
 template <int kDtype>
-__device__ int list_first(const SampleArgs& a, int64_t b, uint64_t k, const Groups& groups, Shared& s) {
-    uint32_t edge = edge_of(s, k, [&](auto f) { groups.each(f); });
-    for (int turn = 0;; ++turn) {
-        const int n = list_tokens<kDtype>(a, b, groups, edge, s, [&](uint32_t key) { return key >= edge; });
-        if (n <= kMostListed || turn) return n;
-        // groups with many such tokens (neighbours that are alike): the edge of tokens
-        edge = edge_of(s, k, [&](auto f) {
-            for_groups<kDtype>(a, b, groups, edge, s, [&](int, uint32_t key) { f(key); });
+__device__ __forceinline__ int list_first(const SampleArgs& a, int64_t b, const Rules& r, const Groups& groups, Shared& s) {
+    const uint32_t k = (uint32_t)r.k, high = key_of_place(r.first);
+    uint32_t edge = edge_of(s, k, high, [&](auto f) { groups.each(f); });
+    for (;;) {
+        const int n = list_tokens<kDtype, true>(a, b, groups, edge, s, [&](uint32_t key) { return key >= edge; });
+        if (n <= kMostListed) return n;
+        // groups with many such tokens (neighbours that are alike): a key that k of those
+        // that found room reach
+        const uint32_t higher = edge_of(s, k, high, [&](auto f) {
+            for (int i = threadIdx.x; i < kMostListed; i += kThreads) f(key_of_place(s.list[i]));
         });
+        if (higher <= edge) return n;
+        edge = higher;
     }
 }
 
 // A row's cuts from its bins, the sums of those that are kept whole into slice_sums.
-__device__ Cuts cuts_of_row(const SampleArgs& a, int64_t b, const Rules& r, Shared& s,
+__device__ __forceinline__ Cuts cuts_of_row(const SampleArgs& a, int64_t b, const Rules& r, Shared& s,
                             unsigned long long* slice_sums) {
     constexpr int kAll = kBins + 1;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -839,7 +911,7 @@ __device__ void sort_list(Shared& s, int n) {
     for (int i = tid; i < n; i += kThreads) atomicAdd(&s.bucket[bucket_of(s.list[i])], 1u);
     __syncthreads();
     const uint32_t first = s.bucket[2 * tid], both = first + s.bucket[2 * tid + 1];
-    uint32_t upto = (uint32_t)wave_scan((uint64_t)both);
+    uint32_t upto = wave_scan32(both);
     if (lane == 63) s.part[wave] = upto;
     __syncthreads();
     for (int i = 0; i < wave; ++i) upto += (uint32_t)s.part[i];
@@ -1030,12 +1102,12 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
         __syncthreads();
         int listed = 0;
         if (few) {
-            listed = list_first<kDtype>(a, b, (uint64_t)r.k, most, s);
+            listed = list_first<kDtype>(a, b, r, most, s);
             c.one = true;
         } else {
             c = cuts_of_row(a, b, r, s, slice_sums);
             if (!(c.low > c.high)) {
-                listed = list_tokens<kDtype>(a, b, most, max(key_of(c.low), 1u), s, [&](uint32_t key) {
+                listed = list_tokens<kDtype, false>(a, b, most, max(key_of(c.low), 1u), s, [&](uint32_t key) {
                     const float x = logit_of(key);
                     return !(x < c.low || x > c.high) && c.listed(bin_of(r.w.log2_of(key)));   // (T = inf: no high)
                 });
@@ -1110,8 +1182,8 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
     }
     // the slice is split over the waves, a large one's part with the token again
     int lo = part * a.length, hi = min(lo + a.length, a.V);
-    constexpr int kAtOnce = 16;   // groups of 64 tokens of a wave
-    while (hi - lo > kThreads * kAtOnce) {
+    constexpr int kInHand = 16;   // groups of 64 tokens of a wave
+    while (hi - lo > kThreads * kInHand) {
         const int each = ((hi - lo + kWaves - 1) / kWaves + 63) / 64 * 64;
         const int begin = min(lo + wave * each, hi), end = min(begin + each, hi);
         uint64_t sum = 0;
@@ -1128,16 +1200,16 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
     // then its weights are in registers, 64 neighbours in those of a number
     const int groups = (hi - lo + kThreads - 1) / kThreads;   // of a wave
     const int begin = lo + wave * groups * 64;
-    uint64_t weights[kAtOnce], sum = 0;
+    uint64_t weights[kInHand], sum = 0;
     {
-        uint32_t keys[kAtOnce];
+        uint32_t keys[kInHand];
 #pragma unroll
-        for (int g = 0; g < kAtOnce; ++g) {
+        for (int g = 0; g < kInHand; ++g) {
             const int v = begin + g * 64 + lane;
             keys[g] = g < groups && v < hi ? key_at<kDtype>(a, b, v) : 0;
         }
 #pragma unroll
-        for (int g = 0; g < kAtOnce; ++g) {
+        for (int g = 0; g < kInHand; ++g) {
             weights[g] = g < groups ? kept.weight(r.w, keys[g], begin + g * 64 + lane) : 0;
             sum += weights[g];
         }
@@ -1149,7 +1221,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
     for (part = 0; part < kWaves - 1 && rest >= s.part[part]; ++part) rest -= s.part[part];
     if (wave != part) return;
 #pragma unroll
-    for (int g = 0; g < kAtOnce; ++g) {
+    for (int g = 0; g < kInHand; ++g) {
         const uint64_t upto = wave_scan(weights[g]), all = lane_of(upto, 63);
         if (rest < all) {
             if (upto > rest && upto - weights[g] <= rest) {   // one lane
