@@ -1,5 +1,5 @@
 """Serving several requests of different lengths with one 8-bit key / value
-cache: the cache, and greedy generation over it.
+cache: the cache, and generation over it.
 
 ``PagedCache`` holds, for every layer of a ``PackedGPT``, blocks of 64 tokens
 (int8 codes, one fp32 scale for each block and head) that the requests share:
