@@ -16,6 +16,7 @@
 #include <type_traits>
 
 #include "nb_linear8.h"
+#include "nb_linear8_forms.h"
 
 namespace nb {
 namespace {
@@ -419,66 +420,32 @@ __global__ __launch_bounds__(64 * kN * kM * kSplit, 2) void linear8_tiles_kernel
     }
 }
 
-template <int kWaves, int kI, int kJ>
+template <int kForm, int kWaves, int kI, int kJ>
 void launch_rows(const Args& a, bool bf16, hipStream_t stream) {
-    const dim3 grid((unsigned)((a.N + 16 * kI - 1) / (16 * kI)), (unsigned)((a.M + 16 * kJ - 1) / (16 * kJ)));
+    constexpr Form f = kForms[kForm];
+    static_assert(!f.tiles && f.outputs == 16 * kI && f.rows == 16 * kJ && f.split == kWaves, "the form");
+    const dim3 grid((unsigned)output_groups(f, a.N), (unsigned)row_groups(f, a.M));
     constexpr size_t lds = (size_t)kWaves * kI * kJ * 64 * 16;
     auto* kernel = bf16 ? linear8_rows_kernel<kWaves, kI, kJ, true> : linear8_rows_kernel<kWaves, kI, kJ, false>;
     hipLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), lds, stream, a);
 }
 
-template <int kI, int kJ, int kN, int kM, int kStages, int kSplit>
+template <int kForm, int kI, int kJ, int kN, int kM, int kStages, int kSplit>
 void launch_tiles(const Args& a, bool bf16, hipStream_t stream) {
     using T = Tile<kI, kJ, kN, kM, kStages, kSplit>;
-    const int64_t grid = (int64_t)((a.N + T::kOutputs - 1) / T::kOutputs) * ((a.M + T::kRows - 1) / T::kRows);
+    constexpr Form f = kForms[kForm];
+    static_assert(f.tiles && f.outputs == T::kOutputs && f.rows == T::kRows && f.split == kSplit, "the form");
+    const dim3 grid((unsigned)(output_groups(f, a.N) * row_groups(f, a.M)));
     auto* kernel = bf16 ? linear8_tiles_kernel<kI, kJ, kN, kM, kStages, kSplit, true>
                         : linear8_tiles_kernel<kI, kJ, kN, kM, kStages, kSplit, false>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(T::kThreads), T::kLds, stream, a);
+    hipLaunchKernelGGL(kernel, grid, dim3(T::kThreads), T::kLds, stream, a);
 }
 
-// The forms, and what each costs in microseconds: `launch` once, `start` for the
-// workgroups that a CU holds at once, `step[c - 1]` for a block of K (of `split`) with c of
-// them.  Fitted to 413 shapes (1 to 2500 rows, 64 to 16000 outputs, K of 128 to 8192)
-// times 10 forms on MI355X; the form of least estimated time is 2 % slower than
-// the fastest one on the mean, half as long again at worst (long K, few outputs,
-// hundreds of rows).  What the other forms lose where each is taken: 9 rows of 7680 x 2560
-// 4.4 us by 32 x 32 (rows), 5.2 by 16 x 16, 6.4 by 64 x 32; 129 of 2560 x 6912 13.0 by 64 x
-// 32, 14.4 by 64 x 64, 18.3 by rows; 512 of 2560 x 6912 20.2 by 128 x 64 of two
-// groups, 27.3 of one, 27.9 by 64 x 64; 1500 of it 30.7 by 128 x 128 of two groups, 36.0 by
-// 128 x 64, 36.8 of one; 1500 of 13824 x 2560 67 by 128 x 128 of one, 85 of two, 75 by 256
-// x 256; 2048 of it 79.5 by 256 x 256, 85 by 128 x 128.
-struct Form {
-    int outputs, rows, split, resident;
-    float launch, start, step[2];
-    void (*run)(const Args&, bool, hipStream_t);
+void (*const kRun[kFormCount])(const Args&, bool, hipStream_t) = {
+    launch_rows<0, 8, 1, 1>,           launch_rows<1, 8, 2, 2>,           launch_tiles<2, 1, 2, 4, 1, 4, 2>,
+    launch_tiles<3, 1, 4, 4, 1, 4, 2>, launch_tiles<4, 2, 4, 4, 1, 3, 2>, launch_tiles<5, 2, 4, 4, 1, 3, 1>,
+    launch_tiles<6, 2, 8, 4, 1, 3, 2>, launch_tiles<7, 2, 8, 4, 1, 3, 1>, launch_tiles<8, 4, 8, 4, 2, 3, 1>,
 };
-const Form kForms[] = {
-    {16, 16, 8, 1, 3.11f, 0.f, {0.276f}, launch_rows<8, 1, 1>},
-    {32, 32, 8, 2, 3.0f, 0.f, {0.58f, 1.21f}, launch_rows<8, 2, 2>},
-    {64, 32, 2, 2, 1.65f, 1.98f, {0.287f, 0.516f}, launch_tiles<1, 2, 4, 1, 4, 2>},
-    {64, 64, 2, 1, 1.03f, 2.46f, {0.397f}, launch_tiles<1, 4, 4, 1, 4, 2>},
-    {128, 64, 2, 1, 0.38f, 3.25f, {0.603f}, launch_tiles<2, 4, 4, 1, 3, 2>},
-    {128, 64, 1, 2, 1.25f, 2.36f, {0.392f, 0.546f}, launch_tiles<2, 4, 4, 1, 3, 1>},
-    {128, 128, 2, 1, 0.f, 4.53f, {0.919f}, launch_tiles<2, 8, 4, 1, 3, 2>},
-    {128, 128, 1, 1, 2.12f, 2.32f, {0.497f}, launch_tiles<2, 8, 4, 1, 3, 1>},
-    {256, 256, 1, 1, 0.f, 6.93f, {1.446f}, launch_tiles<4, 8, 4, 2, 3, 1>},
-};
-
-const Form& form_of(int M, int N, int K) {
-    const int64_t cus = device_cu_count();
-    const Form* best = &kForms[0];
-    float least = INFINITY;
-    for (const Form& f : kForms) {
-        const int64_t grid = ((int64_t)N + f.outputs - 1) / f.outputs * (((int64_t)M + f.rows - 1) / f.rows);
-        if (grid >= 1 << 22) continue;   // (a launch is under 2^32 threads; M N < 2^36: 256 x 256 fits)
-        const int64_t each = (grid + cus - 1) / cus, rest = each % f.resident;
-        const float steps = (float)((K / 128 + f.split - 1) / f.split);
-        float t = f.launch + (float)(each / f.resident) * (f.start + steps * f.step[f.resident - 1]);
-        if (rest) t += f.start + steps * f.step[rest - 1];
-        if (t < least) least = t, best = &f;
-    }
-    return *best;
-}
 
 }  // namespace
 
@@ -501,7 +468,7 @@ int launch_linear8(const int8_t* x, int64_t ld_x, const float* x_scale, const ui
                    hipStream_t stream) {
     const Args a{x, ld_x, x_scale, tiles, scale, bias, residual, ld_residual, y, ld_y, M, N, K,
                  activation};
-    form_of(M, N, K).run(a, y_dtype == NB_BF16, stream);
+    kRun[form_of(M, N, K, device_cu_count())](a, y_dtype == NB_BF16, stream);
     return check_launch("nb_linear8");
 }
 
