@@ -96,6 +96,14 @@ __device__ __forceinline__ float wave64_max(float v) {
                  fmaxf(lane_value(v, 32), lane_value(v, 48)));
 }
 
+// Between LDS accesses of one wave's lanes to the same words: the wave's LDS operations
+// run in order, and this keeps the compiler from putting them in another.
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // f rounded to the nearest bfloat16 (ties to even), kept as a float.
 __device__ __forceinline__ float round_bf16(float f) {
     return bf16_to_f32(f32_to_bf16_rne(f));

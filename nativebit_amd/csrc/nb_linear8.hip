@@ -372,7 +372,11 @@ __global__ __launch_bounds__(64 * kN * kM * kSplit, 2) void linear8_tiles_kernel
     for (int j0 = 0; j0 < kJ; j0 += T::kHalf) {
         const int first = m0 + (wm * kJ + j0) * 16;
         const float xs = a.x_scale[min(first + lane, a.M - 1)];   // of 16 kHalf <= 64 rows
-        if (kSplit > 1 && j0) __syncthreads();
+        // (of one group: written and read by the wave itself)
+        if (j0) {
+            if (kSplit > 1) __syncthreads();
+            else wave_lds_order();
+        }
 #pragma unroll
         for (int i = 0; i < kI; ++i)
 #pragma unroll
@@ -380,7 +384,8 @@ __global__ __launch_bounds__(64 * kN * kM * kSplit, 2) void linear8_tiles_kernel
                 *reinterpret_cast<i4*>(sums + all * kRegion + (j * 16 + fr) * T::kPitch + i * 16 +
                                        fq * 4) = sum[i][j0 + j];
             }
-        if (kSplit > 1) __syncthreads();   // (else read by the wave itself, in order)
+        if (kSplit > 1) __syncthreads();
+        else wave_lds_order();
         by_activation(a.activation, [&](auto act) {
             constexpr int kAct = decltype(act)::value;
             auto leave = [&](auto residual) {

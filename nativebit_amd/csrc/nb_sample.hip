@@ -948,8 +948,10 @@ __device__ uint64_t last_of_few(const SampleArgs& a, const Rules& r, const Cuts&
     int rank = 0;
 #pragma unroll 8
     for (int j = 0; j < n; ++j) rank += list[j] > place;
-    // (into the order; the wave's LDS operations are in order)
+    // into the order
+    wave_lds_order();
     if (lane < n) list[rank] = place;
+    wave_lds_order();
     place = lane < n ? list[lane] : 0;
     const uint32_t key = key_of_place(place);
     const double z = key ? r.w.log2_of(key) : 0.0;
