@@ -44,7 +44,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib, formats, ops, synth
-from .linear import PackedLinear, PackedLinear8, check_rows8
+from .linear import PackedLinear, PackedLinear8
 from .ops import _stream
 from .paged import PagedCache, PagedLayer
 
@@ -309,15 +309,23 @@ class TransformerBlock8(nn.Module):
     them in 8 bits (nb_rmsnorm8), the attention's and the gated products are
     quantized (nb_quantize8); the projections add to the stream in their
     epilogue, gate and up are one layer with the gated product in its
-    (nb_linear8).  The stream, attention and its cache are what they were."""
+    (nb_linear8).  The stream, attention and its cache are what they were.
+    ``layers``: those of ``layers_of(block)``, if they are made already."""
 
-    def __init__(self, block: TransformerBlock):
+    def __init__(self, block: TransformerBlock, layers: tuple | None = None):
         super().__init__()
+        qkv, out_proj, gate_up, down = layers or self.layers_of(block)
         self.ln1, self.ln2, self.attn = block.ln1, block.ln2, block.attn
-        self.attn.qkv = PackedLinear8.from_packed_linear(block.attn.qkv)
-        self.attn.out_proj = PackedLinear8.from_packed_linear(block.attn.out_proj)
-        self.gate_up = PackedLinear8.from_pairs(block.ffn.gate, block.ffn.up)
-        self.down = PackedLinear8.from_packed_linear(block.ffn.down)
+        self.attn.qkv, self.attn.out_proj = qkv, out_proj
+        self.gate_up, self.down = gate_up, down
+
+    @staticmethod
+    def layers_of(block: TransformerBlock) -> tuple:
+        """The block's four products for rows in 8 bits; it is left as it is."""
+        return (PackedLinear8.from_packed_linear(block.attn.qkv),
+                PackedLinear8.from_packed_linear(block.attn.out_proj),
+                PackedLinear8.from_pairs(block.ffn.gate, block.ffn.up),
+                PackedLinear8.from_packed_linear(block.ffn.down))
 
     def forward(self, x, kv_cache=None, pos_offset=0):
         B, T, C = x.shape
@@ -410,12 +418,10 @@ def quantize_activations(model: PackedGPT) -> PackedGPT:
     returned.  Its layers are PackedLinear of 3 bits, 8 entries and blocks of
     128; the packed streams are replaced by the layout that the products
     read, so DecodeEngine and to_nbpack_params take a model before it."""
-    for block in model.blocks:      # (all before the first is changed)
-        if not isinstance(block, TransformerBlock8):
-            for layer in (block.attn.qkv, block.attn.out_proj, block.ffn.gate, block.ffn.up, block.ffn.down):
-                check_rows8(layer)
-    model.blocks = nn.ModuleList([block if isinstance(block, TransformerBlock8) else
-                                  TransformerBlock8(block) for block in model.blocks])
+    layers = {block: TransformerBlock8.layers_of(block) for block in model.blocks
+              if not isinstance(block, TransformerBlock8)}      # (all before the first is changed)
+    made = {block: TransformerBlock8(block, of) for block, of in layers.items()}
+    model.blocks = nn.ModuleList([made.get(block, block) for block in model.blocks])
     return model
 
 
