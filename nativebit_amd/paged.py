@@ -232,8 +232,11 @@ def generate(model, prompts, n_generate: int, *, repetition=None, frequency=None
         u = torch.as_tensor(u, dtype=torch.float32)
         if u.shape != (n, n_generate):
             raise ValueError(f"u must be ({n}, {n_generate}), got {tuple(u.shape)}")
-    if top_k is not None and torch.as_tensor(top_k).is_floating_point():
-        raise ValueError("top_k must be whole numbers")
+    if top_k is not None:
+        top_k = torch.as_tensor(top_k)
+        if top_k.is_floating_point() or top_k.is_complex():
+            raise ValueError("top_k must be whole numbers")
+        top_k = top_k.long().clamp(0, 2 ** 31 - 1)      # (0 and all of a vocabulary keep all)
     draws = {"temperature": _per_request(temperature, n, dev),
              "top_k": _per_request(top_k, n, dev, torch.int32),
              "top_p": _per_request(top_p, n, dev), "min_p": _per_request(min_p, n, dev)}
