@@ -197,6 +197,8 @@ class PackedLinear8(torch.nn.Module):
             if x.dim() == 0 or x.shape[-1] != self.in_features:
                 raise ValueError(f"x last dim must be {self.in_features}, got {tuple(x.shape)}")
             shape = x.shape[:-1]
+            if residual is not None and (residual.dim() == 0 or residual.shape[:-1] != shape):
+                raise ValueError(f"residual must be {(*shape, '...')}, got {tuple(residual.shape)}")
             x = ops.quantize8(x.reshape(-1, self.in_features))
         weights = ops.Weights8(self.tiles, self.scale, self.out_features, self.in_features)
         if residual is not None and shape is not None:
