@@ -746,7 +746,8 @@ int nb_logits_rules(const void* logits, int dtype, int64_t ld, int rows, int V,
  * a temperature of 1 and rules that keep all.  Weights are whole multiples of
  * 2^-45 (2^-38 at the largest V), their sums exact, so the same call gives the
  * same tokens.  The workspace needs nb_sample_ws_bytes(rows, V) bytes, 16-byte
- * aligned (0: may be NULL).
+ * aligned (0: may be NULL).  It, tokens and logprobs overlap neither an input nor one
+ * another.
  */
 int64_t nb_sample_ws_bytes(int rows, int V);
 int nb_sample(const void* logits, int dtype, int64_t ld, int rows, int V, const float* u,
@@ -758,6 +759,7 @@ int nb_sample(const void* logits, int dtype, int64_t ld, int rows, int V, const 
  * Rows in 8 bits through the packed layers.  No counterpart in the reference
  * (its layers multiply fp32 or bf16 activations, inference/triton_kernel.py:
  * 240-275); the layers' indices are its own, their codebooks rounded once.
+ * Outputs overlap neither inputs nor one another, but where a call says so.
  * ------------------------------------------------------------------------ */
 /*
  * Rows in 8 bits with a scale each: codes int8 [rows][width] and scale fp32

@@ -1188,6 +1188,19 @@ bool rows_overlap(const void* in, int in_dtype, int64_t ld_in, int64_t in_width,
     return column < in_width * in_size || column + out_width * out_size > pitch;
 }
 
+// Whether `rows` rows of `width` bytes, `pitch` apart, reach into `bytes` bytes (both ways
+// round: one of the two is written).
+bool rows_reach(const void* rows_at, int64_t pitch, int64_t width, int64_t rows, const void* span, int64_t bytes) {
+    if (!rows_at || !span || rows < 1 || width < 1 || bytes < 1) return false;
+    const int64_t from = (int64_t)(reinterpret_cast<uintptr_t>(span) - reinterpret_cast<uintptr_t>(rows_at));
+    if (from + bytes <= 0 || from >= (rows - 1) * pitch + width) return false;
+    const int64_t row = from < width ? 0 : (from - width) / pitch + 1;   // the first that ends past its start
+    return row * pitch < from + bytes;
+}
+bool spans_meet(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+    return rows_reach(a, a_bytes, a_bytes, 1, b, b_bytes);
+}
+
 // Chunks times the workgroups of each in one dimension of a grid of 256
 // threads each (under 2^32 work-items).
 int check_chunks(const char* fn, const void* chunks, int n_chunks, int64_t per_chunk) {
@@ -1471,6 +1484,18 @@ int nb_sample(const void* logits, int dtype, int64_t ld, int rows, int V, const 
         return fail(NB_EINVAL, "%s: workspace of %lld bytes < %lld", fn, (long long)ws_bytes, (long long)need);
     }
     if (!aligned(workspace, 16)) return fail(NB_EALIGN, "%s: workspace not 16-byte aligned", fn);
+    const int64_t each = (int64_t)rows * 4, size = (int64_t)dtype_size(dtype);
+    const void* outputs[] = {tokens, logprobs, workspace};
+    const int64_t bytes[] = {each, each, need};
+    for (int i = 0; i < 3; ++i) {
+        bool meets = rows_reach(logits, ld * size, V * size, rows, outputs[i], bytes[i]);
+        for (const void* p : {(const void*)u, (const void*)temperature, (const void*)top_k,
+                              (const void*)top_p, (const void*)min_p}) {
+            meets = meets || spans_meet(p, each, outputs[i], bytes[i]);
+        }
+        for (int j = 0; j < i; ++j) meets = meets || spans_meet(outputs[j], bytes[j], outputs[i], bytes[i]);
+        if (meets) return fail(NB_EINVAL, "%s: tokens, logprobs or workspace overlap an input or one another", fn);
+    }
     st = ensure_device();
     if (st) return st;
     return launch_sample(logits, dtype, ld, rows, V, u, temperature, top_k, top_p, min_p, tokens,
@@ -1514,8 +1539,15 @@ extern "C" {
 
 int nb_quantize8(const void* x, int dtype, int64_t ld, int rows, int width, int8_t* codes,
                  float* scale, void* stream) {
-    int st = check_rows8("nb_quantize8", x, dtype, ld, rows, width, codes, scale);
+    const char* fn = "nb_quantize8";
+    int st = check_rows8(fn, x, dtype, ld, rows, width, codes, scale);
     if (st || rows == 0) return st;
+    const int64_t size = (int64_t)dtype_size(dtype), total = (int64_t)rows * width;
+    if (rows_reach(x, ld * size, width * size, rows, codes, total) ||
+        rows_reach(x, ld * size, width * size, rows, scale, (int64_t)rows * 4) ||
+        spans_meet(codes, total, scale, (int64_t)rows * 4)) {
+        return fail(NB_EINVAL, "%s: codes or scale overlap x or one another", fn);
+    }
     st = ensure_device();
     if (st) return st;
     return launch_quantize8(x, dtype, ld, rows, width, codes, scale, static_cast<hipStream_t>(stream));
@@ -1554,6 +1586,11 @@ int nb_rows8_values(const int8_t* codes, const float* scale, int rows, int width
     const char* fn = "nb_rows8_values";
     int st = check_rows8(fn, out, out_dtype, ld_out, rows, width, codes, scale);
     if (st || rows == 0) return st;
+    const int64_t size = (int64_t)dtype_size(out_dtype);
+    if (rows_reach(out, ld_out * size, width * size, rows, codes, (int64_t)rows * width) ||
+        rows_reach(out, ld_out * size, width * size, rows, scale, (int64_t)rows * 4)) {
+        return fail(NB_EINVAL, "%s: out overlaps codes or scale", fn);
+    }
     st = ensure_device();
     if (st) return st;
     return launch_rows8_values(codes, scale, rows, width, out, out_dtype, ld_out,
@@ -1572,6 +1609,18 @@ int nb_linear8_layout(const uint8_t* packed, const float* codebook, int N, int K
     if (!packed || !codebook || !tiles || !scale) return fail(NB_EINVAL, "%s: NULL pointer", fn);
     if (!aligned(packed, 4) || !aligned(codebook, 4) || !aligned(tiles, 16) || !aligned(scale, 4)) {
         return fail(NB_EALIGN, "%s: tiles 16-byte, the others 4-byte alignment", fn);
+    }
+    const int64_t blocks = (int64_t)N * (K / 128);
+    const void* inputs[] = {packed, codebook};
+    for (int i = 0; i < 2; ++i) {
+        const int64_t bytes = blocks * (i ? 32 : 48);
+        if (spans_meet(inputs[i], bytes, tiles, linear8_tiles_bytes(N, K)) ||
+            spans_meet(inputs[i], bytes, scale, (int64_t)N * 4)) {
+            return fail(NB_EINVAL, "%s: tiles or scale overlap packed or codebook", fn);
+        }
+    }
+    if (spans_meet(tiles, linear8_tiles_bytes(N, K), scale, (int64_t)N * 4)) {
+        return fail(NB_EINVAL, "%s: tiles overlap scale", fn);
     }
     st = ensure_device();
     if (st) return st;
@@ -1610,6 +1659,14 @@ int nb_linear8(const int8_t* x, int64_t ld_x, const float* x_scale, const uint8_
         if (rows_overlap(residual, y_dtype, ld_residual, out, y, y_dtype, ld_y, out, M)) {
             return fail(NB_EINVAL, "%s: y overlaps residual (in place: of the same stride)", fn);
         }
+    }
+    const int64_t size = (int64_t)dtype_size(y_dtype);
+    if (rows_overlap(x, NB_U8, ld_x, K, y, y_dtype, ld_y, out, M) ||
+        rows_reach(y, ld_y * size, out * size, M, x_scale, (int64_t)M * 4) ||
+        rows_reach(y, ld_y * size, out * size, M, tiles, linear8_tiles_bytes(N, K)) ||
+        rows_reach(y, ld_y * size, out * size, M, scale, (int64_t)N * 4) ||
+        rows_reach(y, ld_y * size, out * size, M, bias, (int64_t)N * 4)) {
+        return fail(NB_EINVAL, "%s: y overlaps x, x_scale, tiles, scale or bias", fn);
     }
     st = ensure_device();
     if (st) return st;

@@ -1096,6 +1096,9 @@ def rmsnorm8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
             ld_out = width
         else:
             ld_out = _rows("out", out, rows, width, dev)
+            at, end = out.data_ptr(), out.data_ptr() + ((rows - 1) * ld_out + width) * out.element_size()
+            if rows and at < weight + 4 * width and weight < end:
+                raise ValueError("out overlaps weight")
         if residual.dtype != x.dtype or out.dtype != x.dtype:
             raise TypeError(f"x is {x.dtype}, residual {residual.dtype}, out {out.dtype}")
     codes = torch.empty((rows, width), dtype=torch.int8, device=x.device)
