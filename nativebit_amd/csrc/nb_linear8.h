@@ -178,28 +178,33 @@ __device__ __forceinline__ Column column(const Args& a, int n) {
     return c;
 }
 
-// v Phi(v).  Phi(-a) = exp(-a^2 / 2) t P(t) for a >= 0 with t = 1 / (1 + 0.21 a), the
-// form of Abramowitz and Stegun 7.1.26: what is left beside the exponential is smooth in
-// t from 1/2 at 0 to its end, and a polynomial of degree 8 (least largest relative
-// error, fitted in 64 bits for t of a up to 15, where the exponential is below fp32) is
-// within 5.2e-8 of it with its coefficients in fp32.
+// v Phi(v).  Phi(-a) = exp(-a^2 / 2) P(u) for a >= 0 with u = 0.21 a / (1 + 0.21 a), the
+// form of Abramowitz and Stegun 7.1.26 in 1 - t: what is left beside the exponential is
+// smooth in u from 1/2 at 0 to its end, and a polynomial of degree 9 (least largest
+// relative error, fitted in 64 bits for a up to 15, where the exponential is below fp32)
+// is within 1.4e-8 of it.  (In t = 1 / (1 + 0.21 a) the polynomial is as short, but its
+// value near 0 moves four times as far as t does.)
 // Nothing cancels: a product on the left, at most half of v taken off on the right
 // (by a finite factor: of an infinity nothing is, where v tail would be inf * 0).
-// 19 instructions, no branch: 500 rows of 5003 x 1280 without an activation 11.8 us,
-// with this 13.7, with erfcf 3 more (launches of a graph).
+// Errors of 2^20 outputs in fp32 against 64 bits, of v of deviation 0.1, 0.3, 1 and 3:
+// 4.0e-8, 3.8e-8, 2.9e-8 and 2.2e-8; v (1 + erf) / 2 in fp32 3.8e-8, 4.1e-8, 3.9e-8 and 3.0e-8.
+// No branch: 500 rows of 5003 x 1280 in bf16 12.6 us, without an activation 11.0, with
+// erfcf 3 more (launches of a graph).
 __device__ __forceinline__ float gelu(float v) {
-    const float a = __builtin_fabsf(v), t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.21f, a, 1.f));
-    float p = -0.07094477862119675f;
-    p = __builtin_fmaf(p, t, 0.2800799608230591f);
-    p = __builtin_fmaf(p, t, -0.3228669762611389f);
-    p = __builtin_fmaf(p, t, 0.34074342250823975f);
-    p = __builtin_fmaf(p, t, -0.08775527775287628f);
-    p = __builtin_fmaf(p, t, 0.12213890254497528f);
-    p = __builtin_fmaf(p, t, 0.06992674618959427f);
-    p = __builtin_fmaf(p, t, 0.08495952934026718f);
-    p = __builtin_fmaf(p, t, 0.0837184712290764f);
-    const float tail = __builtin_amdgcn_exp2f(a * a * -0.72134752f) * (t * p);
-    return v < 0.f ? v * tail : __builtin_fmaf(-__builtin_fminf(a, 3.4e38f), tail, v);
+    const float a = __builtin_fminf(__builtin_fabsf(v), 3.4e38f), c = 0.21f * a;
+    const float u = c * __builtin_amdgcn_rcpf(1.f + c);
+    float p = 0.07293546944856644f;
+    p = __builtin_fmaf(p, u, -0.3659140467643738f);
+    p = __builtin_fmaf(p, u, 0.6481500864028931f);
+    p = __builtin_fmaf(p, u, -0.04684164747595787f);
+    p = __builtin_fmaf(p, u, -1.916527509689331f);
+    p = __builtin_fmaf(p, u, 4.159022331237793f);
+    p = __builtin_fmaf(p, u, -4.920256614685059f);
+    p = __builtin_fmaf(p, u, 3.7691614627838135f);
+    p = __builtin_fmaf(p, u, -1.8997241258621216f);
+    p = __builtin_fmaf(p, u, 0.5f);
+    const float tail = __builtin_amdgcn_exp2f(a * a * -0.72134752f) * p;
+    return v < 0.f ? v * tail : __builtin_fmaf(-a, tail, v);
 }
 
 // The outputs of four sums: row m, layer outputs n .. n + 3.  Loads, arithmetic and
