@@ -744,10 +744,10 @@ int nb_logits_rules(const void* logits, int dtype, int64_t ld, int rows, int V,
  * u is clamped to [0, 1).  A row of nothing but -inf and NaN gives -1 and -inf.
  * u, temperature, top_k, top_p and min_p have an entry a row; but for u, NULL is
  * a temperature of 1 and rules that keep all.  Weights are whole multiples of
- * 2^-45 (2^-38 at the largest V), their sums exact, so the same call gives the
- * same tokens.  The workspace needs nb_sample_ws_bytes(rows, V) bytes, 16-byte
- * aligned (0: may be NULL).  It, tokens and logprobs overlap neither an input nor one
- * another.
+ * 2^-45 (2^-38 at the largest V; one that rounds to 0 is never drawn), their sums
+ * exact, so the same call gives the same tokens.  The workspace needs
+ * nb_sample_ws_bytes(rows, V) bytes, 16-byte aligned (0: may be NULL).  It, tokens
+ * and logprobs overlap neither an input nor one another.
  */
 int64_t nb_sample_ws_bytes(int rows, int V);
 int nb_sample(const void* logits, int dtype, int64_t ld, int rows, int V, const float* u,
@@ -817,7 +817,8 @@ enum nb_activation {
  * bias fp32 [N] and residual (of y's type, stride ld_residual) may be NULL; y
  * NB_F32 or NB_BF16, stride ld_y; it may be the residual itself, of the same
  * stride, and else overlaps it in no element.  The sums over k are whole numbers
- * and exact, the rest is fp32, rounded to y's type once.  M <= 2^20, M N < 2^36,
+ * and exact, the rest is fp32 (the product of the two scales first), rounded to
+ * y's type once.  M <= 2^20, M N < 2^36,
  * ld_x <= 2^22.
  * (PackedLinear.forward, inference/triton_kernel.py:240-275, and what follows
  * it in a block, inference/generate_torch.py:109-132.)

@@ -6,8 +6,8 @@
 // by the LDS reads of rows and units beside the products (about 1700 of the 2048
 // cycles that a 256 x 256 x 128 step's products take, in a step of 3000; without
 // barriers 2600, without operands made 2400, loads alone 100), and at the ends by
-// whole rounds of tiles and the epilogue: 13824 x 2560 at 2048 rows 79 us, 1830
-// TOP/s.  Measured and not faster there: units straight to registers (88 us against
+// whole rounds of tiles and the epilogue: 13824 x 2560 at 2048 rows 78 to 81 us in
+// launches of a graph (1790 to 1860 TOP/s), 82 under the profiler.  Measured and not faster there: units straight to registers (88 us against
 // 82 with 128 x 128 tiles: 12 and 8 bytes a lane are many small requests), waits a block
 // later, tiles of an XCD in the other order.
 #include <math.h>

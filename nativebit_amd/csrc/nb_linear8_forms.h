@@ -17,8 +17,10 @@ namespace linear8 {
 // 4.4 us by 32 x 32 (rows), 5.2 by 16 x 16, 6.4 by 64 x 32; 129 of 2560 x 6912 13.0 by 64 x
 // 32, 14.4 by 64 x 64, 18.3 by rows; 512 of 2560 x 6912 20.2 by 128 x 64 of two
 // groups, 27.3 of one, 27.9 by 64 x 64; 1500 of it 30.7 by 128 x 128 of two groups, 36.0 by
-// 128 x 64, 36.8 of one; 1500 of 13824 x 2560 67 by 128 x 128 of one, 85 of two, 75 by 256
-// x 256; 2048 of it 79.5 by 256 x 256, 85 by 128 x 128.
+// 128 x 64, 36.8 of one; 2048 of 13824 x 2560 80 by 256 x 256, 88 by 128 x 128 of one.  Where
+// whole rounds of the CUs meet the estimate is the other way round by a little: 1500 rows
+// of 13824 x 2560 take 76 by 256 x 256, estimated at 72, and would take 73 by 128 x 128 of
+// one, estimated at 76 (1200 to 1400 and 1700 rows are the same by both).
 struct Form {
     int outputs, rows;   // of a workgroup
     int split;           // groups of waves that share K

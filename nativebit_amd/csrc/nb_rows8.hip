@@ -13,9 +13,9 @@
 // Bound by memory: each value is read once, held in registers (as it was stored)
 // over the row's one reduction, and its code written.  2048 rows of 6912 fp32 values
 // 14.9 us (71 MB, 4.8 TB/s) and back 12.9 (5.5 TB/s); the norm of 2048 rows of 2560 with
-// its residual and the sum written 16.4 (68 MB, 4.2 TB/s), without them 9.3, where the
-// 64-bit products and quotients are half of it; one row 2 to 4 us, a launch and the
-// reduction's waits.
+// its residual and the sum written 15.9 (68 MB, 4.3 TB/s), without them 11.2 (9.3 again and
+// again on one input), where the 64-bit products and quotients are half of it; one row
+// 2 to 4 us, a launch and the reduction's waits.
 #include <math.h>
 
 #include <algorithm>

@@ -28,17 +28,22 @@
 // tokens that reach it, and those are in the groups that do; k of them, but for
 // ties.  They are listed, and that is all that is read again of the row.
 // What it takes: 160 rows of 131077 fp32 logits with every rule and top_k of 1 to 1024
-// 47 us, 84 MB.  1 reads them at 3.6 TB/s in 23.5; 2 finds nothing to do in 4; 3 is
+// 46 us, 84 MB.  1 reads them at 3.6 TB/s in 23.5; 2 finds nothing to do in 4.6; 3 is
 // one memory round trip after the other (rules, groups, tokens, 2 us each) and some
-// twenty waits of a workgroup between, 20.  Without top_k 90 us: 2 takes 41, an exp in
-// 64 bits and an atomic in LDS for every token.  One row of 50257 with top_p 25 to 36 us
-// by how many tokens are listed (4, 6, and 11 to 20).
+// twenty waits of a workgroup between, 21.  With top_p or min_p alone 89 to 93 us (logits
+// of deviation 4, T = 0.8): 2 takes 44, an exp in 64 bits and an atomic in LDS for every
+// token.  With a temperature alone 69 (21, 34 and 12).  One row of 50257 with top_p 25 to
+// 36 us by how many tokens are listed (4, 6, and 11 to 20), with a temperature alone 16.
 // Other ways measured: cuts and list as launches of their own, a slice each, 34 and
 // 59 us where one took 29 and 48 (48 rows of 50257, 160 of 131077); a list that scans the
 // slice again instead of its groups 21 us at 160 rows, now 2 to 5; 1000 tokens sorted by
 // merging 40 us, through buckets 2.
-// A row with over kMostListed listed tokens (equal logits, mostly) is worked out by
-// its last workgroup alone: radix selection over the row.
+// A row with over kMostListed tokens in the bins that the rules cut through is worked out
+// by its workgroup alone: radix selection, some ten passes over the row.  Equal logits are
+// such rows (48 of 50257 with top_p 245 us, with top_k of 1000 194), and logits next to
+// each other where a cut falls: an eighth of an octave holds over 4096 of 131077 whose
+// deviation over T is about 1 (160 rows with top_p of 0.9 514 us, one 325), and of 262144
+// at 4/3 (48 rows 833 us, one 571).
 #include <math.h>
 
 #include <algorithm>

@@ -958,7 +958,9 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: torch.Tensor |
     that are ``min_p[b]`` or more; the token is the lowest whose running sum of
     kept weights is over ``u[b]`` of their total.  Each rule is a (B,) tensor,
     float32 (top_k int32), or None; 0 tokens, a share of 1 and a least weight of
-    0 keep all; a temperature of 0 takes the first of the order.  Returns int32
+    0 keep all; a temperature of 0 takes the first of the order.  Weights are whole
+    multiples of 2^-45 of the largest (2^-38 at 2^24 tokens): one that rounds to 0 is
+    never drawn.  Returns int32
     (B,) tokens, -1 where a row has nothing but -inf and NaN, and with
     ``logprobs`` also their float32 log-probabilities among the kept ones."""
     _require_cuda("logits", logits)
@@ -1043,7 +1045,7 @@ _ACTIVATIONS = {None: _lib.NB_ACT_NONE, "silu": _lib.NB_ACT_SILU, "gelu": _lib.N
 
 
 def _rows8_out(x):
-    """(device, rows, width, codes, scale) for rows x."""
+    """(device, rows, width) of rows x."""
     _require_cuda("x", x)
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f"x must be (rows, width), got {tuple(x.shape)}")
